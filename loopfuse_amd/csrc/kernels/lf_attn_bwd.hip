@@ -47,6 +47,17 @@ struct LfAttnBwdParams {
   long long ds_sh;        // elements of it per (batch, query head)
 };
 
+#ifndef LF_PACKED
+#define LF_PACKED 0        /* 1: sequences of different lengths packed into one tensor (lf_packed.hip.h): B = 1, Sq = Sk = its rows, and
+                              lf_attn_bwd_dkdv and lf_attn_bwd_dq take the tiles of a list, for which those are one sequence's */
+#endif
+#if LF_PACKED
+struct LfPackedBwdParams : LfAttnBwdParams {
+  const LfPackedTile* dkdv_tiles;      // of as many keys as a workgroup of lf_attn_bwd_dkdv has
+  const LfPackedTile* dq_tiles;        // of as many queries as one of lf_attn_bwd_dq has
+};
+#endif
+
 #define LF_BW_NT 256
 #ifndef LF_BW_GROUP
 #define LF_BW_GROUP 4      /* (batch, kv head) pairs of one XCD whose workgroups are dispatched together */
@@ -362,7 +373,12 @@ template <int kMost, int kMore> __device__ __forceinline__ void lf_bw_wait(int m
 // 89 -> 60 us.
 // With LF_BW_DS the B operands dS also leave for memory, two stores per 32 x 32 block between the MFMAs that take them, and the
 // barrier does not wait for them: 297 -> 340 us of the above for 545 MB (352 with plain stores, which take L2 from Q and dO).
+#if LF_PACKED
+extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const LfPackedBwdParams pk) {
+  LfAttnBwdParams p = pk;
+#else
 extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const LfAttnBwdParams p) {
+#endif
   constexpr int KB = LF_BW_W, kKeyWaves = LF_BW_QSPLIT ? 2 : 4, kStages = LF_BW_QSPLIT ? 4 : 3;
   constexpr int kKeys = 32 * KB * kKeyWaves;
   __shared__ __attribute__((aligned(256))) lf_elem tiles[kStages][2][64 * LF_D];        // Q, dO
@@ -377,13 +393,33 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
   const int l32 = lane & 31;
   const int g = lane >> 5;
 
-  const int nkt = (p.Sk + kKeys - 1) / kKeys;
   // All key blocks of a (batch, kv head) share the Q / dO tiles they walk in one XCD's L2; the first key
   // block has the most steps under a causal mask.
+#if LF_PACKED
+  const int entry = (int)blockIdx.x / p.Hkv, hkv = (int)blockIdx.x - entry * p.Hkv, b = 0;
+  const LfPackedTile mine = lf_packed_tile(pk.dkdv_tiles, entry);
+  if (mine.len == 0) return;
+  if (mine.seq < 0) {
+    lf_packed_clear<LF_BW_NT>(p.dk + (long long)mine.row0 * p.dk_ss + hkv * p.dk_sh, 0, p.dk_ss, 1, mine.tile * kKeys, kKeys, mine.len);
+    lf_packed_clear<LF_BW_NT>(p.dv + (long long)mine.row0 * p.dv_ss + hkv * p.dv_sh, 0, p.dv_ss, 1, mine.tile * kKeys, kKeys, mine.len);
+    return;
+  }
+  const int kt = mine.tile, stat_rows = p.Sq;
+  p.q += (long long)mine.row0 * p.q_ss;
+  p.k += (long long)mine.row0 * p.k_ss;
+  p.v += (long long)mine.row0 * p.v_ss;
+  p.dout += (long long)mine.row0 * p.do_ss;
+  p.lse += mine.row0;
+  p.delta += mine.row0;
+  p.Sq = p.Sk = mine.len;
+#else
+  const int nkt = (p.Sk + kKeys - 1) / kKeys;
   int bhkv, kt;
   if (!lf_slot_of_block(blockIdx.x, p.B * p.Hkv, nkt, LF_BW_GROUP, bhkv, kt)) return;
   const int hkv = bhkv % p.Hkv;
   const int b = bhkv / p.Hkv;
+  const int stat_rows = p.Sq;
+#endif
   const int group = p.Hq / p.Hkv;
   const int key0 = kKeys * kt + 32 * KB * (wave % kKeyWaves);    // first key of this wave
   const int my_qb = wave / kKeyWaves;                            // LF_BW_QSPLIT: the wave's 32 queries of a tile
@@ -460,7 +496,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
   int ld_step = 0, ld_tile = qt_begin, ld_q0 = 0;
   const lf_elem* ld_q = p.q + (long long)b * p.q_sb + (long long)(hkv * group) * p.q_sh;
   const lf_elem* ld_g = p.dout + (long long)b * p.do_sb + (long long)(hkv * group) * p.do_sh;
-  const float* ld_stat = (wave == 0 ? p.lse : p.delta) + ((long long)b * p.Hq + hkv * group) * p.Sq;
+  const float* ld_stat = (wave == 0 ? p.lse : p.delta) + ((long long)b * p.Hq + hkv * group) * stat_rows;
   lf_u32x4 q_rs, g_rs, stat_rs;
   auto aim = [&]() {
     const bool real = ld_step < nsteps;
@@ -473,7 +509,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
       ld_tile = qt_begin;
       ld_q += p.q_sh;
       ld_g += p.do_sh;
-      ld_stat += p.Sq;
+      ld_stat += stat_rows;
     }
   };
   const unsigned stat0 = lf_lds_addr(stats);
@@ -851,6 +887,11 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
   auto ep = (const LfAttnBwdParams __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(ep));
   const float scale = ep->scale;
+#if LF_PACKED
+  const long long out0 = mine.row0;
+#else
+  const long long out0 = 0;
+#endif
 #if LF_BW_QSPLIT
   const unsigned rows_lds = lds0 + (unsigned)(KB * LF_NDB * 8 * 128 * 16 + wave * LF_BW_ROWS_LDS);      // behind the sums
   static_assert(KB * LF_NDB * 8 * 128 * 16 + kKeyWaves * LF_BW_ROWS_LDS <= (int)sizeof(tiles), "sums and rows fit the tiles");
@@ -868,9 +909,9 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
     for (int db = 0; db < LF_NDB; ++db)
 #pragma unroll
       for (int i = 0; i < 16; ++i) dk[kb][db][i] *= scale;
-    lf_bw_store_rows(dk[kb], rows_lds, ep->dk + (long long)b * ep->dk_sb + (long long)hkv * ep->dk_sh + (long long)first * ep->dk_ss, ep->dk_ss,
+    lf_bw_store_rows(dk[kb], rows_lds, ep->dk + (long long)b * ep->dk_sb + (long long)hkv * ep->dk_sh + (out0 + first) * ep->dk_ss, ep->dk_ss,
                      p.Sk - first, lane);
-    lf_bw_store_rows(dv[kb], rows_lds, ep->dv + (long long)b * ep->dv_sb + (long long)hkv * ep->dv_sh + (long long)first * ep->dv_ss, ep->dv_ss,
+    lf_bw_store_rows(dv[kb], rows_lds, ep->dv + (long long)b * ep->dv_sb + (long long)hkv * ep->dv_sh + (out0 + first) * ep->dv_ss, ep->dv_ss,
                      p.Sk - first, lane);
   }
 }
@@ -1040,7 +1081,12 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
 //   causal B4 H32 S2048 D128 223 -> 222, B2 32/8 S4096 378 -> 373, B2 16/8 S777 35 -> 25, B1 32/8 S2048 85 -> 71
 //   the same with a softcap 383 -> 275; window 256 B4 32/8 S2048 151 -> 107, window 1024 259 -> 179
 //   causal B8 16/4 S1000 D64 fp16 47 -> 42, B16 32/8 S300 48 -> 32
+#if LF_PACKED
+extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_attn_bwd_dq(const LfPackedBwdParams pk) {
+  LfAttnBwdParams p = pk;
+#else
 extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_attn_bwd_dq(const LfAttnBwdParams p) {
+#endif
   constexpr int kBM = LF_BW_DQ_NT / 2;                           // query rows of a workgroup
   __shared__ __attribute__((aligned(256))) lf_elem tiles[3][2][64 * LF_D];        // K, V
 
@@ -1050,9 +1096,30 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   const int l32 = lane & 31;
   const int g = lane >> 5;
 
-  const int nqt = (p.Sq + kBM - 1) / kBM;
   // As in lf_attn_bwd_dkdv: the q tiles of all query heads of a (batch, kv head) share its K / V tiles in one
   // XCD's L2, the long q tiles first.
+#if LF_PACKED
+  const int entry = (int)blockIdx.x / p.Hq, unit = (int)blockIdx.x - entry * p.Hq, b = 0;
+  const int hkv = unit % p.Hkv, h = hkv * (p.Hq / p.Hkv) + unit / p.Hkv;
+  const LfPackedTile mine = lf_packed_tile(pk.dq_tiles, entry);
+  if (mine.len == 0) return;
+  p.dq += (long long)mine.row0 * p.dq_ss;
+  if (mine.seq < 0) {
+    lf_packed_clear<LF_BW_DQ_NT>(p.dq + h * p.dq_sh, 0, p.dq_ss, 1, mine.tile * kBM, kBM, mine.len);
+    return;
+  }
+  const int stat_rows = p.Sq;
+  p.q += (long long)mine.row0 * p.q_ss;
+  p.k += (long long)mine.row0 * p.k_ss;
+  p.v += (long long)mine.row0 * p.v_ss;
+  p.o += (long long)mine.row0 * p.o_ss;
+  p.dout += (long long)mine.row0 * p.do_ss;
+  p.lse += mine.row0;
+  p.delta += mine.row0;
+  p.Sq = p.Sk = mine.len;
+  const int qt = (p.Sq + kBM - 1) / kBM - 1 - mine.tile;
+#else
+  const int nqt = (p.Sq + kBM - 1) / kBM;
   const int nrow = (p.Hq / p.Hkv) * nqt;                  // (query head of the group, q tile) per pair
   int bhkv, row;
   if (!lf_slot_of_block(blockIdx.x, p.B * p.Hkv, nrow, LF_BW_GROUP, bhkv, row)) return;
@@ -1060,6 +1127,8 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   const int hkv = bhkv % p.Hkv;
   const int b = bhkv / p.Hkv;
   const int h = hkv * (p.Hq / p.Hkv) + row % (p.Hq / p.Hkv);
+  const int stat_rows = p.Sq;
+#endif
   const int q0 = kBM * qt;
   const int wq0 = q0 + 32 * wave;                    // first row of this wave
   const int nkt = (p.Sk + 63) / 64;
@@ -1101,7 +1170,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
 #pragma unroll
     for (int ks = 0; ks < LF_NKS; ++ks) asm volatile("" : "+a"(qf[ks]), "+a"(gf[ks]));
   }
-  const long long ridx = ((long long)b * p.Hq + h) * p.Sq + qr;
+  const long long ridx = ((long long)b * p.Hq + h) * stat_rows + qr;
   const float lse_q = my_q < p.Sq ? p.lse[ridx] : __builtin_inff();
 #if LF_BW_DQ_NT == 256
   if (my_q < p.Sq && g == 0) p.delta[ridx] = -delta_q;     // for lf_attn_bwd_dkdv

@@ -109,7 +109,18 @@
 #define LF_SPLIT_EXP (!LF_SOFTCAP || !LF_BIAS)     /* second key block's exponentials between the MFMAs of the first (config 2: -0.7 %; no gain with a softcap) */
 #endif
 
+#ifndef LF_PACKED
+#define LF_PACKED 0      /* 1: the tiles of sequences of different lengths packed into one tensor (lf_packed.hip.h) */
+#endif
+#if LF_PACKED && (LF_PAGED || LF_BIAS)
+#error "packed sequences go with dense operands and the flag masks"
+#endif
+#if LF_PACKED
+extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(const LfPackedAttnParams pk) {
+  LfAttnParams p = pk;
+#else
 extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(const LfAttnParams p) {
+#endif
   // one array, K slots first
   __shared__ __attribute__((aligned(16))) lf_elem lds_all[(LF_KSLOTS + LF_VSLOTS) * LF_BN * LF_D];
 
@@ -119,13 +130,35 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
   const int l32 = lane & 31;
   const int g = lane >> 5;
 
+  const int nhv = p.Hq / LF_HEADS_PER_WG;     // head units per batch element (heads, or packs of heads)
+#if LF_PACKED
+  const int entry = (int)blockIdx.x / nhv, bh = (int)blockIdx.x - entry * nhv, b = 0;
+  const LfPackedTile mine = lf_packed_tile(pk.tiles, entry);
+  if (mine.len == 0) return;
+  if (mine.seq < 0) {
+    if (pk.clear)
+      lf_packed_clear<LF_NT>(p.o + (long long)mine.row0 * p.o_ss + (long long)(bh * LF_HEADS_PER_WG) * p.o_sh, p.o_sh, p.o_ss, LF_HEADS_PER_WG,
+                             mine.tile * LF_BM, LF_BM, mine.len);
+    return;
+  }
+  p.q += (long long)mine.row0 * p.q_ss;
+  p.k += (long long)mine.row0 * p.k_ss;
+  p.v += (long long)mine.row0 * p.v_ss;
+  p.o += (long long)mine.row0 * p.o_ss;
+  if (p.part_ml != nullptr) p.part_ml += mine.row0;
+  const int lse_rows = p.Sq;
+  p.Sq = p.Sk = mine.len;
+  const int nqt = (p.Sq + LF_BM - 1) / LF_BM;
+  const int slot_qt = nqt - 1 - mine.tile;    // the last q tile, which has the most kv tiles under a causal mask, comes first
+#else
   // ---- workgroup -> (batch*head, q tile): lf_slot_of_block; under a causal mask the last q tile has the most kv tiles
   const int nqt = (p.Sq + LF_BM - 1) / LF_BM;
-  const int nhv = p.Hq / LF_HEADS_PER_WG;     // head units per batch element (heads, or packs of heads)
   int bh, from_end;
   if (!lf_slot_of_block(blockIdx.x, p.B * nhv, nqt, LF_QGROUP, bh, from_end)) return;
   const int slot_qt = nqt - 1 - from_end;
   const int b = bh / nhv;
+  const int lse_rows = p.Sq;
+#endif
 #if LF_GQAPACK
   const int h = (bh % nhv) * LF_GQAPACK + wave % LF_GQAPACK;    // this wave's query head
 #else
@@ -786,9 +819,9 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     if (p.part_ml != nullptr && g == 0 && my_q < p.Sq)
 #if LF_SOFTCAP && !LF_CAPPOLY
       // the kernel's scores are the capped ones minus the cap: the cap comes back in here
-      p.part_ml[((long long)b * p.Hq + h) * p.Sq + my_q] = mc_ref + __builtin_log2f(l_tot) + p.softcap * LF_LOG2E;
+      p.part_ml[((long long)b * p.Hq + h) * lse_rows + my_q] = mc_ref + __builtin_log2f(l_tot) + p.softcap * LF_LOG2E;
 #else
-      p.part_ml[((long long)b * p.Hq + h) * p.Sq + my_q] = mc_ref + __builtin_log2f(l_tot);
+      p.part_ml[((long long)b * p.Hq + h) * lse_rows + my_q] = mc_ref + __builtin_log2f(l_tot);
 #endif
     {
 #if LF_SAFE

@@ -1,0 +1,47 @@
+// lf_packed.hip.h — sequences of different lengths, one behind the other in one tensor, for the attention kernels
+// (-DLF_PACKED=1): row i of Q, K, V, O [rows, heads, D] belongs to sequence n where offsets[n] <= i < offsets[n + 1].
+//
+// The work items are the tiles of a list that lf_packed_plan (lf_packed_plan.hip) leaves on the GPU: the host knows the
+// number of rows and of sequences, not the lengths, and launches a workgroup per head and entry that the list can have.  A kernel takes its
+// tile's sequence for the whole problem: B = 1, Sq = Sk = its length, pointers at its first row.
+//   Workgroup -> (entry, head): the heads of an entry are neighbours, so that with a multiple of 8 of them each XCD walks
+// its own heads over the entries in their order, and the tiles of a (sequence, head) share its K / V (or Q / dO) in one L2.
+#ifndef LF_PACKED_HIP_H
+#define LF_PACKED_HIP_H
+
+struct LfPackedTile {
+  int row0;        // first row of the sequence
+  int len;         // its rows; 0: no tile
+  int tile;        // number of the tile in it; a tile has as many rows as the list is for
+  int seq;         // number of the sequence; -1: rows of no sequence
+};
+typedef const LfPackedTile __attribute__((address_space(4))) lf_ctile;
+
+// the tile of an entry, through scalar loads
+__device__ __forceinline__ LfPackedTile lf_packed_tile(const LfPackedTile* tiles, int entry) {
+  const lf_ctile* t = reinterpret_cast<const lf_ctile*>(reinterpret_cast<unsigned long long>(tiles)) + entry;
+  LfPackedTile r;
+  r.row0 = t->row0;
+  r.len = t->len;
+  r.tile = t->tile;
+  r.seq = t->seq;
+  return r;
+}
+
+// Rows of no sequence: zeros into rows first .. first + rows - 1 (those below `end`) of `heads` neighbouring heads.
+template <int NT>
+__device__ __forceinline__ void lf_packed_clear(lf_elem* x, long long sh, long long ss, int heads, int first, int rows, int end) {
+  constexpr int kChunks = LF_HEAD_DIM / 8;
+  rows = min(rows, end - first);
+  for (int i = threadIdx.x; i < rows * heads * kChunks; i += NT) {
+    const int c = i % kChunks, h = i / kChunks % heads, r = i / (kChunks * heads);
+    *reinterpret_cast<lf_u32x4*>(x + (long long)(first + r) * ss + h * sh + 8 * c) = lf_u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+struct LfPackedAttnParams : LfAttnParams {      // Sq = Sk = rows of the tensors, B = 1
+  const LfPackedTile* tiles;
+  int clear;               // 1: rows of no sequence are set to zero, 0: they are left as they are
+};
+
+#endif  // LF_PACKED_HIP_H

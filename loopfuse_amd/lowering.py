@@ -97,6 +97,7 @@ class KernelSpec:
     bn: int = 0            # prefill_swp: keys per LDS tile, 32 (three workgroups per CU) or 0 / 64 (two)
     extra: tuple = ()      # further -D options (tuning experiments)
     stay: bool = False     # prefill_swp, bwd: results by plain stores (prefill_out_stays, bwd_grads_stay)
+    packed: bool = False   # prefill_swp, bwd: the tiles of sequences of different lengths in one tensor (lf_packed.hip.h)
 
     def __hash__(self):    # formed once: a call looks its kernels up by it, several times
         h = self.__dict__.get("_hash")
@@ -142,13 +143,19 @@ class KernelSpec:
                 o += ["-DLF_BIAS=2" if self.bias == MASK_BITS else "-DLF_BIAS=1"]
         if self.stay:
             o += ["-DLF_STAY=1"]
+        if self.packed:
+            o += ["-DLF_PACKED=1"]
         if self.safe:
             o += ["-DLF_SAFE=1"]
         return o + list(self.extra)
 
     def files(self) -> tuple[str, ...]:
         kernel = {"prefill": "lf_attn_prefill.hip", "prefill_swp": "lf_attn_prefill_swp.hip",
-                  "decode": "lf_attn_decode.hip", "bwd": "lf_attn_bwd.hip"}[self.family]
+                  "decode": "lf_attn_decode.hip", "bwd": "lf_attn_bwd.hip", "packed_plan": "lf_packed_plan.hip"}[self.family]
+        if self.family == "packed_plan":
+            return ("lf_common.hip.h", "lf_packed.hip.h", kernel)
+        if self.packed:
+            return ("lf_common.hip.h", "lf_packed.hip.h", "lf_prefill_blocks.hip.h", kernel)
         if self.family == "decode":
             return ("lf_common.hip.h", kernel)
         # the two prefill kernels: their own tuning macros come first (the shared blocks use LF_BN)
@@ -160,13 +167,13 @@ class KernelSpec:
 
     def entry(self) -> str:
         return {"prefill": "lf_attn_prefill", "prefill_swp": "lf_attn_prefill_swp", "decode": "lf_attn_decode",
-                "bwd": "lf_attn_bwd_dq"}[self.family]
+                "bwd": "lf_attn_bwd_dq", "packed_plan": "lf_packed_plan"}[self.family]
 
     def name(self) -> str:
         return (f"lf_{self.family}_t{self.dtype}_d{self.head_dim}_m{self.mask}_c{int(self.softcap)}"
                 f"_p{self.paged}x{self.page_size}i{int(self.table_i64)}_r{self.rows}w{self.waves}v{int(self.v_tr)}h{int(self.headwave)}b{self.bias}n{int(self.denom)}"
                 + (f"_q{self.d2}" if self.d2 else "") + (f"_gp{int(self.pack)}" if self.pack else "") + (f"_pv{self.page_size_v}" if self.page_size_v else "")
-                + ("_z" if self.safe else "") + (f"_bn{self.bn}" if self.bn else "") + ("_co" if self.coop else "") + ("_rl" if self.rowload else "") + ("_st" if self.stay else "")
+                + ("_z" if self.safe else "") + (f"_bn{self.bn}" if self.bn else "") + ("_co" if self.coop else "") + ("_rl" if self.rowload else "") + ("_st" if self.stay else "") + ("_pk" if self.packed else "")
                 + "".join("_" + e.replace("-D", "").replace("=", "") for e in self.extra))
 
     def source(self) -> str:

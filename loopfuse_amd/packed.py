@@ -1,0 +1,291 @@
+"""Attention over sequences of different lengths packed into one tensor, forward and backward.
+
+A batch whose sequences differ in length stands here as one tensor ``[rows, heads, D]``, one sequence behind the other, with
+their bounds ``offsets`` (``N + 1`` numbers on the GPU): no padding is stored, read or computed.
+
+    layout = packed_layout(offsets, total)                  # once per batch, for all layers
+    o = attention_packed(q, k, v, AttnPlan("causal", scale=D ** -0.5), layout)
+
+Every query sees the keys of its own sequence under the plan's mask (none, causal, causal sliding window; positions count from the
+sequence's first row).  The kernels are those of the dense operators (``lowering.attention``, ``lowering.attention_backward``)
+built with ``-DLF_PACKED=1``: their workgroups take the tiles of a list that ``packed_layout`` leaves on the GPU, so that nothing
+waits for the lengths.  The reference has no counterpart: its graphs hold one length for a batch (reference README.md:62-99).
+"""
+from __future__ import annotations
+
+import ctypes
+import dataclasses
+import math
+from typing import Optional
+
+import torch
+
+from . import lowering, runtime
+from .lowering import AttnPlan, UnsupportedPlan
+
+TILE_HEIGHTS = (32, 64, 128, 256)      # rows of a tile, list by list
+
+
+class _PlanParams(ctypes.Structure):
+    """Mirror of ``struct LfPackedPlanParams`` in csrc/kernels/lf_packed_plan.hip."""
+
+    _fields_ = [("offsets", ctypes.c_void_p), ("tiles", ctypes.c_void_p), ("N", ctypes.c_int), ("T", ctypes.c_int), ("cap", ctypes.c_int * 4)]
+
+
+class PackedAttnParams(lowering.AttnParams):
+    """Mirror of ``struct LfPackedAttnParams`` in csrc/kernels/lf_packed.hip.h."""
+
+    _fields_ = [("tiles", ctypes.c_void_p), ("clear", ctypes.c_int)]
+
+
+class PackedBwdParams(lowering.AttnBwdParams):
+    """Mirror of ``struct LfPackedBwdParams`` in csrc/kernels/lf_attn_bwd.hip."""
+
+    _fields_ = [("dkdv_tiles", ctypes.c_void_p), ("dq_tiles", ctypes.c_void_p)]
+
+
+@dataclasses.dataclass(frozen=True, eq=False)
+class PackedLayout:
+    """Where the sequences of a packed batch lie, and the lists of their tiles (``packed_layout``)."""
+
+    offsets: torch.Tensor      # int32 [N + 1]
+    total: int                 # rows of the packed tensors
+    tiles: torch.Tensor        # int32 [entries of all lists, 4]
+    caps: tuple                # entries of each list
+
+    @property
+    def count(self) -> int:
+        return self.offsets.shape[0] - 1
+
+    def tiles_of(self, rows: int) -> tuple:
+        """(address, entries) of the list of tiles of so many rows."""
+        i = TILE_HEIGHTS.index(rows)
+        return self.tiles.data_ptr() + 16 * sum(self.caps[:i]), self.caps[i]
+
+
+def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
+    """The layout of a batch of ``N`` packed sequences: sequence ``n`` is rows ``offsets[n] ... offsets[n + 1]`` of tensors of
+    ``total`` rows.  ``offsets``: int32 or int64 ``[N + 1]`` on the GPU, not descending (as a cumulative sum of the lengths is); sequences may be
+    empty.  One launch on the current stream, nothing waits for it; the layout serves every call over this batch, forward and
+    backward, on that stream or on one that waits for it.  Offsets beyond ``0 ... total`` count as the nearer bound."""
+    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype not in (torch.int32, torch.int64):
+        raise UnsupportedPlan("offsets must be an int32 or int64 tensor of one more than the number of sequences")
+    if not offsets.is_cuda:
+        raise RuntimeError("loopfuse_amd: offsets are not on the GPU; the HIP path has no CPU fallback")
+    total = int(total)
+    if total < 0 or total >= 1 << 31:
+        raise UnsupportedPlan("the number of rows must be between 0 and 2**31 - 1")
+    with torch.cuda.device(offsets.device):
+        offsets = offsets.clamp(0, total).to(torch.int32) if offsets.dtype == torch.int64 else offsets.contiguous()
+        count = offsets.shape[0] - 1
+        # a sequence ends with a tile that is not full; so do the rows of no sequence at either end
+        caps = tuple(total // rows + count + 2 for rows in TILE_HEIGHTS)
+        tiles = torch.empty((sum(caps), 4), dtype=torch.int32, device=offsets.device)
+        P = _PlanParams(offsets.data_ptr(), tiles.data_ptr(), count, total, caps)
+        spec = lowering._spec("packed_plan", 0, 64)
+        lowering.get_kernel(spec, spec.entry()).launch((-(-(count + 2) // 256), len(TILE_HEIGHTS), 1), (256, 1, 1), P)
+    return PackedLayout(offsets, total, tiles, caps)
+
+
+def _rows(name: str, t: torch.Tensor, layout: PackedLayout, dtype, D: Optional[int] = None) -> None:
+    if t.dim() != 3 or t.shape[0] != layout.total:
+        raise UnsupportedPlan(f"{name} must be [{layout.total}, heads, D]")
+    if D is not None and t.shape[2] != D:
+        raise UnsupportedPlan(f"{name} has head dim {t.shape[2]}, Q has {D}")
+    lowering._check_tensor(name, t, dtype)
+    if t.device != layout.tiles.device:
+        raise RuntimeError(f"loopfuse_amd: {name} is on {t.device}, the layout on {layout.tiles.device}")
+
+
+def _constants(plan: AttnPlan) -> tuple:
+    """(mask, window, scale, softcap or None) of a plan that the packed kernels serve."""
+    if plan.k_paged or plan.v_paged or plan.denom_add != 0.0:
+        raise UnsupportedPlan("packed sequences go with dense K/V and the plain softmax denominator")
+    if plan.mask not in lowering._MASK_NAMES:
+        raise UnsupportedPlan(f"mask {plan.mask!r} not served")
+    mask = lowering._MASK_NAMES[plan.mask]
+    if mask == lowering.MASK_SLIDING and plan.window < 1:
+        raise UnsupportedPlan("sliding mask needs window >= 1")
+    if not (plan.scale > 0.0) or not math.isfinite(plan.scale):
+        raise UnsupportedPlan("score scale must be positive and finite")
+    cap = None
+    if plan.softcap is not None:
+        cap = abs(float(plan.softcap))
+        if not (cap > 0.0) or not math.isfinite(cap):
+            raise UnsupportedPlan("softcap must be finite and non-zero")
+    # a window beyond the rows keeps what a causal mask keeps; the kernels add it to positions in 32 bits
+    return mask, min(int(plan.window), 1 << 30) if mask == lowering.MASK_SLIDING else 0, float(plan.scale), cap
+
+
+def _heads(q, k, v, layout) -> tuple:
+    dtype = q.dtype
+    if dtype not in lowering._DTYPE_CODE:
+        raise UnsupportedPlan(f"dtype {dtype} not supported by the MFMA kernels (bf16/fp16 only)")
+    if q.dim() != 3 or q.shape[2] not in (64, 128):
+        raise UnsupportedPlan("Q must be [rows, Hq, D] with head dim 64 or 128")
+    D = q.shape[2]
+    for name, t in (("Q", q), ("K", k), ("V", v)):
+        _rows(name, t, layout, dtype, D)
+    Hq, Hkv = q.shape[1], k.shape[1]
+    if v.shape[1] != Hkv or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise UnsupportedPlan(f"{Hq} query heads over {Hkv} / {v.shape[1]} kv heads")
+    return dtype, D, Hq, Hkv
+
+
+def _grid(entries: int, heads: int, threads: int) -> int:
+    if entries * heads * threads >= 1 << 32:
+        raise UnsupportedPlan(f"a launch of {entries} tiles x {heads} heads is too large")
+    return entries * heads
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPlan, layout: PackedLayout, *,
+                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of every packed sequence over itself: q ``[rows, Hq, D]``, k and v ``[rows, Hkv, D]`` (views will do: rows of a
+    fused projection) to O ``[rows, Hq, D]``.  bf16 / fp16, Hq a multiple of Hkv, D 64 or 128, any other below 128 by zero-padding;
+    ``plan``: mask, window, scale and softcap.  Rows of no sequence, in front of the first offset or behind the last,
+    come out as zeros, or stay as they are in an ``out`` that is given.  ``lse``: float32 ``[Hq, rows]``, contiguous, to be given the
+    rows' log-sum-exp in log2 units, as ``lowering.attention`` does.
+
+    Differentiable where gradients are recorded and neither ``out`` nor ``lse`` is given; gradients of rows of no sequence are zero."""
+    if not isinstance(layout, PackedLayout):
+        raise UnsupportedPlan("layout must come from packed_layout")
+    if q.dim() == 3 and q.shape[2] not in (64, 128) and 1 <= q.shape[2] < 128:
+        if out is not None or lse is not None or k.dim() != 3 or v.dim() != 3 or k.shape[2] != q.shape[2] or v.shape[2] != q.shape[2]:
+            raise UnsupportedPlan(f"head dim {q.shape[2]}: by zero-padding, without out and lse")
+        D = q.shape[2]
+        q, k, v = (torch.nn.functional.pad(t, (0, (64 if D < 64 else 128) - D)) for t in (q, k, v))
+        return attention_packed(q, k, v, plan, layout)[..., :D].contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        if out is not None or lse is not None:
+            raise UnsupportedPlan("out and lse are for calls without gradients")
+        return _Packed.apply(q, k, v, plan, layout)
+    return _forward(q, k, v, plan, layout, out, lse)
+
+
+@lowering._on_device_of_first_argument
+def _forward(q, k, v, plan, layout, out, lse):
+    dtype, D, Hq, Hkv = _heads(q, k, v, layout)
+    mask, window, scale, cap = _constants(plan)
+    T = layout.total
+    for name, t in (("K", k), ("V", v)):
+        # direct-to-LDS loads address a sequence with 32-bit byte offsets, up to three tiles past its end
+        if t.stride(0) < 0 or 2 * (T + 192) * t.stride(0) + 2 * D >= 1 << 31:
+            raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
+    fresh = out is None
+    if fresh:
+        out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
+    else:
+        _rows("O", out, layout, dtype, D)
+        if out.shape[1] != Hq or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+            raise UnsupportedPlan(f"O must be [{T}, {Hq}, {D}], every element with a place of its own")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or not lse.is_contiguous() or lse.device != q.device):
+        raise UnsupportedPlan(f"lse must be a contiguous float32 [{Hq}, {T}] tensor on the device of Q")
+    if T == 0:
+        return out
+    P = PackedAttnParams()
+    P.q, P.k, P.v, P.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    P.q_ss, P.q_sh = q.stride()[:2]
+    P.k_ss, P.k_sh = k.stride()[:2]
+    P.v_ss, P.v_sh = v.stride()[:2]
+    P.o_ss, P.o_sh = out.stride()[:2]
+    P.B, P.Hq, P.Hkv, P.Sq, P.Sk, P.window = 1, Hq, Hkv, T, T, window
+    P.scale, P.softcap = scale, cap or 0.0
+    P.nsplit, P.rows = 1, 1
+    P.part_ml = None if lse is None else lse.data_ptr()
+    P.clear = int(fresh)
+    group = Hq // Hkv
+    pack = 4 if group % 4 == 0 else 2 if group % 2 == 0 else 0
+    bm, heads = 128 // (pack or 1), Hq // (pack or 1)
+    P.tiles, entries = layout.tiles_of(bm)
+    mean = T // max(1, layout.count)
+    spec = lowering._spec("prefill_swp", lowering._DTYPE_CODE[dtype], D, mask, cap is not None, pack=pack, packed=True,
+                          bn=lowering.prefill_kv_tile(D, 0, None, heads * (T // bm + layout.count // 2),
+                                                      min(mean, window) if mask == lowering.MASK_SLIDING else mean),
+                          stay=lowering.prefill_out_stays(2 * T * Hq * D))
+    grid = _grid(entries, heads, 256)
+    lowering.get_kernel(spec, spec.entry()).launch((grid, 1, 1), (256, 1, 1), P)
+    lowering._last_launch.set({"kernels": [spec.entry()], "grid": grid, "block": 256, "q_tile_rows": bm, "kv_tile_rows": spec.bn or 64,
+                               "heads_per_workgroup": pack or 1})
+    return out
+
+
+def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, dout: torch.Tensor,
+                              plan: AttnPlan, layout: PackedLayout):
+    """Gradients of ``attention_packed(q, k, v, plan, layout)``: ``(dq, dk, dv)`` in the operands' dtype, zeros in rows of no
+    sequence.  ``o`` and ``lse`` are the forward's output and row log-sum-exp.  As ``lowering.attention_backward``: delta with dQ
+    or in front of it, dK and dV, no atomics."""
+    if not isinstance(layout, PackedLayout):
+        raise UnsupportedPlan("layout must come from packed_layout")
+    return _backward(q, k, v, o, lse, dout, plan, layout)
+
+
+@lowering._on_device_of_first_argument
+def _backward(q, k, v, o, lse, dout, plan, layout):
+    dtype, D, Hq, Hkv = _heads(q, k, v, layout)
+    mask, window, scale, cap = _constants(plan)
+    T, dev = layout.total, q.device
+    for name, t in (("O", o), ("dO", dout)):
+        _rows(name, t, layout, dtype, D)
+        if t.shape[1] != Hq:
+            raise UnsupportedPlan(f"{name} must have the shape of Q")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or not lse.is_contiguous() or lse.device != dev:
+        raise UnsupportedPlan(f"lse must be a contiguous float32 [{Hq}, {T}] tensor on the device of Q")
+    for name, t in (("Q", q), ("dO", dout), ("K", k), ("V", v)):
+        if t.stride(0) < 0 or 2 * (T + 64) * t.stride(0) + 2 * D >= 1 << 32:
+            raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
+    dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=dev) for t in (q, k, v))
+    if T == 0:
+        return dq, dk, dv
+    delta = torch.empty((Hq, T), dtype=torch.float32, device=dev)
+    P = PackedBwdParams()
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv), ("lse", lse), ("delta", delta)):
+        setattr(P, name, t.data_ptr())
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+        setattr(P, name + "_ss", t.stride(0))
+        setattr(P, name + "_sh", t.stride(1))
+    P.B, P.Hq, P.Hkv, P.Sq, P.Sk, P.window = 1, Hq, Hkv, T, T, window
+    P.scale, P.softcap = scale, cap or 0.0
+    count = max(1, layout.count)
+    mean = max(1, T // count)
+    keys = lowering.bwd_key_blocks(D, mask, cap is not None, count * Hkv, mean)
+    nt = lowering.bwd_dq_threads(D, mask, cap is not None, count * Hq, mean, mean)
+    q_split = lowering.bwd_q_split(D, mask, count * Hkv, mean)
+    if q_split:
+        keys = 1
+    spec = bwd_spec(dtype, D, mask, cap is not None, keys, nt, q_split, lowering.bwd_grads_stay(2 * T * Hq * D))
+    P.dkdv_tiles, dkdv_entries = layout.tiles_of(64 if q_split else 128 * keys)
+    P.dq_tiles, dq_entries = layout.tiles_of(nt // 2)
+    steps = {"lf_attn_bwd_delta": (-(-Hq * T // 16), 256), "lf_attn_bwd_dkdv": (_grid(dkdv_entries, Hkv, 256), 256),
+             "lf_attn_bwd_dq": (_grid(dq_entries, Hq, nt), nt)}
+    names = ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"] if nt == 256 else list(steps)
+    named = lowering._kernels_of(spec)
+    for name in names:
+        grid, block = steps[name]
+        lowering.get_kernel(spec, name, named).launch((grid, 1, 1), (block, 1, 1), P)
+    lowering._last_launch.set({"kernels": names})
+    return dq, dk, dv
+
+
+def bwd_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool = False, key_blocks: int = 1, dq_threads: int = 512, q_split: bool = False,
+             stay: bool = False) -> lowering.KernelSpec:
+    return dataclasses.replace(lowering.bwd_spec(dtype, D, mask, softcap, key_blocks, dq_threads, False, q_split, stay), packed=True)
+
+
+class _Packed(torch.autograd.Function):
+    """As the fused training graphs: gradients can be asked for with ``create_graph=True`` but not differentiated again."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, plan, layout):
+        lse = torch.empty((q.shape[1], layout.total), dtype=torch.float32, device=q.device)
+        out = _forward(q, k, v, plan, layout, None, lse)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.plan, ctx.layout = dataclasses.replace(plan), layout      # (the caller may change a plan)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        if dout.stride(-1) != 1 or dout.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(dout.shape[:-1], dout.stride()[:-1])):
+            dout = dout.contiguous()
+        return (*_backward(q, k, v, out, lse, dout, ctx.plan, ctx.layout), None, None)
