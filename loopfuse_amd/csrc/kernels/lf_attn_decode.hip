@@ -66,6 +66,40 @@
                                 tensor of 0 / -inf; travels with the K/V registers of its step */
 #endif
 
+#ifndef LF_SHARED
+#define LF_SHARED 0          /* 1: a piece of one request's own keys, 2: a split of the prefix that all requests share, for 16 of their rows
+                                (lf_shared.hip.h); grid: 1 (pieces * units), 2 (units, nsplit) */
+#endif
+#if LF_SHARED
+#if LF_BIAS || LF_PAGED != 3
+#error "LF_SHARED: K and V in pages, no score bias"
+#endif
+#define LF_DEC_PARAMS LfSharedParams
+#define LF_K_TABLE (LF_SHARED == 2 ? p.prefix_k : p.k_table)
+#define LF_V_TABLE (LF_SHARED == 2 ? p.prefix_v : p.v_table)
+#define LF_KEYS keys         /* of this unit's sequence */
+#define LF_SPLIT_PARTIAL (LF_SHARED == 2 || p.Sk != 0 || keys > split)
+#define LF_PART_ACC (LF_SHARED == 2 ? p.pre_acc : p.part_acc)
+#define LF_PART_ML (LF_SHARED == 2 ? p.pre_ml : p.part_ml)
+#define LF_SLOT(qr) (LF_SHARED == 2 ? ((long long)hkv * p.B * p.rows + (qr)) * p.nsplit + z \
+                                    : ((long long)((int)blockIdx.x / p.units) * p.Hkv + hkv) * p.rows + (qr))
+#define LF_ALL_ROWS (LF_SHARED == 2 ? p.B * p.rows : p.rows)
+/* row r of a unit: of the group of one request, or of all requests one behind the other */
+#define LF_Q_ROW(r) (p.q + (LF_SHARED == 2 ? (long long)((r) / p.rows) * p.q_sb + (long long)((r) % p.rows) * p.q_ss \
+                                           : (long long)b * p.q_sb + (long long)(r) * p.q_ss) + (long long)hkv * p.q_sh)
+#else
+#define LF_DEC_PARAMS LfAttnParams
+#define LF_K_TABLE p.k_table
+#define LF_V_TABLE p.v_table
+#define LF_KEYS p.Sk
+#define LF_SPLIT_PARTIAL (p.nsplit != 1)
+#define LF_PART_ACC p.part_acc
+#define LF_PART_ML p.part_ml
+#define LF_SLOT(qr) (((long long)bh * p.rows + (qr)) * p.nsplit + z)
+#define LF_ALL_ROWS p.rows
+#define LF_Q_ROW(r) (p.q + (long long)b * p.q_sb + (long long)hkv * p.q_sh + (long long)(r) * p.q_ss)
+#endif
+
 struct LfDecStage {
   lf_u32x4 k[LF_NJ];
   lf_u32x4 v[LF_NJ];
@@ -110,7 +144,7 @@ struct LfCoopStage {
 //   LDS -> MFMA         : S^T = K Q^T with ds_read_b128 (row = token, 32 d per k-step) on the
 //                         16x16x32 MFMA; O^T += V^T P^T with transposed 8-byte reads on the
 //                         16x16x16 MFMA, whose k extent is the 16 tokens of a step
-extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(const LfAttnParams p) {
+extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(const LF_DEC_PARAMS p) {
   constexpr int kRowB = LF_DW * LF_D * 2;            // bytes of one token row over the workgroup's heads
   constexpr int kPieces = kRowB / 16;                // 16-byte pieces per row
   constexpr int kKStride = kRowB + 16;               // LDS row strides
@@ -125,27 +159,41 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   const int c = lane & 15;      // token of a step (K rows) / query column (MFMA results)
   const int g = lane >> 4;
 
-  const int z = blockIdx.y;
-  const int chunks = (p.rows + LF_QROWS - 1) / LF_QROWS;   // row chunks per (b, kv head)
-  const int unit = blockIdx.x;
-  const int rc = unit % chunks;
+  const int chunks = (LF_ALL_ROWS + LF_QROWS - 1) / LF_QROWS;   // row chunks per (b, kv head)
   const int hchunks = p.Hkv / LF_DW;                        // the host checks Hkv % LF_DW == 0
+#if LF_SHARED == 1
+  const int unit = blockIdx.x % p.units;
+  const int split = lf_shared_split(p);
+  int b, z, keys;
+  if (!lf_shared_piece(p, split, (int)blockIdx.x / p.units, b, z, keys)) return;
+  b = __builtin_amdgcn_readfirstlane(b);      // (in scalar registers: they make the wave's addresses)
+  z = __builtin_amdgcn_readfirstlane(z);
+  keys = __builtin_amdgcn_readfirstlane(keys);
+  const int split_len = split;
+#else
+  const int z = blockIdx.y;
+  const int unit = blockIdx.x;
+  const int b = unit / (chunks * hchunks);
+  const int split_len = p.split_len;
+#if LF_SHARED
+  const int keys = p.Sk, split = 0;
+#endif
+#endif
+  const int rc = unit % chunks;
   const int hkv0 = ((unit / chunks) % hchunks) * LF_DW;
   const int hkv = hkv0 + wave;
-  const int b = unit / (chunks * hchunks);
   const int bh = b * p.Hkv + hkv;
   const int row0 = rc * LF_QROWS;
-  const int nrows = min(p.rows - row0, LF_QROWS);
+  const int nrows = min(LF_ALL_ROWS - row0, LF_QROWS);
 
-  const int tok_begin = z * p.split_len;
-  const int tok_end = min(tok_begin + p.split_len, p.Sk);
+  const int tok_begin = z * split_len;
+  const int tok_end = min(tok_begin + split_len, LF_KEYS);
   const int nsteps = (max(tok_end - tok_begin, 0) + 15) / 16;   // the same for every wave of the workgroup
 
   // ---- B operand of S^T = K Q^T: lane (q = c, g) holds Q[row0 + q][32*j + 8*g .. +7]
   lf_elem8 qb[LF_NJ];
   {
-    const lf_elem* qrow = p.q + (long long)b * p.q_sb + (long long)hkv * p.q_sh +
-                          (long long)(row0 + min(c, nrows - 1)) * p.q_ss;
+    const lf_elem* qrow = LF_Q_ROW(row0 + min(c, nrows - 1));
 #pragma unroll
     for (int j = 0; j < LF_NJ; ++j) {
       lf_u32x4 raw = *reinterpret_cast<const lf_u32x4*>(qrow + 32 * j + 8 * g);
@@ -180,9 +228,9 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   auto load_ids = [&](int st0) -> lf_table_t {
     const int l = lane & 31;
     const int row = kIds == 1 ? 0 : row_w + kRowStep * (l % kIds);
-    const int tok = min(tok_begin + 16 * (st0 + l / kIds) + row, p.Sk - 1);   // steps past the end: the last page (never issued)
-    return lane < 32 ? reinterpret_cast<const lf_table_t*>(p.k_table)[(long long)b * p.kt_stride + tok / LF_PAGE_SIZE]
-                     : reinterpret_cast<const lf_table_t*>(p.v_table)[(long long)b * p.vt_stride + tok / LF_PAGE_SIZE_V];
+    const int tok = min(tok_begin + 16 * (st0 + l / kIds) + row, LF_KEYS - 1);   // steps past the end: the last page (never issued)
+    return lane < 32 ? reinterpret_cast<const lf_table_t*>(LF_K_TABLE)[(long long)b * p.kt_stride + tok / LF_PAGE_SIZE]
+                     : reinterpret_cast<const lf_table_t*>(LF_V_TABLE)[(long long)b * p.vt_stride + tok / LF_PAGE_SIZE_V];
   };
   lf_table_t ids_cur = load_ids(0), ids_nxt = load_ids(kChunk);
   auto id_of = [&](int st, int u, int which) -> long long {
@@ -208,7 +256,7 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
       const long long idk = id_of(st, kIds == 1 ? 0 : u, 0), idv = id_of(st, kIds == 1 ? 0 : u, 1);
       const int piece = tid + LF_DT * u;
       const int row = row_w + kRowStep * u;                  // the same for the whole wave: scalar addresses
-      const int tk = min(tok0 + row, p.Sk - 1);              // rows past Sk: clamped, masked later
+      const int tk = min(tok0 + row, LF_KEYS - 1);              // rows past Sk: clamped, masked later
       const int within = 8 * (piece % kPieces);              // elements
       // every byte is read once, whole lines at a time: streaming (non-temporal) loads
       sg.k[u] = __builtin_nontemporal_load(reinterpret_cast<const lf_u32x4*>(
@@ -331,7 +379,7 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   l_wave += __shfl_xor(l_wave, 32, 64);
   if (c < nrows) {
     const int qr = row0 + c;
-    if (p.nsplit == 1) {
+    if (!LF_SPLIT_PARTIAL) {
       lf_elem* orow = p.o + (long long)b * p.o_sb + (long long)hkv * p.o_sh + (long long)qr * p.o_ss;
       const float inv = lf_inv_sum(l_wave);
 #pragma unroll
@@ -342,19 +390,19 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
         *reinterpret_cast<lf_elem4*>(orow + 16 * db + 4 * g) = w4;
       }
     } else {
-      const long long slot = ((long long)bh * p.rows + qr) * p.nsplit + z;
+      const long long slot = LF_SLOT(qr);
 #pragma unroll
       for (int db = 0; db < LF_NDB; ++db)
-        *reinterpret_cast<lf_f32x4*>(&p.part_acc[slot * LF_D + 16 * db + 4 * g]) = o[db];
+        *reinterpret_cast<lf_f32x4*>(&LF_PART_ACC[slot * LF_D + 16 * db + 4 * g]) = o[db];
       if (g == 0) {
-        p.part_ml[slot * 2 + 0] = mc;            // exponent offset, log2 units
-        p.part_ml[slot * 2 + 1] = l_wave;
+        LF_PART_ML[slot * 2 + 0] = mc;            // exponent offset, log2 units
+        LF_PART_ML[slot * 2 + 1] = l_wave;
       }
     }
   }
 }
 #else   // !LF_COOP
-extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(const LfAttnParams p) {
+extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(const LF_DEC_PARAMS p) {
   // One buffer, two lives: wave-private V tiles of the pair being consumed
   // ([LF_DW][2][16*D] elements) during the loop, merge buffer
   // ([LF_DW][16][LF_OSTRIDE] floats) after it.
@@ -372,16 +420,36 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   const int c = lane & 15;      // token of a step (loads) / query column (MFMA results)
   const int g = lane >> 4;
 
+  const int chunks = (LF_ALL_ROWS + LF_QROWS - 1) / LF_QROWS;   // row chunks per (b, kv head)
+#if LF_SHARED == 1
+  const int unit = blockIdx.x % p.units;
+  const int split = lf_shared_split(p);
+  int b, z, keys;
+  if (!lf_shared_piece(p, split, (int)blockIdx.x / p.units, b, z, keys)) return;
+  b = __builtin_amdgcn_readfirstlane(b);      // (in scalar registers: they make the wave's addresses)
+  z = __builtin_amdgcn_readfirstlane(z);
+  keys = __builtin_amdgcn_readfirstlane(keys);
+  const int split_len = split;
+#else
   const int z = blockIdx.y;
-  const int chunks = (p.rows + LF_QROWS - 1) / LF_QROWS;   // row chunks per (b, kv head)
   const int unit = blockIdx.x;
+  const int split_len = p.split_len;
+#if LF_SHARED
+  const int keys = p.Sk, split = 0;
+#endif
+#endif
   const int rc = unit % chunks;
 #if LF_HEADWAVE
   // grid.x = B * ceil(Hkv / LF_DW) * chunks; wave w serves head LF_DW*hc + w
   const int hchunks = (p.Hkv + LF_DW - 1) / LF_DW;
   const int hkv = ((unit / chunks) % hchunks) * LF_DW + wave;
+#if LF_SHARED != 1
   const int b = unit / (chunks * hchunks);
+#endif
   if (hkv >= p.Hkv) return;          // no workgroup barrier in this mode
+  const int bh = b * p.Hkv + hkv;
+#elif LF_SHARED == 1
+  const int hkv = unit / chunks;
   const int bh = b * p.Hkv + hkv;
 #else
   const int bh = unit / chunks;
@@ -389,10 +457,10 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   const int b = bh / p.Hkv;
 #endif
   const int row0 = rc * LF_QROWS;
-  const int nrows = min(p.rows - row0, LF_QROWS);          // query rows of this unit
+  const int nrows = min(LF_ALL_ROWS - row0, LF_QROWS);          // query rows of this unit
 
-  int tok_begin = z * p.split_len;
-  int tok_end = min(tok_begin + p.split_len, p.Sk);
+  int tok_begin = z * split_len;
+  int tok_end = min(tok_begin + split_len, LF_KEYS);
 #if LF_BIAS
   // Keys whose bias is -inf for every query row of the unit add nothing.  The split is narrowed
   // to the span from its first to its last live key (the left padding of a batch, the unused
@@ -435,8 +503,7 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   // columns past nrows are zero
   lf_elem8 qb[LF_NJ];
   {
-    const lf_elem* qrow = p.q + (long long)b * p.q_sb + (long long)hkv * p.q_sh +
-                          (long long)(row0 + min(c, nrows - 1)) * p.q_ss;
+    const lf_elem* qrow = LF_Q_ROW(row0 + min(c, nrows - 1));
 #pragma unroll
     for (int j = 0; j < LF_NJ; ++j) {
       lf_u32x4 raw = *reinterpret_cast<const lf_u32x4*>(qrow + 32 * j + 8 * g);
@@ -468,9 +535,9 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
     LfDecIds id = {0, 0};
     if (kPagedK || kPagedV) {
       // clamp: steps past the end re-read the last page (their scores are masked)
-      const int tok = min(step_tok0(st) + (kUniformPage ? 0 : c), p.Sk - 1);
-      if (kPagedK) id.k = reinterpret_cast<const lf_table_t*>(p.k_table)[(long long)b * p.kt_stride + tok / LF_PAGE_SIZE];
-      if (kPagedV) id.v = reinterpret_cast<const lf_table_t*>(p.v_table)[(long long)b * p.vt_stride + tok / LF_PAGE_SIZE_V];
+      const int tok = min(step_tok0(st) + (kUniformPage ? 0 : c), LF_KEYS - 1);
+      if (kPagedK) id.k = reinterpret_cast<const lf_table_t*>(LF_K_TABLE)[(long long)b * p.kt_stride + tok / LF_PAGE_SIZE];
+      if (kPagedV) id.v = reinterpret_cast<const lf_table_t*>(LF_V_TABLE)[(long long)b * p.vt_stride + tok / LF_PAGE_SIZE_V];
     }
     return id;
   };
@@ -487,7 +554,7 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
     const int lt = lane / kCpr, piece = lane % kCpr;
 #pragma unroll
     for (int u = 0; u < LF_NJ; ++u) {
-      const int tok = min(step_tok0(st) + kTokPerLoad * u + lt, p.Sk - 1);   // clamp: masked later, never out of bounds
+      const int tok = min(step_tok0(st) + kTokPerLoad * u + lt, LF_KEYS - 1);   // clamp: masked later, never out of bounds
       const lf_elem *kp, *vp;
       if (kPagedK)
         kp = p.k + id.k * p.k_sb + (long long)(tok % LF_PAGE_SIZE) * p.k_ss + (long long)hkv * p.k_sh;
@@ -501,7 +568,7 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
       sg.v[u] = __builtin_nontemporal_load(reinterpret_cast<const lf_u32x4*>(vp + 8 * piece));
     }
 #else
-    const int tok = min(step_tok0(st) + c, p.Sk - 1);      // clamp: masked later, never out of bounds
+    const int tok = min(step_tok0(st) + c, LF_KEYS - 1);      // clamp: masked later, never out of bounds
     const lf_elem *kp, *vp;
     if (kPagedK)
       kp = p.k + id.k * p.k_sb + (long long)(tok % LF_PAGE_SIZE) * p.k_ss + (long long)hkv * p.k_sh + 8 * g;
@@ -729,7 +796,7 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   // each wave owns its (batch, head): lane (q = c, g) writes d = 16*db + 4*g .. +3 of row q
   if (c < nrows) {
     const int qr = row0 + c;
-    if (p.nsplit == 1) {
+    if (!LF_SPLIT_PARTIAL) {
       lf_elem* orow = p.o + (long long)b * p.o_sb + (long long)hkv * p.o_sh + (long long)qr * p.o_ss;
       const float inv = lf_inv_sum(l_wave);
 #pragma unroll
@@ -740,13 +807,13 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
         *reinterpret_cast<lf_elem4*>(orow + 16 * db + 4 * g) = w4;
       }
     } else {
-      const long long slot = ((long long)bh * p.rows + qr) * p.nsplit + z;
+      const long long slot = LF_SLOT(qr);
 #pragma unroll
       for (int db = 0; db < LF_NDB; ++db)
-        *reinterpret_cast<lf_f32x4*>(&p.part_acc[slot * LF_D + 16 * db + 4 * g]) = o[db];
+        *reinterpret_cast<lf_f32x4*>(&LF_PART_ACC[slot * LF_D + 16 * db + 4 * g]) = o[db];
       if (g == 0) {
-        p.part_ml[slot * 2 + 0] = mc;            // exponent offset, log2 units
-        p.part_ml[slot * 2 + 1] = l_wave;
+        LF_PART_ML[slot * 2 + 0] = mc;            // exponent offset, log2 units
+        LF_PART_ML[slot * 2 + 1] = l_wave;
       }
     }
   }
@@ -788,7 +855,7 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] += red_o[(w * LF_QROWS + qi) * LF_OSTRIDE + d0 + e];
     const int qr = row0 + qi;
-    if (p.nsplit == 1) {
+    if (!LF_SPLIT_PARTIAL) {
       lf_elem* orow = p.o + (long long)b * p.o_sb + (long long)hkv * p.o_sh + (long long)qr * p.o_ss;
       const float inv = lf_inv_sum(l_tot);
       lf_elem8 w8;
@@ -796,12 +863,12 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
       for (int e = 0; e < 8; ++e) w8[e] = lf_from_float(sum[e] * inv);
       *reinterpret_cast<lf_elem8*>(orow + d0) = w8;
     } else {
-      const long long slot = ((long long)bh * p.rows + qr) * p.nsplit + z;
+      const long long slot = LF_SLOT(qr);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p.part_acc[slot * LF_D + d0 + e] = sum[e];
+      for (int e = 0; e < 8; ++e) LF_PART_ACC[slot * LF_D + d0 + e] = sum[e];
       if (d0 == 0) {
-        p.part_ml[slot * 2 + 0] = m_all;       // exponent offset, log2 units
-        p.part_ml[slot * 2 + 1] = l_tot;
+        LF_PART_ML[slot * 2 + 0] = m_all;       // exponent offset, log2 units
+        LF_PART_ML[slot * 2 + 1] = l_tot;
       }
     }
   }
@@ -810,6 +877,7 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
 
 #endif  // LF_COOP
 
+#if !LF_SHARED
 // Merge nsplit partial results per query row.  A thread owns 4 consecutive d of one row; block = 256 threads = 1024 /
 // LF_HEAD_DIM rows, grid = ceil(B*Hkv*rows / rows per block), or one row per block, its splits shared by the block's groups of
 // threads and their results merged through LDS.  Bound by its chain of loads, a round trip per four splits: with one group
@@ -888,3 +956,4 @@ extern "C" __global__ void __launch_bounds__(256) lf_attn_decode_combine(const L
   for (int e = 0; e < 4; ++e) w[e] = lf_from_float(a[e] * inv);
   *reinterpret_cast<lf_elem4*>(orow + d0) = w;
 }
+#endif  // !LF_SHARED

@@ -1,0 +1,34 @@
+// lf_store_kv.hip — rows of new keys and values into their slots of the page pools: pool[slot[t]] = row t.
+// A thread moves one 16-byte piece of a token's K row and the same one of its V row; neighbouring threads the pieces of one row, so
+// that reads and writes are whole lines.  Bound by HBM: 2 rows read and 2 written per token, and their slot.
+
+struct LfStoreParams {
+  const lf_u32x4* k;           // [T, Hkv, D], strides below
+  const lf_u32x4* v;
+  lf_u32x4* k_pool;            // [pages, page, Hkv, D]
+  lf_u32x4* v_pool;
+  const int* slots;            // [T]; below 0 or behind the last: the row is left out
+  long long k_ss, k_sh, v_ss, v_sh;                    // strides in 16-byte pieces: rows, heads
+  long long kp_sb, kp_ss, kp_sh, vp_sb, vp_ss, vp_sh;  // pages, tokens of a page, heads
+  long long last;              // slots of a pool
+  int T, heads, per_head;      // pieces of a head's row
+  int shift;                   // log2 of the tokens per page
+};
+
+#define LF_STORE_NT 256
+extern "C" __global__ void __launch_bounds__(LF_STORE_NT) lf_store_kv(const LfStoreParams p) {
+  const int pieces = p.heads * p.per_head;
+  const int tokens = max(LF_STORE_NT / pieces, 1);      // of a block
+  const int in = threadIdx.x / pieces;
+  const int t = blockIdx.x * tokens + (pieces > LF_STORE_NT ? 0 : in);
+  if (t >= p.T || (pieces <= LF_STORE_NT && in >= tokens)) return;
+  const int slot = p.slots[t];
+  if (slot < 0 || slot >= p.last) return;
+  const long long page = slot >> p.shift, at = slot & ((1 << p.shift) - 1);
+  for (int i = pieces > LF_STORE_NT ? (int)threadIdx.x : (int)threadIdx.x - in * pieces; i < pieces; i += LF_STORE_NT) {
+    const int h = i / p.per_head, c = i - h * p.per_head;
+    const lf_u32x4 k = p.k[t * p.k_ss + h * p.k_sh + c], v = p.v[t * p.v_ss + h * p.v_sh + c];
+    p.k_pool[page * p.kp_sb + at * p.kp_ss + h * p.kp_sh + c] = k;
+    p.v_pool[page * p.vp_sb + at * p.vp_ss + h * p.vp_sh + c] = v;
+  }
+}

@@ -98,6 +98,7 @@ class KernelSpec:
     extra: tuple = ()      # further -D options (tuning experiments)
     stay: bool = False     # prefill_swp, bwd: results by plain stores (prefill_out_stays, bwd_grads_stay)
     packed: bool = False   # prefill_swp, bwd: the tiles of sequences of different lengths in one tensor (lf_packed.hip.h)
+    shared: int = 0        # decode: 1 the own keys of requests of different lengths, 2 the prefix they share (lf_shared.hip.h)
 
     def __hash__(self):    # formed once: a call looks its kernels up by it, several times
         h = self.__dict__.get("_hash")
@@ -129,6 +130,8 @@ class KernelSpec:
                 o += ["-DLF_ROWLOAD=1"]
             if self.bias:
                 o += ["-DLF_BIAS=1"]
+            if self.shared:
+                o += [f"-DLF_SHARED={self.shared}"]
         elif self.family == "prefill":
             o += [f"-DLF_V_TR={int(self.v_tr)}", f"-DLF_BIAS={self.bias}", f"-DLF_DENOM={int(self.denom)}"]
             if self.d2:
@@ -151,9 +154,14 @@ class KernelSpec:
 
     def files(self) -> tuple[str, ...]:
         kernel = {"prefill": "lf_attn_prefill.hip", "prefill_swp": "lf_attn_prefill_swp.hip",
-                  "decode": "lf_attn_decode.hip", "bwd": "lf_attn_bwd.hip", "packed_plan": "lf_packed_plan.hip"}[self.family]
+                  "decode": "lf_attn_decode.hip", "bwd": "lf_attn_bwd.hip", "packed_plan": "lf_packed_plan.hip",
+                  "shared_combine": "lf_shared_combine.hip", "paged_tables": "lf_paged_tables.hip", "store_kv": "lf_store_kv.hip"}[self.family]
         if self.family == "packed_plan":
             return ("lf_common.hip.h", "lf_packed.hip.h", kernel)
+        if self.shared or self.family == "shared_combine":
+            return ("lf_common.hip.h", "lf_shared.hip.h", kernel)
+        if self.family in ("paged_tables", "store_kv"):
+            return ("lf_common.hip.h", kernel)
         if self.packed:
             return ("lf_common.hip.h", "lf_packed.hip.h", "lf_prefill_blocks.hip.h", kernel)
         if self.family == "decode":
@@ -167,13 +175,14 @@ class KernelSpec:
 
     def entry(self) -> str:
         return {"prefill": "lf_attn_prefill", "prefill_swp": "lf_attn_prefill_swp", "decode": "lf_attn_decode",
-                "bwd": "lf_attn_bwd_dq", "packed_plan": "lf_packed_plan"}[self.family]
+                "bwd": "lf_attn_bwd_dq", "packed_plan": "lf_packed_plan", "shared_combine": "lf_shared_combine",
+                "paged_tables": "lf_paged_tables", "store_kv": "lf_store_kv"}[self.family]
 
     def name(self) -> str:
         return (f"lf_{self.family}_t{self.dtype}_d{self.head_dim}_m{self.mask}_c{int(self.softcap)}"
                 f"_p{self.paged}x{self.page_size}i{int(self.table_i64)}_r{self.rows}w{self.waves}v{int(self.v_tr)}h{int(self.headwave)}b{self.bias}n{int(self.denom)}"
                 + (f"_q{self.d2}" if self.d2 else "") + (f"_gp{int(self.pack)}" if self.pack else "") + (f"_pv{self.page_size_v}" if self.page_size_v else "")
-                + ("_z" if self.safe else "") + (f"_bn{self.bn}" if self.bn else "") + ("_co" if self.coop else "") + ("_rl" if self.rowload else "") + ("_st" if self.stay else "") + ("_pk" if self.packed else "")
+                + ("_z" if self.safe else "") + (f"_bn{self.bn}" if self.bn else "") + ("_co" if self.coop else "") + ("_rl" if self.rowload else "") + ("_st" if self.stay else "") + ("_pk" if self.packed else "") + (f"_sh{self.shared}" if self.shared else "")
                 + "".join("_" + e.replace("-D", "").replace("=", "") for e in self.extra))
 
     def source(self) -> str:

@@ -1,0 +1,272 @@
+"""Key / value caches in pages for requests of different lengths: their tables, the storing of new tokens, attention over them.
+
+A serving step over a batch of requests, nothing of which waits for the lengths, which live on the GPU:
+
+    step = extend_tables(lengths, new, table, free, page_size, total)    # pages for the new tokens, and each one's slot
+    store_kv(k, v, k_pool, v_pool, step.slots)                           # their keys and values into the pools
+    o = attention_shared(q, k_pool, v_pool, plan, table, step.lengths,   # one new token per request over its keys,
+                         prefix_table=prefix, prefix_len=n)              # and over a prefix that all requests share
+
+Pools are ``[pages, page, Hkv, D]`` (or ``[pages, Hkv, D]`` for one-token pages), as ``lowering.attention`` takes them; a table
+row names a request's pages in the order of its tokens.  The reference reads caches of one length through
+``paged_load`` (reference loopfuse/torch_backend/__init__.py:46-56) and leaves tables and stores to its user.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import lowering
+from .lowering import AttnPlan, UnsupportedPlan
+
+_TABLE_DTYPES = (torch.int32, torch.int64)
+
+
+class _TablesParams(ctypes.Structure):
+    """Mirror of ``struct LfTablesParams`` in csrc/kernels/lf_paged_tables.hip."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("cached", "fresh", "table", "free", "offsets", "lengths", "slots", "positions", "pages")]
+                + [("table_stride", ctypes.c_longlong)] + [(n, ctypes.c_int) for n in ("B", "width", "count", "T", "shift")])
+
+
+class _StoreParams(ctypes.Structure):
+    """Mirror of ``struct LfStoreParams`` in csrc/kernels/lf_store_kv.hip."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_pool", "v_pool", "slots")]
+                + [(n, ctypes.c_longlong) for n in ("k_ss", "k_sh", "v_ss", "v_sh", "kp_sb", "kp_ss", "kp_sh", "vp_sb", "vp_ss", "vp_sh", "last")]
+                + [(n, ctypes.c_int) for n in ("T", "heads", "per_head", "shift")])
+
+
+class SharedParams(lowering.AttnParams):
+    """Mirror of ``struct LfSharedParams`` in csrc/kernels/lf_shared.hip.h."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("lengths", "prefix_k", "prefix_v", "pre_acc", "pre_ml")]
+                + [(n, ctypes.c_int) for n in ("room", "units", "target", "least")])
+
+
+class PagedStep(NamedTuple):
+    """What ``extend_tables`` leaves."""
+
+    offsets: torch.Tensor      # int32 [B + 1]: request b's new tokens are rows offsets[b] ... offsets[b + 1]
+    lengths: torch.Tensor      # int32 [B]: tokens of each request with the new ones
+    slots: torch.Tensor        # int32 [total]: page * page_size + place in the page, -1 for rows of no token
+    positions: torch.Tensor    # int32 [total]: place in the request, -1 for rows of no token
+    pages: torch.Tensor        # int32 [1]: free pages that the new tokens need
+
+
+def _on_gpu(name: str, t: torch.Tensor, dtypes, dim: int, device=None) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.dim() != dim:
+        raise UnsupportedPlan(f"{name} must be a tensor of {dim} dim(s), {' or '.join(str(d).replace('torch.', '') for d in dtypes)}")
+    if not t.is_cuda:
+        raise RuntimeError(f"loopfuse_amd: {name} is not on the GPU; the HIP path has no CPU fallback")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"loopfuse_amd: {name} is on {t.device}, not on {device}")
+
+
+def _shift(page_size: int) -> int:
+    if not isinstance(page_size, int) or page_size < 1 or page_size & (page_size - 1):
+        raise UnsupportedPlan("page size must be a power of two")
+    return page_size.bit_length() - 1
+
+
+def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, page_size: int, total: int) -> PagedStep:
+    """Pages for the new tokens of a batch, and the slot of each of them, from lengths on the GPU.
+
+    cached, new : int32 [B], tokens that a request has in its pages and tokens that come (0 for both: an empty place of the batch);
+    below 0 counts as 0.  table : [B, width], int32 or int64, rows contiguous; request ``b``'s first ``ceil(cached / page_size)`` entries are
+    read, those of its new pages are WRITTEN, the others stay as they are.  free : pages to take, [count], of the table's dtype; the
+    requests take ``pages`` of them from the front, in the order of the batch.  total : rows of the step's packed tensors (a padded
+    size will do).
+
+    Nothing is raised for what only the GPU knows: where no free page is left, the row of the table is too short or a token lies behind
+    ``total``, the token's slot (and the new entry) is -1, which ``store_kv`` leaves out; ``pages`` above ``len(free)`` says so."""
+    _on_gpu("cached", cached, (torch.int32,), 1)
+    dev, B = cached.device, cached.shape[0]
+    _on_gpu("new", new, (torch.int32,), 1, dev)
+    _on_gpu("table", table, _TABLE_DTYPES, 2, dev)
+    _on_gpu("free", free, (table.dtype,), 1, dev)
+    if new.shape[0] != B or table.shape[0] != B:
+        raise UnsupportedPlan(f"new and table must be of {B} requests")
+    if table.shape[1] and B and table.stride(1) != 1 or (B > 1 and table.stride(0) < table.shape[1]):
+        raise UnsupportedPlan("rows of the table must be contiguous and apart")
+    shift, total = _shift(page_size), int(total)
+    if total < 0 or total >= 1 << 31:
+        raise UnsupportedPlan("the number of rows must be between 0 and 2**31 - 1")
+    with torch.cuda.device(dev):
+        made = torch.empty(2 * B + 2 + 2 * total, dtype=torch.int32, device=dev)
+        offsets, lengths, pages, slots, positions = made.split((B + 1, B, 1, total, total))
+        cached, new, free = cached.contiguous(), new.contiguous(), free.contiguous()
+        P = _TablesParams(cached.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr(), offsets.data_ptr(), lengths.data_ptr(),
+                          slots.data_ptr(), positions.data_ptr(), pages.data_ptr(), table.stride(0), B, table.shape[1], free.shape[0], total, shift)
+        spec = lowering._spec("paged_tables", 0, 64, table_i64=table.dtype == torch.int64)
+        # a block per request and 1024 rows of the mean one
+        share = max(1, min(64, total // (1024 * max(B, 1))))
+        lowering.get_kernel(spec, spec.entry()).launch((max(B, 1), share, 1), (256, 1, 1), P)
+    return PagedStep(offsets, lengths, slots, positions, pages)
+
+
+def _pool(name: str, t: torch.Tensor) -> tuple:
+    """(pages, page size, heads, D, page stride, token stride, head stride) of a page pool."""
+    if t.dim() == 3:
+        return t.shape[0], 1, t.shape[1], t.shape[2], t.stride(0), 0, t.stride(1)
+    if t.dim() == 4:
+        return (*t.shape, *t.stride()[:3])
+    raise UnsupportedPlan(f"{name} pool must be [N, Hkv, D] or [N, P, Hkv, D]")
+
+
+def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Tensor) -> None:
+    """Write rows of new keys and values, k and v ``[rows, Hkv, D]``, into the page pools: row t into token ``slots[t] % page`` of page
+    ``slots[t] // page``.  bf16 / fp16, D a multiple of 8; views will do.  ``slots``: int32 [rows] (``PagedStep.slots``); rows whose slot is below 0 or
+    behind the pool's last are left out.  Slots that are not left out are distinct, as those of ``extend_tables`` are:
+    of two rows with one slot, either may be found there afterwards, or a part of each."""
+    if k.dtype not in lowering._DTYPE_CODE:
+        raise UnsupportedPlan(f"dtype {k.dtype} not supported (bf16/fp16 only)")
+    for name, t in (("K", k), ("V", v), ("K pool", k_pool), ("V pool", v_pool)):
+        lowering._check_tensor(name, t, k.dtype)
+        if t.device != k.device:
+            raise RuntimeError(f"loopfuse_amd: {name} is on {t.device}, K on {k.device}")
+    _on_gpu("slots", slots, (torch.int32,), 1, k.device)
+    if k.dim() != 3 or k.shape != v.shape or slots.shape[0] != k.shape[0] or k.shape[2] % 8:
+        raise UnsupportedPlan("K and V must be [rows, Hkv, D], D a multiple of 8, slots [rows]")
+    T, heads, D = k.shape
+    pages, page, hk, dk, *ks = _pool("K", k_pool)
+    pages_v, page_v, hv, dv, *vs = _pool("V", v_pool)
+    if (pages, page) != (pages_v, page_v) or (hk, dk) != (heads, D) or (hv, dv) != (heads, D):
+        raise UnsupportedPlan("the pools must agree in pages and page size with each other, in heads and head dim with K and V")
+    if any(n > 1 and s == 0 for p in (k_pool, v_pool) for n, s in zip(p.shape, p.stride())):
+        raise UnsupportedPlan("every element of a pool must have a place of its own")
+    shift = _shift(page)
+    if T == 0 or pages == 0 or heads == 0 or D == 0:
+        return
+    with torch.cuda.device(k.device):
+        slots = slots.contiguous()
+        P = _StoreParams(k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), slots.data_ptr(),
+                         *(x // 8 for x in (*k.stride()[:2], *v.stride()[:2], *ks, *vs)), pages * page, T, heads, D // 8, shift)
+        spec = lowering._spec("store_kv", 0, 64)
+        lowering.get_kernel(spec, spec.entry()).launch((-(-T // max(256 // (heads * D // 8), 1)), 1, 1), (256, 1, 1), P)
+
+
+def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, plan: AttnPlan, table: torch.Tensor, lengths: torch.Tensor, *,
+                     prefix_table: Optional[torch.Tensor] = None, prefix_len: int = 0, v_table: Optional[torch.Tensor] = None,
+                     prefix_v_table: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per request over a prefix that all requests share and over the request's own keys.
+
+    q : [B, Hq, 1, D], bf16 / fp16, D 64 or 128.  k_pool, v_pool : page pools of one page size.  table : [B, width], int32 or int64,
+    the pages of each request's own keys, of which it has ``lengths[b]`` (int32 [B], on the GPU; what a row of the table has no room for is
+    left out); entries behind the last page are not read.  prefix_table : [ceil(prefix_len / page)], the pages of the prefix, of
+    the table's dtype.  ``v_table`` / ``prefix_v_table``: those of V where they differ from K's.  ``plan``: scale and softcap, no mask.
+    Returns O [B, Hq, 1, D]; a request without a key, e.g. an empty place of a padded batch, gets zeros.
+
+    The prefix is read once for all requests together: its keys meet the rows of the whole batch as a matrix product, the requests'
+    own keys are streamed, and the partial results are joined in a second launch.  Page ids are trusted, as those of
+    ``lowering.attention`` are."""
+    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, int(prefix_len), v_table, prefix_v_table, out)
+
+
+@lowering._on_device_of_first_argument
+def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v_table, prefix_v_table, out):
+    dtype = q.dtype
+    if dtype not in lowering._DTYPE_CODE:
+        raise UnsupportedPlan(f"dtype {dtype} not supported by the MFMA kernels (bf16/fp16 only)")
+    if q.dim() != 4 or q.shape[2] != 1 or q.shape[3] not in (64, 128):
+        raise UnsupportedPlan("Q must be [B, Hq, 1, D] with head dim 64 or 128")
+    B, Hq, _, D = q.shape
+    lowering._check_tensor("Q", q, dtype)
+    for name, t in (("K pool", k_pool), ("V pool", v_pool)):
+        lowering._check_tensor(name, t, dtype)
+        if t.device != q.device:
+            raise RuntimeError(f"loopfuse_amd: {name} is on {t.device}, Q on {q.device}")
+    if plan.mask not in (None, "none") or plan.denom_add != 0.0:
+        raise UnsupportedPlan("attention over a shared prefix takes no mask and the plain softmax denominator")
+    if not (plan.scale > 0.0) or not math.isfinite(plan.scale):
+        raise UnsupportedPlan("score scale must be positive and finite")
+    softcap = None
+    if plan.softcap is not None:
+        softcap = abs(float(plan.softcap))
+        if not (softcap > 0.0) or not math.isfinite(softcap):
+            raise UnsupportedPlan("softcap must be finite and non-zero")
+    pages, page, Hkv, Dk, *ks = _pool("K", k_pool)
+    pages_v, page_v, Hkv_v, Dv, *vs = _pool("V", v_pool)
+    if page != page_v or Hkv != Hkv_v or Dk != D or Dv != D:
+        raise UnsupportedPlan("the pools must have one page size, the same kv heads and Q's head dim")
+    _shift(page)
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise UnsupportedPlan("Hq must be a multiple of Hkv")
+    group = Hq // Hkv
+    _on_gpu("table", table, _TABLE_DTYPES, 2, q.device)
+    _on_gpu("lengths", lengths, (torch.int32,), 1, q.device)
+    v_table = table if v_table is None else v_table
+    _on_gpu("V table", v_table, (table.dtype,), 2, q.device)
+    if table.shape[0] != B or v_table.shape != table.shape or lengths.shape[0] != B:
+        raise UnsupportedPlan(f"tables and lengths must be of {B} requests, the tables of one width")
+    if prefix_len < 0 or prefix_len >= 1 << 31 or table.shape[1] * page >= 1 << 31:
+        raise UnsupportedPlan("more keys than positions in 32 bits")
+    if prefix_len:
+        if prefix_table is None:
+            raise UnsupportedPlan("a prefix needs its table")
+        prefix_v_table = prefix_table if prefix_v_table is None else prefix_v_table
+        for name, t in (("prefix table", prefix_table), ("V prefix table", prefix_v_table)):
+            _on_gpu(name, t, (table.dtype,), 1, q.device)
+            if t.shape[0] * page < prefix_len:
+                raise UnsupportedPlan(f"{name} has room for {t.shape[0] * page} of {prefix_len} keys")
+        prefix_table, prefix_v_table = prefix_table.contiguous(), prefix_v_table.contiguous()
+    table = table if table.stride(1) == 1 else table.contiguous()
+    v_table = v_table if v_table.stride(1) == 1 else v_table.contiguous()
+    lengths = lengths.contiguous()
+    if out is None:
+        out = torch.empty((B, Hq, 1, D), dtype=dtype, device=q.device)
+    else:
+        lowering._check_tensor("O", out, dtype)
+        if tuple(out.shape) != (B, Hq, 1, D) or out.device != q.device or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+            raise UnsupportedPlan(f"O must be [{B}, {Hq}, 1, {D}] on the device of Q, every element with a place of its own")
+    if B == 0:
+        return out
+    P = SharedParams()
+    P.q, P.k, P.v, P.o = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
+    P.q_sb, P.q_sh, P.q_ss = q.stride(0), group * q.stride(1), q.stride(1)
+    P.o_sb, P.o_sh, P.o_ss = out.stride(0), group * out.stride(1), out.stride(1)
+    P.k_sb, P.k_ss, P.k_sh = ks
+    P.v_sb, P.v_ss, P.v_sh = vs
+    P.k_table, P.v_table, P.kt_stride, P.vt_stride = table.data_ptr(), v_table.data_ptr(), table.stride(0), v_table.stride(0)
+    P.lengths = lengths.data_ptr()
+    P.B, P.Hq, P.Hkv, P.rows, P.Sq = B, Hq, Hkv, group, 1
+    P.scale, P.softcap = float(plan.scale), softcap or 0.0
+    P.room = table.shape[1] * page
+    P.Sk = prefix_len
+    coop = lowering._decode_coop_waves(3, page, 0, 0, Hkv, P, D)
+    chunks = -(-group // lowering.DECODE_QROWS)
+    heads = Hkv // coop if coop else Hkv
+    P.units, P.target, P.least = heads * chunks, 256 if coop else 512, 160 if coop else 512
+    items = P.target // P.units + B if P.room else 0
+    pre_rows, pre_units, splits = B * group, heads * -(-B * group // lowering.DECODE_QROWS), 0
+    P.nsplit = 1
+    if prefix_len:
+        splits = max(1, min(64, prefix_len // 160, 512 // pre_units))
+        splits, P.split_len = lowering._split_lengths(splits, prefix_len)
+        P.nsplit = splits
+        P.prefix_k, P.prefix_v = prefix_table.data_ptr(), prefix_v_table.data_ptr()
+    own, pre = items * Hq, splits * B * Hq            # rows of partial results
+    args = dict(rows=lowering.DECODE_QROWS, waves=coop or 4, headwave=coop > 0, coop=coop > 0,
+                rowload=not coop and lowering._decode_rowload(3, page, 0, 0))
+    make = lambda which: lowering._spec("decode", lowering._DTYPE_CODE[dtype], D, lowering.MASK_NONE, softcap is not None, 3, page,
+                                        table.dtype == torch.int64, shared=which, **args)
+    with lowering._scratch_lock:        # no other thread's step on this stream between the launches
+        scratch = lowering._get_scratch(q.device, (own + pre) * (D + 2))
+        at = scratch.data_ptr()
+        P.part_acc, P.part_ml = at, at + 4 * own * D
+        P.pre_acc, P.pre_ml = at + 4 * own * (D + 2), at + 4 * own * (D + 2) + 4 * pre * D
+        names = []
+        if splits:
+            lowering.get_kernel(make(2), "lf_attn_decode").launch((pre_units, splits, 1), (64 * args["waves"], 1, 1), P)
+            names.append("lf_attn_decode")
+        if items:
+            lowering.get_kernel(make(1), "lf_attn_decode").launch((items * P.units, 1, 1), (64 * args["waves"], 1, 1), P)
+            names.append("lf_attn_decode")
+        spec = lowering._spec("shared_combine", lowering._DTYPE_CODE[dtype], D)
+        lowering.get_kernel(spec, spec.entry()).launch((B * -(-Hq // (1024 // D)), 1, 1), (256, 1, 1), P)
+        names.append(spec.entry())
+    lowering._last_launch.set({"kernels": names})
+    return out
