@@ -115,9 +115,25 @@
 #if LF_PACKED && (LF_PAGED || LF_BIAS)
 #error "packed sequences go with dense operands and the flag masks"
 #endif
+#ifndef LF_PREFIX
+#define LF_PREFIX 0      /* 1: a split of a prefix that all requests of a batch share, for 128 of their rows (lf_shared.hip.h); leaves partial
+                            results; grid: row tiles x nsplit x Hkv, in units of whole KV tiles.  Pages may lie anywhere: a load's page is
+                            its buffer's base */
+#endif
+#if LF_PREFIX && (LF_PAGED != 3 || LF_BIAS || LF_MASK || LF_GQAPACK || LF_PACKED)
+#error "a shared prefix: K and V in pages, no mask, rows of all heads of a group"
+#endif
 #if LF_PACKED
 extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(const LfPackedAttnParams pk) {
   LfAttnParams p = pk;
+#elif LF_PREFIX
+extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(const LfSharedParams sp) {
+  LfAttnParams p = sp;
+  p.k_table = sp.prefix_k;
+  p.v_table = sp.prefix_v;
+  p.Hq = p.Hkv;
+  p.Sq = sp.B * sp.rows;
+  p.visits = nullptr;
 #else
 extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(const LfAttnParams p) {
 #endif
@@ -150,6 +166,12 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
   p.Sq = p.Sk = mine.len;
   const int nqt = (p.Sq + LF_BM - 1) / LF_BM;
   const int slot_qt = nqt - 1 - mine.tile;    // the last q tile, which has the most kv tiles under a causal mask, comes first
+#elif LF_PREFIX
+  // the row tiles of a (split, kv head) are neighbours but for the heads: they share its K and V in one L2
+  const int nqt = (p.Sq + LF_BM - 1) / LF_BM, b = 0;
+  const int bh = (int)blockIdx.x % p.Hkv, slot_qt = (int)blockIdx.x / p.Hkv % nqt, part = (int)blockIdx.x / p.Hkv / nqt;
+  const int lse_rows = 0;
+  (void)nhv;
 #else
   // ---- workgroup -> (batch*head, q tile): lf_slot_of_block; under a causal mask the last q tile has the most kv tiles
   const int nqt = (p.Sq + LF_BM - 1) / LF_BM;
@@ -190,13 +212,35 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
   const int wave_u = wave;
   // page id (as a byte offset of the page + this kv head) for the rows of this wave in
   // pass ps of tile kt; tiles / rows past Sk re-use the last page (their rows are zeroed)
-  auto page_off = [&](int which, int kt, int ps) -> unsigned {
+#if LF_PREFIX
+  typedef long long lf_page_t;
+#else
+  typedef unsigned lf_page_t;
+#endif
+  auto page_off = [&](int which, int kt, int ps) -> lf_page_t {
     const int tok = min(kt * LF_BN + (LF_NT / LF_CPR) * ps + (64 / LF_CPR) * wave_u, p.Sk - 1);
     const lf_table_t* tab = reinterpret_cast<const lf_table_t*>(which ? p.v_table : p.k_table);
     const int psz = which ? LF_PAGE_SIZE_V : LF_PAGE_SIZE;
+#if LF_PREFIX
+    const long long page = tab[tok / psz];
+    return 2 * (which ? page * p.v_sb + hkv * p.v_sh : page * p.k_sb + hkv * p.k_sh);
+#else
     const unsigned id = (unsigned)tab[(long long)b * (which ? p.vt_stride : p.kt_stride) + tok / psz];
     return which ? id * (unsigned)(p.v_sb * 2) + (unsigned)hkv * (unsigned)(p.v_sh * 2)
                  : id * (unsigned)(p.k_sb * 2) + (unsigned)hkv * (unsigned)(p.k_sh * 2);
+#endif
+  };
+  // the buffer of a load from page `pg` and what of `pg` is left for its offset
+  auto of_page = [&](const lf_u32x4& rs, const lf_elem* base, lf_page_t& pg) {
+#if LF_PREFIX
+    lf_u32x4 r = lf_make_buffer(reinterpret_cast<const char*>(base) + pg, 0xfffffff0u);
+    r[2] = rs[2] == 0u ? 0u : r[2];
+    pg = 0;
+    return r;
+#else
+    (void)base;
+    return rs;
+#endif
   };
   const lf_u32x4 k_rsq = lf_make_buffer(k_uni, k_bytes), v_rsq = lf_make_buffer(v_uni, v_bytes);
   // per-lane part of the offset: dense = row inside the pass, paged = row inside the wave's load
@@ -209,27 +253,29 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
   // pg: page_off() of the pass (paged operands only; fetched a tile ahead by the caller)
   // `rs`: k_rsq / v_rsq, or the same with an empty range for a tile past the last one (nothing is
   // fetched then; the slot it would fill is free)
-  auto dma_k_pass = [&](const lf_u32x4& rs, int kt, int sl, int ps, unsigned pg) {
+  auto dma_k_pass = [&](const lf_u32x4& rs, int kt, int sl, int ps, lf_page_t pg) {
     unsigned off;
+    const lf_u32x4 buf = of_page(rs, p.k, pg);
     if (kPagedK) {
       const int tokw = kt * LF_BN + kRowsPerPass * ps + kRowsPerWave * wave_u;     // first row of this wave's load
-      off = pg + (unsigned)(tokw % LF_PAGE_SIZE) * k_rowb + k_doff;
+      off = (unsigned)pg + (unsigned)(tokw % LF_PAGE_SIZE) * k_rowb + k_doff;
       if (tokw + (int)(srow % kRowsPerWave) >= p.Sk) off = 0xffffffffu;
     } else {
       off = k_doff + (unsigned)(kt * LF_BN + kRowsPerPass * ps) * k_rowb;
     }
-    lf_dma_to_lds_at(rs, off, k_row_addr(sl, kRowsPerPass * ps + kRowsPerWave * wave_u));
+    lf_dma_to_lds_at(buf, off, k_row_addr(sl, kRowsPerPass * ps + kRowsPerWave * wave_u));
   };
-  auto dma_v_pass = [&](const lf_u32x4& rs, int kt, int sl, int ps, unsigned pg) {
+  auto dma_v_pass = [&](const lf_u32x4& rs, int kt, int sl, int ps, lf_page_t pg) {
     unsigned off;
+    const lf_u32x4 buf = of_page(rs, p.v, pg);
     if (kPagedV) {
       const int tokw = kt * LF_BN + kRowsPerPass * ps + kRowsPerWave * wave_u;
-      off = pg + (unsigned)(tokw % LF_PAGE_SIZE_V) * v_rowb + v_doff;
+      off = (unsigned)pg + (unsigned)(tokw % LF_PAGE_SIZE_V) * v_rowb + v_doff;
       if (tokw + (int)(srow % kRowsPerWave) >= p.Sk) off = 0xffffffffu;
     } else {
       off = v_doff + (unsigned)(kt * LF_BN + kRowsPerPass * ps) * v_rowb;
     }
-    lf_dma_to_lds_at(rs, off, v_row_addr(sl, kRowsPerPass * ps + kRowsPerWave * wave_u));
+    lf_dma_to_lds_at(buf, off, v_row_addr(sl, kRowsPerPass * ps + kRowsPerWave * wave_u));
   };
 
 #if LF_CAPPOLY
@@ -316,6 +362,10 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     // ---- block skip: KV tiles [kt_begin, kt_end) hold an unmasked (i, j) for rows q0..qlast
     int kt_begin, kt_end;
     lf_tile_range(q0, qlast, nkt, p.window, kt_begin, kt_end);
+#if LF_PREFIX
+    kt_begin = min(part * (p.split_len / LF_BN), nkt);
+    kt_end = min(kt_begin + p.split_len / LF_BN, nkt);
+#endif
 #if LF_BIAS == 2
     // The mask's words for this (batch, head): one per 32 rows and 1024 keys; broadcast dims of the mask collapse
     constexpr int kRb = LF_BM / 32, kPer = LF_BN / 32;         // blocks of 32 rows per q tile, of 32 keys per tile
@@ -393,9 +443,9 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     // registers, which counts only the loads it knows, also covers the older direct loads).
     // Paged operands: page offsets of the passes issued during the coming tile (K two
     // tiles ahead, V one tile ahead), fetched a tile before they are needed
-    unsigned kpg[LF_NPASS], vpg[LF_NPASS];
+    lf_page_t kpg[LF_NPASS], vpg[LF_NPASS];
     {
-      unsigned k0pg[LF_NPASS], k1pg[LF_NPASS], v0pg[LF_NPASS];
+      lf_page_t k0pg[LF_NPASS], k1pg[LF_NPASS], v0pg[LF_NPASS];
 #pragma unroll
       for (int ps = 0; ps < LF_NPASS; ++ps) {
         k0pg[ps] = kPagedK ? page_off(0, kt_begin, ps) : 0u;
@@ -414,8 +464,13 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     // Q^T fragments (B operand): lane holds row my_q, d = 16*ks + 8*g .. +7.
     lf_elem8 qf[LF_NKS];
     {
+#if LF_PREFIX
+      const int r = min(my_q, p.Sq - 1);
+      const lf_elem* qrow = p.q + (long long)(r / p.rows) * p.q_sb + (long long)h * p.q_sh + (long long)(r % p.rows) * p.q_ss;
+#else
       const lf_elem* qrow = p.q + (long long)b * p.q_sb + (long long)h * p.q_sh +
                             (long long)min(my_q, p.Sq - 1) * p.q_ss;
+#endif
 #pragma unroll
       for (int ks = 0; ks < LF_NKS; ++ks)
         qf[ks] = __builtin_bit_cast(lf_elem8, *reinterpret_cast<const lf_u32x4*>(qrow + 16 * ks + 8 * g));
@@ -534,7 +589,7 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
         else dma_v_pass(v_cur, kt + 1, vs_ld, d - LF_NPASS, vpg[d - LF_NPASS]);
       };
       // page offsets for the next tile's loads (table reads: in flight during this tile)
-      unsigned kpg_n[LF_NPASS], vpg_n[LF_NPASS];
+      lf_page_t kpg_n[LF_NPASS], vpg_n[LF_NPASS];
 #pragma unroll
       for (int ps = 0; ps < LF_NPASS; ++ps) {
         kpg_n[ps] = kPagedK ? page_off(0, kt + 3, ps) : 0u;
@@ -814,6 +869,19 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     // ---- epilogue: O[q][d] = O^T[d][q] / l.  Element i of block db is
     // d = 32*db + 8*(i/4) + 4*g + i%4.
     const float l_tot = l_run + lf_swap32(l_run);
+#if LF_PREFIX
+    // the row's partial result, as lf_attn_decode leaves it: offset and sum in log2 units, and sum of e V
+    if (my_q < p.Sq) {
+      const long long slot = ((long long)h * p.Sq + my_q) * p.nsplit + part;
+#pragma unroll
+      for (int db = 0; db < LF_NDB; ++db)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+          *reinterpret_cast<lf_f32x4*>(&sp.pre_acc[slot * LF_D + 32 * db + 8 * i4 + 4 * g]) =
+              lf_f32x4{o[db][4 * i4], o[db][4 * i4 + 1], o[db][4 * i4 + 2], o[db][4 * i4 + 3]};
+      if (g == 0) *reinterpret_cast<lf_f32x2*>(&sp.pre_ml[slot * 2]) = lf_f32x2{mc_ref, l_tot};
+    }
+#else
     // optional: the row's log-sum-exp of the scaled, masked scores in log2 units (what a
     // backward pass recomputes the probabilities from); -inf for a row that saw no key
     if (p.part_ml != nullptr && g == 0 && my_q < p.Sq)
@@ -879,6 +947,7 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
       }
 #endif
     }
+#endif   // LF_PREFIX
   };
 
   run_q_tile(slot_qt);

@@ -98,7 +98,7 @@ class KernelSpec:
     extra: tuple = ()      # further -D options (tuning experiments)
     stay: bool = False     # prefill_swp, bwd: results by plain stores (prefill_out_stays, bwd_grads_stay)
     packed: bool = False   # prefill_swp, bwd: the tiles of sequences of different lengths in one tensor (lf_packed.hip.h)
-    shared: int = 0        # decode: 1 the own keys of requests of different lengths, 2 the prefix they share (lf_shared.hip.h)
+    shared: int = 0        # decode: 1 the own keys of requests of different lengths, 2 the prefix they share (lf_shared.hip.h); prefill_swp: 2
 
     def __hash__(self):    # formed once: a call looks its kernels up by it, several times
         h = self.__dict__.get("_hash")
@@ -144,6 +144,8 @@ class KernelSpec:
                 o += [f"-DLF_GQAPACK={int(self.pack)}"]
             if self.bias:
                 o += ["-DLF_BIAS=2" if self.bias == MASK_BITS else "-DLF_BIAS=1"]
+            if self.shared:
+                o += ["-DLF_PREFIX=1"]
         if self.stay:
             o += ["-DLF_STAY=1"]
         if self.packed:
@@ -158,6 +160,8 @@ class KernelSpec:
                   "shared_combine": "lf_shared_combine.hip", "paged_tables": "lf_paged_tables.hip", "store_kv": "lf_store_kv.hip"}[self.family]
         if self.family == "packed_plan":
             return ("lf_common.hip.h", "lf_packed.hip.h", kernel)
+        if self.shared and self.family == "prefill_swp":
+            return ("lf_common.hip.h", "lf_shared.hip.h", "lf_prefill_blocks.hip.h", kernel)
         if self.shared or self.family == "shared_combine":
             return ("lf_common.hip.h", "lf_shared.hip.h", kernel)
         if self.family in ("paged_tables", "store_kv"):
@@ -817,6 +821,49 @@ def _keep(key, kept: _Kept) -> None:
     if len(_kept) >= _MAX_KEPT:
         _kept.clear()
     _kept[key] = kept
+
+
+class _Repeat:
+    """The launches of a call of one of the other operators (``packed``, ``paged``), recorded for its signature (``_call_key``):
+    ``block``: the parameter block, its pointers still to be set; ``more``: what the operator keeps beside it."""
+
+    __slots__ = ("block", "launches", "record", "more")
+
+    def __init__(self, params, steps, record, more=None):
+        self.block, self.launches, self.record, self.more = bytes(params), runtime.LaunchList(steps), record, more
+
+
+def _call_key(kind: str, data, ints, plan: Optional[AttnPlan], more: tuple):
+    """As ``_signature``: key of a call over operands ``data``, read 16 bytes at a time, and index tensors ``ints`` (None in the place of
+    one that is not given), with further plain values ``more``; None: not to be kept."""
+    if os.environ is not _ENVIRON or _VARIABLES is None or b"LOOPFUSE_CHECK_TABLES" in _VARIABLES:
+        return None
+    device, operands = runtime.current_device(), []
+    try:
+        for t in data:
+            if t is None:
+                operands.append(None)
+            elif t.get_device() != device or t.data_ptr() % 16:
+                return None
+            else:
+                operands.append((t.shape, t.stride(), t.dtype))
+        for t in ints:
+            if t is None:
+                operands.append(None)
+            elif t.get_device() != device:
+                return None
+            else:
+                operands.append((t.shape, t.stride(), t.dtype))
+    except AttributeError:
+        return None
+    fields = None
+    if plan is not None:
+        fields = (plan.mask, plan.window, plan.scale, plan.softcap, plan.k_paged, plan.v_paged, plan.denom_add)
+        if not _PLAIN_TYPES.issuperset(map(type, fields)):
+            return None
+    if not _PLAIN_TYPES.issuperset(map(type, more)):
+        return None
+    return (kind, device, fields, more, tuple(map(_VARIABLES.get, _SWITCHES)), tuple(operands))
 
 
 class _LastLaunch:

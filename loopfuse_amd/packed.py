@@ -58,9 +58,9 @@ class PackedLayout:
         return self.offsets.shape[0] - 1
 
     def tiles_of(self, rows: int) -> tuple:
-        """(address, entries) of the list of tiles of so many rows."""
+        """(first byte in ``tiles``, entries) of the list of tiles of so many rows."""
         i = TILE_HEIGHTS.index(rows)
-        return self.tiles.data_ptr() + 16 * sum(self.caps[:i]), self.caps[i]
+        return 16 * sum(self.caps[:i]), self.caps[i]
 
 
 def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
@@ -162,8 +162,29 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
     return _forward(q, k, v, plan, layout, out, lse)
 
 
-@lowering._on_device_of_first_argument
 def _forward(q, k, v, plan, layout, out, lse):
+    key = lowering._call_key("packed", (q, k, v, out), (lse, layout.tiles), plan, (layout.total, layout.caps[-1]))
+    kept = lowering._kept.get(key)
+    if kept is not None:
+        return _forward_again(q, k, v, layout, out, lse, kept)
+    return _forward_general(q, k, v, plan, layout, out, lse, key)
+
+
+def _forward_again(q, k, v, layout, out, lse, repeat):
+    P = PackedAttnParams.from_buffer_copy(repeat.block)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    P.q, P.k, P.v, P.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    if lse is not None:
+        P.part_ml = lse.data_ptr()
+    P.tiles = layout.tiles.data_ptr() + repeat.more
+    repeat.launches.launch(P)
+    lowering._last_launch.set(repeat.record)
+    return out
+
+
+@lowering._on_device_of_first_argument
+def _forward_general(q, k, v, plan, layout, out, lse, key):
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
     mask, window, scale, cap = _constants(plan)
     T = layout.total
@@ -171,41 +192,38 @@ def _forward(q, k, v, plan, layout, out, lse):
         # direct-to-LDS loads address a sequence with 32-bit byte offsets, up to three tiles past its end
         if t.stride(0) < 0 or 2 * (T + 192) * t.stride(0) + 2 * D >= 1 << 31:
             raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
-    fresh = out is None
-    if fresh:
-        out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
-    else:
+    if out is not None:
         _rows("O", out, layout, dtype, D)
         if out.shape[1] != Hq or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
             raise UnsupportedPlan(f"O must be [{T}, {Hq}, {D}], every element with a place of its own")
     if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or not lse.is_contiguous() or lse.device != q.device):
         raise UnsupportedPlan(f"lse must be a contiguous float32 [{Hq}, {T}] tensor on the device of Q")
     if T == 0:
-        return out
+        return torch.empty(q.shape, dtype=dtype, device=q.device) if out is None else out
     P = PackedAttnParams()
-    P.q, P.k, P.v, P.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     P.q_ss, P.q_sh = q.stride()[:2]
     P.k_ss, P.k_sh = k.stride()[:2]
     P.v_ss, P.v_sh = v.stride()[:2]
-    P.o_ss, P.o_sh = out.stride()[:2]
+    P.o_ss, P.o_sh = (Hq * D, D) if out is None else out.stride()[:2]
     P.B, P.Hq, P.Hkv, P.Sq, P.Sk, P.window = 1, Hq, Hkv, T, T, window
     P.scale, P.softcap = scale, cap or 0.0
     P.nsplit, P.rows = 1, 1
-    P.part_ml = None if lse is None else lse.data_ptr()
-    P.clear = int(fresh)
+    P.clear = int(out is None)
     group = Hq // Hkv
     pack = 4 if group % 4 == 0 else 2 if group % 2 == 0 else 0
     bm, heads = 128 // (pack or 1), Hq // (pack or 1)
-    P.tiles, entries = layout.tiles_of(bm)
+    tiles_at, entries = layout.tiles_of(bm)
     mean = T // max(1, layout.count)
     spec = lowering._spec("prefill_swp", lowering._DTYPE_CODE[dtype], D, mask, cap is not None, pack=pack, packed=True,
                           bn=lowering.prefill_kv_tile(D, 0, None, heads * (T // bm + layout.count // 2),
                                                       min(mean, window) if mask == lowering.MASK_SLIDING else mean),
                           stay=lowering.prefill_out_stays(2 * T * Hq * D))
     grid = _grid(entries, heads, 256)
-    lowering.get_kernel(spec, spec.entry()).launch((grid, 1, 1), (256, 1, 1), P)
-    lowering._last_launch.set({"kernels": [spec.entry()], "grid": grid, "block": 256, "q_tile_rows": bm, "kv_tile_rows": spec.bn or 64,
-                               "heads_per_workgroup": pack or 1})
+    record = {"kernels": [spec.entry()], "grid": grid, "block": 256, "q_tile_rows": bm, "kv_tile_rows": spec.bn or 64, "heads_per_workgroup": pack or 1}
+    repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (grid, 1, 1), 256)], record, tiles_at)
+    out = _forward_again(q, k, v, layout, out, lse, repeat)
+    if key is not None:
+        lowering._keep(key, repeat)
     return out
 
 
@@ -219,8 +237,30 @@ def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return _backward(q, k, v, o, lse, dout, plan, layout)
 
 
-@lowering._on_device_of_first_argument
 def _backward(q, k, v, o, lse, dout, plan, layout):
+    key = lowering._call_key("packed bwd", (q, k, v, o, dout), (lse, layout.tiles), plan, (layout.total, layout.caps[-1]))
+    kept = lowering._kept.get(key)
+    if kept is not None:
+        return _backward_again(q, k, v, o, lse, dout, layout, kept)
+    return _backward_general(q, k, v, o, lse, dout, plan, layout, key)
+
+
+def _backward_again(q, k, v, o, lse, dout, layout, repeat):
+    P = PackedBwdParams.from_buffer_copy(repeat.block)
+    dtype, dev = q.dtype, q.device
+    dq, dk, dv = torch.empty(q.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
+    delta = torch.empty(lse.shape, dtype=torch.float32, device=dev)
+    P.q, P.k, P.v, P.o, P.dout = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr()
+    P.dq, P.dk, P.dv, P.lse, P.delta = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), lse.data_ptr(), delta.data_ptr()
+    at = layout.tiles.data_ptr()
+    P.dkdv_tiles, P.dq_tiles = at + repeat.more[0], at + repeat.more[1]
+    repeat.launches.launch(P)
+    lowering._last_launch.set(repeat.record)
+    return dq, dk, dv
+
+
+@lowering._on_device_of_first_argument
+def _backward_general(q, k, v, o, lse, dout, plan, layout, key):
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
     mask, window, scale, cap = _constants(plan)
     T, dev = layout.total, q.device
@@ -233,16 +273,15 @@ def _backward(q, k, v, o, lse, dout, plan, layout):
     for name, t in (("Q", q), ("dO", dout), ("K", k), ("V", v)):
         if t.stride(0) < 0 or 2 * (T + 64) * t.stride(0) + 2 * D >= 1 << 32:
             raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
-    dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=dev) for t in (q, k, v))
     if T == 0:
-        return dq, dk, dv
-    delta = torch.empty((Hq, T), dtype=torch.float32, device=dev)
+        return tuple(torch.empty(t.shape, dtype=dtype, device=dev) for t in (q, k, v))
     P = PackedBwdParams()
-    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv), ("lse", lse), ("delta", delta)):
-        setattr(P, name, t.data_ptr())
-    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("do", dout)):
         setattr(P, name + "_ss", t.stride(0))
         setattr(P, name + "_sh", t.stride(1))
+    for name, heads in (("dq", Hq), ("dk", Hkv), ("dv", Hkv)):
+        setattr(P, name + "_ss", heads * D)
+        setattr(P, name + "_sh", D)
     P.B, P.Hq, P.Hkv, P.Sq, P.Sk, P.window = 1, Hq, Hkv, T, T, window
     P.scale, P.softcap = scale, cap or 0.0
     count = max(1, layout.count)
@@ -253,17 +292,18 @@ def _backward(q, k, v, o, lse, dout, plan, layout):
     if q_split:
         keys = 1
     spec = bwd_spec(dtype, D, mask, cap is not None, keys, nt, q_split, lowering.bwd_grads_stay(2 * T * Hq * D))
-    P.dkdv_tiles, dkdv_entries = layout.tiles_of(64 if q_split else 128 * keys)
-    P.dq_tiles, dq_entries = layout.tiles_of(nt // 2)
+    dkdv_at, dkdv_entries = layout.tiles_of(64 if q_split else 128 * keys)
+    dq_at, dq_entries = layout.tiles_of(nt // 2)
     steps = {"lf_attn_bwd_delta": (-(-Hq * T // 16), 256), "lf_attn_bwd_dkdv": (_grid(dkdv_entries, Hkv, 256), 256),
              "lf_attn_bwd_dq": (_grid(dq_entries, Hq, nt), nt)}
     names = ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"] if nt == 256 else list(steps)
     named = lowering._kernels_of(spec)
-    for name in names:
-        grid, block = steps[name]
-        lowering.get_kernel(spec, name, named).launch((grid, 1, 1), (block, 1, 1), P)
-    lowering._last_launch.set({"kernels": names})
-    return dq, dk, dv
+    launches = [(lowering.get_kernel(spec, name, named), (steps[name][0], 1, 1), steps[name][1]) for name in names]
+    repeat = lowering._Repeat(P, launches, {"kernels": names}, (dkdv_at, dq_at))
+    res = _backward_again(q, k, v, o, lse, dout, layout, repeat)
+    if key is not None:
+        lowering._keep(key, repeat)
+    return res
 
 
 def bwd_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool = False, key_blocks: int = 1, dq_threads: int = 512, q_split: bool = False,

@@ -83,6 +83,10 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
 
     Nothing is raised for what only the GPU knows: where no free page is left, the row of the table is too short or a token lies behind
     ``total``, the token's slot (and the new entry) is -1, which ``store_kv`` leaves out; ``pages`` above ``len(free)`` says so."""
+    key = lowering._call_key("tables", (), (cached, new, table, free), None, (page_size, total))
+    kept = lowering._kept.get(key)
+    if kept is not None:
+        return _tables(cached, new, table, free, total, kept)
     _on_gpu("cached", cached, (torch.int32,), 1)
     dev, B = cached.device, cached.shape[0]
     _on_gpu("new", new, (torch.int32,), 1, dev)
@@ -96,15 +100,32 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
     if total < 0 or total >= 1 << 31:
         raise UnsupportedPlan("the number of rows must be between 0 and 2**31 - 1")
     with torch.cuda.device(dev):
-        made = torch.empty(2 * B + 2 + 2 * total, dtype=torch.int32, device=dev)
-        offsets, lengths, pages, slots, positions = made.split((B + 1, B, 1, total, total))
-        cached, new, free = cached.contiguous(), new.contiguous(), free.contiguous()
-        P = _TablesParams(cached.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr(), offsets.data_ptr(), lengths.data_ptr(),
-                          slots.data_ptr(), positions.data_ptr(), pages.data_ptr(), table.stride(0), B, table.shape[1], free.shape[0], total, shift)
+        packed = [t if t.is_contiguous() else t.contiguous() for t in (cached, new, free)]
+        P = _TablesParams(table_stride=table.stride(0), B=B, width=table.shape[1], count=free.shape[0], T=total, shift=shift)
         spec = lowering._spec("paged_tables", 0, 64, table_i64=table.dtype == torch.int64)
         # a block per request and 1024 rows of the mean one
         share = max(1, min(64, total // (1024 * max(B, 1))))
-        lowering.get_kernel(spec, spec.entry()).launch((max(B, 1), share, 1), (256, 1, 1), P)
+        repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (max(B, 1), share, 1), 256)], {"kernels": [spec.entry()]},
+                                  (2 * B + 2 + 2 * total, (B + 1, B, 1, total, total)))
+        step = _tables(packed[0], packed[1], table, packed[2], total, repeat)
+    if key is not None and packed[0] is cached and packed[1] is new and packed[2] is free:
+        lowering._keep(key, repeat)
+    return step
+
+
+def _tables(cached, new, table, free, total, repeat) -> PagedStep:
+    size, parts = repeat.more
+    made = torch.empty(size, dtype=torch.int32, device=table.device)
+    offsets, lengths, pages, slots, positions = made.split_with_sizes(parts)
+    P = _TablesParams.from_buffer_copy(repeat.block)
+    P.cached, P.fresh, P.table, P.free = cached.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr()
+    P.offsets = at = made.data_ptr()
+    P.lengths = at = at + 4 * parts[0]
+    P.pages = at = at + 4 * parts[1]
+    P.slots = at = at + 4
+    P.positions = at + 4 * total
+    repeat.launches.launch(P)
+    lowering._last_launch.set(repeat.record)
     return PagedStep(offsets, lengths, slots, positions, pages)
 
 
@@ -122,6 +143,10 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     ``slots[t] // page``.  bf16 / fp16, D a multiple of 8; views will do.  ``slots``: int32 [rows] (``PagedStep.slots``); rows whose slot is below 0 or
     behind the pool's last are left out.  Slots that are not left out are distinct, as those of ``extend_tables`` are:
     of two rows with one slot, either may be found there afterwards, or a part of each."""
+    key = lowering._call_key("store", (k, v, k_pool, v_pool), (slots,), None, ())
+    kept = lowering._kept.get(key)
+    if kept is not None:
+        return _store(k, v, k_pool, v_pool, slots, kept)
     if k.dtype not in lowering._DTYPE_CODE:
         raise UnsupportedPlan(f"dtype {k.dtype} not supported (bf16/fp16 only)")
     for name, t in (("K", k), ("V", v), ("K pool", k_pool), ("V pool", v_pool)):
@@ -142,16 +167,27 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     if T == 0 or pages == 0 or heads == 0 or D == 0:
         return
     with torch.cuda.device(k.device):
-        slots = slots.contiguous()
-        P = _StoreParams(k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), slots.data_ptr(),
-                         *(x // 8 for x in (*k.stride()[:2], *v.stride()[:2], *ks, *vs)), pages * page, T, heads, D // 8, shift)
+        packed = slots.contiguous()
+        P = _StoreParams(0, 0, 0, 0, 0, *(x // 8 for x in (*k.stride()[:2], *v.stride()[:2], *ks, *vs)), pages * page, T, heads, D // 8, shift)
         spec = lowering._spec("store_kv", 0, 64)
-        lowering.get_kernel(spec, spec.entry()).launch((-(-T // max(256 // (heads * D // 8), 1)), 1, 1), (256, 1, 1), P)
+        grid = (-(-T // max(256 // (heads * D // 8), 1)), 1, 1)
+        repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), grid, 256)], {"kernels": [spec.entry()]})
+        _store(k, v, k_pool, v_pool, packed, repeat)
+    if key is not None and packed is slots:
+        lowering._keep(key, repeat)
+
+
+def _store(k, v, k_pool, v_pool, slots, repeat) -> None:
+    P = _StoreParams.from_buffer_copy(repeat.block)
+    P.k, P.v, P.k_pool, P.v_pool, P.slots = k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), slots.data_ptr()
+    repeat.launches.launch(P)
+    lowering._last_launch.set(repeat.record)
 
 
 def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, plan: AttnPlan, table: torch.Tensor, lengths: torch.Tensor, *,
                      prefix_table: Optional[torch.Tensor] = None, prefix_len: int = 0, v_table: Optional[torch.Tensor] = None,
-                     prefix_v_table: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     prefix_v_table: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                     choice: Optional[dict] = None) -> torch.Tensor:
     """Attention of one new token per request over a prefix that all requests share and over the request's own keys.
 
     q : [B, Hq, 1, D], bf16 / fp16, D 64 or 128.  k_pool, v_pool : page pools of one page size.  table : [B, width], int32 or int64,
@@ -162,12 +198,19 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
 
     The prefix is read once for all requests together: its keys meet the rows of the whole batch as a matrix product, the requests'
     own keys are streamed, and the partial results are joined in a second launch.  Page ids are trusted, as those of
-    ``lowering.attention`` are."""
-    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, int(prefix_len), v_table, prefix_v_table, out)
+    ``lowering.attention`` are.  ``choice`` overrides the rules of the work split: ``{"prefix": "tiles" | "stream", "splits": n,
+    "target": n, "least": n}``."""
+    key = None if choice else lowering._call_key("shared", (q, k_pool, v_pool, out), (table, lengths, prefix_table, v_table, prefix_v_table),
+                                                 plan, (prefix_len,))
+    kept = lowering._kept.get(key)
+    if kept is not None:
+        return _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_table, out, kept)
+    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, int(prefix_len), v_table, prefix_v_table, out, choice or {}, key)
 
 
 @lowering._on_device_of_first_argument
-def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v_table, prefix_v_table, out):
+def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v_table, prefix_v_table, out, choice, key):
+    given = (table, lengths, prefix_table, v_table, prefix_v_table)
     dtype = q.dtype
     if dtype not in lowering._DTYPE_CODE:
         raise UnsupportedPlan(f"dtype {dtype} not supported by the MFMA kernels (bf16/fp16 only)")
@@ -202,7 +245,7 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     _on_gpu("V table", v_table, (table.dtype,), 2, q.device)
     if table.shape[0] != B or v_table.shape != table.shape or lengths.shape[0] != B:
         raise UnsupportedPlan(f"tables and lengths must be of {B} requests, the tables of one width")
-    if prefix_len < 0 or prefix_len >= 1 << 31 or table.shape[1] * page >= 1 << 31:
+    if not isinstance(prefix_len, int) or prefix_len < 0 or prefix_len >= 1 << 31 or table.shape[1] * page >= 1 << 31:
         raise UnsupportedPlan("more keys than positions in 32 bits")
     if prefix_len:
         if prefix_table is None:
@@ -216,22 +259,19 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     table = table if table.stride(1) == 1 else table.contiguous()
     v_table = v_table if v_table.stride(1) == 1 else v_table.contiguous()
     lengths = lengths.contiguous()
-    if out is None:
-        out = torch.empty((B, Hq, 1, D), dtype=dtype, device=q.device)
-    else:
+    if out is not None:
         lowering._check_tensor("O", out, dtype)
         if tuple(out.shape) != (B, Hq, 1, D) or out.device != q.device or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
             raise UnsupportedPlan(f"O must be [{B}, {Hq}, 1, {D}] on the device of Q, every element with a place of its own")
     if B == 0:
-        return out
+        return torch.empty(q.shape, dtype=dtype, device=q.device) if out is None else out
     P = SharedParams()
-    P.q, P.k, P.v, P.o = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
     P.q_sb, P.q_sh, P.q_ss = q.stride(0), group * q.stride(1), q.stride(1)
-    P.o_sb, P.o_sh, P.o_ss = out.stride(0), group * out.stride(1), out.stride(1)
+    o_sb, o_sh = (Hq * D, D) if out is None else out.stride()[:2]
+    P.o_sb, P.o_sh, P.o_ss = o_sb, group * o_sh, o_sh
     P.k_sb, P.k_ss, P.k_sh = ks
     P.v_sb, P.v_ss, P.v_sh = vs
-    P.k_table, P.v_table, P.kt_stride, P.vt_stride = table.data_ptr(), v_table.data_ptr(), table.stride(0), v_table.stride(0)
-    P.lengths = lengths.data_ptr()
+    P.kt_stride, P.vt_stride = table.stride(0), v_table.stride(0)
     P.B, P.Hq, P.Hkv, P.rows, P.Sq = B, Hq, Hkv, group, 1
     P.scale, P.softcap = float(plan.scale), softcap or 0.0
     P.room = table.shape[1] * page
@@ -239,34 +279,69 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     coop = lowering._decode_coop_waves(3, page, 0, 0, Hkv, P, D)
     chunks = -(-group // lowering.DECODE_QROWS)
     heads = Hkv // coop if coop else Hkv
-    P.units, P.target, P.least = heads * chunks, 256 if coop else 512, 160 if coop else 512
+    P.units = heads * chunks
+    P.target, P.least = choice.get("target", 256 if coop else 512), choice.get("least", 160 if coop else 512)
     items = P.target // P.units + B if P.room else 0
-    pre_rows, pre_units, splits = B * group, heads * -(-B * group // lowering.DECODE_QROWS), 0
+    splits, rows, pre_grid = 0, B * group, None
+    tiles = False
     P.nsplit = 1
     if prefix_len:
-        splits = max(1, min(64, prefix_len // 160, 512 // pre_units))
-        splits, P.split_len = lowering._split_lengths(splits, prefix_len)
+        # direct-to-LDS loads of whole rows from a page at a time, a page's bytes within 32-bit offsets
+        tiles = page % 8 == 0 and page * max(P.k_ss, P.v_ss) < 1 << 30 and P.k_ss >= 0 and P.v_ss >= 0
+        if tiles:
+            tiles = choice.get("prefix", "tiles" if rows > lowering.DECODE_QROWS else "stream") == "tiles"
+        if tiles:
+            units, keys = Hkv * -(-rows // 128), -(-prefix_len // 64)
+            splits = max(1, min(64, keys // 2, choice.get("splits", -(-512 // units))))
+            P.split_len = 64 * -(-keys // splits)
+            splits = -(-prefix_len // P.split_len)
+            pre_grid = (units * splits, 1, 1)
+            P.k_span = P.v_span = 1
+        else:
+            units = heads * -(-rows // lowering.DECODE_QROWS)
+            splits = max(1, min(64, prefix_len // 160, choice.get("splits", 512 // units)))
+            splits, P.split_len = lowering._split_lengths(splits, prefix_len)
+            pre_grid = (units, splits, 1)
         P.nsplit = splits
-        P.prefix_k, P.prefix_v = prefix_table.data_ptr(), prefix_v_table.data_ptr()
     own, pre = items * Hq, splits * B * Hq            # rows of partial results
     args = dict(rows=lowering.DECODE_QROWS, waves=coop or 4, headwave=coop > 0, coop=coop > 0,
                 rowload=not coop and lowering._decode_rowload(3, page, 0, 0))
     make = lambda which: lowering._spec("decode", lowering._DTYPE_CODE[dtype], D, lowering.MASK_NONE, softcap is not None, 3, page,
                                         table.dtype == torch.int64, shared=which, **args)
+    steps = []
+    if splits:
+        spec = lowering._spec("prefill_swp", lowering._DTYPE_CODE[dtype], D, lowering.MASK_NONE, softcap is not None, 3, page,
+                              table.dtype == torch.int64, shared=2) if tiles else make(2)
+        steps.append((lowering.get_kernel(spec, spec.entry()), pre_grid, 256 if tiles else 64 * args["waves"]))
+    if items:
+        steps.append((lowering.get_kernel(make(1), "lf_attn_decode"), (items * P.units, 1, 1), 64 * args["waves"]))
+    spec = lowering._spec("shared_combine", lowering._DTYPE_CODE[dtype], D)
+    steps.append((lowering.get_kernel(spec, spec.entry()), (B * -(-Hq // (1024 // D)), 1, 1), 256))
+    repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps], "prefix": "tiles" if tiles else "stream", "splits": splits},
+                              ((own + pre) * (D + 2), 4 * own * D, 4 * own * (D + 2), 4 * own * (D + 2) + 4 * pre * D))
+    res = _again(q, k_pool, v_pool, table, lengths, prefix_table if prefix_len else None, v_table, prefix_v_table, out, repeat)
+    if key is not None and all(a is b for a, b in zip(given[:3] , (table, lengths, prefix_table))) and (given[3] is None or given[3] is v_table) \
+            and (given[4] is None or given[4] is prefix_v_table):
+        lowering._keep(key, repeat)
+    return res
+
+
+def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_table, out, repeat):
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    P = SharedParams.from_buffer_copy(repeat.block)
+    P.q, P.k, P.v, P.o = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
+    P.k_table = table.data_ptr()
+    P.v_table = P.k_table if v_table is None else v_table.data_ptr()
+    P.lengths = lengths.data_ptr()
+    if prefix_table is not None:
+        P.prefix_k = prefix_table.data_ptr()
+        P.prefix_v = P.prefix_k if prefix_v_table is None else prefix_v_table.data_ptr()
+    floats, ml, pre_acc, pre_ml = repeat.more
     with lowering._scratch_lock:        # no other thread's step on this stream between the launches
-        scratch = lowering._get_scratch(q.device, (own + pre) * (D + 2))
+        scratch = lowering._get_scratch(q.device, floats)
         at = scratch.data_ptr()
-        P.part_acc, P.part_ml = at, at + 4 * own * D
-        P.pre_acc, P.pre_ml = at + 4 * own * (D + 2), at + 4 * own * (D + 2) + 4 * pre * D
-        names = []
-        if splits:
-            lowering.get_kernel(make(2), "lf_attn_decode").launch((pre_units, splits, 1), (64 * args["waves"], 1, 1), P)
-            names.append("lf_attn_decode")
-        if items:
-            lowering.get_kernel(make(1), "lf_attn_decode").launch((items * P.units, 1, 1), (64 * args["waves"], 1, 1), P)
-            names.append("lf_attn_decode")
-        spec = lowering._spec("shared_combine", lowering._DTYPE_CODE[dtype], D)
-        lowering.get_kernel(spec, spec.entry()).launch((B * -(-Hq // (1024 // D)), 1, 1), (256, 1, 1), P)
-        names.append(spec.entry())
-    lowering._last_launch.set({"kernels": names})
+        P.part_acc, P.part_ml, P.pre_acc, P.pre_ml = at, at + ml, at + pre_acc, at + pre_ml
+        repeat.launches.launch(P)
+    lowering._last_launch.set(repeat.record)
     return out
