@@ -57,6 +57,7 @@
 #define LF_DT (LF_DW * 64)
 #define LF_D LF_HEAD_DIM
 #define LF_NJ (LF_D / 32)    /* 16-byte pieces of a row held by one lane = k-steps of QK^T */
+#undef LF_NDB                /* (of another kernel in front of this one) */
 #define LF_NDB (LF_D / 16)   /* 16-row blocks of O^T */
 #define LF_QROWS 16          /* query rows one unit can hold (MFMA N) */
 #define LF_OSTRIDE (LF_D + 4) /* floats per row of the merge buffer */
@@ -67,37 +68,42 @@
 #endif
 
 #ifndef LF_SHARED
-#define LF_SHARED 0          /* 1: a piece of one request's own keys, 2: a split of the prefix that all requests share, for 16 of their rows
-                                (lf_shared.hip.h); grid: 1 (pieces * units), 2 (units, nsplit) */
+#define LF_SHARED 0          /* 1: requests of different lengths behind a prefix that they share (lf_shared.hip.h): a workgroup has a piece of one
+                                request's own keys or a split of the prefix for 16 rows of all requests; one-dimensional grid */
+#endif
+#ifndef LF_PREFIX
+#define LF_PREFIX 0          /* 1: ... or, with 4 waves, a split of the prefix for 128 rows, on the tiles of lf_attn_prefill_swp.hip in front of
+                                this file */
 #endif
 #if LF_SHARED
-#if LF_BIAS || LF_PAGED != 3
-#error "LF_SHARED: K and V in pages, no score bias"
+#if LF_BIAS || LF_PAGED != 3 || (LF_PREFIX && LF_DW != 4)
+#error "LF_SHARED: K and V in pages, no score bias; LF_PREFIX: 4 waves"
 #endif
 #define LF_DEC_PARAMS LfSharedParams
-#define LF_K_TABLE (LF_SHARED == 2 ? p.prefix_k : p.k_table)
-#define LF_V_TABLE (LF_SHARED == 2 ? p.prefix_v : p.v_table)
-#define LF_KEYS keys         /* of this unit's sequence */
-#define LF_SPLIT_PARTIAL (LF_SHARED == 2 || p.Sk != 0 || keys > split)
-#define LF_PART_ACC (LF_SHARED == 2 ? p.pre_acc : p.part_acc)
-#define LF_PART_ML (LF_SHARED == 2 ? p.pre_ml : p.part_ml)
-#define LF_SLOT(qr) (LF_SHARED == 2 ? ((long long)hkv * p.B * p.rows + (qr)) * p.nsplit + z \
-                                    : ((long long)((int)blockIdx.x / p.units) * p.Hkv + hkv) * p.rows + (qr))
-#define LF_ALL_ROWS (LF_SHARED == 2 ? p.B * p.rows : p.rows)
+#define LF_K_TABLE su.k_table
+#define LF_V_TABLE su.v_table
+#define LF_KEYS su.keys       /* of this unit's sequence */
+#define LF_SPLIT_LEN su.split_len
+#define LF_ALL_ROWS su.rows
 /* row r of a unit: of the group of one request, or of all requests one behind the other */
-#define LF_Q_ROW(r) (p.q + (LF_SHARED == 2 ? (long long)((r) / p.rows) * p.q_sb + (long long)((r) % p.rows) * p.q_ss \
-                                           : (long long)b * p.q_sb + (long long)(r) * p.q_ss) + (long long)hkv * p.q_sh)
+#define LF_Q_ROW(r) (p.q + (su.prefix ? (long long)((r) / p.rows) * p.q_sb + (long long)((r) % p.rows) * p.q_ss \
+                                     : (long long)b * p.q_sb + (long long)(r) * p.q_ss) + (long long)hkv * p.q_sh)
+#define LF_SPLIT_PARTIAL (su.prefix || p.Sk != 0 || su.keys > su.split_len)
+#define LF_PART_ACC (su.prefix ? p.pre_acc : p.part_acc)
+#define LF_PART_ML (su.prefix ? p.pre_ml : p.part_ml)
+#define LF_SLOT(qr) (su.prefix ? ((long long)hkv * p.nsplit + z) * su.rows + (qr) : ((long long)su.piece * p.Hkv + hkv) * p.rows + (qr))
 #else
 #define LF_DEC_PARAMS LfAttnParams
 #define LF_K_TABLE p.k_table
 #define LF_V_TABLE p.v_table
 #define LF_KEYS p.Sk
+#define LF_SPLIT_LEN p.split_len
+#define LF_ALL_ROWS p.rows
+#define LF_Q_ROW(r) (p.q + (long long)b * p.q_sb + (long long)hkv * p.q_sh + (long long)(r) * p.q_ss)
 #define LF_SPLIT_PARTIAL (p.nsplit != 1)
 #define LF_PART_ACC p.part_acc
 #define LF_PART_ML p.part_ml
 #define LF_SLOT(qr) (((long long)bh * p.rows + (qr)) * p.nsplit + z)
-#define LF_ALL_ROWS p.rows
-#define LF_Q_ROW(r) (p.q + (long long)b * p.q_sb + (long long)hkv * p.q_sh + (long long)(r) * p.q_ss)
 #endif
 
 struct LfDecStage {
@@ -151,7 +157,16 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   constexpr int kVStride = kRowB + 32;
   constexpr int kBufB = 16 * (kKStride + kVStride);
   static_assert(16 * kPieces == LF_NJ * LF_DT, "a step is LF_NJ pieces per thread");
+#if LF_PREFIX
+  unsigned char* const smem = lf_pool;
+  static_assert(2 * kBufB <= (int)sizeof(lf_pool), "both parts of the kernel fit the pool");
+  if ((int)blockIdx.x < p.pre_blocks) {
+    lf_prefix_tile(p, (int)blockIdx.x);
+    return;
+  }
+#else
   __shared__ __attribute__((aligned(16))) unsigned char smem[2 * kBufB];
+#endif
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -159,35 +174,32 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   const int c = lane & 15;      // token of a step (K rows) / query column (MFMA results)
   const int g = lane >> 4;
 
-  const int chunks = (LF_ALL_ROWS + LF_QROWS - 1) / LF_QROWS;   // row chunks per (b, kv head)
-  const int hchunks = p.Hkv / LF_DW;                        // the host checks Hkv % LF_DW == 0
-#if LF_SHARED == 1
-  const int unit = blockIdx.x % p.units;
-  const int split = lf_shared_split(p);
-  int b, z, keys;
-  if (!lf_shared_piece(p, split, (int)blockIdx.x / p.units, b, z, keys)) return;
-  b = __builtin_amdgcn_readfirstlane(b);      // (in scalar registers: they make the wave's addresses)
-  z = __builtin_amdgcn_readfirstlane(z);
-  keys = __builtin_amdgcn_readfirstlane(keys);
-  const int split_len = split;
+#if LF_SHARED
+  LfSharedUnit su;
+  if (!lf_shared_unit(p, (int)blockIdx.x, su)) return;
+  const int z = su.z, unit = su.unit;
 #else
   const int z = blockIdx.y;
   const int unit = blockIdx.x;
-  const int b = unit / (chunks * hchunks);
-  const int split_len = p.split_len;
-#if LF_SHARED
-  const int keys = p.Sk, split = 0;
 #endif
+  const int chunks = (LF_ALL_ROWS + LF_QROWS - 1) / LF_QROWS;   // row chunks per (b, kv head)
+  const int hchunks = p.Hkv / LF_DW;                        // the host checks Hkv % LF_DW == 0
+#if LF_SHARED
+  const int b = su.b;
+#else
+  const int b = unit / (chunks * hchunks);
 #endif
   const int rc = unit % chunks;
   const int hkv0 = ((unit / chunks) % hchunks) * LF_DW;
   const int hkv = hkv0 + wave;
+#if !LF_SHARED
   const int bh = b * p.Hkv + hkv;
+#endif
   const int row0 = rc * LF_QROWS;
   const int nrows = min(LF_ALL_ROWS - row0, LF_QROWS);
 
-  const int tok_begin = z * split_len;
-  const int tok_end = min(tok_begin + split_len, LF_KEYS);
+  const int tok_begin = z * LF_SPLIT_LEN;
+  const int tok_end = min(tok_begin + LF_SPLIT_LEN, LF_KEYS);
   const int nsteps = (max(tok_end - tok_begin, 0) + 15) / 16;   // the same for every wave of the workgroup
 
   // ---- B operand of S^T = K Q^T: lane (q = c, g) holds Q[row0 + q][32*j + 8*g .. +7]
@@ -408,7 +420,16 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   // ([LF_DW][16][LF_OSTRIDE] floats) after it.
   constexpr int kVBytes = LF_DW * 2 * 16 * LF_D * 2 * (LF_ROWLOAD ? 2 : 1);   // wave-private V (and K) tiles of a pair
   constexpr int kOBytes = LF_DW * LF_QROWS * LF_OSTRIDE * 4;
+#if LF_PREFIX
+  unsigned char* const smem = lf_pool;
+  static_assert((kVBytes > kOBytes ? kVBytes : kOBytes) <= (int)sizeof(lf_pool), "both parts of the kernel fit the pool");
+  if ((int)blockIdx.x < p.pre_blocks) {
+    lf_prefix_tile(p, (int)blockIdx.x);
+    return;
+  }
+#else
   __shared__ __attribute__((aligned(16))) unsigned char smem[kVBytes > kOBytes ? kVBytes : kOBytes];
+#endif
 #if !LF_HEADWAVE
   __shared__ float red_m[LF_DW][LF_QROWS];
   __shared__ float red_l[LF_DW][LF_QROWS];
@@ -420,37 +441,25 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   const int c = lane & 15;      // token of a step (loads) / query column (MFMA results)
   const int g = lane >> 4;
 
-  const int chunks = (LF_ALL_ROWS + LF_QROWS - 1) / LF_QROWS;   // row chunks per (b, kv head)
-#if LF_SHARED == 1
-  const int unit = blockIdx.x % p.units;
-  const int split = lf_shared_split(p);
-  int b, z, keys;
-  if (!lf_shared_piece(p, split, (int)blockIdx.x / p.units, b, z, keys)) return;
-  b = __builtin_amdgcn_readfirstlane(b);      // (in scalar registers: they make the wave's addresses)
-  z = __builtin_amdgcn_readfirstlane(z);
-  keys = __builtin_amdgcn_readfirstlane(keys);
-  const int split_len = split;
+#if LF_SHARED
+  LfSharedUnit su;
+  if (!lf_shared_unit(p, (int)blockIdx.x, su)) return;
+  const int z = su.z, unit = su.unit;
 #else
   const int z = blockIdx.y;
   const int unit = blockIdx.x;
-  const int split_len = p.split_len;
-#if LF_SHARED
-  const int keys = p.Sk, split = 0;
 #endif
-#endif
+  const int chunks = (LF_ALL_ROWS + LF_QROWS - 1) / LF_QROWS;   // row chunks per (b, kv head)
   const int rc = unit % chunks;
 #if LF_HEADWAVE
   // grid.x = B * ceil(Hkv / LF_DW) * chunks; wave w serves head LF_DW*hc + w
   const int hchunks = (p.Hkv + LF_DW - 1) / LF_DW;
   const int hkv = ((unit / chunks) % hchunks) * LF_DW + wave;
-#if LF_SHARED != 1
   const int b = unit / (chunks * hchunks);
-#endif
   if (hkv >= p.Hkv) return;          // no workgroup barrier in this mode
   const int bh = b * p.Hkv + hkv;
-#elif LF_SHARED == 1
-  const int hkv = unit / chunks;
-  const int bh = b * p.Hkv + hkv;
+#elif LF_SHARED
+  const int hkv = unit / chunks, b = su.b;
 #else
   const int bh = unit / chunks;
   const int hkv = bh % p.Hkv;
@@ -459,8 +468,8 @@ extern "C" __global__ void __launch_bounds__(LF_DT, 8 / LF_DW) lf_attn_decode(co
   const int row0 = rc * LF_QROWS;
   const int nrows = min(LF_ALL_ROWS - row0, LF_QROWS);          // query rows of this unit
 
-  int tok_begin = z * split_len;
-  int tok_end = min(tok_begin + split_len, LF_KEYS);
+  int tok_begin = z * LF_SPLIT_LEN;
+  int tok_end = min(tok_begin + LF_SPLIT_LEN, LF_KEYS);
 #if LF_BIAS
   // Keys whose bias is -inf for every query row of the unit add nothing.  The split is narrowed
   // to the span from its first to its last live key (the left padding of a batch, the unused

@@ -116,9 +116,9 @@
 #error "packed sequences go with dense operands and the flag masks"
 #endif
 #ifndef LF_PREFIX
-#define LF_PREFIX 0      /* 1: a split of a prefix that all requests of a batch share, for 128 of their rows (lf_shared.hip.h); leaves partial
-                            results; grid: row tiles x nsplit x Hkv, in units of whole KV tiles.  Pages may lie anywhere: a load's page is
-                            its buffer's base */
+#define LF_PREFIX 0      /* 1: not a kernel but a part of lf_attn_decode -DLF_SHARED=1: a split of a prefix that all requests of a batch share,
+                            for 128 of their rows (lf_shared.hip.h); leaves partial results.  Pages may lie anywhere: a load's page
+                            is its buffer's base */
 #endif
 #if LF_PREFIX && (LF_PAGED != 3 || LF_BIAS || LF_MASK || LF_GQAPACK || LF_PACKED)
 #error "a shared prefix: K and V in pages, no mask, rows of all heads of a group"
@@ -127,7 +127,8 @@
 extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(const LfPackedAttnParams pk) {
   LfAttnParams p = pk;
 #elif LF_PREFIX
-extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(const LfSharedParams sp) {
+__shared__ __attribute__((aligned(256))) unsigned char lf_pool[(LF_KSLOTS + LF_VSLOTS) * LF_BN * LF_HEAD_DIM * 2];
+__device__ __forceinline__ void lf_prefix_tile(const LfSharedParams& sp, const int block) {
   LfAttnParams p = sp;
   p.k_table = sp.prefix_k;
   p.v_table = sp.prefix_v;
@@ -138,7 +139,11 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
 extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(const LfAttnParams p) {
 #endif
   // one array, K slots first
+#if LF_PREFIX
+#define lds_all lf_pool
+#else
   __shared__ __attribute__((aligned(16))) lf_elem lds_all[(LF_KSLOTS + LF_VSLOTS) * LF_BN * LF_D];
+#endif
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -169,7 +174,7 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
 #elif LF_PREFIX
   // the row tiles of a (split, kv head) are neighbours but for the heads: they share its K and V in one L2
   const int nqt = (p.Sq + LF_BM - 1) / LF_BM, b = 0;
-  const int bh = (int)blockIdx.x % p.Hkv, slot_qt = (int)blockIdx.x / p.Hkv % nqt, part = (int)blockIdx.x / p.Hkv / nqt;
+  const int bh = block % p.Hkv, slot_qt = block / p.Hkv % nqt, part = block / p.Hkv / nqt;
   const int lse_rows = 0;
   (void)nhv;
 #else
@@ -872,7 +877,7 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
 #if LF_PREFIX
     // the row's partial result, as lf_attn_decode leaves it: offset and sum in log2 units, and sum of e V
     if (my_q < p.Sq) {
-      const long long slot = ((long long)h * p.Sq + my_q) * p.nsplit + part;
+      const long long slot = ((long long)h * p.nsplit + part) * p.Sq + my_q;
 #pragma unroll
       for (int db = 0; db < LF_NDB; ++db)
 #pragma unroll

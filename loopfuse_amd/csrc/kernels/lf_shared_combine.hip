@@ -12,7 +12,7 @@ extern "C" __global__ void __launch_bounds__(256) lf_shared_combine(const LfShar
   if (head >= heads || (p.Sk == 0 && count == 1)) return;       // (one piece and nothing else: written already)
   const int hkv = head / p.rows, qr = head % p.rows;
   const int splits = p.Sk ? p.nsplit : 0, parts = splits + count;
-  const long long pre = ((long long)hkv * p.B * p.rows + (long long)b * p.rows + qr) * p.nsplit;
+  const long long pre = (long long)hkv * p.nsplit * p.B * p.rows + (long long)b * p.rows + qr;
   float m = LF_NEG_INF, l = 0.0f;
   lf_f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int z0 = 0; z0 < parts; z0 += 4) {
@@ -22,7 +22,7 @@ extern "C" __global__ void __launch_bounds__(256) lf_shared_combine(const LfShar
     for (int u = 0; u < 4; ++u) {
       const int z = min(z0 + u, parts - 1);
       const bool own = z >= splits;
-      const long long slot = own ? ((long long)(first + z - splits) * p.Hkv + hkv) * p.rows + qr : pre + z;
+      const long long slot = own ? ((long long)(first + z - splits) * p.Hkv + hkv) * p.rows + qr : pre + (long long)z * p.B * p.rows;
       ml[u] = *reinterpret_cast<const lf_f32x2*>((own ? p.part_ml : p.pre_ml) + slot * 2);
       ac[u] = *reinterpret_cast<const lf_f32x4*>((own ? p.part_acc : p.pre_acc) + slot * LF_HEAD_DIM + d0);
     }

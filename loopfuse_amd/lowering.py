@@ -98,7 +98,7 @@ class KernelSpec:
     extra: tuple = ()      # further -D options (tuning experiments)
     stay: bool = False     # prefill_swp, bwd: results by plain stores (prefill_out_stays, bwd_grads_stay)
     packed: bool = False   # prefill_swp, bwd: the tiles of sequences of different lengths in one tensor (lf_packed.hip.h)
-    shared: int = 0        # decode: 1 the own keys of requests of different lengths, 2 the prefix they share (lf_shared.hip.h); prefill_swp: 2
+    shared: int = 0        # decode: 1 requests of different lengths and the prefix they share (lf_shared.hip.h), 2 with the prefix on 128-row tiles
 
     def __hash__(self):    # formed once: a call looks its kernels up by it, several times
         h = self.__dict__.get("_hash")
@@ -131,7 +131,7 @@ class KernelSpec:
             if self.bias:
                 o += ["-DLF_BIAS=1"]
             if self.shared:
-                o += [f"-DLF_SHARED={self.shared}"]
+                o += ["-DLF_SHARED=1"] + (["-DLF_PREFIX=1"] if self.shared == 2 else [])
         elif self.family == "prefill":
             o += [f"-DLF_V_TR={int(self.v_tr)}", f"-DLF_BIAS={self.bias}", f"-DLF_DENOM={int(self.denom)}"]
             if self.d2:
@@ -144,8 +144,6 @@ class KernelSpec:
                 o += [f"-DLF_GQAPACK={int(self.pack)}"]
             if self.bias:
                 o += ["-DLF_BIAS=2" if self.bias == MASK_BITS else "-DLF_BIAS=1"]
-            if self.shared:
-                o += ["-DLF_PREFIX=1"]
         if self.stay:
             o += ["-DLF_STAY=1"]
         if self.packed:
@@ -160,8 +158,8 @@ class KernelSpec:
                   "shared_combine": "lf_shared_combine.hip", "paged_tables": "lf_paged_tables.hip", "store_kv": "lf_store_kv.hip"}[self.family]
         if self.family == "packed_plan":
             return ("lf_common.hip.h", "lf_packed.hip.h", kernel)
-        if self.shared and self.family == "prefill_swp":
-            return ("lf_common.hip.h", "lf_shared.hip.h", "lf_prefill_blocks.hip.h", kernel)
+        if self.shared == 2:
+            return ("lf_common.hip.h", "lf_shared.hip.h", "lf_prefill_blocks.hip.h", "lf_attn_prefill_swp.hip", kernel)
         if self.shared or self.family == "shared_combine":
             return ("lf_common.hip.h", "lf_shared.hip.h", kernel)
         if self.family in ("paged_tables", "store_kv"):

@@ -44,7 +44,7 @@ class SharedParams(lowering.AttnParams):
     """Mirror of ``struct LfSharedParams`` in csrc/kernels/lf_shared.hip.h."""
 
     _fields_ = ([(n, ctypes.c_void_p) for n in ("lengths", "prefix_k", "prefix_v", "pre_acc", "pre_ml")]
-                + [(n, ctypes.c_int) for n in ("room", "units", "target", "least")])
+                + [(n, ctypes.c_int) for n in ("room", "units", "pre_units", "pre_blocks", "target_log2", "least")])
 
 
 class PagedStep(NamedTuple):
@@ -199,7 +199,7 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     The prefix is read once for all requests together: its keys meet the rows of the whole batch as a matrix product, the requests'
     own keys are streamed, and the partial results are joined in a second launch.  Page ids are trusted, as those of
     ``lowering.attention`` are.  ``choice`` overrides the rules of the work split: ``{"prefix": "tiles" | "stream", "splits": n,
-    "target": n, "least": n}``."""
+    "target_log2": n, "least": n}``."""
     key = None if choice else lowering._call_key("shared", (q, k_pool, v_pool, out), (table, lengths, prefix_table, v_table, prefix_v_table),
                                                  plan, (prefix_len,))
     kept = lowering._kept.get(key)
@@ -277,44 +277,38 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     P.room = table.shape[1] * page
     P.Sk = prefix_len
     coop = lowering._decode_coop_waves(3, page, 0, 0, Hkv, P, D)
+    rows = B * group
+    # direct-to-LDS loads of whole rows from a page at a time, a page's bytes within 32-bit offsets
+    tiles = prefix_len > 0 and page % 8 == 0 and P.k_ss >= 0 and P.v_ss >= 0 and page * max(P.k_ss, P.v_ss) < 1 << 30 and \
+        choice.get("prefix", "tiles" if rows > lowering.DECODE_QROWS else "stream") == "tiles"
+    if tiles and coop:
+        coop = 4 if 4 * D >= 512 else 0         # both parts of the launch have 4 waves
     chunks = -(-group // lowering.DECODE_QROWS)
     heads = Hkv // coop if coop else Hkv
     P.units = heads * chunks
-    P.target, P.least = choice.get("target", 256 if coop else 512), choice.get("least", 160 if coop else 512)
-    items = P.target // P.units + B if P.room else 0
-    splits, rows, pre_grid = 0, B * group, None
-    tiles = False
-    P.nsplit = 1
+    P.target_log2, P.least = choice.get("target_log2", 8 if coop == 8 else 9), choice.get("least", 64)
+    items = (1 << P.target_log2) // P.units + B if P.room else 0
+    splits = 0
+    P.nsplit = P.pre_units = 1
     if prefix_len:
-        # direct-to-LDS loads of whole rows from a page at a time, a page's bytes within 32-bit offsets
-        tiles = page % 8 == 0 and page * max(P.k_ss, P.v_ss) < 1 << 30 and P.k_ss >= 0 and P.v_ss >= 0
         if tiles:
-            tiles = choice.get("prefix", "tiles" if rows > lowering.DECODE_QROWS else "stream") == "tiles"
-        if tiles:
-            units, keys = Hkv * -(-rows // 128), -(-prefix_len // 64)
-            splits = max(1, min(64, keys // 2, choice.get("splits", -(-512 // units))))
+            P.pre_units, keys = Hkv * -(-rows // 128), -(-prefix_len // 64)
+            splits = max(1, min(64, keys, choice.get("splits", min(keys // 8, 256 // P.pre_units))))
             P.split_len = 64 * -(-keys // splits)
             splits = -(-prefix_len // P.split_len)
-            pre_grid = (units * splits, 1, 1)
             P.k_span = P.v_span = 1
         else:
-            units = heads * -(-rows // lowering.DECODE_QROWS)
-            splits = max(1, min(64, prefix_len // 160, choice.get("splits", 512 // units)))
+            P.pre_units = heads * -(-rows // lowering.DECODE_QROWS)
+            splits = max(1, min(64, prefix_len // 32, choice.get("splits", 512 // P.pre_units)))
             splits, P.split_len = lowering._split_lengths(splits, prefix_len)
-            pre_grid = (units, splits, 1)
-        P.nsplit = splits
+        P.nsplit, P.pre_blocks = splits, splits * P.pre_units
     own, pre = items * Hq, splits * B * Hq            # rows of partial results
     args = dict(rows=lowering.DECODE_QROWS, waves=coop or 4, headwave=coop > 0, coop=coop > 0,
                 rowload=not coop and lowering._decode_rowload(3, page, 0, 0))
-    make = lambda which: lowering._spec("decode", lowering._DTYPE_CODE[dtype], D, lowering.MASK_NONE, softcap is not None, 3, page,
-                                        table.dtype == torch.int64, shared=which, **args)
-    steps = []
-    if splits:
-        spec = lowering._spec("prefill_swp", lowering._DTYPE_CODE[dtype], D, lowering.MASK_NONE, softcap is not None, 3, page,
-                              table.dtype == torch.int64, shared=2) if tiles else make(2)
-        steps.append((lowering.get_kernel(spec, spec.entry()), pre_grid, 256 if tiles else 64 * args["waves"]))
-    if items:
-        steps.append((lowering.get_kernel(make(1), "lf_attn_decode"), (items * P.units, 1, 1), 64 * args["waves"]))
+    steps, spec = [], lowering._spec("decode", lowering._DTYPE_CODE[dtype], D, lowering.MASK_NONE, softcap is not None, 3, page,
+                                     table.dtype == torch.int64, shared=2 if tiles else 1, **args)
+    if splits or items:
+        steps.append((lowering.get_kernel(spec, "lf_attn_decode"), (P.pre_blocks + items * P.units, 1, 1), 64 * args["waves"]))
     spec = lowering._spec("shared_combine", lowering._DTYPE_CODE[dtype], D)
     steps.append((lowering.get_kernel(spec, spec.entry()), (B * -(-Hq // (1024 // D)), 1, 1), 256))
     repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps], "prefix": "tiles" if tiles else "stream", "splits": splits},
