@@ -92,6 +92,22 @@ __device__ __forceinline__ int lf_bw_ds_row(int qb, int nkb, int window) {
   return qb * (before + 1) - (qb - before);
 #endif
 }
+#if LF_PACKED
+// Packed sequences: blocks of one in front of those of sequence `seq`, first row row0.  A row of blocks counts as one of the longest
+// sequence that T rows have room for, on the average over its rows (causal: half of it): nothing has to be summed over the sequences in
+// front, and sequences do not overlap, since those of n blocks of rows lie n and more of row0 / 32 + seq apart.
+__device__ __forceinline__ long long lf_bw_ds_before(int row0, int seq, int T, int window) {
+  const int n = (T + 31) / 32;
+#if LF_MASK == 0
+  const int per = n;
+#elif LF_MASK == 1
+  const int per = (n + 2) / 2;
+#else
+  const int per = (window + 30) / 32 + 1;
+#endif
+  return (long long)(row0 / 32 + seq) * per;
+}
+#endif
 // A block holds what the lanes of lf_attn_bwd_dkdv hold as the B operand of dK^T += Q^T dS, 16-byte chunks (half h of the 32
 // queries, lane half g, key) of 8 queries, permuted so that the transposed reads of lf_attn_bwd_dq (4 keys, all 16 queries
 // of both halves at a time) touch every LDS bank once: byte offset of lane (g, key)'s chunk of half 0; half 1 is (it ^ 128) + 1024.
@@ -411,6 +427,9 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
   p.dout += (long long)mine.row0 * p.do_ss;
   p.lse += mine.row0;
   p.delta += mine.row0;
+#if LF_BW_DS
+  p.ds += 1024 * lf_bw_ds_before(mine.row0, mine.seq, p.Sq, p.window);
+#endif
   p.Sq = p.Sk = mine.len;
 #else
   const int nkt = (p.Sk + kKeys - 1) / kKeys;
@@ -928,7 +947,12 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
 // are plain ones and push K out of the L2), against 222 us of the kernel below, which forms dS again.  A step is 64 keys: the
 // K tile, and every wave's own two blocks of dS, 4 KB in a row of memory; three LDS stages, one barrier.  Steps of 32 keys in
 // 3 ... 6 stages: 143 ... 148 us.
+#if LF_PACKED
+extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_attn_bwd_dq(const LfPackedBwdParams pk) {
+  LfAttnBwdParams p = pk;
+#else
 extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_attn_bwd_dq(const LfAttnBwdParams p) {
+#endif
   constexpr int kBM = LF_BW_DQ_NT / 2, kWaves = LF_BW_DQ_NT / 64, kS = 3;
   __shared__ __attribute__((aligned(256))) lf_elem k_tiles[kS][64 * LF_D];
   __shared__ __attribute__((aligned(256))) lf_elem ds_tiles[kS][kWaves][2 * 1024];
@@ -939,6 +963,21 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   const int l32 = lane & 31;
   const int g = lane >> 5;
 
+#if LF_PACKED
+  const int entry = (int)blockIdx.x / p.Hq, head = (int)blockIdx.x - entry * p.Hq, b = 0;
+  const int hkv = head % p.Hkv, h = hkv * (p.Hq / p.Hkv) + head / p.Hkv;
+  const LfPackedTile mine = lf_packed_tile(pk.dq_tiles, entry);
+  if (mine.len == 0) return;
+  p.dq += (long long)mine.row0 * p.dq_ss;
+  if (mine.seq < 0) {
+    lf_packed_clear<LF_BW_DQ_NT>(p.dq + h * p.dq_sh, 0, p.dq_ss, 1, mine.tile * kBM, kBM, mine.len);
+    return;
+  }
+  p.k += (long long)mine.row0 * p.k_ss;
+  p.ds += 1024 * lf_bw_ds_before(mine.row0, mine.seq, p.Sq, p.window);
+  p.Sq = p.Sk = mine.len;
+  const int qt = (p.Sq + kBM - 1) / kBM - 1 - mine.tile;
+#else
   const int nqt = (p.Sq + kBM - 1) / kBM;
   const int group = p.Hq / p.Hkv;
   int bhkv, row;
@@ -947,6 +986,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   const int hkv = bhkv % p.Hkv;
   const int b = bhkv / p.Hkv;
   const int h = hkv * group + row % group;
+#endif
   const int q0 = kBM * qt;
   const int wq0 = q0 + 32 * wave;                    // first row of this wave
 
@@ -1099,8 +1139,8 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   // As in lf_attn_bwd_dkdv: the q tiles of all query heads of a (batch, kv head) share its K / V tiles in one
   // XCD's L2, the long q tiles first.
 #if LF_PACKED
-  const int entry = (int)blockIdx.x / p.Hq, unit = (int)blockIdx.x - entry * p.Hq, b = 0;
-  const int hkv = unit % p.Hkv, h = hkv * (p.Hq / p.Hkv) + unit / p.Hkv;
+  const int entry = (int)blockIdx.x / p.Hq, head = (int)blockIdx.x - entry * p.Hq, b = 0;
+  const int hkv = head % p.Hkv, h = hkv * (p.Hq / p.Hkv) + head / p.Hkv;
   const LfPackedTile mine = lf_packed_tile(pk.dq_tiles, entry);
   if (mine.len == 0) return;
   p.dq += (long long)mine.row0 * p.dq_ss;

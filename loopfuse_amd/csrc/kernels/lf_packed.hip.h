@@ -5,7 +5,9 @@
 // number of rows and of sequences, not the lengths, and launches a workgroup per head and entry that the list can have.  A kernel takes its
 // tile's sequence for the whole problem: B = 1, Sq = Sk = its length, pointers at its first row.
 //   Workgroup -> (entry, head): the heads of an entry are neighbours, so that with a multiple of 8 of them each XCD walks
-// its own heads over the entries in their order, and the tiles of a (sequence, head) share its K / V (or Q / dO) in one L2.
+// its own heads over the entries in their order, and the tiles of a (sequence, head) share its K / V (or Q / dO) in one L2.  A list is
+// ordered by the tiles' work within groups of sequences; launches take the list whose groups make 64 (lf_attn_bwd: 32) (sequence, head) pairs, 8
+// (4) for each XCD, as the dense kernels' slots do.
 #ifndef LF_PACKED_HIP_H
 #define LF_PACKED_HIP_H
 

@@ -1,28 +1,31 @@
-// lf_packed_plan.hip — the tile lists of a packed batch (lf_packed.hip.h) from its offsets.
+// lf_packed_plan.hip — the tile lists of a packed batch (lf_packed.hip.h) from its offsets, in two launches.
 //
-// Four lists, for tiles of 32, 64, 128 and 256 rows.  Sequences come in the order of their lengths, the longest first
-// (equal ones in their own order), the tiles of one together: workgroups are dispatched in this order, so that the long ones
-// do not come last.  Behind them the rows of no sequence (in front of the first offset, behind the last one), then empty entries.
-//   Place of a sequence's first tile = tiles of the sequences in front of it in that order: every thread forms that sum for its own
-// sequence by looking at all N lengths, 256 at a time through LDS.  N^2 / 256 steps per block, of which there are N / 256 per list:
-// no sort, no scan across blocks, one launch.
+// Lists for tiles of 32, 64, 128 and 256 rows (dispatch order = list order).  Sequences are sorted by length, the longest first (equal ones
+// in their own order), and taken in groups of neighbours of 1, 2, 4 or 8, a list for each: in a group the tiles come by their work under
+// a causal mask, the longest first, where tile t of a sequence of n tiles counts n - t (the kernels number them so).  One group for all would
+// balance best and share the least in L2, groups of one the other way round; who launches knows how many heads an XCD has at a time.  Behind
+// the sequences come the rows of no sequence (in front of the first offset, behind the last one), then empty entries.
+//   lf_packed_sort: the rank of a sequence and the tiles in front of it, each a sum over all sequences that every thread forms for its own one:
+// N^2 / 256 steps per block, N / 256 blocks, no scan across them.
+//   lf_packed_plan: a wave per group; the place of tile t of the group's member g, with c = n_g - t, is the tiles in front of the group +
+// sum_j max(0, n_j - c) (longer ones) + g (of those that are as long, the members before it).
 // Whatever the offsets hold, tiles lie inside the T rows and places inside the list: offsets are clamped to 0 .. T, and what
 // overlapping sequences have too many of is left out.
 
+#define LF_PLAN_LISTS 4        /* tile heights */
+#define LF_PLAN_GROUPS 4       /* 1, 2, 4, 8 */
 struct LfPackedPlanParams {
   const int* offsets;          // [N + 1]
-  LfPackedTile* tiles;         // the four lists, one behind the other
+  LfPackedTile* tiles;         // lists [height][group size][cap[height]]
+  int* sorted;                 // [3 + LF_PLAN_LISTS][N + 2], of a rank: first row, rows, number of the sequence, tiles of each height in front of it
   int N, T;
-  int cap[4];                  // entries of each
+  int cap[LF_PLAN_LISTS];
 };
 
 #define LF_PLAN_NT 256
-extern "C" __global__ void __launch_bounds__(LF_PLAN_NT) lf_packed_plan(const LfPackedPlanParams p) {
-  __shared__ int s_len[LF_PLAN_NT], s_tiles[LF_PLAN_NT];
-  const int list = blockIdx.y, shift = 5 + list, up = (1 << shift) - 1;
-  LfPackedTile* out = p.tiles;
-  for (int i = 0; i < list; ++i) out += p.cap[i];
-  const int cap = p.cap[list];
+extern "C" __global__ void __launch_bounds__(LF_PLAN_NT) lf_packed_sort(const LfPackedPlanParams p) {
+  __shared__ int s_len[LF_PLAN_NT];
+  const int M = p.N + 2;
   auto at = [&](int n) { return min(max(p.offsets[n], 0), p.T); };
   // item n < N: a sequence; N: the rows behind the last; N + 1: those in front of the first
   const int n = blockIdx.x * LF_PLAN_NT + threadIdx.x;
@@ -36,33 +39,69 @@ extern "C" __global__ void __launch_bounds__(LF_PLAN_NT) lf_packed_plan(const Lf
   } else if (n == p.N + 1) {
     len = at(0);
   }
-  // places in front of this item, tiles of all sequences
-  long long first = 0;
+  int rank = 0;
+  long long first[LF_PLAN_LISTS] = {0, 0, 0, 0};
   for (int base = 0; base < p.N; base += LF_PLAN_NT) {
     const int j = base + threadIdx.x;
     const int l = j < p.N ? max(at(j + 1) - at(j), 0) : 0;
     __syncthreads();
     s_len[threadIdx.x] = l;
-    s_tiles[threadIdx.x] = (l + up) >> shift;
     __syncthreads();
     const int count = min(p.N - base, LF_PLAN_NT);
     for (int i = 0; i < count; ++i) {
       const int other = s_len[i];
-      if (n >= p.N || other > len || (other == len && base + i < n)) first += s_tiles[i];
+      if (n >= p.N || other > len || (other == len && base + i < n)) {
+        ++rank;
+#pragma unroll
+        for (int k = 0; k < LF_PLAN_LISTS; ++k) first[k] += (other + (32 << k) - 1) >> (5 + k);
+      }
     }
   }
-  if (n == p.N + 1) first += (p.T - at(p.N) + up) >> shift;
-  const int tiles = (len + up) >> shift;
-  const bool last = n == p.N + 1;
-  // entries are written by whole waves, one item after the other
-  const int lane = threadIdx.x & 63;
-  for (int i = 0; i < 64; ++i) {
-    const int item = __builtin_amdgcn_readlane(n, i);
-    if (item > p.N + 1) break;
-    const int f = __builtin_amdgcn_readlane((int)min(first, (long long)cap), i), c = __builtin_amdgcn_readlane(tiles, i);
-    const int r = __builtin_amdgcn_readlane(row0, i), l = __builtin_amdgcn_readlane(len, i);
-    for (int t = lane; t < c && f + t < cap; t += 64) out[f + t] = LfPackedTile{r, l, t, item < p.N ? item : -1};
-    if (__builtin_amdgcn_readlane((int)last, i))
-      for (int t = f + c + lane; t < cap; t += 64) out[t] = LfPackedTile{0, 0, 0, -1};
+  if (n == p.N + 1) {
+    ++rank;
+#pragma unroll
+    for (int k = 0; k < LF_PLAN_LISTS; ++k) first[k] += (p.T - at(p.N) + (32 << k) - 1) >> (5 + k);
+  }
+  if (n >= M) return;
+  p.sorted[rank] = row0;
+  p.sorted[M + rank] = len;
+  p.sorted[2 * M + rank] = n;
+#pragma unroll
+  for (int k = 0; k < LF_PLAN_LISTS; ++k) p.sorted[(3 + k) * M + rank] = (int)min(first[k], (long long)p.cap[k]);
+}
+
+// grid: (blocks of 4 groups, heights x group sizes)
+extern "C" __global__ void __launch_bounds__(LF_PLAN_NT) lf_packed_plan(const LfPackedPlanParams p) {
+  const int height = blockIdx.y / LF_PLAN_GROUPS, size = 1 << (blockIdx.y % LF_PLAN_GROUPS);
+  const int M = p.N + 2, shift = 5 + height, up = (1 << shift) - 1, cap = p.cap[height];
+  LfPackedTile* out = p.tiles;
+  for (int i = 0; i < height; ++i) out += (long long)LF_PLAN_GROUPS * p.cap[i];
+  out += (long long)(blockIdx.y % LF_PLAN_GROUPS) * cap;
+  const int lane = threadIdx.x & 63, wave = blockIdx.x * (LF_PLAN_NT / 64) + (threadIdx.x >> 6);
+  const int groups = (p.N + size - 1) / size;
+  const int* first = p.sorted + (3 + height) * M;
+  if (wave < groups) {
+    const int r0 = wave * size, members = min(size, p.N - r0), at = first[r0];
+    int n[1 << (LF_PLAN_GROUPS - 1)];
+#pragma unroll
+    for (int j = 0; j < 1 << (LF_PLAN_GROUPS - 1); ++j) n[j] = j < members ? (p.sorted[M + r0 + j] + up) >> shift : 0;
+#pragma unroll
+    for (int g = 0; g < 1 << (LF_PLAN_GROUPS - 1); ++g) {
+      if (g >= members) break;
+      const int row0 = p.sorted[r0 + g], len = p.sorted[M + r0 + g], seq = p.sorted[2 * M + r0 + g];
+      for (int t = lane; t < n[g]; t += 64) {
+        const int c = n[g] - t;
+        long long place = (long long)at + g;
+#pragma unroll
+        for (int j = 0; j < 1 << (LF_PLAN_GROUPS - 1); ++j) place += max(n[j] - c, 0);
+        if (place < cap) out[place] = LfPackedTile{row0, len, t, seq};
+      }
+    }
+  } else if (wave < groups + 2) {       // rows of no sequence; the second of the two also leaves the empty entries
+    const int r = p.N + wave - groups, row0 = p.sorted[r], len = p.sorted[M + r], at = first[r], n = (len + up) >> shift;
+    for (int t = lane; t < n; t += 64)
+      if ((long long)at + t < cap) out[at + t] = LfPackedTile{row0, len, t, -1};
+    if (wave == groups + 1)
+      for (long long t = (long long)at + n + lane; t < cap; t += 64) out[t] = LfPackedTile{0, 0, 0, -1};
   }
 }

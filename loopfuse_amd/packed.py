@@ -23,13 +23,15 @@ import torch
 from . import lowering, runtime
 from .lowering import AttnPlan, UnsupportedPlan
 
-TILE_HEIGHTS = (32, 64, 128, 256)      # rows of a tile, list by list
+TILE_HEIGHTS = (32, 64, 128, 256)      # rows of a tile, lists by lists
+GROUP_SIZES = (1, 2, 4, 8)             # sequences whose tiles come together, list by list
 
 
 class _PlanParams(ctypes.Structure):
     """Mirror of ``struct LfPackedPlanParams`` in csrc/kernels/lf_packed_plan.hip."""
 
-    _fields_ = [("offsets", ctypes.c_void_p), ("tiles", ctypes.c_void_p), ("N", ctypes.c_int), ("T", ctypes.c_int), ("cap", ctypes.c_int * 4)]
+    _fields_ = [("offsets", ctypes.c_void_p), ("tiles", ctypes.c_void_p), ("sorted", ctypes.c_void_p), ("N", ctypes.c_int), ("T", ctypes.c_int),
+                ("cap", ctypes.c_int * 4)]
 
 
 class PackedAttnParams(lowering.AttnParams):
@@ -57,16 +59,16 @@ class PackedLayout:
     def count(self) -> int:
         return self.offsets.shape[0] - 1
 
-    def tiles_of(self, rows: int) -> tuple:
-        """(first byte in ``tiles``, entries) of the list of tiles of so many rows."""
-        i = TILE_HEIGHTS.index(rows)
-        return 16 * sum(self.caps[:i]), self.caps[i]
+    def tiles_of(self, rows: int, units: int) -> tuple:
+        """(first byte in ``tiles``, entries) of the list of tiles of so many rows in groups of about ``units`` sequences."""
+        i, g = TILE_HEIGHTS.index(rows), max(j for j, n in enumerate(GROUP_SIZES) if n <= max(1, units))
+        return 16 * (len(GROUP_SIZES) * sum(self.caps[:i]) + g * self.caps[i]), self.caps[i]
 
 
 def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
     """The layout of a batch of ``N`` packed sequences: sequence ``n`` is rows ``offsets[n] ... offsets[n + 1]`` of tensors of
     ``total`` rows.  ``offsets``: int32 or int64 ``[N + 1]`` on the GPU, not descending (as a cumulative sum of the lengths is); sequences may be
-    empty.  One launch on the current stream, nothing waits for it; the layout serves every call over this batch, forward and
+    empty.  Two launches on the current stream, nothing waits for them; the layout serves every call over this batch, forward and
     backward, on that stream or on one that waits for it.  Offsets beyond ``0 ... total`` count as the nearer bound."""
     if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype not in (torch.int32, torch.int64):
         raise UnsupportedPlan("offsets must be an int32 or int64 tensor of one more than the number of sequences")
@@ -80,10 +82,12 @@ def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
         count = offsets.shape[0] - 1
         # a sequence ends with a tile that is not full; so do the rows of no sequence at either end
         caps = tuple(total // rows + count + 2 for rows in TILE_HEIGHTS)
-        tiles = torch.empty((sum(caps), 4), dtype=torch.int32, device=offsets.device)
-        P = _PlanParams(offsets.data_ptr(), tiles.data_ptr(), count, total, caps)
+        made = torch.empty(4 * len(GROUP_SIZES) * sum(caps) + (3 + len(caps)) * (count + 2), dtype=torch.int32, device=offsets.device)
+        tiles = made[:4 * len(GROUP_SIZES) * sum(caps)].view(-1, 4)
+        P = _PlanParams(offsets.data_ptr(), tiles.data_ptr(), tiles.data_ptr() + 16 * tiles.shape[0], count, total, caps)
         spec = lowering._spec("packed_plan", 0, 64)
-        lowering.get_kernel(spec, spec.entry()).launch((-(-(count + 2) // 256), len(TILE_HEIGHTS), 1), (256, 1, 1), P)
+        runtime.LaunchList([(lowering.get_kernel(spec, "lf_packed_sort"), (-(-(count + 2) // 256), 1, 1), 256),
+                            (lowering.get_kernel(spec, "lf_packed_plan"), (-(-(count + 2) // 4), len(caps) * len(GROUP_SIZES), 1), 256)]).launch(P)
     return PackedLayout(offsets, total, tiles, caps)
 
 
@@ -97,7 +101,7 @@ def _rows(name: str, t: torch.Tensor, layout: PackedLayout, dtype, D: Optional[i
         raise RuntimeError(f"loopfuse_amd: {name} is on {t.device}, the layout on {layout.tiles.device}")
 
 
-def _constants(plan: AttnPlan) -> tuple:
+def _constants(plan: AttnPlan, total: int) -> tuple:
     """(mask, window, scale, softcap or None) of a plan that the packed kernels serve."""
     if plan.k_paged or plan.v_paged or plan.denom_add != 0.0:
         raise UnsupportedPlan("packed sequences go with dense K/V and the plain softmax denominator")
@@ -113,8 +117,8 @@ def _constants(plan: AttnPlan) -> tuple:
         cap = abs(float(plan.softcap))
         if not (cap > 0.0) or not math.isfinite(cap):
             raise UnsupportedPlan("softcap must be finite and non-zero")
-    # a window beyond the rows keeps what a causal mask keeps; the kernels add it to positions in 32 bits
-    return mask, min(int(plan.window), 1 << 30) if mask == lowering.MASK_SLIDING else 0, float(plan.scale), cap
+    # (a window beyond all rows keeps what one of their number keeps; the kernels add it to positions in 32 bits)
+    return mask, min(int(plan.window), max(total, 1)) if mask == lowering.MASK_SLIDING else 0, float(plan.scale), cap
 
 
 def _heads(q, k, v, layout) -> tuple:
@@ -186,7 +190,7 @@ def _forward_again(q, k, v, layout, out, lse, repeat):
 @lowering._on_device_of_first_argument
 def _forward_general(q, k, v, plan, layout, out, lse, key):
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
-    mask, window, scale, cap = _constants(plan)
+    mask, window, scale, cap = _constants(plan, layout.total)
     T = layout.total
     for name, t in (("K", k), ("V", v)):
         # direct-to-LDS loads address a sequence with 32-bit byte offsets, up to three tiles past its end
@@ -212,7 +216,7 @@ def _forward_general(q, k, v, plan, layout, out, lse, key):
     group = Hq // Hkv
     pack = 4 if group % 4 == 0 else 2 if group % 2 == 0 else 0
     bm, heads = 128 // (pack or 1), Hq // (pack or 1)
-    tiles_at, entries = layout.tiles_of(bm)
+    tiles_at, entries = layout.tiles_of(bm, 64 // heads)
     mean = T // max(1, layout.count)
     spec = lowering._spec("prefill_swp", lowering._DTYPE_CODE[dtype], D, mask, cap is not None, pack=pack, packed=True,
                           bn=lowering.prefill_kv_tile(D, 0, None, heads * (T // bm + layout.count // 2),
@@ -241,7 +245,8 @@ def _backward(q, k, v, o, lse, dout, plan, layout):
     key = lowering._call_key("packed bwd", (q, k, v, o, dout), (lse, layout.tiles), plan, (layout.total, layout.caps[-1]))
     kept = lowering._kept.get(key)
     if kept is not None:
-        return _backward_again(q, k, v, o, lse, dout, layout, kept)
+        res = _backward_again(q, k, v, o, lse, dout, layout, kept)
+        return _backward_general(q, k, v, o, lse, dout, plan, layout, None, False) if res is None else res
     return _backward_general(q, k, v, o, lse, dout, plan, layout, key)
 
 
@@ -254,15 +259,22 @@ def _backward_again(q, k, v, o, lse, dout, layout, repeat):
     P.dq, P.dk, P.dv, P.lse, P.delta = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), lse.data_ptr(), delta.data_ptr()
     at = layout.tiles.data_ptr()
     P.dkdv_tiles, P.dq_tiles = at + repeat.more[0], at + repeat.more[1]
+    if repeat.more[2]:
+        # last: it may take what room is left, which the results need and it does not
+        try:
+            ds = torch.empty(repeat.more[2], dtype=dtype, device=dev)
+        except torch.OutOfMemoryError:
+            return None
+        P.ds = ds.data_ptr()
     repeat.launches.launch(P)
     lowering._last_launch.set(repeat.record)
     return dq, dk, dv
 
 
 @lowering._on_device_of_first_argument
-def _backward_general(q, k, v, o, lse, dout, plan, layout, key):
+def _backward_general(q, k, v, o, lse, dout, plan, layout, key, room=True):
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
-    mask, window, scale, cap = _constants(plan)
+    mask, window, scale, cap = _constants(plan, layout.total)
     T, dev = layout.total, q.device
     for name, t in (("O", o), ("dO", dout)):
         _rows(name, t, layout, dtype, D)
@@ -291,24 +303,45 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, key):
     q_split = lowering.bwd_q_split(D, mask, count * Hkv, mean)
     if q_split:
         keys = 1
-    spec = bwd_spec(dtype, D, mask, cap is not None, keys, nt, q_split, lowering.bwd_grads_stay(2 * T * Hq * D))
-    dkdv_at, dkdv_entries = layout.tiles_of(64 if q_split else 128 * keys)
-    dq_at, dq_entries = layout.tiles_of(nt // 2)
+    blocks = ds_blocks(mask, window, T, layout.count)
+    keep_ds = room and bwd_keep_ds(D, cap is not None, Hq * blocks)
+    spec = bwd_spec(dtype, D, mask, cap is not None, keys, nt, q_split, lowering.bwd_grads_stay(2 * T * Hq * D), keep_ds)
+    P.ds_sh = blocks * lowering.BWD_DS_BLOCK
+    dkdv_at, dkdv_entries = layout.tiles_of(64 if q_split else 128 * keys, 32 // Hkv)
+    dq_at, dq_entries = layout.tiles_of(nt // 2, 32 // Hkv)
     steps = {"lf_attn_bwd_delta": (-(-Hq * T // 16), 256), "lf_attn_bwd_dkdv": (_grid(dkdv_entries, Hkv, 256), 256),
              "lf_attn_bwd_dq": (_grid(dq_entries, Hq, nt), nt)}
-    names = ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"] if nt == 256 else list(steps)
+    names = ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"] if nt == 256 and not keep_ds else list(steps)
     named = lowering._kernels_of(spec)
     launches = [(lowering.get_kernel(spec, name, named), (steps[name][0], 1, 1), steps[name][1]) for name in names]
-    repeat = lowering._Repeat(P, launches, {"kernels": names}, (dkdv_at, dq_at))
+    repeat = lowering._Repeat(P, launches, {"kernels": names}, (dkdv_at, dq_at, P.ds_sh * Hq if keep_ds else 0))
     res = _backward_again(q, k, v, o, lse, dout, layout, repeat)
+    if res is None:
+        return _backward_general(q, k, v, o, lse, dout, plan, layout, None, False)
     if key is not None:
         lowering._keep(key, repeat)
     return res
 
 
 def bwd_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool = False, key_blocks: int = 1, dq_threads: int = 512, q_split: bool = False,
-             stay: bool = False) -> lowering.KernelSpec:
-    return dataclasses.replace(lowering.bwd_spec(dtype, D, mask, softcap, key_blocks, dq_threads, False, q_split, stay), packed=True)
+             stay: bool = False, keep_ds: bool = False) -> lowering.KernelSpec:
+    return dataclasses.replace(lowering.bwd_spec(dtype, D, mask, softcap, key_blocks, dq_threads, keep_ds, q_split, stay), packed=True)
+
+
+def ds_blocks(mask: int, window: int, total: int, count: int) -> int:
+    """Blocks of dS of one head: those in front of a sequence that begins behind the last row (``lf_bw_ds_before`` in
+    csrc/kernels/lf_attn_bwd.hip); under a window the blocks in front of the first key that the last row's start leaves out."""
+    n = -(-total // 32)
+    per = n if mask == lowering.MASK_NONE else (n + 2) // 2 if mask == lowering.MASK_CAUSAL else (window + 30) // 32 + 1
+    return (total // 32 + count + 1) * per
+
+
+def bwd_keep_ds(D: int, softcap: bool, blocks: int) -> bool:
+    """Does dS stay in memory between the two product kernels (``lowering.bwd_keep_ds``)?  ``blocks`` = of dS in all that the rows have room
+    for, 2 KB each, as if they were one sequence; what the real ones need of them is touched.  Up to 9 GiB, a 32nd of the memory: 16 384 rows
+    of 32 heads under a causal mask.  All launches, us, recomputed / kept: D 128 causal, 8 sequences up to 2048, H32 487 / 454, 32/8 505 / 482, 40 up
+    to 300, 32/8 150 / 124, window 256 343 / 290, unmasked H16 186 / 170; D 64 with a softcap 98 / 83, without 104 / 103 and 304 / 324."""
+    return 2 * lowering.BWD_DS_BLOCK * blocks <= 9 << 30 and (D == 128 or softcap)
 
 
 class _Packed(torch.autograd.Function):
