@@ -38,12 +38,12 @@ __device__ __forceinline__ int lf_wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // row_bcast:31 into rows 2 and 3
   return x;
 }
-// length of a piece: whole pairs of 16-key steps
-__device__ __forceinline__ int lf_shared_split(const LfSharedParams& p) {
+// length of a piece: whole pairs of 16-key steps.  `mine` = lengths of the first 64 requests, one per lane (read once for all scans)
+__device__ __forceinline__ int lf_shared_split(const LfSharedParams& p, int mine) {
   const int lane = __lane_id();
   long long total = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int len = lf_shared_length(p, b0 + lane);
+    const int len = b0 ? lf_shared_length(p, b0 + lane) : mine;
     // (the sum of 64 lengths may not fit 32 bits: their halves do)
     total += (long long)__builtin_amdgcn_readlane(lf_wave_scan(len >> 16), 63) << 16;
     total += __builtin_amdgcn_readlane(lf_wave_scan(len & 0xffff), 63);
@@ -52,11 +52,11 @@ __device__ __forceinline__ int lf_shared_split(const LfSharedParams& p) {
   return max(p.least, (int)min((even + 32) & ~31ll, 1ll << 30));
 }
 // The request of piece `piece`, the piece's number among that request's and the request's keys; false: there is no such piece.
-__device__ __forceinline__ bool lf_shared_piece(const LfSharedParams& p, int split, int piece, int& b, int& number, int& keys) {
+__device__ __forceinline__ bool lf_shared_piece(const LfSharedParams& p, int mine, int split, int piece, int& b, int& number, int& keys) {
   const int lane = __lane_id();
   int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int len = lf_shared_length(p, b0 + lane), n = (len + split - 1) / split;
+    const int len = b0 ? lf_shared_length(p, b0 + lane) : mine, n = (len + split - 1) / split;
     const int upto = lf_wave_scan(n);            // pieces of requests b0 .. b0 + lane
     const unsigned long long past = __builtin_amdgcn_ballot_w64(before + upto > piece);
     if (past != 0ull) {
@@ -71,12 +71,14 @@ __device__ __forceinline__ bool lf_shared_piece(const LfSharedParams& p, int spl
   return false;
 }
 // First piece of request `b` and how many it has.
-__device__ __forceinline__ void lf_shared_pieces_of(const LfSharedParams& p, int split, int b, int& first, int& count) {
+__device__ __forceinline__ void lf_shared_pieces_of(const LfSharedParams& p, int mine, int split, int b, int& first, int& count) {
   const int lane = __lane_id();
-  first = 0;
-  for (int b0 = 0; b0 < b; b0 += 64)
-    first += __builtin_amdgcn_readlane(lf_wave_scan(b0 + lane < b ? (lf_shared_length(p, b0 + lane) + split - 1) / split : 0), 63);
-  count = (lf_shared_length(p, b) + split - 1) / split;
+  first = count = 0;
+  for (int b0 = 0; b0 <= b; b0 += 64) {
+    const int n = ((b0 ? lf_shared_length(p, b0 + lane) : mine) + split - 1) / split;
+    first += __builtin_amdgcn_readlane(lf_wave_scan(b0 + lane < b ? n : 0), 63);
+    if (b - b0 < 64) count = __builtin_amdgcn_readlane(n, b - b0);
+  }
 }
 
 // What a workgroup of lf_attn_decode does: a split of the prefix for 16 rows of all requests, or a piece of one request's own keys.
@@ -99,9 +101,10 @@ __device__ __forceinline__ bool lf_shared_unit(const LfSharedParams& p, int bloc
   }
 #endif
   block -= p.pre_blocks;
-  const int split = lf_shared_split(p), piece = block / p.units;
+  const int mine = lf_shared_length(p, __lane_id());
+  const int split = lf_shared_split(p, mine), piece = block / p.units;
   int b, z, keys;
-  if (!lf_shared_piece(p, split, piece, b, z, keys)) return false;
+  if (!lf_shared_piece(p, mine, split, piece, b, z, keys)) return false;
   u = LfSharedUnit{false, __builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(z), piece, __builtin_amdgcn_readfirstlane(keys),
                    __builtin_amdgcn_readfirstlane(split), block - piece * p.units, p.rows, p.k_table, p.v_table};
   return true;

@@ -184,6 +184,36 @@ def _store(k, v, k_pool, v_pool, slots, repeat) -> None:
     lowering._last_launch.set(repeat.record)
 
 
+def own_loads(D: int, tiles: bool, keys: int) -> int:
+    """Heads whose waves load whole token rows of the own keys together (``-DLF_COOP=1``), where the pools allow it: 4 at head dimension 128;
+    at 64, 8, or none beside the prefix's tiles, whose workgroups have 4 waves (0: four waves share a head).  ``keys`` = that a call can have
+    in all: up to 4096 the shorter chain of the other form wins.  GPU time, us, 32/8 heads, 128, none / 4 / 8 together: 2 requests behind
+    1000 keys 10.3 / 11.4 / 15.3, 1 of 2000 keys 11.3 / 12.4 / 15.8, 1 of 500 behind 4096 17.6 / 14.2 / 17.6, 8 of 500 behind 2000 20.5 / 16.3 / 20.1,
+    8 up to 4000 27.2 / 20.4 / 23.4, 128 up to 2000 103 / 102 / 117; 64 up to 1024 behind 2048, on tiles, 50 / 39 / -."""
+    if D == 128:
+        return 4 if keys > 4096 else 0
+    return 0 if tiles or keys <= 4096 else 8
+
+
+def prefix_splits(units: int, keys: int, rows: int, own_bytes: int) -> int:
+    """Splits of a prefix on 128-row tiles: ``units`` workgroups per split, ``keys`` tiles of 64 keys, ``rows`` (request, head) pairs,
+    ``own_bytes`` of K and V that the own keys have room for.  A tile of a chain takes 2.4 us, a split costs its partials, 0.3 us and 0.25
+    per 1000 rows, and there is one workgroup per CU at most, since the own keys are streamed beside them; where those take longer, on half
+    of their room, than a chain of 8 tiles, finer splits only cost.  GPU time, us, by splits: 16 requests behind 1000 keys 2 21.7, 4 15.9,
+    8 14.1, 16 15.5; 32 behind 8000 8 36.8, 16 26.5, 32 25.1; 128 behind 2000 4 29.8, 8 28.8, 16 34.9; 64 up to 1024 behind 2048 2 47.4,
+    4 39.1, 8 43.5; 128 up to 300 behind 8208 4 67.6, 8 50.3, 16 57.8."""
+    most = max(1, 256 // units)
+    best = int(math.sqrt(keys * 2.4 / (0.3 + rows / 4000)) + 0.5)
+    if own_bytes / 2 > 100e6:
+        best = min(best, max(1, keys // 8))
+    return max(1, min(most, best))
+
+
+def combine_grid(B: int, Hq: int, D: int) -> int:
+    """Blocks of lf_shared_combine: 1024 / D rows of one request each, or one row whose parts the block's groups of threads share."""
+    return B * Hq if B * Hq <= 1024 else B * -(-Hq // (1024 // D))
+
+
 def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, plan: AttnPlan, table: torch.Tensor, lengths: torch.Tensor, *,
                      prefix_table: Optional[torch.Tensor] = None, prefix_len: int = 0, v_table: Optional[torch.Tensor] = None,
                      prefix_v_table: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -276,24 +306,24 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     P.scale, P.softcap = float(plan.scale), softcap or 0.0
     P.room = table.shape[1] * page
     P.Sk = prefix_len
-    coop = lowering._decode_coop_waves(3, page, 0, 0, Hkv, P, D)
     rows = B * group
     # direct-to-LDS loads of whole rows from a page at a time, a page's bytes within 32-bit offsets
     tiles = prefix_len > 0 and page % 8 == 0 and P.k_ss >= 0 and P.v_ss >= 0 and page * max(P.k_ss, P.v_ss) < 1 << 30 and \
         choice.get("prefix", "tiles" if rows > lowering.DECODE_QROWS else "stream") == "tiles"
-    if tiles and coop:
-        coop = 4 if 4 * D >= 512 else 0         # both parts of the launch have 4 waves
+    coop = lowering._decode_coop_waves(3, page, 0, 0, Hkv, P, D)
+    if coop:
+        coop = choice.get("coop", own_loads(D, tiles, prefix_len + B * P.room))
     chunks = -(-group // lowering.DECODE_QROWS)
     heads = Hkv // coop if coop else Hkv
     P.units = heads * chunks
-    P.target_log2, P.least = choice.get("target_log2", 8 if coop == 8 else 9), choice.get("least", 64)
+    P.target_log2, P.least = choice.get("target_log2", 10 if B * P.room >= 100_000 else 9), choice.get("least", 128)
     items = (1 << P.target_log2) // P.units + B if P.room else 0
     splits = 0
     P.nsplit = P.pre_units = 1
     if prefix_len:
         if tiles:
             P.pre_units, keys = Hkv * -(-rows // 128), -(-prefix_len // 64)
-            splits = max(1, min(64, keys, choice.get("splits", min(keys // 8, 256 // P.pre_units))))
+            splits = max(1, min(64, keys, choice.get("splits", prefix_splits(P.pre_units, keys, B * Hq, 4 * B * P.room * Hkv * D))))
             P.split_len = 64 * -(-keys // splits)
             splits = -(-prefix_len // P.split_len)
             P.k_span = P.v_span = 1
@@ -310,7 +340,7 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     if splits or items:
         steps.append((lowering.get_kernel(spec, "lf_attn_decode"), (P.pre_blocks + items * P.units, 1, 1), 64 * args["waves"]))
     spec = lowering._spec("shared_combine", lowering._DTYPE_CODE[dtype], D)
-    steps.append((lowering.get_kernel(spec, spec.entry()), (B * -(-Hq // (1024 // D)), 1, 1), 256))
+    steps.append((lowering.get_kernel(spec, spec.entry()), (combine_grid(B, Hq, D), 1, 1), 256))
     repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps], "prefix": "tiles" if tiles else "stream", "splits": splits},
                               ((own + pre) * (D + 2), 4 * own * D, 4 * own * (D + 2), 4 * own * (D + 2) + 4 * pre * D))
     res = _again(q, k_pool, v_pool, table, lengths, prefix_table if prefix_len else None, v_table, prefix_v_table, out, repeat)
