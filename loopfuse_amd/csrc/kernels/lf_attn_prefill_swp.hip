@@ -117,10 +117,12 @@
 #endif
 #ifndef LF_PREFIX
 #define LF_PREFIX 0      /* 1: not a kernel but a part of lf_attn_decode -DLF_SHARED=1: a split of a prefix that all requests of a batch share,
-                            for 128 of their rows (lf_shared.hip.h); leaves partial results.  Pages may lie anywhere: a load's page
-                            is its buffer's base */
+                            for 128 of their rows (lf_shared.hip.h); leaves partial results.  The pools lie within 4 GiB (k_span, v_span)
+                            and every lane looks up its own row's page and adds it to its offset.  2: pages of a multiple of 8 tokens
+                            anywhere, a load's page is its buffer's base: the whole call, us, 1 / 2: 32 requests behind 8000
+                            keys 28.8 / 30.1, 128 up to 300 behind 8208 48.7 / 52.5, 1 of 500 behind 4096 14.1 / 14.7 */
 #endif
-#if LF_PREFIX && (LF_PAGED != 3 || LF_BIAS || LF_MASK || LF_GQAPACK || LF_PACKED)
+#if LF_PREFIX && (LF_PAGED != 3 || LF_PAGE_SIZE != LF_PAGE_SIZE_V || LF_BIAS || LF_MASK || LF_GQAPACK || LF_PACKED)
 #error "a shared prefix: K and V in pages, no mask, rows of all heads of a group"
 #endif
 #if LF_PACKED
@@ -218,6 +220,8 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
   // page id (as a byte offset of the page + this kv head) for the rows of this wave in
   // pass ps of tile kt; tiles / rows past Sk re-use the last page (their rows are zeroed)
 #if LF_PREFIX
+  constexpr bool kLanePages = LF_PREFIX == 1;
+  static_assert(kLanePages || LF_PAGE_SIZE % 8 == 0, "the rows of a load lie in one page");
   typedef long long lf_page_t;
 #else
   typedef unsigned lf_page_t;
@@ -227,6 +231,12 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     const lf_table_t* tab = reinterpret_cast<const lf_table_t*>(which ? p.v_table : p.k_table);
     const int psz = which ? LF_PAGE_SIZE_V : LF_PAGE_SIZE;
 #if LF_PREFIX
+    if (kLanePages) {          // of this lane's own row, its place in the page with it (rows past Sk: left out below)
+      const int mine = min(kt * LF_BN + (LF_NT / LF_CPR) * ps + srow, p.Sk - 1);
+      const unsigned page = (unsigned)tab[mine / psz], in = (unsigned)(mine % psz);
+      return which ? page * (unsigned)(p.v_sb * 2) + in * v_rowb + (unsigned)hkv * (unsigned)(p.v_sh * 2)
+                   : page * (unsigned)(p.k_sb * 2) + in * k_rowb + (unsigned)hkv * (unsigned)(p.k_sh * 2);
+    }
     const long long page = tab[tok / psz];
     return 2 * (which ? page * p.v_sb + hkv * p.v_sh : page * p.k_sb + hkv * p.k_sh);
 #else
@@ -238,6 +248,7 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
   // the buffer of a load from page `pg` and what of `pg` is left for its offset
   auto of_page = [&](const lf_u32x4& rs, const lf_elem* base, lf_page_t& pg) {
 #if LF_PREFIX
+    if (kLanePages) return rs;
     lf_u32x4 r = lf_make_buffer(reinterpret_cast<const char*>(base) + pg, 0xfffffff0u);
     r[2] = rs[2] == 0u ? 0u : r[2];
     pg = 0;
@@ -263,7 +274,11 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     const lf_u32x4 buf = of_page(rs, p.k, pg);
     if (kPagedK) {
       const int tokw = kt * LF_BN + kRowsPerPass * ps + kRowsPerWave * wave_u;     // first row of this wave's load
+#if LF_PREFIX
+      off = (unsigned)pg + (kLanePages ? 16u * (unsigned)lf_k_phys(srow, sch) : (unsigned)(tokw % LF_PAGE_SIZE) * k_rowb + k_doff);
+#else
       off = (unsigned)pg + (unsigned)(tokw % LF_PAGE_SIZE) * k_rowb + k_doff;
+#endif
       if (tokw + (int)(srow % kRowsPerWave) >= p.Sk) off = 0xffffffffu;
     } else {
       off = k_doff + (unsigned)(kt * LF_BN + kRowsPerPass * ps) * k_rowb;
@@ -275,7 +290,11 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     const lf_u32x4 buf = of_page(rs, p.v, pg);
     if (kPagedV) {
       const int tokw = kt * LF_BN + kRowsPerPass * ps + kRowsPerWave * wave_u;
+#if LF_PREFIX
+      off = (unsigned)pg + (kLanePages ? 16u * (unsigned)lf_v_phys(srow, sch) : (unsigned)(tokw % LF_PAGE_SIZE_V) * v_rowb + v_doff);
+#else
       off = (unsigned)pg + (unsigned)(tokw % LF_PAGE_SIZE_V) * v_rowb + v_doff;
+#endif
       if (tokw + (int)(srow % kRowsPerWave) >= p.Sk) off = 0xffffffffu;
     } else {
       off = v_doff + (unsigned)(kt * LF_BN + kRowsPerPass * ps) * v_rowb;

@@ -98,7 +98,7 @@ class KernelSpec:
     extra: tuple = ()      # further -D options (tuning experiments)
     stay: bool = False     # prefill_swp, bwd: results by plain stores (prefill_out_stays, bwd_grads_stay)
     packed: bool = False   # prefill_swp, bwd: the tiles of sequences of different lengths in one tensor (lf_packed.hip.h)
-    shared: int = 0        # decode: 1 requests of different lengths and the prefix they share (lf_shared.hip.h), 2 with the prefix on 128-row tiles
+    shared: int = 0        # decode: 1 requests of different lengths and the prefix they share (lf_shared.hip.h), 2 with the prefix on 128-row tiles, 3 in pools beyond 4 GiB
 
     def __hash__(self):    # formed once: a call looks its kernels up by it, several times
         h = self.__dict__.get("_hash")
@@ -131,7 +131,7 @@ class KernelSpec:
             if self.bias:
                 o += ["-DLF_BIAS=1"]
             if self.shared:
-                o += ["-DLF_SHARED=1"] + (["-DLF_PREFIX=1"] if self.shared == 2 else [])
+                o += ["-DLF_SHARED=1"] + ([f"-DLF_PREFIX={self.shared - 1}"] if self.shared > 1 else [])
         elif self.family == "prefill":
             o += [f"-DLF_V_TR={int(self.v_tr)}", f"-DLF_BIAS={self.bias}", f"-DLF_DENOM={int(self.denom)}"]
             if self.d2:
@@ -158,7 +158,7 @@ class KernelSpec:
                   "shared_combine": "lf_shared_combine.hip", "paged_tables": "lf_paged_tables.hip", "store_kv": "lf_store_kv.hip"}[self.family]
         if self.family == "packed_plan":
             return ("lf_common.hip.h", "lf_packed.hip.h", kernel)
-        if self.shared == 2:
+        if self.shared > 1:
             return ("lf_common.hip.h", "lf_shared.hip.h", "lf_prefill_blocks.hip.h", "lf_attn_prefill_swp.hip", kernel)
         if self.shared or self.family == "shared_combine":
             return ("lf_common.hip.h", "lf_shared.hip.h", kernel)

@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import dataclasses
 import math
+import operator
 from typing import Optional
 
 import torch
@@ -74,7 +75,9 @@ def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
         raise UnsupportedPlan("offsets must be an int32 or int64 tensor of one more than the number of sequences")
     if not offsets.is_cuda:
         raise RuntimeError("loopfuse_amd: offsets are not on the GPU; the HIP path has no CPU fallback")
-    total = int(total)
+    if isinstance(total, torch.Tensor):
+        raise UnsupportedPlan("the number of rows must be a number of the host's")
+    total = operator.index(total)
     if total < 0 or total >= 1 << 31:
         raise UnsupportedPlan("the number of rows must be between 0 and 2**31 - 1")
     with torch.cuda.device(offsets.device):
@@ -299,7 +302,7 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, key, room=True):
     count = max(1, layout.count)
     mean = max(1, T // count)
     keys = lowering.bwd_key_blocks(D, mask, cap is not None, count * Hkv, mean)
-    nt = lowering.bwd_dq_threads(D, mask, cap is not None, count * Hq, mean, mean)
+    nt = bwd_dq_threads(D, mask, count * Hq * -(-mean // 256))
     q_split = lowering.bwd_q_split(D, mask, count * Hkv, mean)
     if q_split:
         keys = 1
@@ -326,6 +329,14 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, key, room=True):
 def bwd_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool = False, key_blocks: int = 1, dq_threads: int = 512, q_split: bool = False,
              stay: bool = False, keep_ds: bool = False) -> lowering.KernelSpec:
     return dataclasses.replace(lowering.bwd_spec(dtype, D, mask, softcap, key_blocks, dq_threads, keep_ds, q_split, stay), packed=True)
+
+
+def bwd_dq_threads(D: int, mask: int, tiles: int) -> int:
+    """Workgroup size of lf_attn_bwd_dq (``lowering.bwd_dq_threads``), ``tiles`` = of 256 queries in all heads: 512 threads at head dimension 128
+    once all CUs have work, else 256.  All backward launches, us, 512 / 256, recomputed and with dS kept: D 128 causal, 8 sequences up to 2048,
+    H32 487 / 523 and 454 / 458, 32/8 505 / 558 and 489 / 482, window 256 343 / 378 and 290 / 299; D 64 24 up to 1000, 16/4 113 / 104, 3 up to 4001 320 / 304,
+    with a softcap 110 / 98 and 85 / 83."""
+    return 512 if D == 128 and tiles > (256 if mask == lowering.MASK_CAUSAL else 128) else 256
 
 
 def ds_blocks(mask: int, window: int, total: int, count: int) -> int:

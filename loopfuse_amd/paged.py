@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from typing import NamedTuple, Optional
 
 import torch
@@ -66,6 +67,13 @@ def _on_gpu(name: str, t: torch.Tensor, dtypes, dim: int, device=None) -> None:
         raise RuntimeError(f"loopfuse_amd: {name} is on {t.device}, not on {device}")
 
 
+def _whole(name: str, n) -> int:
+    """A size that the host knows (a tensor would have to be waited for)."""
+    if isinstance(n, torch.Tensor):
+        raise UnsupportedPlan(f"{name} must be a number of the host's")
+    return operator.index(n)
+
+
 def _shift(page_size: int) -> int:
     if not isinstance(page_size, int) or page_size < 1 or page_size & (page_size - 1):
         raise UnsupportedPlan("page size must be a power of two")
@@ -96,7 +104,7 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
         raise UnsupportedPlan(f"new and table must be of {B} requests")
     if table.shape[1] and B and table.stride(1) != 1 or (B > 1 and table.stride(0) < table.shape[1]):
         raise UnsupportedPlan("rows of the table must be contiguous and apart")
-    shift, total = _shift(page_size), int(total)
+    shift, total = _shift(page_size), _whole("total", total)
     if total < 0 or total >= 1 << 31:
         raise UnsupportedPlan("the number of rows must be between 0 and 2**31 - 1")
     with torch.cuda.device(dev):
@@ -184,15 +192,24 @@ def _store(k, v, k_pool, v_pool, slots, repeat) -> None:
     lowering._last_launch.set(repeat.record)
 
 
-def own_loads(D: int, tiles: bool, keys: int) -> int:
+def own_loads(D: int, page: int, tiles: bool, keys: int) -> int:
     """Heads whose waves load whole token rows of the own keys together (``-DLF_COOP=1``), where the pools allow it: 4 at head dimension 128;
-    at 64, 8, or none beside the prefix's tiles, whose workgroups have 4 waves (0: four waves share a head).  ``keys`` = that a call can have
-    in all: up to 4096 the shorter chain of the other form wins.  GPU time, us, 32/8 heads, 128, none / 4 / 8 together: 2 requests behind
-    1000 keys 10.3 / 11.4 / 15.3, 1 of 2000 keys 11.3 / 12.4 / 15.8, 1 of 500 behind 4096 17.6 / 14.2 / 17.6, 8 of 500 behind 2000 20.5 / 16.3 / 20.1,
-    8 up to 4000 27.2 / 20.4 / 23.4, 128 up to 2000 103 / 102 / 117; 64 up to 1024 behind 2048, on tiles, 50 / 39 / -."""
+    8 at 64 for many keys in pages shorter than 16 tokens (0: four waves share a head).  ``keys`` = that a call can have in all, without a
+    prefix on ``tiles`` (whose workgroups have 4 waves): up to 4096 the shorter chain of the other form wins.  GPU time, us, 32/8 heads, 128, none / 4 / 8
+    together: 2 requests behind 1000 keys 10.3 / 11.4 / 14.5, 1 of 2000 keys 11.6 / 14.9 / 20.9, 1 of 500 behind 4096 18.2 / 16.9 / 22.6, 8 of 500 behind
+    2000, on tiles, 15.1 / 15.7 / -, 32 of 500 behind 500 28.0 / 17.3 / -, 8 up to 4000 30.7 / 25.3 / 23.6, 128 up to 2000 103 / 102 / 126, 64 up to 1024
+    behind 2048 53 / 39 / -; 64, pages of 16, none / 8: 16 up to 1000 13.4 / 14.9, 8 up to 4000 18.7 / 16.0, 128 up to 2000 63.9 / 72.3; of one token 13.0 /
+    14.6, 17.9 / 16.0, 84.1 / 67.8."""
     if D == 128:
         return 4 if keys > 4096 else 0
-    return 0 if tiles or keys <= 4096 else 8
+    return 8 if page < 16 and keys > 24_000 and not tiles else 0
+
+
+def prefix_on_tiles(rows: int, prefix_len: int) -> bool:
+    """Does a prefix run on tiles of 128 query rows (one read of it for so many), or as the own keys do, for 16?  ``rows`` = B * group.
+    GPU time, us, tiles / 16 rows: 8 rows behind 1000 keys 11.7 / 10.2, 4 behind 4096 13.9 / 17.2, 32 behind 2000 15.1 / 18.0, 64 behind 1000 14 /
+    16, 128 behind 500 17.3 / 24.0, behind 8000 27 / 60, 512 behind 2000 29 / 48."""
+    return rows > lowering.DECODE_QROWS or prefix_len >= 2048
 
 
 def prefix_splits(units: int, keys: int, rows: int, own_bytes: int) -> int:
@@ -229,13 +246,13 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     The prefix is read once for all requests together: its keys meet the rows of the whole batch as a matrix product, the requests'
     own keys are streamed, and the partial results are joined in a second launch.  Page ids are trusted, as those of
     ``lowering.attention`` are.  ``choice`` overrides the rules of the work split: ``{"prefix": "tiles" | "stream", "splits": n,
-    "target_log2": n, "least": n}``."""
+    "target_log2": n, "least": n, "coop": n, "near": bool}``."""
     key = None if choice else lowering._call_key("shared", (q, k_pool, v_pool, out), (table, lengths, prefix_table, v_table, prefix_v_table),
                                                  plan, (prefix_len,))
     kept = lowering._kept.get(key)
     if kept is not None:
         return _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_table, out, kept)
-    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, int(prefix_len), v_table, prefix_v_table, out, choice or {}, key)
+    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, _whole("prefix_len", prefix_len), v_table, prefix_v_table, out, choice or {}, key)
 
 
 @lowering._on_device_of_first_argument
@@ -275,7 +292,7 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     _on_gpu("V table", v_table, (table.dtype,), 2, q.device)
     if table.shape[0] != B or v_table.shape != table.shape or lengths.shape[0] != B:
         raise UnsupportedPlan(f"tables and lengths must be of {B} requests, the tables of one width")
-    if not isinstance(prefix_len, int) or prefix_len < 0 or prefix_len >= 1 << 31 or table.shape[1] * page >= 1 << 31:
+    if prefix_len < 0 or prefix_len >= 1 << 31 or table.shape[1] * page >= 1 << 31:
         raise UnsupportedPlan("more keys than positions in 32 bits")
     if prefix_len:
         if prefix_table is None:
@@ -307,12 +324,17 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     P.room = table.shape[1] * page
     P.Sk = prefix_len
     rows = B * group
-    # direct-to-LDS loads of whole rows from a page at a time, a page's bytes within 32-bit offsets
-    tiles = prefix_len > 0 and page % 8 == 0 and P.k_ss >= 0 and P.v_ss >= 0 and page * max(P.k_ss, P.v_ss) < 1 << 30 and \
-        choice.get("prefix", "tiles" if rows > lowering.DECODE_QROWS else "stream") == "tiles"
+    # direct-to-LDS loads with 32-bit offsets, in the pools or else in a page
+    spans = [sum((n - 1) * abs(st) for n, st in zip(t.shape, t.stride())) + 1 for t in (k_pool, v_pool)]
+    near = max(spans) < (1 << 31) - 64
+    tiles = prefix_len > 0 and all(st >= 0 for t in (k_pool, v_pool) for st in t.stride()) and \
+        (near or (page % 8 == 0 and page * max(P.k_ss, P.v_ss) < 1 << 30)) and \
+        choice.get("prefix", "tiles" if prefix_on_tiles(rows, prefix_len) else "stream") == "tiles"
+    if tiles and not choice.get("near", True) and page % 8 == 0:
+        near = False
     coop = lowering._decode_coop_waves(3, page, 0, 0, Hkv, P, D)
     if coop:
-        coop = choice.get("coop", own_loads(D, tiles, prefix_len + B * P.room))
+        coop = choice.get("coop", own_loads(D, page, tiles, B * P.room + (0 if tiles else prefix_len)))
     chunks = -(-group // lowering.DECODE_QROWS)
     heads = Hkv // coop if coop else Hkv
     P.units = heads * chunks
@@ -326,7 +348,7 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
             splits = max(1, min(64, keys, choice.get("splits", prefix_splits(P.pre_units, keys, B * Hq, 4 * B * P.room * Hkv * D))))
             P.split_len = 64 * -(-keys // splits)
             splits = -(-prefix_len // P.split_len)
-            P.k_span = P.v_span = 1
+            P.k_span, P.v_span = spans if near else (1, 1)
         else:
             P.pre_units = heads * -(-rows // lowering.DECODE_QROWS)
             splits = max(1, min(64, prefix_len // 32, choice.get("splits", 512 // P.pre_units)))
@@ -336,7 +358,7 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     args = dict(rows=lowering.DECODE_QROWS, waves=coop or 4, headwave=coop > 0, coop=coop > 0,
                 rowload=not coop and lowering._decode_rowload(3, page, 0, 0))
     steps, spec = [], lowering._spec("decode", lowering._DTYPE_CODE[dtype], D, lowering.MASK_NONE, softcap is not None, 3, page,
-                                     table.dtype == torch.int64, shared=2 if tiles else 1, **args)
+                                     table.dtype == torch.int64, shared=(2 if near else 3) if tiles else 1, **args)
     if splits or items:
         steps.append((lowering.get_kernel(spec, "lf_attn_decode"), (P.pre_blocks + items * P.units, 1, 1), 64 * args["waves"]))
     spec = lowering._spec("shared_combine", lowering._DTYPE_CODE[dtype], D)

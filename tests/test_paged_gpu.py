@@ -192,8 +192,8 @@ def test_attention_over_a_shared_prefix_is_the_formula(lengths, prefix, page, Hk
     plan = AttnPlan(scale=D ** -0.5, softcap=cap, k_paged=True, v_paged=True)
     out = paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=prefix)
     check(out, oracle(q, kp, vp, table, n, pre, prefix, D ** -0.5, cap))
-    if prefix and page % 8 == 0:       # the other form of the prefix, other splits and pieces
-        for choice in ({"prefix": "tiles", "splits": 3}, {"prefix": "stream", "splits": 2, "least": 32, "target_log2": 12}):
+    if prefix:       # the other form of the prefix, other splits and pieces
+        for choice in ({"prefix": "tiles", "splits": 3}, {"prefix": "tiles", "near": False}, {"prefix": "stream", "splits": 2, "least": 32, "target_log2": 12}):
             other = paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=prefix, choice=choice)
             check(other, oracle(q, kp, vp, table, n, pre, prefix, D ** -0.5, cap), str(choice))
     given = torch.full((len(lengths), 2 * Hkv * group, 1, D), 9.0, dtype=dtype, device=DEV)
