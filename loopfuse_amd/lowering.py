@@ -864,6 +864,21 @@ def _call_key(kind: str, data, ints, plan: Optional[AttnPlan], more: tuple):
     return (kind, device, fields, more, tuple(map(_VARIABLES.get, _SWITCHES)), tuple(operands))
 
 
+def outside_graphs(fn):
+    """An operator that a function under ``torch.compile`` calls as it is, between two graphs: there is nothing in it to trace."""
+    apart = torch.compiler.disable(fn)
+
+    @functools.wraps(fn)
+    def call(*args, **kw):
+        return apart(*args, **kw) if torch.compiler.is_compiling() else fn(*args, **kw)
+    return call
+
+
+def _checks_tables() -> bool:
+    """LOOPFUSE_CHECK_TABLES=1: index tensors are looked at before the launches (waits for the stream, which a capture forbids)."""
+    return _env("LOOPFUSE_CHECK_TABLES", "0") == "1" and not torch.cuda.is_current_stream_capturing()
+
+
 class _LastLaunch:
     """What the calling THREAD's last ``attention`` call launched (kernels, grid, block, tile
     shape): ``attention.last_launch["kernels"]``.  Each thread sees its own record."""

@@ -66,11 +66,13 @@ class PackedLayout:
         return 16 * (len(GROUP_SIZES) * sum(self.caps[:i]) + g * self.caps[i]), self.caps[i]
 
 
+@lowering.outside_graphs
 def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
     """The layout of a batch of ``N`` packed sequences: sequence ``n`` is rows ``offsets[n] ... offsets[n + 1]`` of tensors of
     ``total`` rows.  ``offsets``: int32 or int64 ``[N + 1]`` on the GPU, not descending (as a cumulative sum of the lengths is); sequences may be
     empty.  Two launches on the current stream, nothing waits for them; the layout serves every call over this batch, forward and
-    backward, on that stream or on one that waits for it.  Offsets beyond ``0 ... total`` count as the nearer bound."""
+    backward, on that stream or on one that waits for it.  Offsets beyond ``0 ... total`` count as the nearer bound
+    (``LOOPFUSE_CHECK_TABLES=1`` raises for them and for descending ones)."""
     if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype not in (torch.int32, torch.int64):
         raise UnsupportedPlan("offsets must be an int32 or int64 tensor of one more than the number of sequences")
     if not offsets.is_cuda:
@@ -81,8 +83,12 @@ def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
     if total < 0 or total >= 1 << 31:
         raise UnsupportedPlan("the number of rows must be between 0 and 2**31 - 1")
     with torch.cuda.device(offsets.device):
-        offsets = offsets.clamp(0, total).to(torch.int32) if offsets.dtype == torch.int64 else offsets.contiguous()
         count = offsets.shape[0] - 1
+        if lowering._checks_tables():
+            ends = offsets.tolist()
+            if any(a > b for a, b in zip(ends, ends[1:])) or ends[0] < 0 or ends[-1] > total:
+                raise ValueError(f"loopfuse_amd: offsets must not descend, within 0 ... {total}")
+        offsets = offsets.clamp(0, total).to(torch.int32) if offsets.dtype == torch.int64 else offsets.contiguous()
         # a sequence ends with a tile that is not full; so do the rows of no sequence at either end
         caps = tuple(total // rows + count + 2 for rows in TILE_HEIGHTS)
         made = torch.empty(4 * len(GROUP_SIZES) * sum(caps) + (3 + len(caps)) * (count + 2), dtype=torch.int32, device=offsets.device)
@@ -145,6 +151,7 @@ def _grid(entries: int, heads: int, threads: int) -> int:
     return entries * heads
 
 
+@lowering.outside_graphs
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttnPlan, layout: PackedLayout, *,
                      out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of every packed sequence over itself: q ``[rows, Hq, D]``, k and v ``[rows, Hkv, D]`` (views will do: rows of a
@@ -152,6 +159,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
     ``plan``: mask, window, scale and softcap.  Rows of no sequence, in front of the first offset or behind the last,
     come out as zeros, or stay as they are in an ``out`` that is given.  ``lse``: float32 ``[Hq, rows]``, contiguous, to be given the
     rows' log-sum-exp in log2 units, as ``lowering.attention`` does.
+
+    Inside ``torch.compile`` the call runs as it is, between two graphs.
 
     Differentiable where gradients are recorded and neither ``out`` nor ``lse`` is given; gradients of rows of no sequence are zero."""
     if not isinstance(layout, PackedLayout):
@@ -234,6 +243,7 @@ def _forward_general(q, k, v, plan, layout, out, lse, key):
     return out
 
 
+@lowering.outside_graphs
 def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, dout: torch.Tensor,
                               plan: AttnPlan, layout: PackedLayout):
     """Gradients of ``attention_packed(q, k, v, plan, layout)``: ``(dq, dk, dv)`` in the operands' dtype, zeros in rows of no

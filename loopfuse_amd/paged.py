@@ -80,6 +80,7 @@ def _shift(page_size: int) -> int:
     return page_size.bit_length() - 1
 
 
+@lowering.outside_graphs
 def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, page_size: int, total: int) -> PagedStep:
     """Pages for the new tokens of a batch, and the slot of each of them, from lengths on the GPU.
 
@@ -108,6 +109,8 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
     if total < 0 or total >= 1 << 31:
         raise UnsupportedPlan("the number of rows must be between 0 and 2**31 - 1")
     with torch.cuda.device(dev):
+        if lowering._checks_tables():
+            _check_extension(cached, new, table, free, page_size, total)
         packed = [t if t.is_contiguous() else t.contiguous() for t in (cached, new, free)]
         P = _TablesParams(table_stride=table.stride(0), B=B, width=table.shape[1], count=free.shape[0], T=total, shift=shift)
         spec = lowering._spec("paged_tables", 0, 64, table_i64=table.dtype == torch.int64)
@@ -119,6 +122,14 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
     if key is not None and packed[0] is cached and packed[1] is new and packed[2] is free:
         lowering._keep(key, repeat)
     return step
+
+
+def _check_extension(cached, new, table, free, page_size, total) -> None:
+    c, n = cached.clamp(min=0).long(), new.clamp(min=0).long()
+    pages = (c + n + page_size - 1) // page_size
+    need, width, rows = int((pages - (c + page_size - 1) // page_size).sum()), int(pages.max()) if len(c) else 0, int(n.sum())
+    if need > free.shape[0] or width > table.shape[1] or rows > total:
+        raise ValueError(f"loopfuse_amd: {need} pages of {free.shape[0]} free ones, tables of {width} of {table.shape[1]} entries, {rows} of {total} rows")
 
 
 def _tables(cached, new, table, free, total, repeat) -> PagedStep:
@@ -146,6 +157,7 @@ def _pool(name: str, t: torch.Tensor) -> tuple:
     raise UnsupportedPlan(f"{name} pool must be [N, Hkv, D] or [N, P, Hkv, D]")
 
 
+@lowering.outside_graphs
 def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Tensor) -> None:
     """Write rows of new keys and values, k and v ``[rows, Hkv, D]``, into the page pools: row t into token ``slots[t] % page`` of page
     ``slots[t] // page``.  bf16 / fp16, D a multiple of 8; views will do.  ``slots``: int32 [rows] (``PagedStep.slots``); rows whose slot is below 0 or
@@ -175,6 +187,10 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     if T == 0 or pages == 0 or heads == 0 or D == 0:
         return
     with torch.cuda.device(k.device):
+        if lowering._checks_tables():
+            kept_slots = slots[slots >= 0]
+            if len(kept_slots) and (int(kept_slots.max()) >= pages * page or len(torch.unique(kept_slots)) < len(kept_slots)):
+                raise ValueError(f"loopfuse_amd: slots must be distinct and below {pages * page}")
         packed = slots.contiguous()
         P = _StoreParams(0, 0, 0, 0, 0, *(x // 8 for x in (*k.stride()[:2], *v.stride()[:2], *ks, *vs)), pages * page, T, heads, D // 8, shift)
         spec = lowering._spec("store_kv", 0, 64)
@@ -231,6 +247,7 @@ def combine_grid(B: int, Hq: int, D: int) -> int:
     return B * Hq if B * Hq <= 1024 else B * -(-Hq // (1024 // D))
 
 
+@lowering.outside_graphs
 def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, plan: AttnPlan, table: torch.Tensor, lengths: torch.Tensor, *,
                      prefix_table: Optional[torch.Tensor] = None, prefix_len: int = 0, v_table: Optional[torch.Tensor] = None,
                      prefix_v_table: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -245,7 +262,7 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
 
     The prefix is read once for all requests together: its keys meet the rows of the whole batch as a matrix product, the requests'
     own keys are streamed, and the partial results are joined in a second launch.  Page ids are trusted, as those of
-    ``lowering.attention`` are.  ``choice`` overrides the rules of the work split: ``{"prefix": "tiles" | "stream", "splits": n,
+    ``lowering.attention`` are (``LOOPFUSE_CHECK_TABLES=1`` looks at them).  ``choice`` overrides the rules of the work split: ``{"prefix": "tiles" | "stream", "splits": n,
     "target_log2": n, "least": n, "coop": n, "near": bool}``."""
     key = None if choice else lowering._call_key("shared", (q, k_pool, v_pool, out), (table, lengths, prefix_table, v_table, prefix_v_table),
                                                  plan, (prefix_len,))
@@ -312,6 +329,11 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
             raise UnsupportedPlan(f"O must be [{B}, {Hq}, 1, {D}] on the device of Q, every element with a place of its own")
     if B == 0:
         return torch.empty(q.shape, dtype=dtype, device=q.device) if out is None else out
+    if lowering._checks_tables():
+        used = torch.arange(table.shape[1], device=q.device) < ((lengths.clamp(min=0).long() + page - 1) // page)[:, None]
+        named = [table[used], v_table[used]] + ([t[:-(-prefix_len // page)] for t in (prefix_table, prefix_v_table)] if prefix_len else [])
+        if any(len(t) and (int(t.min()) < 0 or int(t.max()) >= pages) for t in named) or (B and int(lengths.max()) > table.shape[1] * page):
+            raise ValueError(f"loopfuse_amd: page ids outside 0 ... {pages - 1}, or a length beyond its row of the table")
     P = SharedParams()
     P.q_sb, P.q_sh, P.q_ss = q.stride(0), group * q.stride(1), q.stride(1)
     o_sb, o_sh = (Hq * D, D) if out is None else out.stride()[:2]
@@ -391,3 +413,4 @@ def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_ta
         repeat.launches.launch(P)
     lowering._last_launch.set(repeat.record)
     return out
+
