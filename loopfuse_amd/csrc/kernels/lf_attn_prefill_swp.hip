@@ -894,16 +894,29 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
     // d = 32*db + 8*(i/4) + 4*g + i%4.
     const float l_tot = l_run + lf_swap32(l_run);
 #if LF_PREFIX
-    // the row's partial result, as lf_attn_decode leaves it: offset and sum in log2 units, and sum of e V
-    if (my_q < p.Sq) {
-      const long long slot = ((long long)h * p.nsplit + part) * p.Sq + my_q;
+    // The rows' partial results, as lf_attn_decode leaves them: offset and sum in log2 units, and sums of e V.  These meet in the tiles' LDS
+    // (behind the last tile's barrier nobody reads it any more) and leave in whole rows.
+    {
+      constexpr int kStride = LF_D * 4 + 16, kSpace = (LF_KSLOTS + LF_VSLOTS) * LF_BN * LF_D * 2 / LF_NW;      // bytes per wave
+      static_assert(32 * kStride <= kSpace, "a wave's rows fit its part of the LDS");
+      const long long row0 = ((long long)h * p.nsplit + part) * p.Sq + wq0;
+      if (g == 0 && my_q < p.Sq) *reinterpret_cast<lf_f32x2*>(&sp.pre_ml[(row0 + l32) * 2]) = lf_f32x2{mc_ref, l_tot};
+      typedef __attribute__((address_space(3))) lf_f32x4* lf_lds_f32x4;
+      const unsigned mine = lds0 + (unsigned)(wave * kSpace);
 #pragma unroll
       for (int db = 0; db < LF_NDB; ++db)
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4)
-          *reinterpret_cast<lf_f32x4*>(&sp.pre_acc[slot * LF_D + 32 * db + 8 * i4 + 4 * g]) =
+          *(lf_lds_f32x4)(size_t)(mine + (unsigned)(l32 * kStride + 4 * (32 * db + 8 * i4 + 4 * g))) =
               lf_f32x4{o[db][4 * i4], o[db][4 * i4 + 1], o[db][4 * i4 + 2], o[db][4 * i4 + 3]};
-      if (g == 0) *reinterpret_cast<lf_f32x2*>(&sp.pre_ml[slot * 2]) = lf_f32x2{mc_ref, l_tot};
+      lf_wave_exchange();
+      constexpr int kLanes = LF_D / 4, kRows = 64 / kLanes;      // lanes per row, rows per store
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const int r = kRows * i + lane / kLanes, c = lane % kLanes;
+        const lf_f32x4 x = *(lf_lds_f32x4)(size_t)(mine + (unsigned)(r * kStride + 16 * c));
+        if (wq0 + r < p.Sq) *reinterpret_cast<lf_f32x4*>(&sp.pre_acc[(row0 + r) * LF_D + 4 * c]) = x;
+      }
     }
 #else
     // optional: the row's log-sum-exp of the scaled, masked scores in log2 units (what a

@@ -189,7 +189,7 @@ def _forward(q, k, v, plan, layout, out, lse):
 def _forward_again(q, k, v, layout, out, lse, repeat):
     P = PackedAttnParams.from_buffer_copy(repeat.block)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     P.q, P.k, P.v, P.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     if lse is not None:
         P.part_ml = lse.data_ptr()

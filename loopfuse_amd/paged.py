@@ -134,7 +134,7 @@ def _check_extension(cached, new, table, free, page_size, total) -> None:
 
 def _tables(cached, new, table, free, total, repeat) -> PagedStep:
     size, parts = repeat.more
-    made = torch.empty(size, dtype=torch.int32, device=table.device)
+    made = cached.new_empty(size)
     offsets, lengths, pages, slots, positions = made.split_with_sizes(parts)
     P = _TablesParams.from_buffer_copy(repeat.block)
     P.cached, P.fresh, P.table, P.free = cached.data_ptr(), new.data_ptr(), table.data_ptr(), free.data_ptr()
@@ -396,7 +396,7 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
 
 def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_table, out, repeat):
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     P = SharedParams.from_buffer_copy(repeat.block)
     P.q, P.k, P.v, P.o = q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr()
     P.k_table = table.data_ptr()
