@@ -365,21 +365,30 @@ def bwd_keep_ds(D: int, softcap: bool, blocks: int) -> bool:
     return 2 * lowering.BWD_DS_BLOCK * blocks <= 9 << 30 and (D == 128 or softcap)
 
 
+def _gradients(ctx, dout):
+    q, k, v, out, lse = ctx.saved_tensors
+    if dout.stride(-1) != 1 or dout.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(dout.shape[:-1], dout.stride()[:-1])):
+        dout = dout.contiguous()
+    return (*_backward(q, k, v, out, lse, dout, ctx.plan, ctx.layout), None, None)
+
+
+_gradients_once = torch.autograd.function.once_differentiable(_gradients)
+
+
 class _Packed(torch.autograd.Function):
-    """As the fused training graphs: gradients can be asked for with ``create_graph=True`` but not differentiated again."""
+    """As the fused training graphs: gradients can be asked for with ``create_graph=True`` but not differentiated again.  (Only then do
+    they go through the wrapper that says so, which costs 10 us.)"""
 
     @staticmethod
     def forward(ctx, q, k, v, plan, layout):
         lse = torch.empty((q.shape[1], layout.total), dtype=torch.float32, device=q.device)
         out = _forward(q, k, v, plan, layout, None, lse)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.plan, ctx.layout = dataclasses.replace(plan), layout      # (the caller may change a plan)
+        # (the caller may change a plan)
+        ctx.plan = AttnPlan(plan.mask, plan.window, plan.scale, plan.softcap, plan.k_paged, plan.v_paged, plan.denom_add)
+        ctx.layout = layout
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
-        if dout.stride(-1) != 1 or dout.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(dout.shape[:-1], dout.stride()[:-1])):
-            dout = dout.contiguous()
-        return (*_backward(q, k, v, out, lse, dout, ctx.plan, ctx.layout), None, None)
+        return (_gradients_once if torch.is_grad_enabled() else _gradients)(ctx, dout)

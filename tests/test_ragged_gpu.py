@@ -272,6 +272,21 @@ def test_gradients_are_differences():
         assert abs(dot - slope) <= 4 * 2.0 ** -11 * (grad.double().norm() * d.norm()).item()
 
 
+def test_gradients_are_not_differentiated_again():
+    q, k, v, g, layout = packed_args(9)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    plan = AttnPlan("causal", scale=0.1)
+    out = packed.attention_packed(*leaves, plan, layout)
+    plan.scale = 5.0                                    # the call's plan is the one it was given
+    grads = torch.autograd.grad(out, leaves, g, create_graph=True, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(grads, run_train((q, k, v, g, layout))[1:]))
+    with pytest.raises(RuntimeError):
+        grads[0].float().sum().backward()
+    grads = torch.autograd.grad(out, leaves, g.clone().requires_grad_(True), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grads[0].float().sum().backward()
+
+
 def test_other_head_dims_are_padded():
     q, k, v, g, layout = packed_args(3, (30, 40), 4, 2, 40)
     leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
