@@ -6,8 +6,7 @@
 // tile's sequence for the whole problem: B = 1, Sq = Sk = its length, pointers at its first row.
 //   Workgroup -> (entry, head): the heads of an entry are neighbours, so that with a multiple of 8 of them each XCD walks
 // its own heads over the entries in their order, and the tiles of a (sequence, head) share its K / V (or Q / dO) in one L2.  A list is
-// ordered by the tiles' work within groups of sequences; launches take the list whose groups make 64 (lf_attn_bwd: 32) (sequence, head) pairs, 8
-// (4) for each XCD, as the dense kernels' slots do.
+// ordered by the tiles' work within groups of sequences; which list a launch takes: packed.group_size.
 #ifndef LF_PACKED_HIP_H
 #define LF_PACKED_HIP_H
 

@@ -226,9 +226,9 @@ def _forward_general(q, k, v, plan, layout, out, lse, key):
     P.nsplit, P.rows = 1, 1
     P.clear = int(out is None)
     group = Hq // Hkv
-    pack = 4 if group % 4 == 0 else 2 if group % 2 == 0 else 0
+    pack = heads_per_workgroup(group)
     bm, heads = 128 // (pack or 1), Hq // (pack or 1)
-    tiles_at, entries = layout.tiles_of(bm, 64 // heads)
+    tiles_at, entries = layout.tiles_of(bm, group_size(mask, 64 // heads))
     mean = T // max(1, layout.count)
     spec = lowering._spec("prefill_swp", lowering._DTYPE_CODE[dtype], D, mask, cap is not None, pack=pack, packed=True,
                           bn=lowering.prefill_kv_tile(D, 0, None, heads * (T // bm + layout.count // 2),
@@ -241,6 +241,22 @@ def _forward_general(q, k, v, plan, layout, out, lse, key):
     if key is not None:
         lowering._keep(key, repeat)
     return out
+
+
+def group_size(mask: int, causal: int) -> int:
+    """Sequences whose tiles come together by their work: under a causal mask ``causal``, so that an XCD has 8 (sequence, head) pairs at a time,
+    under a window, where K and V of a tile are few, 8, and 1 without a mask, where all tiles of a sequence are alike.
+    Forward, us, 1 / 2 / 4 / 8, 32/8 heads: causal 3 up to 6000 430 / 435 / 422 / 422, 4 of 500 18.2 / 18.2 / 15.8 / 15.9; 32/32 heads 8 up to 2048
+    120 / 120 / 127 / 121; window 256 8 up to 2048 55.4 / 56.9 / 54.6 / 52.5, 5 up to 4001 with a softcap 84 / 84 / 83 / 79; unmasked 8 up to 2048 206 /
+    214 / 222 / 230.  All backward launches: causal 8 up to 2048, 32/8 466 / 487 / 491 / 430, 32/32 441 / 447 / 452 / 443; 24 up to 1000, D 64, 16/4
+    93 / 93 / 94 / 96, 3 up to 4001 305 / 306 / 299 / 299; window 256 286 / 287 / 285 / 281; unmasked 738 / 785 / 790 / 850."""
+    return 1 if mask == lowering.MASK_NONE else 8 if mask == lowering.MASK_SLIDING else causal
+
+
+def heads_per_workgroup(group: int) -> int:
+    """Query heads of a group that share a workgroup's K and V, as in ``lowering.attention``.  1 / 2 / 4, us, 32/8 heads: 12 sequences up to 2048
+    174 / 167 / 162, 64 up to 300 50 / 42 / 37, window 256 8 up to 2048 74 / 59 / 52."""
+    return 4 if group % 4 == 0 else 2 if group % 2 == 0 else 0
 
 
 @lowering.outside_graphs
@@ -320,8 +336,8 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, key, room=True):
     keep_ds = room and bwd_keep_ds(D, cap is not None, Hq * blocks)
     spec = bwd_spec(dtype, D, mask, cap is not None, keys, nt, q_split, lowering.bwd_grads_stay(2 * T * Hq * D), keep_ds)
     P.ds_sh = blocks * lowering.BWD_DS_BLOCK
-    dkdv_at, dkdv_entries = layout.tiles_of(64 if q_split else 128 * keys, 32 // Hkv)
-    dq_at, dq_entries = layout.tiles_of(nt // 2, 32 // Hkv)
+    dkdv_at, dkdv_entries = layout.tiles_of(64 if q_split else 128 * keys, group_size(mask, 64 // Hkv if Hkv <= 16 else 1))
+    dq_at, dq_entries = layout.tiles_of(nt // 2, group_size(mask, 64 // Hkv if Hkv <= 16 else 1))
     steps = {"lf_attn_bwd_delta": (-(-Hq * T // 16), 256), "lf_attn_bwd_dkdv": (_grid(dkdv_entries, Hkv, 256), 256),
              "lf_attn_bwd_dq": (_grid(dq_entries, Hq, nt), nt)}
     names = ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"] if nt == 256 and not keep_ds else list(steps)
