@@ -55,6 +55,7 @@ struct LfAttnBwdParams {
 struct LfPackedBwdParams : LfAttnBwdParams {
   const LfPackedTile* dkdv_tiles;      // of as many keys as a workgroup of lf_attn_bwd_dkdv has
   const LfPackedTile* dq_tiles;        // of as many queries as one of lf_attn_bwd_dq has
+  const lf_elem* low;                  // optional, strides of O: what rounding left of it
 };
 #endif
 
@@ -116,7 +117,11 @@ __device__ __forceinline__ unsigned lf_bw_ds_chunk(int key, int g) {
 }
 
 // delta[row] = sum_d dO[row][d] * O[row][d]; 16 lanes per row, 8 elements per lane
+#if LF_PACKED
+extern "C" __global__ void __launch_bounds__(LF_BW_NT) lf_attn_bwd_delta(const LfPackedBwdParams p) {
+#else
 extern "C" __global__ void __launch_bounds__(LF_BW_NT) lf_attn_bwd_delta(const LfAttnBwdParams p) {
+#endif
   const long long row = (long long)blockIdx.x * (LF_BW_NT / 16) + threadIdx.x / 16;
   const int piece = threadIdx.x % 16;
   const long long nrows = (long long)p.B * p.Hq * p.Sq;
@@ -129,6 +134,13 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT) lf_attn_bwd_delta(const L
     const lf_elem8 gv = *reinterpret_cast<const lf_elem8*>(p.dout + b * p.do_sb + h * p.do_sh + qi * p.do_ss + 8 * piece);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += (float)ov[e] * (float)gv[e];
+#if LF_PACKED
+    if (p.low != nullptr) {
+      const lf_elem8 lv = *reinterpret_cast<const lf_elem8*>(p.low + h * p.o_sh + qi * p.o_ss + 8 * piece);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += (float)lv[e] * (float)gv[e];
+    }
+#endif
   }
   s += __shfl_xor(s, 1, 64);
   s += __shfl_xor(s, 2, 64);
@@ -1204,6 +1216,19 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[e] += (float)ov[e] * (float)gv[e];
     }
+#if LF_PACKED
+    if (pk.low != nullptr) {
+      const lf_elem* lrow = pk.low + (long long)mine.row0 * p.o_ss + (long long)h * p.o_sh + (long long)qr * p.o_ss;
+#pragma unroll
+      for (int ks = 0; ks < LF_NKS; ++ks) of[ks] = *reinterpret_cast<const lf_u32x4*>(lrow + 16 * ks + 8 * g);
+#pragma unroll
+      for (int ks = 0; ks < LF_NKS; ++ks) {
+        const lf_elem8 lv = __builtin_bit_cast(lf_elem8, of[ks]), gv = __builtin_bit_cast(lf_elem8, gf[ks]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] += (float)lv[e] * (float)gv[e];
+      }
+    }
+#endif
     const float half = ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
     delta_q = half + __shfl_xor(half, 32, 64);
 #endif

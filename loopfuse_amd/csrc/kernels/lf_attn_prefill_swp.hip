@@ -169,7 +169,7 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
   p.v += (long long)mine.row0 * p.v_ss;
   p.o += (long long)mine.row0 * p.o_ss;
   if (p.part_ml != nullptr) p.part_ml += mine.row0;
-  const int lse_rows = p.Sq;
+  const int lse_rows = p.Sq, tile_row0 = mine.row0;
   p.Sq = p.Sk = mine.len;
   const int nqt = (p.Sq + LF_BM - 1) / LF_BM;
   const int slot_qt = nqt - 1 - mine.tile;    // the last q tile, which has the most kv tiles under a causal mask, comes first
@@ -935,10 +935,24 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
       const float inv = 1.0f / l_tot;
 #endif
       lf_elem* ohead = p.o + (long long)b * p.o_sb + (long long)h * p.o_sh;
+#if LF_PACKED
+      float inv_l = inv;
+      // the rows of O, or (`low`) of what rounding leaves of it
+      auto put = [&](lf_elem* ohead, const bool low) {
+#endif
       auto chunk = [&](int db, int i4) {       // d = 32*db + 8*i4 + 4*g + 0..3 of row my_q
         lf_elem4 w;
 #pragma unroll
+#if LF_PACKED
+        for (int e = 0; e < 4; ++e) {
+          float x = o[db][4 * i4 + e] * inv_l;
+          asm("" : "+v"(x));      // (the product is rounded to 32 bits in both passes: a product that is rounded to 16 at once may differ by a step)
+          w[e] = lf_from_float(x);
+          if (low) w[e] = lf_from_float(x - lf_to_float(w[e]));
+        }
+#else
         for (int e = 0; e < 4; ++e) w[e] = lf_from_float(o[db][4 * i4 + e] * inv);
+#endif
         return __builtin_bit_cast(lf_u32x2, w);
       };
 #if LF_STAY
@@ -981,6 +995,19 @@ extern "C" __global__ void __launch_bounds__(LF_NT, LF_WPE) lf_attn_prefill_swp(
           const lf_u32x4 x = *(lf_lds_u32x4_ptr)(size_t)(mine + (unsigned)(r * kStride + 16 * c));
           if (q < p.Sq) __builtin_nontemporal_store(x, reinterpret_cast<lf_u32x4*>(ohead + (long long)q * p.o_ss + 8 * c));
         }
+      }
+#endif
+#if LF_PACKED
+      };
+      put(ohead, false);
+      // for a backward (LfPackedAttnParams); the pointer is read only now: held over the loop it would cost registers
+      auto ep = (const LfPackedAttnParams __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+      asm volatile("" : "+s"(ep));
+      if (ep->low != nullptr) {
+        asm volatile("" : "+v"(inv_l));        // (formed again, not kept)
+        __builtin_amdgcn_sched_barrier(0);
+        lf_wave_exchange();
+        put(ep->low + (long long)tile_row0 * p.o_ss + (long long)h * p.o_sh, true);
       }
 #endif
     }

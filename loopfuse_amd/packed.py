@@ -38,13 +38,13 @@ class _PlanParams(ctypes.Structure):
 class PackedAttnParams(lowering.AttnParams):
     """Mirror of ``struct LfPackedAttnParams`` in csrc/kernels/lf_packed.hip.h."""
 
-    _fields_ = [("tiles", ctypes.c_void_p), ("clear", ctypes.c_int)]
+    _fields_ = [("tiles", ctypes.c_void_p), ("low", ctypes.c_void_p), ("clear", ctypes.c_int)]
 
 
 class PackedBwdParams(lowering.AttnBwdParams):
     """Mirror of ``struct LfPackedBwdParams`` in csrc/kernels/lf_attn_bwd.hip."""
 
-    _fields_ = [("dkdv_tiles", ctypes.c_void_p), ("dq_tiles", ctypes.c_void_p)]
+    _fields_ = [("dkdv_tiles", ctypes.c_void_p), ("dq_tiles", ctypes.c_void_p), ("low", ctypes.c_void_p)]
 
 
 @dataclasses.dataclass(frozen=True, eq=False)
@@ -162,7 +162,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
 
     Inside ``torch.compile`` the call runs as it is, between two graphs.
 
-    Differentiable where gradients are recorded and neither ``out`` nor ``lse`` is given; gradients of rows of no sequence are zero."""
+    Differentiable where gradients are recorded and neither ``out`` nor ``lse`` is given; gradients of rows of no sequence are zero.
+    Kept for the backward besides Q, K, V and O: lse, and what rounding takes from O, as large as O (it halves what delta is off by)."""
     if not isinstance(layout, PackedLayout):
         raise UnsupportedPlan("layout must come from packed_layout")
     if q.dim() == 3 and q.shape[2] not in (64, 128) and 1 <= q.shape[2] < 128:
@@ -178,21 +179,23 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
     return _forward(q, k, v, plan, layout, out, lse)
 
 
-def _forward(q, k, v, plan, layout, out, lse):
+def _forward(q, k, v, plan, layout, out, lse, low=None):
     key = lowering._call_key("packed", (q, k, v, out), (lse, layout.tiles), plan, (layout.total, layout.caps[-1]))
     kept = lowering._kept.get(key)
     if kept is not None:
-        return _forward_again(q, k, v, layout, out, lse, kept)
-    return _forward_general(q, k, v, plan, layout, out, lse, key)
+        return _forward_again(q, k, v, layout, out, lse, low, kept)
+    return _forward_general(q, k, v, plan, layout, out, lse, low, key)
 
 
-def _forward_again(q, k, v, layout, out, lse, repeat):
+def _forward_again(q, k, v, layout, out, lse, low, repeat):
     P = PackedAttnParams.from_buffer_copy(repeat.block)
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     P.q, P.k, P.v, P.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     if lse is not None:
         P.part_ml = lse.data_ptr()
+    if low is not None:
+        P.low = low.data_ptr()
     P.tiles = layout.tiles.data_ptr() + repeat.more
     repeat.launches.launch(P)
     lowering._last_launch.set(repeat.record)
@@ -200,7 +203,7 @@ def _forward_again(q, k, v, layout, out, lse, repeat):
 
 
 @lowering._on_device_of_first_argument
-def _forward_general(q, k, v, plan, layout, out, lse, key):
+def _forward_general(q, k, v, plan, layout, out, lse, low, key):
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
     mask, window, scale, cap = _constants(plan, layout.total)
     T = layout.total
@@ -237,7 +240,7 @@ def _forward_general(q, k, v, plan, layout, out, lse, key):
     grid = _grid(entries, heads, 256)
     record = {"kernels": [spec.entry()], "grid": grid, "block": 256, "q_tile_rows": bm, "kv_tile_rows": spec.bn or 64, "heads_per_workgroup": pack or 1}
     repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (grid, 1, 1), 256)], record, tiles_at)
-    out = _forward_again(q, k, v, layout, out, lse, repeat)
+    out = _forward_again(q, k, v, layout, out, lse, low, repeat)
     if key is not None:
         lowering._keep(key, repeat)
     return out
@@ -270,22 +273,24 @@ def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return _backward(q, k, v, o, lse, dout, plan, layout)
 
 
-def _backward(q, k, v, o, lse, dout, plan, layout):
+def _backward(q, k, v, o, lse, dout, plan, layout, low=None):
     key = lowering._call_key("packed bwd", (q, k, v, o, dout), (lse, layout.tiles), plan, (layout.total, layout.caps[-1]))
     kept = lowering._kept.get(key)
     if kept is not None:
-        res = _backward_again(q, k, v, o, lse, dout, layout, kept)
-        return _backward_general(q, k, v, o, lse, dout, plan, layout, None, False) if res is None else res
-    return _backward_general(q, k, v, o, lse, dout, plan, layout, key)
+        res = _backward_again(q, k, v, o, lse, dout, layout, low, kept)
+        return _backward_general(q, k, v, o, lse, dout, plan, layout, low, None, False) if res is None else res
+    return _backward_general(q, k, v, o, lse, dout, plan, layout, low, key)
 
 
-def _backward_again(q, k, v, o, lse, dout, layout, repeat):
+def _backward_again(q, k, v, o, lse, dout, layout, low, repeat):
     P = PackedBwdParams.from_buffer_copy(repeat.block)
     dtype, dev = q.dtype, q.device
     dq, dk, dv = torch.empty(q.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
     delta = torch.empty(lse.shape, dtype=torch.float32, device=dev)
     P.q, P.k, P.v, P.o, P.dout = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr()
     P.dq, P.dk, P.dv, P.lse, P.delta = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), lse.data_ptr(), delta.data_ptr()
+    if low is not None:
+        P.low = low.data_ptr()
     at = layout.tiles.data_ptr()
     P.dkdv_tiles, P.dq_tiles = at + repeat.more[0], at + repeat.more[1]
     if repeat.more[2]:
@@ -301,7 +306,7 @@ def _backward_again(q, k, v, o, lse, dout, layout, repeat):
 
 
 @lowering._on_device_of_first_argument
-def _backward_general(q, k, v, o, lse, dout, plan, layout, key, room=True):
+def _backward_general(q, k, v, o, lse, dout, plan, layout, low, key, room=True):
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
     mask, window, scale, cap = _constants(plan, layout.total)
     T, dev = layout.total, q.device
@@ -344,9 +349,9 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, key, room=True):
     named = lowering._kernels_of(spec)
     launches = [(lowering.get_kernel(spec, name, named), (steps[name][0], 1, 1), steps[name][1]) for name in names]
     repeat = lowering._Repeat(P, launches, {"kernels": names}, (dkdv_at, dq_at, P.ds_sh * Hq if keep_ds else 0))
-    res = _backward_again(q, k, v, o, lse, dout, layout, repeat)
+    res = _backward_again(q, k, v, o, lse, dout, layout, low, repeat)
     if res is None:
-        return _backward_general(q, k, v, o, lse, dout, plan, layout, None, False)
+        return _backward_general(q, k, v, o, lse, dout, plan, layout, low, None, False)
     if key is not None:
         lowering._keep(key, repeat)
     return res
@@ -382,10 +387,10 @@ def bwd_keep_ds(D: int, softcap: bool, blocks: int) -> bool:
 
 
 def _gradients(ctx, dout):
-    q, k, v, out, lse = ctx.saved_tensors
+    q, k, v, out, lse, low = ctx.saved_tensors
     if dout.stride(-1) != 1 or dout.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(dout.shape[:-1], dout.stride()[:-1])):
         dout = dout.contiguous()
-    return (*_backward(q, k, v, out, lse, dout, ctx.plan, ctx.layout), None, None)
+    return (*_backward(q, k, v, out, lse, dout, ctx.plan, ctx.layout, low), None, None)
 
 
 _gradients_once = torch.autograd.function.once_differentiable(_gradients)
@@ -398,8 +403,9 @@ class _Packed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, plan, layout):
         lse = torch.empty((q.shape[1], layout.total), dtype=torch.float32, device=q.device)
-        out = _forward(q, k, v, plan, layout, None, lse)
-        ctx.save_for_backward(q, k, v, out, lse)
+        low = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _forward(q, k, v, plan, layout, None, lse, low)
+        ctx.save_for_backward(q, k, v, out, lse, low)
         # (the caller may change a plan)
         ctx.plan = AttnPlan(plan.mask, plan.window, plan.scale, plan.softcap, plan.k_paged, plan.v_paged, plan.denom_add)
         ctx.layout = layout

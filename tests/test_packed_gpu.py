@@ -137,3 +137,33 @@ def test_forward_and_gradients_are_the_formulas(lengths, Hq, Hkv, D, dtype, mask
     assert torch.equal(given[lo:hi], out[lo:hi]) and (given[:lo] == 7).all() and (given[hi:] == 7).all()
     assert (lse[:, :lo] == 5).all() and (lse[:, hi:] == 5).all()
     assert (lse[:, lo:hi].double() - lse_ref[:, lo:hi]).abs().max().item() <= 2e-3 if hi > lo else True
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,Hkv,D,mask", [(2, 2, 64, "causal"), (8, 2, 128, "causal"), (4, 2, 128, None), (8, 1, 64, "sliding")])
+def test_what_rounding_takes_from_the_result_is_kept_for_the_backward(Hq, Hkv, D, mask, dtype):
+    # Q = 0: every probability is 1 / (number of keys), exact before the sum, so that O in 32 bits is the mean of V but for what its n
+    # sums, the reciprocal and one product round, and O + low is off by that and by half a step of low
+    lengths, lead = [1, 2, 0, 31, 130, 257], 3
+    bounds = [lead]
+    for n in lengths:
+        bounds.append(bounds[-1] + n)
+    T = bounds[-1] + 5
+    g = torch.Generator(DEV).manual_seed(4)
+    q = torch.zeros(T, Hq, D, dtype=dtype, device=DEV)
+    k, v = ((2 * torch.rand(T, Hkv, D, generator=g, device=DEV) - 1).to(dtype) for _ in range(2))
+    layout = packed.packed_layout(torch.tensor(bounds, dtype=torch.int32, device=DEV), T)
+    plan = AttnPlan(mask, window=40, scale=1.0)
+    lse, low = torch.empty(Hq, T, device=DEV), torch.full_like(q, math.nan)
+    out = packed._forward(q, k, v, plan, layout, None, lse, low)
+    want, _ = oracle(q, k, v, torch.zeros_like(q), bounds, mask, 40, 1.0, None)
+    rows = slice(lead, bounds[-1])
+    value, l64 = want["out"][0][rows], low[rows].double()
+    off = (out[rows].double() + l64 - value).abs()
+    bound = (257 + 4) * 2.0 ** -24 + torch.finfo(dtype).eps / 2 * l64.abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    assert (off <= bound).all(), (off - bound).max()
+    assert (out[rows].double() - value).abs().max() > 8 * bound.max()      # (what O alone is off by)
+    assert torch.isnan(low[:lead]).all() and torch.isnan(low[bounds[-1]:]).all()
+    dout = torch.randn(q.shape, generator=g, device=DEV).to(dtype)
+    for name, t in zip(("dq", "dk", "dv"), packed._backward(q, k, v, out, lse, dout, plan, layout, low)):
+        assert torch.isfinite(t).all(), name
