@@ -4,11 +4,13 @@
 //   have = ceil(c / P), need = ceil((c + n) / P) - have, first = sum of `need` of the requests before it,
 //   table[b, have + i] = free[first + i], i < need,
 //   offsets[b] = sum of `new` of the requests before it: the packed row of its first new token,
-//   positions[offsets[b] + t] = c + t, slots[...] = table[b, (c + t) / P] * P + (c + t) % P, t < n.
+//   positions[offsets[b] + t] = c + t, slots[...] = table[b, (c + t) / P] * P + (c + t) % P, t < n,
+//   lengths[b] = c + the number of its new tokens that fit.
 // A block has one request (and a share of its tokens): it forms the two sums itself from all B lengths, which are in L2 after the first
 // block, so that no block waits for another.  Slots of new pages come from the list of free ones, not from the table, so blocks of one
 // request do not wait for each other's entries either.  Bound by its chain of round trips (lengths, then the page, then the stores).
-// What does not fit -- no free page left, a row of the table too short, a token behind the last row -- gets page and slot -1.
+// What does not fit -- no free page left, a row of the table too short, a token behind the last row -- gets page and slot -1 and is not
+// counted, so that nothing reads keys that are not there: of each kind it is the request's last tokens.
 
 struct LfTablesParams {
   const int* cached;          // [B]
@@ -16,7 +18,7 @@ struct LfTablesParams {
   lf_table_t* table;          // [B, width], rows table_stride apart
   const lf_table_t* free;     // [count]
   int* offsets;               // [B + 1]
-  int* lengths;               // [B] cached + new
+  int* lengths;               // [B]
   int* slots;                 // [T]
   int* positions;             // [T]
   int* pages;                 // [1] pages that the requests need
@@ -62,17 +64,18 @@ extern "C" __global__ void __launch_bounds__(LF_TABLES_NT) lf_paged_tables(const
   if (b < p.B) {
     const long long c = cached(b), n = fresh(b), have = pages(c), need = pages(c + n) - have;
     lf_table_t* mine = p.table + b * p.table_stride;
+    const long long end = min(n, p.T - row);
     if (share == 0) {
+      const long long named = min((long long)p.width, have + min(need, max(p.count - first, 0ll)));      // entries of its row that name pages
       p.offsets[b] = clamp32(row);
-      p.lengths[b] = clamp32(c + n);
+      p.lengths[b] = clamp32(c + max(0ll, min(end, (named << p.shift) - c)));
     }
     for (long long i = share; i < need && have + i < p.width; i += step) mine[have + i] = page_at(first + i);
-    const long long end = min(n, p.T - row);
     for (long long t = share; t < end; t += step) {
       const long long at = (c + t) >> p.shift;
       const lf_table_t page = at >= p.width ? (lf_table_t)-1 : at < have ? mine[at] : page_at(first + at - have);
       p.positions[row + t] = clamp32(c + t);
-      p.slots[row + t] = page < 0 ? -1 : (int)((page << p.shift) | ((c + t) & up));
+      p.slots[row + t] = page < 0 || page > (0x7fffffff >> p.shift) ? -1 : (int)((page << p.shift) | ((c + t) & up));
     }
   }
   if (b == 0 && share == 0) {

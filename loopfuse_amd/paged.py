@@ -52,7 +52,7 @@ class PagedStep(NamedTuple):
     """What ``extend_tables`` leaves."""
 
     offsets: torch.Tensor      # int32 [B + 1]: request b's new tokens are rows offsets[b] ... offsets[b + 1]
-    lengths: torch.Tensor      # int32 [B]: tokens of each request with the new ones
+    lengths: torch.Tensor      # int32 [B]: tokens of each request with the new ones that have a slot
     slots: torch.Tensor        # int32 [total]: page * page_size + place in the page, -1 for rows of no token
     positions: torch.Tensor    # int32 [total]: place in the request, -1 for rows of no token
     pages: torch.Tensor        # int32 [1]: free pages that the new tokens need
@@ -75,8 +75,8 @@ def _whole(name: str, n) -> int:
 
 
 def _shift(page_size: int) -> int:
-    if not isinstance(page_size, int) or page_size < 1 or page_size & (page_size - 1):
-        raise UnsupportedPlan("page size must be a power of two")
+    if not isinstance(page_size, int) or page_size < 1 or page_size & (page_size - 1) or page_size > 1 << 30:
+        raise UnsupportedPlan("page size must be a power of two, 2**30 at most")
     return page_size.bit_length() - 1
 
 
@@ -91,7 +91,8 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
     size will do).
 
     Nothing is raised for what only the GPU knows: where no free page is left, the row of the table is too short or a token lies behind
-    ``total``, the token's slot (and the new entry) is -1, which ``store_kv`` leaves out; ``pages`` above ``len(free)`` says so."""
+    ``total``, the token's slot (and the new entry) is -1, which ``store_kv`` leaves out, and ``lengths`` ends in front of it;
+    ``pages`` above ``len(free)`` says so.  Slots are numbers in 32 bits: a page behind those counts as none."""
     key = lowering._call_key("tables", (), (cached, new, table, free), None, (page_size, total))
     kept = lowering._kept.get(key)
     if kept is not None:
@@ -309,8 +310,9 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     _on_gpu("V table", v_table, (table.dtype,), 2, q.device)
     if table.shape[0] != B or v_table.shape != table.shape or lengths.shape[0] != B:
         raise UnsupportedPlan(f"tables and lengths must be of {B} requests, the tables of one width")
-    if prefix_len < 0 or prefix_len >= 1 << 31 or table.shape[1] * page >= 1 << 31:
-        raise UnsupportedPlan("more keys than positions in 32 bits")
+    # (the kernels round keys up to pieces, 2**30 keys at most, in 32 bits)
+    if prefix_len < 0 or max(prefix_len, table.shape[1] * page) > 1 << 30:
+        raise UnsupportedPlan("a request or the prefix has room for more than 2**30 keys")
     if prefix_len:
         if prefix_table is None:
             raise UnsupportedPlan("a prefix needs its table")
@@ -376,6 +378,8 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
             splits = max(1, min(64, prefix_len // 32, choice.get("splits", 512 // P.pre_units)))
             splits, P.split_len = lowering._split_lengths(splits, prefix_len)
         P.nsplit, P.pre_blocks = splits, splits * P.pre_units
+    if (P.pre_blocks + items * P.units) * 64 * max(4, coop) >= 1 << 32:
+        raise UnsupportedPlan(f"a launch for {B} requests of {Hq} heads is too large")
     own, pre = items * Hq, splits * B * Hq            # rows of partial results
     args = dict(rows=lowering.DECODE_QROWS, waves=coop or 4, headwave=coop > 0, coop=coop > 0,
                 rowload=not coop and lowering._decode_rowload(3, page, 0, 0))

@@ -29,12 +29,14 @@ def plain_tables(cached, new, table, free, page, total):
             if i < len(table[b]):
                 table[b][i] = free[taken] if taken < len(free) else -1
             taken += 1
+        length = c
         for t in range(c, c + n):
             positions.append(t)
             i = t // page
             slots.append(table[b][i] * page + t % page if i < len(table[b]) and table[b][i] >= 0 else -1)
+            length += slots[-1] >= 0 and len(slots) <= total
         offsets.append(offsets[-1] + n)
-        lengths.append(c + n)
+        lengths.append(length)
     rest = [-1] * max(0, total - len(slots))
     return table, offsets, lengths, (slots + rest)[:total], (positions + rest)[:total], taken
 
@@ -49,6 +51,8 @@ TABLES = [
     ([10, 20, 30], [50, 50, 50], 16, 9, -4, 6),           # not enough free pages
     ([10, 20, 30], [50, 50, 500], 16, 9, 0, 6),           # a row too short
     ([1, 2, 3], [70, 80, 90], 64, 9, 0, -100),            # tokens behind the last row
+    ([10, 20, 30, 64, 3], [50, 50, 0, 50, 5], 16, 3, -5, -40),      # all of it
+    ([100, 5], [3, 3], 16, 2, 0, 0),                      # more in the cache than the table has room for
     ([i * 7 % 50 for i in range(700)], [i * 5 % 13 for i in range(700)], 2, 40, 0, 100),
     ([0], [20000], 16, 1250, 0, 0),
     ([], [], 16, 4, 3, 9),
@@ -75,6 +79,31 @@ def test_tables_slots_and_positions_are_the_plain_loops(cached, new, page, width
     assert (wide[:, 0] == -5).all() and (wide[:, 1 + width:] == -5).all()
     assert step.offsets.tolist() == want[1] and step.lengths.tolist() == want[2]
     assert step.slots.tolist() == want[3] and step.positions.tolist() == want[4] and step.pages.tolist() == [want[5]]
+
+
+def test_pages_whose_slots_pass_32_bits_are_none():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    for dtype in (torch.int32, torch.int64):
+        pages = [2 ** 27 - 1, 2 ** 27, 2 ** 28] + ([2 ** 33 + 1] if dtype == torch.int64 else [2 ** 31 - 1])
+        step = paged.extend_tables(i32([0] * 4), i32([16] * 4), torch.zeros((4, 1), dtype=dtype, device=DEV), torch.tensor(pages, dtype=dtype, device=DEV), 16, 64)
+        assert step.slots.tolist() == list(range(2 ** 31 - 16, 2 ** 31)) + [-1] * 48
+
+
+def test_attention_after_pages_ran_out_reads_what_was_stored():
+    # 3 free pages for the 5 that are asked for: the entries that got none are -1, and no key is looked for there
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    page, Hkv, D, new = 16, 2, 128, [20, 30, 10]
+    kp, vp = (torch.full((4, page, Hkv, D), math.nan, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    k, v = (torch.randn((60, Hkv, D), generator=gen, device=DEV).to(torch.bfloat16) for _ in range(2))
+    table = torch.full((3, 4), -1, dtype=torch.int32, device=DEV)
+    step = paged.extend_tables(i32([0, 0, 0]), i32(new), table, i32([2, 0, 3]), page, 60)
+    assert step.lengths.tolist() == [20, 16, 0] and step.pages.tolist() == [5]
+    assert table.tolist() == [[2, 0, -1, -1], [3, -1, -1, -1], [-1, -1, -1, -1]]
+    paged.store_kv(k, v, kp, vp, step.slots)
+    q = torch.randn((3, 4, 1, D), generator=gen, device=DEV).to(torch.bfloat16)
+    plan = AttnPlan(scale=D ** -0.5, k_paged=True, v_paged=True)
+    check(paged.attention_shared(q, kp, vp, plan, table, step.lengths), oracle(q, kp, vp, table, step.lengths, None, 0, D ** -0.5, None))
 
 
 # ---- store_kv ------------------------------------------------------------------------------------------------

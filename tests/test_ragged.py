@@ -125,6 +125,7 @@ TABLES = {
     "dims": lambda c, n, t, f: (c, n, t[0], f, 16, 10),
     "page size": lambda c, n, t, f: (c, n, t, f, 12, 10),
     "no page": lambda c, n, t, f: (c, n, t, f, 0, 10),
+    "pages beyond 32 bits": lambda c, n, t, f: (c, n, t, f, 1 << 31, 10),
     "total": lambda c, n, t, f: (c, n, t, f, 16, -1),
     "columns apart": lambda c, n, t, f: (c, n, fake((3, 8), torch.int32)[:, ::2], f, 16, 10),
     "rows of one": lambda c, n, t, f: (c, n, fake((1, 4), torch.int32).expand(3, 4), f, 16, 10),
@@ -181,6 +182,8 @@ SHARED = {
     "type of the prefix table": dict(prefix_table=fake((2,), torch.int64)), "a negative prefix": dict(prefix_len=-1),
     "V table": dict(v_table=fake((3, 4), torch.int32)), "page sizes": dict(v_pool=fake((18, 2, 2, 64))), "page size": dict(k_pool=fake((9, 6, 2, 64)), v_pool=fake((9, 6, 2, 64))),
     "out": dict(out=fake((3, 4, 64))), "out of one row": dict(out=fake((1, 4, 1, 64)).expand(3, 4, 1, 64)), "kv heads": dict(v_pool=fake((9, 4, 1, 64))),
+    "room beyond 2**30 keys": dict(table=fake((3, 1), torch.int32).expand(3, (1 << 28) + 1)),
+    "a prefix beyond 2**30 keys": dict(prefix_table=fake((1,), torch.int32).expand((1 << 28) + 1), prefix_len=(1 << 30) + 1),
     "a prefix length that is no number": dict(prefix_len=torch.tensor(7)),
 }
 
