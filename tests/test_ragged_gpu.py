@@ -177,6 +177,72 @@ def test_repeated_captured_and_on_another_stream(form):
         assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_a_captured_step_replays_with_other_lengths():
+    """One graph of a serving step and of a packed batch: what it replays follows the lengths, new tokens and offsets that its buffers hold then."""
+    Hq, Hkv, D, page, B, width = 16, 4, 128, 16, 4, 40
+    pool = [rnd((B * width + 38, page, Hkv, D), s) for s in (1, 2)]
+    prefix_table = i32(list(range(B * width + 30, B * width + 37)))
+    plan = AttnPlan(scale=0.1, k_paged=True, v_paged=True)
+
+    def run(a):
+        step = paged.extend_tables(a["cached"], a["new"], a["table"], a["free"], page, 50)
+        paged.store_kv(a["k"][:, :Hkv], a["k"][:, Hkv:], *a["pool"], step.slots)
+        out = paged.attention_shared(a["q"], *a["pool"], plan, a["table"], step.lengths, prefix_table=prefix_table, prefix_len=100)
+        rows = packed.attention_packed(a["k"].repeat(1, 2, 1), a["k"][:, :Hkv], a["k"][:, Hkv:], AttnPlan("causal", scale=0.1),
+                                       packed.packed_layout(step.offsets, 50))
+        return (*step, out, rows, *a["pool"], a["table"])
+
+    def inputs(cached, new, seed):
+        ids = torch.randperm(B * width + 30, generator=torch.Generator().manual_seed(seed)).to(torch.int32).to(DEV)
+        return {"cached": i32(cached), "new": i32(new), "table": ids[30:].view(B, width).clone(), "free": ids[:30].clone(), "q": rnd((B, Hq, 1, D), seed), "k": rnd((50, 2 * Hkv, D), seed + 1),
+                "pool": [p.clone() for p in pool]}
+
+    steps = [([0, 3, 600, 16], [1, 1, 1, 1]), ([0, 0, 0, 0], [0, 0, 0, 0]), ([100, 20, 0, 33], [0, 50, 0, 0]), ([639, 1, 1, 500], [1, 20, 9, 20]), ([5, 6, 7, 8], [40, 40, 40, 40])]
+    wants = [run(inputs(c, n, 10 + i)) for i, (c, n) in enumerate(steps)]
+    held = inputs(*steps[0], 10)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(held)
+    for i in (3, 1, 4, 0, 2, 3):
+        for name, x in inputs(*steps[i], 10 + i).items():
+            for to, t in zip(held[name], x) if name == "pool" else ((held[name], x),):
+                to.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        for j, (x, y) in enumerate(zip(got, wants[i])):
+            assert torch.equal(x, y), (i, j)
+
+
+def test_a_captured_call_refuses_leaves_of_a_living_eager_graph():
+    q, k, v, g, layout = packed_args(5)
+    leaves, plan = [t.requires_grad_(True) for t in (q, k, v)], AttnPlan("causal", scale=0.1)
+    eager = packed.attention_packed(*leaves, plan, layout)
+    want = torch.autograd.grad(eager, leaves, g, retain_graph=True)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        g.add_(0)
+        with pytest.raises(UnsupportedPlan, match="leaves"):
+            packed.attention_packed(*leaves, plan, layout)
+        padded = [t[..., :40].contiguous().detach().requires_grad_(True) for t in leaves]
+        held = [t * 2 for t in padded]
+        with pytest.raises(UnsupportedPlan, match="leaves"):
+            packed.attention_packed(*padded, plan, layout)
+        del held
+        with torch.no_grad():
+            packed.attention_packed(*leaves, plan, layout)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(packed.attention_packed(*leaves, plan, layout), leaves, g)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_two_graphs_and_a_larger_eager_call_do_not_share_room():
     """Partial results of captured calls live in the graphs, those of eager calls in a buffer that a larger call replaces."""
     a, b = shared_args(1), shared_args(2, lengths=(700, 3))
