@@ -229,18 +229,20 @@ def prefix_on_tiles(rows: int, prefix_len: int) -> bool:
     return rows > lowering.DECODE_QROWS or prefix_len >= 2048
 
 
-def prefix_splits(units: int, keys: int, rows: int, own_bytes: int) -> int:
-    """Splits of a prefix on 128-row tiles: ``units`` workgroups per split, ``keys`` tiles of 64 keys, ``rows`` (request, head) pairs,
-    ``own_bytes`` of K and V that the own keys have room for.  A tile of a chain takes 2.4 us, a split costs its partials, 0.3 us and 0.25
-    per 1000 rows, and there is one workgroup per CU at most, since the own keys are streamed beside them; where those take longer, on half
-    of their room, than a chain of 8 tiles, finer splits only cost.  GPU time, us, by splits: 16 requests behind 1000 keys 2 21.7, 4 15.9,
-    8 14.1, 16 15.5; 32 behind 8000 8 36.8, 16 26.5, 32 25.1; 128 behind 2000 4 29.8, 8 28.8, 16 34.9; 64 up to 1024 behind 2048 2 47.4,
-    4 39.1, 8 43.5; 128 up to 300 behind 8208 4 67.6, 8 50.3, 16 57.8."""
-    most = max(1, 256 // units)
-    best = int(math.sqrt(keys * 2.4 / (0.3 + rows / 4000)) + 0.5)
-    if own_bytes / 2 > 100e6:
-        best = min(best, max(1, keys // 8))
-    return max(1, min(most, best))
+def prefix_splits(units: int, keys: int, rows: int, D: int, prefix_bytes: int, own_bytes: int) -> int:
+    """Splits of a prefix on 128-row tiles, the least of a sum: ``units`` workgroups per split, ``keys`` tiles of 64 keys, ``rows`` (request, head)
+    pairs, bytes of K and V of the prefix and of what the own keys have room for.  A tile of a chain takes 1.3 us (0.86 at head dimension 64), more
+    with more than one workgroup per CU; chains gain nothing below what HBM takes for the prefix and part of the own keys; a split leaves its
+    partial results, 0.46 us per 1000 rows.  225 drawn batches, 2 ... 256 requests of 20 ... 2000 keys behind 500 ... 16 000: 1.025 of the best number's
+    time in the mean, 1.2 at most.  GPU time, us, by splits, 32/8 heads: 64 requests up to 1024 behind 2048 keys 2 42.5, 3 37.3, 4 38.6, 8 43.7; 128 up to 300
+    behind 8208 4 61.5, 8 45.2, 9 42.9, 10 49.8, 15 55.8; 32 up to 100 behind 8000 8 36.2, 16 25.4, 21 28.1, 32 30.0; 8/2 heads, 11 up to 194 behind 4154 8 22.5, 17
+    15.3, 33 13.5."""
+    tile, best = 1.3 if D == 128 else 0.86, (math.inf, 1)
+    stream = (prefix_bytes + own_bytes / 5) / 4.2e6
+    for n in range(1, min(64, keys) + 1):
+        chain = -(-keys // n) * tile * (1 + 0.4 * max(0.0, units * n / 256 - 1))
+        best = min(best, (max(chain, stream) + n * (0.025 + 0.46e-3 * rows * D / 128), n))
+    return best[1]
 
 
 def combine_grid(B: int, Hq: int, D: int) -> int:
@@ -369,7 +371,7 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     if prefix_len:
         if tiles:
             P.pre_units, keys = Hkv * -(-rows // 128), -(-prefix_len // 64)
-            splits = max(1, min(64, keys, choice.get("splits", prefix_splits(P.pre_units, keys, B * Hq, 4 * B * P.room * Hkv * D))))
+            splits = max(1, min(64, keys, choice.get("splits", prefix_splits(P.pre_units, keys, B * Hq, D, 4 * prefix_len * Hkv * D, 4 * B * P.room * Hkv * D))))
             P.split_len = 64 * -(-keys // splits)
             splits = -(-prefix_len // P.split_len)
             P.k_span, P.v_span = spans if near else (1, 1)

@@ -315,5 +315,6 @@ def test_splits_of_a_prefix_are_whole_tiles_and_few():
     for units in (1, 3, 8, 32, 300):
         for keys in (1, 2, 16, 129, 4000):
             for own in (0, 1 << 40):
-                n = paged.prefix_splits(units, keys, 128, own)
-                assert 1 <= n and (n == 1 or n * units <= 256)
+                for D in (64, 128):
+                    n = paged.prefix_splits(units, keys, 128, D, keys << 17, own)
+                    assert 1 <= n <= min(64, keys) and (own == 0 or n == 1)
