@@ -9,7 +9,7 @@
 // A block has one request (and a share of its tokens): it forms the two sums itself from all B lengths, which are in L2 after the first
 // block, so that no block waits for another.  Slots of new pages come from the list of free ones, not from the table, so blocks of one
 // request do not wait for each other's entries either.  Bound by its chain of round trips (lengths, then the page, then the stores): 64 requests of one
-// new token 4.1 us, 256 of 2048 and fewer (2.2 MB) 6.1; the call's host time is 10.8.
+// new token 4.1 us, 256 of 2048 and fewer (2.2 MB) 6.1, as long as the call takes the host.
 // What does not fit -- no free page left, a row of the table too short, a token behind the last row -- gets page and slot -1 and is not
 // counted, so that nothing reads keys that are not there: of each kind it is the request's last tokens.
 

@@ -822,7 +822,7 @@ def _keep(key, kept: _Kept) -> None:
 
 
 class _Repeat:
-    """The launches of a call of one of the other operators (``packed``, ``paged``), recorded for its signature (``_call_key``):
+    """The launches of a call of one of the other operators (``packed``, ``paged``), recorded for its signature (``_call_key``) in csrc/lf_host.cpp:
     ``block``: the parameter block, its pointers still to be set; ``more``: what the operator keeps beside it."""
 
     __slots__ = ("block", "launches", "record", "more")
@@ -831,37 +831,27 @@ class _Repeat:
         self.block, self.launches, self.record, self.more = bytes(params), runtime.LaunchList(steps), record, more
 
 
+def _host():
+    """The module that takes repeated calls of the operators ``packed`` and ``paged`` (csrc/lf_host.cpp), set up."""
+    module = runtime.host()
+    if _VARIABLES is not None:
+        def failed(rc):
+            runtime._check("lf_launch_list", rc)
+        from .paged import PagedStep
+        module.setup(os, _ENVIRON, _VARIABLES, _SWITCHES, b"LOOPFUSE_CHECK_TABLES", _last_launch._tls, failed, PagedStep,
+                     ctypes.cast(runtime.lib().lf_launch_list, ctypes.c_void_p).value)
+    return module
+
+
 def _call_key(kind: str, data, ints, plan: Optional[AttnPlan], more: tuple):
-    """As ``_signature``: key of a call over operands ``data``, read 16 bytes at a time, and index tensors ``ints`` (None in the place of
-    one that is not given), with further plain values ``more``; None: not to be kept."""
-    if os.environ is not _ENVIRON or _VARIABLES is None or b"LOOPFUSE_CHECK_TABLES" in _VARIABLES:
-        return None
-    device, operands = runtime.current_device(), []
-    try:
-        for t in data:
-            if t is None:
-                operands.append(None)
-            elif t.get_device() != device or t.data_ptr() % 16:
-                return None
-            else:
-                operands.append((t.shape, t.stride(), t.dtype))
-        for t in ints:
-            if t is None:
-                operands.append(None)
-            elif t.get_device() != device:
-                return None
-            else:
-                operands.append((t.shape, t.stride(), t.dtype))
-    except AttributeError:
-        return None
-    fields = None
-    if plan is not None:
-        fields = (plan.mask, plan.window, plan.scale, plan.softcap, plan.k_paged, plan.v_paged, plan.denom_add)
-        if not _PLAIN_TYPES.issuperset(map(type, fields)):
-            return None
-    if not _PLAIN_TYPES.issuperset(map(type, more)):
-        return None
-    return (kind, device, fields, more, tuple(map(_VARIABLES.get, _SWITCHES)), tuple(operands))
+    """Signature of a call over operands ``data``, read 16 bytes at a time, and index tensors ``ints`` (None in the place of one that is
+    not given), with further plain values ``more``; None: not to be kept."""
+    return runtime.host().key(kind, data, ints, plan, more)
+
+
+def _keep_call(key, repeat: "_Repeat", more: tuple) -> None:
+    if key is not None:
+        runtime.host().keep(key, repeat.block, bytes(repeat.launches._items), repeat.record, repeat, more)
 
 
 def outside_graphs(fn):

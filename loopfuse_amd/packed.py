@@ -181,7 +181,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
         return attention_packed(q, k, v, plan, layout)[..., :D].contiguous()
     if grads:
         return _Packed.apply(q, k, v, plan, layout)
-    return _forward(q, k, v, plan, layout, out, lse)
+    done = _host.attention_packed(q, k, v, out, lse, layout.tiles, plan, layout.total, layout.caps[-1], False)
+    return _forward(q, k, v, plan, layout, out, lse) if done is None else done
 
 
 def in_a_graph(leaf: torch.Tensor) -> bool:
@@ -191,14 +192,6 @@ def in_a_graph(leaf: torch.Tensor) -> bool:
     edge = torch.autograd.graph.get_gradient_edge
     edge(leaf).node.metadata["loopfuse_amd"] = True
     return edge(leaf).node.metadata.pop("loopfuse_amd", False)
-
-
-def _forward(q, k, v, plan, layout, out, lse, low=None):
-    key = lowering._call_key("packed", (q, k, v, out), (lse, layout.tiles), plan, (layout.total, layout.caps[-1]))
-    kept = lowering._kept.get(key)
-    if kept is not None:
-        return _forward_again(q, k, v, layout, out, lse, low, kept)
-    return _forward_general(q, k, v, plan, layout, out, lse, low, key)
 
 
 def _forward_again(q, k, v, layout, out, lse, low, repeat):
@@ -217,7 +210,7 @@ def _forward_again(q, k, v, layout, out, lse, low, repeat):
 
 
 @lowering._on_device_of_first_argument
-def _forward_general(q, k, v, plan, layout, out, lse, low, key):
+def _forward(q, k, v, plan, layout, out, lse, low=None):
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
     mask, window, scale, cap = _constants(plan, layout.total)
     T = layout.total
@@ -254,9 +247,9 @@ def _forward_general(q, k, v, plan, layout, out, lse, low, key):
     grid = _grid(entries, heads, 256)
     record = {"kernels": [spec.entry()], "grid": grid, "block": 256, "q_tile_rows": bm, "kv_tile_rows": spec.bn or 64, "heads_per_workgroup": pack or 1}
     repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (grid, 1, 1), 256)], record, tiles_at)
+    key = lowering._call_key("p", (q, k, v, out), (None if low is not None else lse, layout.tiles), plan, (T, layout.caps[-1], low is not None))
     out = _forward_again(q, k, v, layout, out, lse, low, repeat)
-    if key is not None:
-        lowering._keep(key, repeat)
+    lowering._keep_call(key, repeat, (tiles_at,))
     return out
 
 
@@ -288,12 +281,9 @@ def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 
 def _backward(q, k, v, o, lse, dout, plan, layout, low=None):
-    key = lowering._call_key("packed bwd", (q, k, v, o, dout), (lse, layout.tiles), plan, (layout.total, layout.caps[-1]))
-    kept = lowering._kept.get(key)
-    if kept is not None:
-        res = _backward_again(q, k, v, o, lse, dout, layout, low, kept)
-        return _backward_general(q, k, v, o, lse, dout, plan, layout, low, None, False) if res is None else res
-    return _backward_general(q, k, v, o, lse, dout, plan, layout, low, key)
+    done = _host.attention_packed_backward(q, k, v, o, dout, lse, layout.tiles, low, plan, layout.total, layout.caps[-1])
+    # (False: there was no room for dS)
+    return done or _backward_general(q, k, v, o, lse, dout, plan, layout, low, done is None)
 
 
 def _backward_again(q, k, v, o, lse, dout, layout, low, repeat):
@@ -320,7 +310,7 @@ def _backward_again(q, k, v, o, lse, dout, layout, low, repeat):
 
 
 @lowering._on_device_of_first_argument
-def _backward_general(q, k, v, o, lse, dout, plan, layout, low, key, room=True):
+def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
     mask, window, scale, cap = _constants(plan, layout.total)
     T, dev = layout.total, q.device
@@ -365,9 +355,10 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, key, room=True):
     repeat = lowering._Repeat(P, launches, {"kernels": names}, (dkdv_at, dq_at, P.ds_sh * Hq if keep_ds else 0))
     res = _backward_again(q, k, v, o, lse, dout, layout, low, repeat)
     if res is None:
-        return _backward_general(q, k, v, o, lse, dout, plan, layout, low, None, False)
-    if key is not None:
-        lowering._keep(key, repeat)
+        return _backward_general(q, k, v, o, lse, dout, plan, layout, low, False)
+    if room:
+        key = lowering._call_key("b", (q, k, v, o, dout), (lse, layout.tiles, low), plan, (T, layout.caps[-1]))
+        lowering._keep_call(key, repeat, repeat.more)
     return res
 
 
@@ -416,9 +407,12 @@ class _Packed(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, plan, layout):
-        lse = torch.empty((q.shape[1], layout.total), dtype=torch.float32, device=q.device)
-        low = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        out = _forward(q, k, v, plan, layout, None, lse, low)
+        done = _host.attention_packed(q, k, v, None, None, layout.tiles, plan, layout.total, layout.caps[-1], True)
+        if done is None:
+            lse = torch.empty((q.shape[1], layout.total), dtype=torch.float32, device=q.device)
+            low = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            done = _forward(q, k, v, plan, layout, None, lse, low), lse, low
+        out, lse, low = done
         ctx.save_for_backward(q, k, v, out, lse, low)
         # (the caller may change a plan)
         ctx.plan = AttnPlan(plan.mask, plan.window, plan.scale, plan.softcap, plan.k_paged, plan.v_paged, plan.denom_add)
@@ -428,3 +422,6 @@ class _Packed(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         return (_gradients_once if torch.is_grad_enabled() else _gradients)(ctx, dout)
+
+
+_host = lowering._host()

@@ -93,10 +93,9 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
     Nothing is raised for what only the GPU knows: where no free page is left, the row of the table is too short or a token lies behind
     ``total``, the token's slot (and the new entry) is -1, which ``store_kv`` leaves out, and ``lengths`` ends in front of it;
     ``pages`` above ``len(free)`` says so.  Slots are numbers in 32 bits: a page behind those counts as none."""
-    key = lowering._call_key("tables", (), (cached, new, table, free), None, (page_size, total))
-    kept = lowering._kept.get(key)
-    if kept is not None:
-        return _tables(cached, new, table, free, total, kept)
+    done = _host.extend_tables(cached, new, table, free, page_size, total)
+    if done is not None:
+        return done
     _on_gpu("cached", cached, (torch.int32,), 1)
     dev, B = cached.device, cached.shape[0]
     _on_gpu("new", new, (torch.int32,), 1, dev)
@@ -120,8 +119,8 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
         repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (max(B, 1), share, 1), 256)], {"kernels": [spec.entry()]},
                                   (2 * B + 2 + 2 * total, (B + 1, B, 1, total, total)))
         step = _tables(packed[0], packed[1], table, packed[2], total, repeat)
-    if key is not None and packed[0] is cached and packed[1] is new and packed[2] is free:
-        lowering._keep(key, repeat)
+        if packed[0] is cached and packed[1] is new and packed[2] is free:
+            lowering._keep_call(lowering._call_key("t", (), (cached, new, table, free), None, (page_size, total)), repeat, (repeat.more[0], *repeat.more[1]))
     return step
 
 
@@ -164,10 +163,8 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     ``slots[t] // page``.  bf16 / fp16, D a multiple of 8; views will do.  ``slots``: int32 [rows] (``PagedStep.slots``); rows whose slot is below 0 or
     behind the pool's last are left out.  Slots that are not left out are distinct, as those of ``extend_tables`` are:
     of two rows with one slot, either may be found there afterwards, or a part of each."""
-    key = lowering._call_key("store", (k, v, k_pool, v_pool), (slots,), None, ())
-    kept = lowering._kept.get(key)
-    if kept is not None:
-        return _store(k, v, k_pool, v_pool, slots, kept)
+    if _host.store_kv(k, v, k_pool, v_pool, slots):
+        return
     if k.dtype not in lowering._DTYPE_CODE:
         raise UnsupportedPlan(f"dtype {k.dtype} not supported (bf16/fp16 only)")
     for name, t in (("K", k), ("V", v), ("K pool", k_pool), ("V pool", v_pool)):
@@ -198,8 +195,8 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
         grid = (-(-T // max(256 // (heads * D // 8), 1)), 1, 1)
         repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), grid, 256)], {"kernels": [spec.entry()]})
         _store(k, v, k_pool, v_pool, packed, repeat)
-    if key is not None and packed is slots:
-        lowering._keep(key, repeat)
+        if packed is slots:
+            lowering._keep_call(lowering._call_key("s", (k, v, k_pool, v_pool), (slots,), None, ()), repeat, ())
 
 
 def _store(k, v, k_pool, v_pool, slots, repeat) -> None:
@@ -267,16 +264,15 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     own keys are streamed, and the partial results are joined in a second launch.  Page ids are trusted, as those of
     ``lowering.attention`` are (``LOOPFUSE_CHECK_TABLES=1`` looks at them).  ``choice`` overrides the rules of the work split: ``{"prefix": "tiles" | "stream", "splits": n,
     "target_log2": n, "least": n, "coop": n, "near": bool}``."""
-    key = None if choice else lowering._call_key("shared", (q, k_pool, v_pool, out), (table, lengths, prefix_table, v_table, prefix_v_table),
-                                                 plan, (prefix_len,))
-    kept = lowering._kept.get(key)
-    if kept is not None:
-        return _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_table, out, kept)
-    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, _whole("prefix_len", prefix_len), v_table, prefix_v_table, out, choice or {}, key)
+    if not choice:
+        done = _host.attention_shared(q, k_pool, v_pool, out, table, lengths, prefix_table, v_table, prefix_v_table, plan, prefix_len)
+        if done is not None:
+            return done
+    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, _whole("prefix_len", prefix_len), v_table, prefix_v_table, out, choice or {})
 
 
 @lowering._on_device_of_first_argument
-def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v_table, prefix_v_table, out, choice, key):
+def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v_table, prefix_v_table, out, choice):
     given = (table, lengths, prefix_table, v_table, prefix_v_table)
     dtype = q.dtype
     if dtype not in lowering._DTYPE_CODE:
@@ -394,9 +390,9 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps], "prefix": "tiles" if tiles else "stream", "splits": splits},
                               ((own + pre) * (D + 2), 4 * own * D, 4 * own * (D + 2), 4 * own * (D + 2) + 4 * pre * D))
     res = _again(q, k_pool, v_pool, table, lengths, prefix_table if prefix_len else None, v_table, prefix_v_table, out, repeat)
-    if key is not None and all(a is b for a, b in zip(given[:3] , (table, lengths, prefix_table))) and (given[3] is None or given[3] is v_table) \
+    if not choice and all(a is b for a, b in zip(given[:3], (table, lengths, prefix_table))) and (given[3] is None or given[3] is v_table) \
             and (given[4] is None or given[4] is prefix_v_table):
-        lowering._keep(key, repeat)
+        lowering._keep_call(lowering._call_key("h", (q, k_pool, v_pool, out), given, plan, (prefix_len,)), repeat, repeat.more)
     return res
 
 
@@ -420,3 +416,5 @@ def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_ta
     lowering._last_launch.set(repeat.record)
     return out
 
+
+_host = lowering._host()

@@ -1,6 +1,6 @@
 """ctypes binding of the C-ABI shim (``liblf_shim.so``, declared in ``include/lf_shim.h``).
 
-This is the only place Python touches native code.  It replaces the reference's
+This and ``_lf_host.so`` (csrc/lf_host.cpp, ``host`` below) are the only places where Python touches native code.  It replaces the reference's
 "write the generated Triton module to a temp file and import it" step
 (reference ``loopfuse/torch_backend/interface.py:624-638``): HIP source goes in,
 a loaded gfx950 kernel handle comes out, and launches go to the HIP stream
@@ -21,6 +21,7 @@ import torch  # noqa: F401  (loaded first so the shim binds to torch's HIP runti
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 SHIM_PATH = os.path.join(_PKG_DIR, "liblf_shim.so")
+HOST_PATH = os.path.join(_PKG_DIR, "_lf_host.so")
 KERNEL_DIR = os.path.join(_PKG_DIR, "csrc", "kernels")
 CACHE_DIR = os.environ.get("LOOPFUSE_CACHE_DIR", os.path.join(_PKG_DIR, "_cache"))
 DEFAULT_ARCH = "gfx950"
@@ -110,6 +111,14 @@ def lib() -> ctypes.CDLL:
         L.lf_device_count.restype = ctypes.c_int
         _lib = L
         return L
+
+
+def host():
+    """The module of csrc/lf_host.cpp, which takes repeated calls of the operators for different lengths."""
+    if not os.path.exists(HOST_PATH):
+        raise RuntimeError(f"{HOST_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    from . import _lf_host
+    return _lf_host
 
 
 def _check(what: str, rc: int) -> None:

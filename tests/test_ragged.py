@@ -195,6 +195,20 @@ def test_shared_calls_that_are_refused(case):
         paged.attention_shared(**shared(**SHARED[case]))
 
 
+def test_the_host_module_leaves_other_operands_to_the_general_path():
+    host = runtime.host()
+    q, k, v = qkv()
+    lay = layout(10)
+    for a in ((q, k, v), tuple(t.as_subclass(torch.Tensor) for t in (q, k, v)), (None, 3, "x")):
+        assert host.attention_packed(*a, None, None, lay.tiles, PLAN, 10, 1, False) is None
+        assert host.key("p", a, (lay.tiles,), PLAN, (10,)) is None
+        assert host.store_kv(*a, v, None) is None
+    assert host.attention_packed(q, k, v, None, None, lay.tiles, object(), 10, 1, False) is None
+    for call in (lambda: host.store_kv(q), lambda: host.key("p", q), lambda: host.keep(b"", b"", b"", {}, None, ()[:0] + (1.5,)), lambda: host.keep(b"", b"x" * 2000, b"", {}, None, ())):
+        with pytest.raises(TypeError):
+            call()
+
+
 def test_a_leaf_of_a_living_graph_is_known():
     q = torch.randn(3, requires_grad=True)
     assert not packed.in_a_graph(q)

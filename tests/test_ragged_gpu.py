@@ -155,7 +155,7 @@ def test_repeated_captured_and_on_another_stream(form):
     run(make(1))
     args, other = make(11), make(21)
     again = run(args)
-    lowering._kept.clear()
+    paged._host.clear()
     want = run(args)
     assert all(torch.equal(x, y) for x, y in zip(again, want))
     side = torch.cuda.Stream()
@@ -409,10 +409,86 @@ def test_dS_is_formed_again_where_there_is_no_room(monkeypatch):
 
     monkeypatch.setattr(torch, "empty", full)
     for _ in range(2):
+        paged._host.clear()
         got = packed.attention_packed_backward(q, k, v, o, lse, g, plan, layout)
         assert lowering._last_launch["kernels"] == ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"]
         # dK and dV keep their bits but for delta, which is summed in another order; dQ its value: products of the same 16-bit dS
         assert all(rel(x, y.double()) <= 2.0 ** -8 for x, y in zip(got, want))
+
+
+def test_dS_is_formed_again_where_a_repeated_call_has_no_room():
+    q, k, v, g, layout = packed_args(4, (4000,), 16, 16, 128)
+    plan, lse = AttnPlan("causal", scale=0.1), torch.empty((16, len(q)), device=DEV)
+    o = packed.attention_packed(q, k, v, plan, layout, lse=lse)
+    for _ in range(2):
+        want = packed.attention_packed_backward(q, k, v, o, lse, g, plan, layout)
+    assert "lf_attn_bwd_delta" in lowering._last_launch["kernels"]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    # room for the results, 100 MB with those of the call before, and not for 266 MB of dS
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (200 << 20)) / torch.cuda.get_device_properties(0).total_memory)
+    try:
+        got = [(packed.attention_packed_backward(q, k, v, o, lse, g, plan, layout), lowering._last_launch["kernels"]) for _ in range(2)]
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    for grads, kernels in got:
+        assert kernels == ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"]
+        assert all(rel(x, y.double()) <= 2.0 ** -8 for x, y in zip(grads, want))
+
+
+def test_repeated_calls_are_taken_by_the_host_module(monkeypatch):
+    """... for plain operands of a signature that ran before; others, and those under another environment, take the general path to the same bits."""
+    paged._host.clear()
+    a = shared_args(7)
+    want = run_shared(a)
+    assert paged._host.size() == 1
+    monkeypatch.setattr(paged, "_shared", None)
+    assert torch.equal(run_shared(a), want)
+    b = shared_args(8)                              # other tensors of the same sizes
+    assert torch.equal(run_shared(b), run_shared(b)) and not torch.equal(run_shared(b), want)
+    out = torch.empty_like(want)
+    monkeypatch.undo()
+    plan = AttnPlan(scale=0.1, k_paged=True, v_paged=True)
+    given = lambda: paged.attention_shared(*a[:3], plan, *a[3:5], prefix_table=a[5], prefix_len=a[6], out=out)
+    assert given() is out and given() is out and torch.equal(out, want)
+    size = paged._host.size()
+    assert size == 2
+    for change in ({"LOOPFUSE_DECODE_COOP": "0"}, {"LOOPFUSE_CHECK_TABLES": "1"}):
+        for name, value in change.items():
+            monkeypatch.setenv(name, value)
+        assert rel(run_shared(a), want.double()) <= TOL
+        monkeypatch.undo()
+    assert paged._host.size() == size + 1           # (the first of the two is a signature of its own)
+    assert torch.equal(run_shared(a), want)
+    # a plan that is changed, and one whose fields are no plain numbers
+    other = AttnPlan(scale=torch.tensor(0.1), k_paged=True, v_paged=True)
+    kept = paged._host.size()
+    with torch.inference_mode():
+        assert torch.equal(run_shared(a), want)
+    assert rel(paged.attention_shared(*a[:3], other, *a[3:5], prefix_table=a[5], prefix_len=a[6]), want.double()) <= TOL
+    assert paged._host.size() == kept
+
+    class Sub(torch.Tensor):
+        pass
+
+    assert torch.equal(run_shared((a[0].as_subclass(Sub), *a[1:])).as_subclass(torch.Tensor), want) and paged._host.size() == kept
+
+
+def test_the_parts_of_a_step_are_tensors_of_their_own():
+    cached, new = i32([3, 0, 40]), i32([1, 20, 5])
+    table, free = torch.zeros((3, 8), dtype=torch.int32, device=DEV), i32(list(range(20)))
+    for _ in range(3):
+        step = paged.extend_tables(cached, new, table, free, 16, 30)
+        assert type(step) is paged.PagedStep and [t.shape[0] for t in step] == [4, 3, 30, 30, 1]
+        assert step.offsets.tolist() == [0, 1, 21, 26] and step.lengths.tolist() == [4, 20, 45] and step.pages.tolist() == [2]
+        assert all(t.dtype == torch.int32 and t.is_contiguous() and not t.requires_grad for t in step)
+        lengths = step.lengths
+        before = step.slots.clone()
+        lengths += 1
+        assert torch.equal(step.slots, before) and (lengths - 1).tolist() == [4, 20, 45]
+        assert lengths.storage_offset() == 4 and step.positions[-4:].tolist() == [-1] * 4
+        del step
+        assert lengths.tolist() == [5, 21, 46]
 
 
 def test_pools_beyond_32_bits():
