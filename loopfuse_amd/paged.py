@@ -230,7 +230,7 @@ def prefix_splits(units: int, keys: int, rows: int, D: int, prefix_bytes: int, o
     """Splits of a prefix on 128-row tiles, the least of a sum: ``units`` workgroups per split, ``keys`` tiles of 64 keys, ``rows`` (request, head)
     pairs, bytes of K and V of the prefix and of what the own keys have room for.  A tile of a chain takes 1.3 us (0.86 at head dimension 64), more
     with more than one workgroup per CU; chains gain nothing below what HBM takes for the prefix and part of the own keys; a split leaves its
-    partial results, 0.46 us per 1000 rows.  225 drawn batches, 2 ... 256 requests of 20 ... 2000 keys behind 500 ... 16 000: 1.025 of the best number's
+    partial results, 0.46 us per 1000 rows.  300 drawn batches, 2 ... 256 requests of 20 ... 2000 keys behind 500 ... 16 000: 1.025 of the best number's
     time in the mean, 1.2 at most.  GPU time, us, by splits, 32/8 heads: 64 requests up to 1024 behind 2048 keys 2 42.5, 3 37.3, 4 38.6, 8 43.7; 128 up to 300
     behind 8208 4 61.5, 8 45.2, 9 42.9, 10 49.8, 15 55.8; 32 up to 100 behind 8000 8 36.2, 16 25.4, 21 28.1, 32 30.0; 8/2 heads, 11 up to 194 behind 4154 8 22.5, 17
     15.3, 33 13.5."""
