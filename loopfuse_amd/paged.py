@@ -206,17 +206,29 @@ def _store(k, v, k_pool, v_pool, slots, repeat) -> None:
     lowering._last_launch.set(repeat.record)
 
 
-def own_loads(D: int, page: int, tiles: bool, keys: int) -> int:
-    """Heads whose waves load whole token rows of the own keys together (``-DLF_COOP=1``), where the pools allow it: 4 at head dimension 128;
-    8 at 64 for many keys in pages shorter than 16 tokens (0: four waves share a head).  ``keys`` = that a call can have in all, without a
-    prefix on ``tiles`` (whose workgroups have 4 waves): up to 4096 the shorter chain of the other form wins.  GPU time, us, 32/8 heads, 128, none / 4 / 8
-    together: 2 requests behind 1000 keys 10.3 / 11.4 / 14.5, 1 of 2000 keys 11.6 / 14.9 / 20.9, 1 of 500 behind 4096 18.2 / 16.9 / 22.6, 8 of 500 behind
-    2000, on tiles, 15.1 / 15.7 / -, 32 of 500 behind 500 28.0 / 17.3 / -, 8 up to 4000 30.7 / 25.3 / 23.6, 128 up to 2000 103 / 102 / 126, 64 up to 1024
-    behind 2048 53 / 39 / -; 64, pages of 16, none / 8: 16 up to 1000 13.4 / 14.9, 8 up to 4000 18.7 / 16.0, 128 up to 2000 63.9 / 72.3; of one token 13.0 /
-    14.6, 17.9 / 16.0, 84.1 / 67.8."""
+def own_loads(D: int, Hkv: int, tiles: bool, requests: int, keys: int) -> int:
+    """Heads whose waves load whole token rows of the own keys together (``-DLF_COOP=1``), where the pools allow it: 4 at head dimension 128, 8 at 64 (0: four
+    waves share a head).  ``keys`` = that a call can have in all, without a prefix on ``tiles`` (whose workgroups have 4 waves).  Each wave then walks
+    its head's keys alone: four times the steps for a fourth of the workgroups, which pays where there are many (request, head) pairs or many keys.  GPU time,
+    us, none / together: 128, 32/8 heads, without a prefix 3 requests up to 128 keys 8.8 / 11.3, 14 up to 510 11.3 / 12.7, 20 up to 60 7.9 / 7.8, 95 up to 512 27.6 / 22.3, 238
+    of 6 21.3 / 11.8; behind 1000 ... 12 000 on tiles 3 up to 1008 15.7 / 15.6, 12 up to 1088 20.1 / 16.3, 38 up to 64 27.7 / 22.7, 157 up to 64 59.9 / 31.7; 64, 32/8
+    heads, 4 up to 110 7.0 / 10.6, 134 of 16 12.7 / 9.2, 55 up to 1904 32.5 / 25.7."""
     if D == 128:
-        return 4 if keys > 4096 else 0
-    return 8 if page < 16 and keys > 24_000 and not tiles else 0
+        return 4 if requests * Hkv >= (100 if tiles else 300) or keys * Hkv > (32_000 if tiles else 64_000) else 0
+    return 8 if not tiles and (requests * Hkv >= 500 or keys > 24_000) else 0
+
+
+def own_pieces(coop: int, workgroups: int, room: int, keys: int) -> tuple:
+    """(log2 of the workgroups that the own keys are cut for, least length of a piece).  ``workgroups`` = with one piece per request, ``room`` = keys that a
+    request can have, ``keys`` = all of them.  About one or two workgroups per CU, four from 150 000 keys on, and of 8 waves half as many of the small calls; pieces of 128 keys,
+    or of 256 where the requests fill the GPU in one piece each and where ends of pieces are few.  300 drawn batches, 1 ... 256 requests of 5 ... 8000 keys, with own_loads:
+    1.025 of the best choice's time in the mean, 1.3 at most; us, by log2: 72 up to 2432
+    keys, 32/8 heads, 8 158, 9 136, 10 123, 134 of 16, D 64, 9.2, 10.7, 13.4; by least length, 128 / 256: 214 of 178, 2/2 heads, 28.3 / 17.5, 78 of 157, 64/8, 25.9 / 17.5, 55 up to
+    1904, D 64, 31.0 / 25.7, 2 up to 3819, 16/4, 15.2 / 20.8."""
+    least = 256 if workgroups >= 128 and room <= 256 else 128
+    if coop == 8:
+        return (8, least) if keys < 50_000 else (9, 256)
+    return (9, least) if keys < 150_000 else (10, least if coop else 256)
 
 
 def prefix_on_tiles(rows: int, prefix_len: int) -> bool:
@@ -356,11 +368,12 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
         near = False
     coop = lowering._decode_coop_waves(3, page, 0, 0, Hkv, P, D)
     if coop:
-        coop = choice.get("coop", own_loads(D, page, tiles, B * P.room + (0 if tiles else prefix_len)))
+        coop = choice.get("coop", own_loads(D, Hkv, tiles, B, B * P.room + (0 if tiles else prefix_len)))
     chunks = -(-group // lowering.DECODE_QROWS)
     heads = Hkv // coop if coop else Hkv
     P.units = heads * chunks
-    P.target_log2, P.least = choice.get("target_log2", 10 if B * P.room >= 100_000 else 9), choice.get("least", 128)
+    target, least = own_pieces(coop, B * P.units, P.room, B * P.room)
+    P.target_log2, P.least = choice.get("target_log2", target), choice.get("least", least)
     items = (1 << P.target_log2) // P.units + B if P.room else 0
     splits = 0
     P.nsplit = P.pre_units = 1
