@@ -45,6 +45,7 @@ typedef struct LfPackedBwdParamsHost {
   const LfPackedTileHost* dkdv_tiles;      /* lists for tiles of as many keys, and queries, as a workgroup has */
   const LfPackedTileHost* dq_tiles;
   const void* low;         /* optional, strides of O: as the forward wrote it */
+  int32_t dkdv_blocks;     /* lf_attn_bwd_both (-DLF_BW_BOTH=1): workgroups of dK and dV, in front of those of dQ */
 } LfPackedBwdParamsHost;
 
 /* lf_attn_decode -DLF_SHARED=1, then lf_shared_combine.  attn: q_sb, q_sh, q_ss = request, kv head, row of its group, o likewise;

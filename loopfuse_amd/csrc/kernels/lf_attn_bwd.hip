@@ -56,7 +56,16 @@ struct LfPackedBwdParams : LfAttnBwdParams {
   const LfPackedTile* dkdv_tiles;      // of as many keys as a workgroup of lf_attn_bwd_dkdv has
   const LfPackedTile* dq_tiles;        // of as many queries as one of lf_attn_bwd_dq has
   const lf_elem* low;                  // optional, strides of O: what rounding left of it
+  int dkdv_blocks;                     // LF_BW_BOTH: workgroups of dK and dV, in front of those of dQ
 };
+#endif
+#ifndef LF_BW_BOTH
+#define LF_BW_BOTH 0       /* 1 (packed, 256 threads, dS not kept): dK, dV and dQ in one launch, lf_attn_bwd_both, behind lf_attn_bwd_delta.
+                              The longest chain of tiles of dK and dV is several times the mean where sequences differ, and dQ fills what it
+                              leaves empty: 24 sequences up to 1000, 16/4 heads of 64, 98 -> 77 us (packed.bwd_both) */
+#endif
+#if LF_BW_BOTH && !LF_PACKED
+#error "one launch for all gradients: packed sequences"
 #endif
 
 #define LF_BW_NT 256
@@ -118,10 +127,40 @@ __device__ __forceinline__ unsigned lf_bw_ds_chunk(int key, int g) {
 
 // delta[row] = sum_d dO[row][d] * O[row][d]; 16 lanes per row, 8 elements per lane
 #if LF_PACKED
+// ... or, of packed rows, as many lanes as a row has pieces of 16 bytes, for LF_BW_DELTA_ROWS rows whose loads go out together, the heads of a row one
+// behind the other, with indexes in 32 bits (Hq T stays below 2^31: the other launches).  Bound by HBM: O, what rounding took from it and dO, 52 MB
+// in 10.7 us at 24 sequences up to 1000, 16 heads of 64 (4.9 TB/s; 13.7 with 16 lanes per row and 64-bit divisions), 226 MB in 42.
+#define LF_BW_DELTA_ROWS 2
 extern "C" __global__ void __launch_bounds__(LF_BW_NT) lf_attn_bwd_delta(const LfPackedBwdParams p) {
+  constexpr unsigned kGroups = LF_BW_NT / LF_CPR;
+  const unsigned group = threadIdx.x / LF_CPR, piece = threadIdx.x % LF_CPR, n = (unsigned)p.Hq * (unsigned)p.Sq;
+  const unsigned first = blockIdx.x * (kGroups * LF_BW_DELTA_ROWS) + group;
+  lf_elem8 ov[LF_BW_DELTA_ROWS], gv[LF_BW_DELTA_ROWS], lv[LF_BW_DELTA_ROWS];
+  unsigned h[LF_BW_DELTA_ROWS], q[LF_BW_DELTA_ROWS];
+#pragma unroll
+  for (int u = 0; u < LF_BW_DELTA_ROWS; ++u) {
+    const unsigned i = min(first + u * kGroups, n - 1);
+    q[u] = i / (unsigned)p.Hq;
+    h[u] = i - q[u] * (unsigned)p.Hq;
+    const long long at = (long long)h[u] * p.o_sh + (long long)q[u] * p.o_ss + 8 * piece;
+    ov[u] = *reinterpret_cast<const lf_elem8*>(p.o + at);
+    gv[u] = *reinterpret_cast<const lf_elem8*>(p.dout + (long long)h[u] * p.do_sh + (long long)q[u] * p.do_ss + 8 * piece);
+    lv[u] = p.low != nullptr ? *reinterpret_cast<const lf_elem8*>(p.low + at) : lf_elem8{};
+  }
+#pragma unroll
+  for (int u = 0; u < LF_BW_DELTA_ROWS; ++u) {
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (float)ov[u][e] * (float)gv[u][e];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (float)lv[u][e] * (float)gv[u][e];
+#pragma unroll
+    for (int d = 1; d < LF_CPR; d <<= 1) s += __shfl_xor(s, d, 64);
+    if (first + u * kGroups < n && piece == 0) p.delta[(long long)h[u] * p.Sq + q[u]] = -s;
+  }
+}
 #else
 extern "C" __global__ void __launch_bounds__(LF_BW_NT) lf_attn_bwd_delta(const LfAttnBwdParams p) {
-#endif
   const long long row = (long long)blockIdx.x * (LF_BW_NT / 16) + threadIdx.x / 16;
   const int piece = threadIdx.x % 16;
   const long long nrows = (long long)p.B * p.Hq * p.Sq;
@@ -134,13 +173,6 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT) lf_attn_bwd_delta(const L
     const lf_elem8 gv = *reinterpret_cast<const lf_elem8*>(p.dout + b * p.do_sb + h * p.do_sh + qi * p.do_ss + 8 * piece);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += (float)ov[e] * (float)gv[e];
-#if LF_PACKED
-    if (p.low != nullptr) {
-      const lf_elem8 lv = *reinterpret_cast<const lf_elem8*>(p.low + h * p.o_sh + qi * p.o_ss + 8 * piece);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += (float)lv[e] * (float)gv[e];
-    }
-#endif
   }
   s += __shfl_xor(s, 1, 64);
   s += __shfl_xor(s, 2, 64);
@@ -148,6 +180,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT) lf_attn_bwd_delta(const L
   s += __shfl_xor(s, 8, 64);
   if (row < nrows && piece == 0) p.delta[row] = -s;
 }
+#endif
 
 // wait for this wave's direct loads and LDS writes, then meet the other waves.  The wait is the
 // builtin, not inline asm, so that the compiler's wait-counter pass sees that nothing is
@@ -401,16 +434,31 @@ template <int kMost, int kMore> __device__ __forceinline__ void lf_bw_wait(int m
 // 89 -> 60 us.
 // With LF_BW_DS the B operands dS also leave for memory, two stores per 32 x 32 block between the MFMAs that take them, and the
 // barrier does not wait for them: 297 -> 340 us of the above for 545 MB (352 with plain stores, which take L2 from Q and dO).
-#if LF_PACKED
+#if LF_BW_BOTH
+#if LF_BW_DS
+#error "one launch for all gradients: dQ forms dS itself"
+#endif
+constexpr int kBwPool = (LF_BW_QSPLIT ? 4 : 3) * (2 * 64 * LF_D * 2 + 2 * 64 * 4);      // of dK and dV; dQ's three stages fit
+__shared__ __attribute__((aligned(256))) unsigned char lf_bw_pool[kBwPool];
+__device__ __forceinline__ void lf_bw_dkdv(const LfPackedBwdParams& pk, const int place) {
+  LfAttnBwdParams p = pk;
+#elif LF_PACKED
 extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const LfPackedBwdParams pk) {
   LfAttnBwdParams p = pk;
+  const int place = (int)blockIdx.x;
 #else
 extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const LfAttnBwdParams p) {
 #endif
   constexpr int KB = LF_BW_W, kKeyWaves = LF_BW_QSPLIT ? 2 : 4, kStages = LF_BW_QSPLIT ? 4 : 3;
   constexpr int kKeys = 32 * KB * kKeyWaves;
+#if LF_BW_BOTH
+  auto& tiles = *reinterpret_cast<lf_elem(*)[kStages][2][64 * LF_D]>(lf_bw_pool);
+  auto& stats = *reinterpret_cast<float(*)[kStages][2][64]>(lf_bw_pool + sizeof(tiles));
+  static_assert(sizeof(tiles) + sizeof(stats) <= kBwPool && LF_BW_NT == LF_BW_DQ_NT && !LF_BW_VL, "both parts fit the pool");
+#else
   __shared__ __attribute__((aligned(256))) lf_elem tiles[kStages][2][64 * LF_D];        // Q, dO
   __shared__ __attribute__((aligned(16))) float stats[kStages][2][64];                  // of the 64 rows: L, start of dP
+#endif
 #if LF_BW_VL
   __shared__ lf_u32x4 v_lds[LF_BW_VL][KB][LF_BW_NT];                               // V^T operands that the registers have no room for
 #endif
@@ -424,7 +472,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
   // All key blocks of a (batch, kv head) share the Q / dO tiles they walk in one XCD's L2; the first key
   // block has the most steps under a causal mask.
 #if LF_PACKED
-  const int entry = (int)blockIdx.x / p.Hkv, hkv = (int)blockIdx.x - entry * p.Hkv, b = 0;
+  const int entry = place / p.Hkv, hkv = place - entry * p.Hkv, b = 0;
   const LfPackedTile mine = lf_packed_tile(pk.dkdv_tiles, entry);
   if (mine.len == 0) return;
   if (mine.seq < 0) {
@@ -1133,14 +1181,22 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
 //   causal B4 H32 S2048 D128 223 -> 222, B2 32/8 S4096 378 -> 373, B2 16/8 S777 35 -> 25, B1 32/8 S2048 85 -> 71
 //   the same with a softcap 383 -> 275; window 256 B4 32/8 S2048 151 -> 107, window 1024 259 -> 179
 //   causal B8 16/4 S1000 D64 fp16 47 -> 42, B16 32/8 S300 48 -> 32
-#if LF_PACKED
+#if LF_BW_BOTH
+__device__ __forceinline__ void lf_bw_dq(const LfPackedBwdParams& pk, const int place) {
+  LfAttnBwdParams p = pk;
+#elif LF_PACKED
 extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_attn_bwd_dq(const LfPackedBwdParams pk) {
   LfAttnBwdParams p = pk;
+  const int place = (int)blockIdx.x;
 #else
 extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_attn_bwd_dq(const LfAttnBwdParams p) {
 #endif
   constexpr int kBM = LF_BW_DQ_NT / 2;                           // query rows of a workgroup
+#if LF_BW_BOTH
+  auto& tiles = *reinterpret_cast<lf_elem(*)[3][2][64 * LF_D]>(lf_bw_pool);
+#else
   __shared__ __attribute__((aligned(256))) lf_elem tiles[3][2][64 * LF_D];        // K, V
+#endif
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -1151,7 +1207,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   // As in lf_attn_bwd_dkdv: the q tiles of all query heads of a (batch, kv head) share its K / V tiles in one
   // XCD's L2, the long q tiles first.
 #if LF_PACKED
-  const int entry = (int)blockIdx.x / p.Hq, head = (int)blockIdx.x - entry * p.Hq, b = 0;
+  const int entry = place / p.Hq, head = place - entry * p.Hq, b = 0;
   const int hkv = head % p.Hkv, h = hkv * (p.Hq / p.Hkv) + head / p.Hkv;
   const LfPackedTile mine = lf_packed_tile(pk.dq_tiles, entry);
   if (mine.len == 0) return;
@@ -1197,7 +1253,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
       qf[ks] = *reinterpret_cast<const lf_u32x4*>(qrow + 16 * ks + 8 * g);
       gf[ks] = *reinterpret_cast<const lf_u32x4*>(grow + 16 * ks + 8 * g);
     }
-#if LF_BW_DQ_NT == 256
+#if LF_BW_DQ_NT == 256 && !LF_BW_BOTH
     // delta of the row, half of its elements in each of two lanes: eight sums of LF_NKS products, then a tree, i.e. chains
     // as short as those of lf_attn_bwd_delta.  dO is in registers here anyway, so this costs a read of O, where a launch of
     // its own reads both.  Both launches against this one, us: causal B8 16/4 S1000 D64 52 / 43, B2 16/8 S777 D128 31 / 26,
@@ -1237,7 +1293,7 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   }
   const long long ridx = ((long long)b * p.Hq + h) * stat_rows + qr;
   const float lse_q = my_q < p.Sq ? p.lse[ridx] : __builtin_inff();
-#if LF_BW_DQ_NT == 256
+#if LF_BW_DQ_NT == 256 && !LF_BW_BOTH
   if (my_q < p.Sq && g == 0) p.delta[ridx] = -delta_q;     // for lf_attn_bwd_dkdv
 #else
   delta_q = my_q < p.Sq ? -p.delta[ridx] : 0.0f;
@@ -1488,5 +1544,15 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
 #endif
   lf_bw_store_rows(dq, lds0 + (unsigned)(wave * LF_BW_ROWS_LDS), p.dq + (long long)b * p.dq_sb + (long long)h * p.dq_sh + (long long)wq0 * p.dq_ss,
                    p.dq_ss, p.Sq - wq0, lane);
+}
+#endif
+
+#if LF_BW_BOTH
+// All gradients of packed sequences in one launch, behind lf_attn_bwd_delta: the workgroups of dK and dV come first, the longest of a group of
+// sequences in front, those of dQ take the places that they leave.
+extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_both(const LfPackedBwdParams pk) {
+  const int place = (int)blockIdx.x;
+  if (place < pk.dkdv_blocks) lf_bw_dkdv(pk, place);
+  else lf_bw_dq(pk, place - pk.dkdv_blocks);
 }
 #endif

@@ -9,7 +9,7 @@
 // ordered by the tiles' work within groups of sequences; which list a launch takes: packed.group_size.
 //   MFMA- and exponential-bound as the dense kernels are, with the longest chain of tiles on top where sequences are few.  bf16 causal, head dim 128, 12
 // sequences up to 2048, 32/8 heads: 175 us (887 TFLOP/s); window 256 and softcap, fp16, 5 up to 4001: 87 us (2.8 TB/s of Q, K, V and O); forward
-// and backward, 8 up to 2048, 32/32 heads 142 + 452 us (646 TFLOP/s), 24 up to 1000, fp16, D 64, 16/4 heads 25 + 97 us (its longest key tile).
+// and backward, 8 up to 2048, 32/32 heads 142 + 452 us (646 TFLOP/s), 24 up to 1000, fp16, D 64, 16/4 heads 25 + 77 us (its longest key tile).
 #ifndef LF_PACKED_HIP_H
 #define LF_PACKED_HIP_H
 

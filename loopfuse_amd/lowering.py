@@ -154,7 +154,7 @@ class KernelSpec:
 
     def files(self) -> tuple[str, ...]:
         kernel = {"prefill": "lf_attn_prefill.hip", "prefill_swp": "lf_attn_prefill_swp.hip",
-                  "decode": "lf_attn_decode.hip", "bwd": "lf_attn_bwd.hip", "packed_plan": "lf_packed_plan.hip",
+                  "decode": "lf_attn_decode.hip", "bwd": "lf_attn_bwd.hip", "bwd_both": "lf_attn_bwd.hip", "packed_plan": "lf_packed_plan.hip",
                   "shared_combine": "lf_shared_combine.hip", "paged_tables": "lf_paged_tables.hip", "store_kv": "lf_store_kv.hip"}[self.family]
         if self.family == "packed_plan":
             return ("lf_common.hip.h", "lf_packed.hip.h", kernel)
@@ -177,7 +177,7 @@ class KernelSpec:
 
     def entry(self) -> str:
         return {"prefill": "lf_attn_prefill", "prefill_swp": "lf_attn_prefill_swp", "decode": "lf_attn_decode",
-                "bwd": "lf_attn_bwd_dq", "packed_plan": "lf_packed_plan", "shared_combine": "lf_shared_combine",
+                "bwd": "lf_attn_bwd_dq", "bwd_both": "lf_attn_bwd_both", "packed_plan": "lf_packed_plan", "shared_combine": "lf_shared_combine",
                 "paged_tables": "lf_paged_tables", "store_kv": "lf_store_kv"}[self.family]
 
     def name(self) -> str:
@@ -234,7 +234,7 @@ def compile_spec(spec: KernelSpec, arch: str = runtime.DEFAULT_ARCH) -> Compiled
     # outside the lock: different specialisations compile concurrently (the shim is re-entrant;
     # two threads asking for the same one both compile, the results are identical)
     code, hit, log = runtime.compile_source(spec.source(), spec.name(), spec.options(), arch)
-    if spec.family == "bwd" and _env("USE_HARDCODE_KERNEL", "0") != "1":
+    if spec.family in ("bwd", "bwd_both") and _env("USE_HARDCODE_KERNEL", "0") != "1":
         # the product kernels hand their accumulators to inline MFMAs as inputs: one that is spilled loses what the loop
         # added to it, and nothing at run time says so
         spilled = {name: n for name, n in runtime.private_segment_bytes(code).items() if n}

@@ -44,7 +44,7 @@ class PackedAttnParams(lowering.AttnParams):
 class PackedBwdParams(lowering.AttnBwdParams):
     """Mirror of ``struct LfPackedBwdParams`` in csrc/kernels/lf_attn_bwd.hip."""
 
-    _fields_ = [("dkdv_tiles", ctypes.c_void_p), ("dq_tiles", ctypes.c_void_p), ("low", ctypes.c_void_p)]
+    _fields_ = [("dkdv_tiles", ctypes.c_void_p), ("dq_tiles", ctypes.c_void_p), ("low", ctypes.c_void_p), ("dkdv_blocks", ctypes.c_int)]
 
 
 @dataclasses.dataclass(frozen=True, eq=False)
@@ -343,13 +343,19 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
         keys = 1
     blocks = ds_blocks(mask, window, T, layout.count)
     keep_ds = room and bwd_keep_ds(D, cap is not None, Hq * blocks)
-    spec = bwd_spec(dtype, D, mask, cap is not None, keys, nt, q_split, lowering.bwd_grads_stay(2 * T * Hq * D), keep_ds)
+    rows = 64 if q_split else 128 * keys
+    both = bwd_both(D, nt, keep_ds)
+    spec = bwd_spec(dtype, D, mask, cap is not None, keys, nt, q_split, lowering.bwd_grads_stay(2 * T * Hq * D), keep_ds, both)
     P.ds_sh = blocks * lowering.BWD_DS_BLOCK
-    dkdv_at, dkdv_entries = layout.tiles_of(64 if q_split else 128 * keys, group_size(mask, 64 // Hkv if Hkv <= 16 else 1))
+    dkdv_at, dkdv_entries = layout.tiles_of(rows, group_size(mask, 64 // Hkv if Hkv <= 16 else 1))
     dq_at, dq_entries = layout.tiles_of(nt // 2, group_size(mask, 64 // Hkv if Hkv <= 16 else 1))
-    steps = {"lf_attn_bwd_delta": (-(-Hq * T // 16), 256), "lf_attn_bwd_dkdv": (_grid(dkdv_entries, Hkv, 256), 256),
+    steps = {"lf_attn_bwd_delta": (-(-Hq * T // (4096 // D)), 256), "lf_attn_bwd_dkdv": (_grid(dkdv_entries, Hkv, 256), 256),
              "lf_attn_bwd_dq": (_grid(dq_entries, Hq, nt), nt)}
     names = ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"] if nt == 256 and not keep_ds else list(steps)
+    if both:
+        P.dkdv_blocks = steps["lf_attn_bwd_dkdv"][0]
+        steps["lf_attn_bwd_both"] = _grid(1, P.dkdv_blocks + steps["lf_attn_bwd_dq"][0], 256), 256
+        names = ["lf_attn_bwd_delta", "lf_attn_bwd_both"]
     named = lowering._kernels_of(spec)
     launches = [(lowering.get_kernel(spec, name, named), (steps[name][0], 1, 1), steps[name][1]) for name in names]
     repeat = lowering._Repeat(P, launches, {"kernels": names}, (dkdv_at, dq_at, P.ds_sh * Hq if keep_ds else 0))
@@ -363,8 +369,17 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
 
 
 def bwd_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool = False, key_blocks: int = 1, dq_threads: int = 512, q_split: bool = False,
-             stay: bool = False, keep_ds: bool = False) -> lowering.KernelSpec:
-    return dataclasses.replace(lowering.bwd_spec(dtype, D, mask, softcap, key_blocks, dq_threads, keep_ds, q_split, stay), packed=True)
+             stay: bool = False, keep_ds: bool = False, both: bool = False) -> lowering.KernelSpec:
+    spec = lowering.bwd_spec(dtype, D, mask, softcap, key_blocks, dq_threads, keep_ds, q_split, stay)
+    return dataclasses.replace(spec, packed=True, **({"family": "bwd_both", "extra": spec.extra + ("-DLF_BW_BOTH=1",)} if both else {}))
+
+
+def bwd_both(D: int, dq_threads: int, keep_ds: bool) -> bool:
+    """All gradients in one launch behind delta's (``-DLF_BW_BOTH=1``), where dQ forms dS itself and two workgroups of it and of dK and dV fit a CU (head
+    dimension 64)?  The longest chain of tiles of dK and dV is several times the mean where sequences differ or are few, and dQ fills what it leaves empty.  us, dQ then dK and dV /
+    delta then all: 24 sequences up to 1000, 16/4 heads 98 / 77, 3 up to 4001, 16/4 304 / 248, 2 up to 4708, 2/1 197 / 121, 5 of 576, 2/2 26 / 17, 28 up to 208, 2/2 17 / 12, 16
+    of 300, 32/8 66 / 64, 64 up to 500, 16/16 88 / 91, 8 of 2048, 32/8 588 / 585, 32/32 608 / 616; 35 batches 0.84 of the time in the mean."""
+    return D == 64 and dq_threads == 256 and not keep_ds
 
 
 def bwd_dq_threads(D: int, mask: int, tiles: int) -> int:

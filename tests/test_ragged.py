@@ -11,6 +11,7 @@ import torch
 
 from loopfuse_amd import lowering, packed, paged, runtime
 from loopfuse_amd.lowering import AttnPlan, UnsupportedPlan
+import test_kernel_codegen as codegen
 
 BF = torch.bfloat16
 
@@ -218,6 +219,31 @@ def test_a_leaf_of_a_living_graph_is_known():
     assert packed.in_a_graph(q)
     del out
     assert not packed.in_a_graph(q)
+
+
+def _both_builds():
+    import __graft_entry__
+    return sorted({s for s in __graft_entry__.ragged_specs() if s.family == "bwd_both"}, key=lambda s: s.name())
+
+
+@pytest.mark.parametrize("spec", _both_builds(), ids=lambda s: s.name()[12:])
+def test_the_launch_of_all_gradients_keeps_its_accumulators(spec):
+    """As for the other backward builds: no spill, results of MFMAs left alone until they are there, and in each of the two parts no other
+    instruction on an AGPR between its first and its last MFMA."""
+    if not os.path.exists(codegen.OBJDUMP):
+        pytest.skip("needs the ROCm LLVM tools")
+    lines = codegen._kernels(spec)["lf_attn_bwd_both"]
+    codegen._check("both", lines)
+    codegen._check_settled("both", lines)
+    mfma = [i for i, ln in enumerate(lines) if ln.startswith("v_mfma")]
+    cut = max(range(1, len(mfma)), key=lambda j: mfma[j] - mfma[j - 1])
+    assert mfma[cut] - mfma[cut - 1] > 200          # (the end of one part and the begin of the other)
+    for part in (mfma[:cut], mfma[cut:]):
+        for ln in lines[part[0]:part[-1]]:
+            assert ln.startswith("v_mfma") or not re.search(r"\ba(\d+|\[\d+:\d+\])", ln), ln
+    for ln in lines:
+        m = re.match(r"v_mfma_\S+ (a\[\d+:\d+\]),.*, (\S+)$", ln)
+        assert m is None or m.group(1) == m.group(2), ln
 
 
 # ---- parameter blocks and rules --------------------------------------------------------------------------------

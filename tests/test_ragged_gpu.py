@@ -491,6 +491,26 @@ def test_the_parts_of_a_step_are_tensors_of_their_own():
         assert lengths.tolist() == [5, 21, 46]
 
 
+@pytest.mark.parametrize("mask,window,cap", [("causal", 0, None), ("sliding", 100, None), (None, 0, None), ("causal", 0, 20.0)])
+def test_gradients_in_one_launch_by_both_splits(monkeypatch, mask, window, cap):
+    """At head dimension 64 all gradients come from one launch; whole keys or queries shared by two waves, dQ keeps its bits and the others differ by the order
+    of their sums.  With a softcap, dS formed again."""
+    q, k, v, g, layout = packed_args(6, (700, 0, 64, 333, 1, 129), 8, 2, 64)
+    plan, lse = AttnPlan(mask, window=window, scale=0.125, softcap=cap), torch.empty((8, len(q)), device=DEV)
+    o = packed.attention_packed(q, k, v, plan, layout, lse=lse)
+    monkeypatch.setattr(packed, "bwd_keep_ds", lambda *a: False)
+    res = []
+    for q_split in (False, True):
+        monkeypatch.setattr(lowering, "bwd_q_split", lambda *a: q_split)
+        paged._host.clear()
+        res.append(packed.attention_packed_backward(q, k, v, o, lse, g, plan, layout))
+        assert lowering._last_launch["kernels"] == ["lf_attn_bwd_delta", "lf_attn_bwd_both"]
+    paged._host.clear()
+    assert torch.equal(res[0][0], res[1][0])
+    for x, y in zip(*res):
+        assert rel(x, y.double()) <= 2.0 ** -8
+
+
 def test_pools_beyond_32_bits():
     """A pool of 5 GiB whose last pages are used, by stores and by both forms of the prefix."""
     pages, page, Hkv, D = 170_000, 16, 8, 128
