@@ -424,6 +424,7 @@ class _Packed(torch.autograd.Function):
     def forward(ctx, q, k, v, plan, layout):
         done = _host.attention_packed(q, k, v, None, None, layout.tiles, plan, layout.total, layout.caps[-1], True)
         if done is None:
+            _heads(q, k, v, layout)
             lse = torch.empty((q.shape[1], layout.total), dtype=torch.float32, device=q.device)
             low = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             done = _forward(q, k, v, plan, layout, None, lse, low), lse, low

@@ -106,6 +106,16 @@ def test_packed_calls_that_are_refused(case, monkeypatch):
         packed.attention_packed(*args, plan, lay, **kw)
 
 
+@pytest.mark.parametrize("case", [c for c in PACKED if "32 bits" not in c])
+def test_packed_calls_with_gradients_that_are_refused(case, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    args, plan, lay, kw = PACKED[case](*qkv())
+    with pytest.raises(UnsupportedPlan):
+        packed.attention_packed(*(t.detach().as_subclass(OnGpu).requires_grad_() for t in args), plan, lay, **kw)
+    with pytest.raises(UnsupportedPlan):
+        packed.attention_packed(args[0].detach()[0, 0].as_subclass(OnGpu).requires_grad_(), *args[1:], plan, lay, **kw)
+
+
 def test_packed_backward_calls_that_are_refused():
     q, k, v = qkv()
     lse = fake((4, 10), torch.float32)

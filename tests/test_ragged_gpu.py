@@ -279,6 +279,32 @@ def test_threads_share_a_stream():
     assert not bad
 
 
+def test_threads_on_streams_of_their_own_and_a_cache_that_is_emptied():
+    forms = ["packed", "packed training", "shared", "shared, no prefix", "tables", "store"]
+    args = {f: [FORMS[f][0](s) for s in (1, 11, 21)] for f in forms}
+    want = {f: [FORMS[f][1](a) for a in args[f]] for f in forms}
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream() if i % 2 else torch.cuda.default_stream()
+        with torch.cuda.stream(stream):
+            for n in range(30):
+                f, j = forms[(n + i) % len(forms)], (n * 7 + i) % 3
+                got = FORMS[f][1](args[f][j])
+                stream.synchronize()
+                if not all(torch.equal(x, y) for x, y in zip(got, want[f][j])):
+                    bad.append((i, n, f))
+                if n % 8 == i:
+                    paged._host.clear()
+                torch.cuda.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
 def test_packed_operands_that_are_views_of_one_projection():
     """Q, K and V as slices of [rows, (Hq + 2 Hkv) D]; an output and a gradient of other strides."""
     lengths, Hq, Hkv, D = (100, 31), 8, 2, 64
