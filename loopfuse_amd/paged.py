@@ -332,8 +332,8 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
             if t.shape[0] * page < prefix_len:
                 raise UnsupportedPlan(f"{name} has room for {t.shape[0] * page} of {prefix_len} keys")
         prefix_table, prefix_v_table = prefix_table.contiguous(), prefix_v_table.contiguous()
-    table = table if table.stride(1) == 1 else table.contiguous()
-    v_table = v_table if v_table.stride(1) == 1 else v_table.contiguous()
+    # (the kernels have 32 bits for the distance of a table's rows)
+    table, v_table = (t if t.stride(1) == 1 and t.stride(0) < 1 << 31 else t.contiguous() for t in (table, v_table))
     lengths = lengths.contiguous()
     if out is not None:
         lowering._check_tensor("O", out, dtype)

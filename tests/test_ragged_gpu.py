@@ -557,6 +557,19 @@ def test_pools_beyond_32_bits():
         assert rel(out[0].transpose(0, 1), want) <= TOL
 
 
+def test_rows_of_a_table_far_apart():
+    a = shared_args(9, lengths=(40, 90))
+    want, wide = run_shared(a), torch.empty(2 ** 31 + 64, dtype=torch.int32, device=DEV)
+    far = wide.as_strided((2, a[3].shape[1]), (2 ** 31 + 8, 1))
+    far.copy_(a[3])
+    for _ in range(2):
+        assert torch.equal(run_shared((*a[:3], far, *a[4:])), want)
+    table = wide.as_strided((2, 8), (2 ** 31 + 8, 1))
+    table.fill_(-1)
+    step = paged.extend_tables(i32([0, 20]), i32([17, 13]), table, i32(list(range(5))), 16, 30)
+    assert table.tolist() == [[0, 1] + [-1] * 6, [-1, -1, 2] + [-1] * 5] and step.slots[:17].tolist() == list(range(17))
+
+
 def test_tables_of_v_of_their_own_and_views_of_tables():
     q, kp, vp, table, n, pre, prefix = shared_args(6)
     want = run_shared((q, kp, vp, table, n, pre, prefix))
