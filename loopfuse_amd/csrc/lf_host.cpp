@@ -3,7 +3,7 @@
 // the environment switches alone.  The first call of such a signature goes through the Python module, which checks it and leaves here the parameter
 // block and the launches (`keep`); the next ones form the signature, the results and the block here.  A function returns None where nothing is
 // kept for the signature, or for operands that are no plain GPU tensors: the Python module then takes the call, or refuses it.
-//   The kernels of small calls run for 3 ... 6 us.  us a call, with the same steps in Python / here: extend_tables 10.9 / 6.2, store_kv of 64 rows 8.3 / 4.6,
+//   The kernels of small calls run for 3 ... 6 us.  us a call, with the same steps in Python / here: extend_tables 10.9 / 6.2, packed_layout, two launches, 16.4 / 7.0, store_kv of 64 rows 8.3 / 4.6,
 // attention_packed of 3 short prompts 10.9 / 6.8, attention_shared of 2 requests, two launches, 15.5 / 10.9, a training step of 24 short sequences, 121 us of
 // kernels, 135 / 123.
 #define PY_SSIZE_T_CLEAN
@@ -198,8 +198,8 @@ at::TensorOptions like(const at::Tensor& t) { return at::TensorOptions().dtype(t
 
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
-// the launches, without the GIL; false: the error is set
-bool launch(const Entry& e, Block& block, void* stream) {
+// the launches, without the GIL; false: the error is set.  `told`: last_launch says so
+bool launch(const Entry& e, Block& block, void* stream, bool told = true) {
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = env.launch(reinterpret_cast<const lf_launch_item*>(e.items.data()), e.count, block.bytes, stream);
@@ -208,7 +208,7 @@ bool launch(const Entry& e, Block& block, void* stream) {
     Py_XDECREF(PyObject_CallFunction(env.fail, "i", rc));
     return false;
   }
-  return PyObject_SetAttr(env.last, name_record, e.record) == 0;
+  return !told || PyObject_SetAttr(env.last, name_record, e.record) == 0;
 }
 
 // ---- module functions ------------------------------------------------------------------------------------------
@@ -330,6 +330,30 @@ PyObject* extend_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_XDECREF(args);
   Py_DECREF(parts);
   return step;
+  END_HANDLE_TH_ERRORS
+}
+
+// packed_layout(offsets, total) -> (tiles, caps); owner: a tuple whose second item is caps; more: entries of the lists, numbers in all
+PyObject* packed_layout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 2)) return nullptr;
+  auto e = find('l', a, 1, 0, nullptr, a + 1, 1);
+  if (!e) return none();
+  const at::Tensor& offsets = THPVariable_Unpack(a[0]);
+  at::Tensor all = made({e->more[1]}, like(offsets));
+  Block block(*e);
+  auto* p = block.as<LfPackedPlanParamsHost>();
+  p->offsets = at_<int32_t>(a[0]);
+  p->tiles = static_cast<LfPackedTileHost*>(all.mutable_data_ptr());
+  p->sorted = reinterpret_cast<int32_t*>(p->tiles + e->more[0]);
+  if (!launch(*e, block, stream_of(offsets), false)) return nullptr;
+  auto tiles = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+  tiles.unsafeGetTensorImpl()->set_sizes_contiguous({e->more[0], 4});
+  PyObject* x = THPVariable_Wrap(std::move(tiles));
+  if (!x) return nullptr;
+  PyObject* r = PyTuple_Pack(2, x, PyTuple_GET_ITEM(e->owner, 1));
+  Py_DECREF(x);
+  return r;
   END_HANDLE_TH_ERRORS
 }
 
@@ -491,7 +515,7 @@ PyObject* attention_packed_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
 
 #define LF_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LF_FAST(setup), LF_FAST(key), LF_FAST(keep), {"clear", clear, METH_NOARGS, nullptr}, {"size", size, METH_NOARGS, nullptr},
-                         LF_FAST(extend_tables), LF_FAST(store_kv), LF_FAST(attention_shared), LF_FAST(attention_packed), LF_FAST(attention_packed_backward),
+                         LF_FAST(packed_layout), LF_FAST(extend_tables), LF_FAST(store_kv), LF_FAST(attention_shared), LF_FAST(attention_packed), LF_FAST(attention_packed_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lf_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -849,9 +849,9 @@ def _call_key(kind: str, data, ints, plan: Optional[AttnPlan], more: tuple):
     return runtime.host().key(kind, data, ints, plan, more)
 
 
-def _keep_call(key, repeat: "_Repeat", more: tuple) -> None:
+def _keep_call(key, repeat: "_Repeat", more: tuple, owner=None) -> None:
     if key is not None:
-        runtime.host().keep(key, repeat.block, bytes(repeat.launches._items), repeat.record, repeat, more)
+        runtime.host().keep(key, repeat.block, bytes(repeat.launches._items), repeat.record, owner or repeat, more)
 
 
 def outside_graphs(fn):

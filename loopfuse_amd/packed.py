@@ -73,6 +73,9 @@ def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
     empty.  Two launches on the current stream, nothing waits for them; the layout serves every call over this batch, forward and
     backward, on that stream or on one that waits for it.  Offsets beyond ``0 ... total`` count as the nearer bound
     (``LOOPFUSE_CHECK_TABLES=1`` raises for them and for descending ones)."""
+    done = _host.packed_layout(offsets, total)
+    if done is not None:
+        return PackedLayout(offsets, total, *done)
     if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 1 or offsets.dtype not in (torch.int32, torch.int64):
         raise UnsupportedPlan("offsets must be an int32 or int64 tensor of one more than the number of sequences")
     if not offsets.is_cuda:
@@ -88,15 +91,18 @@ def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
             ends = offsets.tolist()
             if any(a > b for a, b in zip(ends, ends[1:])) or ends[0] < 0 or ends[-1] > total:
                 raise ValueError(f"loopfuse_amd: offsets must not descend, within 0 ... {total}")
-        offsets = offsets.clamp(0, total).to(torch.int32) if offsets.dtype == torch.int64 else offsets.contiguous()
+        given, offsets = offsets, offsets.clamp(0, total).to(torch.int32) if offsets.dtype == torch.int64 else offsets.contiguous()
         # a sequence ends with a tile that is not full; so do the rows of no sequence at either end
         caps = tuple(total // rows + count + 2 for rows in TILE_HEIGHTS)
         made = torch.empty(4 * len(GROUP_SIZES) * sum(caps) + (3 + len(caps)) * (count + 2), dtype=torch.int32, device=offsets.device)
         tiles = made[:4 * len(GROUP_SIZES) * sum(caps)].view(-1, 4)
         P = _PlanParams(offsets.data_ptr(), tiles.data_ptr(), tiles.data_ptr() + 16 * tiles.shape[0], count, total, caps)
         spec = lowering._spec("packed_plan", 0, 64)
-        runtime.LaunchList([(lowering.get_kernel(spec, "lf_packed_sort"), (-(-(count + 2) // 256), 1, 1), 256),
-                            (lowering.get_kernel(spec, "lf_packed_plan"), (-(-(count + 2) // 4), len(caps) * len(GROUP_SIZES), 1), 256)]).launch(P)
+        repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, "lf_packed_sort"), (-(-(count + 2) // 256), 1, 1), 256),
+                                      (lowering.get_kernel(spec, "lf_packed_plan"), (-(-(count + 2) // 4), len(caps) * len(GROUP_SIZES), 1), 256)], None)
+        repeat.launches.launch(P)
+        if given is offsets:
+            lowering._keep_call(lowering._call_key("l", (), (offsets,), None, (total,)), repeat, (tiles.shape[0], made.shape[0]), (repeat, caps))
     return PackedLayout(offsets, total, tiles, caps)
 
 
