@@ -279,15 +279,26 @@ def heads_per_workgroup(group: int) -> int:
 def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, dout: torch.Tensor,
                               plan: AttnPlan, layout: PackedLayout):
     """Gradients of ``attention_packed(q, k, v, plan, layout)``: ``(dq, dk, dv)`` in the operands' dtype, zeros in rows of no
-    sequence.  ``o`` and ``lse`` are the forward's output and row log-sum-exp.  As ``lowering.attention_backward``: delta with dQ
-    or in front of it, dK and dV, no atomics."""
+    sequence.  ``o`` and ``lse`` are the forward's output and row log-sum-exp; Q, K, V and dO whose rows are not apart (one row expanded)
+    are copied.  As ``lowering.attention_backward``: delta with dQ or in front of it, dK and dV, no atomics."""
     if not isinstance(layout, PackedLayout):
         raise UnsupportedPlan("layout must come from packed_layout")
     return _backward(q, k, v, o, lse, dout, plan, layout)
 
 
+def rows_apart(t):
+    """``t`` or, where rows lie closer than a row is long (one row expanded over all), a copy.  The kernels take what lies behind a sequence's last
+    row for zeros, which the ranges of their buffers make of it only where it lies behind that row's last element too."""
+    return t if t.dim() != 3 or t.stride(0) >= t.shape[2] else t.clone(memory_format=torch.contiguous_format)
+
+
 def _backward(q, k, v, o, lse, dout, plan, layout, low=None):
     done = _host.attention_packed_backward(q, k, v, o, dout, lse, layout.tiles, low, plan, layout.total, layout.caps[-1])
+    if done is None:      # (operands with rows that are not apart are of no signature that is kept)
+        apart = [rows_apart(t) for t in (q, k, v, dout)]
+        if any(a is not b for a, b in zip(apart, (q, k, v, dout))):
+            q, k, v, dout = apart
+            done = _host.attention_packed_backward(q, k, v, o, dout, lse, layout.tiles, low, plan, layout.total, layout.caps[-1])
     # (False: there was no room for dS)
     return done or _backward_general(q, k, v, o, lse, dout, plan, layout, low, done is None)
 
@@ -327,7 +338,7 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
     if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or not lse.is_contiguous() or lse.device != dev:
         raise UnsupportedPlan(f"lse must be a contiguous float32 [{Hq}, {T}] tensor on the device of Q")
     for name, t in (("Q", q), ("dO", dout), ("K", k), ("V", v)):
-        if t.stride(0) < 0 or 2 * (T + 64) * t.stride(0) + 2 * D >= 1 << 32:
+        if t.stride(0) < D or 2 * (T + 64) * t.stride(0) + 2 * D >= 1 << 32:
             raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
     if T == 0:
         return tuple(torch.empty(t.shape, dtype=dtype, device=dev) for t in (q, k, v))
