@@ -26,6 +26,8 @@ from .lowering import AttnPlan, UnsupportedPlan
 
 TILE_HEIGHTS = (32, 64, 128, 256)      # rows of a tile, lists by lists
 GROUP_SIZES = (1, 2, 4, 8)             # sequences whose tiles come together, list by list
+MAX_ROWS = (1 << 31) - 1024            # of a packed batch
+MAX_SEQUENCES = 1 << 22                # each is ranked among all of them, some seconds for so many
 
 
 class _PlanParams(ctypes.Structure):
@@ -68,8 +70,8 @@ class PackedLayout:
 
 @lowering.outside_graphs
 def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
-    """The layout of a batch of ``N`` packed sequences: sequence ``n`` is rows ``offsets[n] ... offsets[n + 1]`` of tensors of
-    ``total`` rows.  ``offsets``: int32 or int64 ``[N + 1]`` on the GPU, not descending (as a cumulative sum of the lengths is); sequences may be
+    """The layout of a batch of ``N`` packed sequences, ``MAX_SEQUENCES`` at most: sequence ``n`` is rows ``offsets[n] ... offsets[n + 1]`` of
+    tensors of ``total`` rows, ``MAX_ROWS`` at most.  ``offsets``: int32 or int64 ``[N + 1]`` on the GPU, not descending (as a cumulative sum of the lengths is); sequences may be
     empty.  Two launches on the current stream, nothing waits for them; the layout serves every call over this batch, forward and
     backward, on that stream or on one that waits for it.  Offsets beyond ``0 ... total`` count as the nearer bound
     (``LOOPFUSE_CHECK_TABLES=1`` raises for them and for descending ones)."""
@@ -83,8 +85,11 @@ def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
     if isinstance(total, torch.Tensor):
         raise UnsupportedPlan("the number of rows must be a number of the host's")
     total = operator.index(total)
-    if total < 0 or total >= 1 << 31:
-        raise UnsupportedPlan("the number of rows must be between 0 and 2**31 - 1")
+    # (the kernels round rows up to tiles, and walk a few tiles ahead, in 32 bits)
+    if total < 0 or total > MAX_ROWS:
+        raise UnsupportedPlan(f"the number of rows must be between 0 and {MAX_ROWS}")
+    if offsets.shape[0] > MAX_SEQUENCES + 1:
+        raise UnsupportedPlan(f"more than {MAX_SEQUENCES} sequences")
     with torch.cuda.device(offsets.device):
         count = offsets.shape[0] - 1
         if lowering._checks_tables():

@@ -1,0 +1,25 @@
+"""The largest sizes, overridden choices and derivatives that the operators for different lengths refuse; how they lay out what they keep; no GPU."""
+import pytest
+import torch
+
+from loopfuse_amd import packed
+from loopfuse_amd.lowering import UnsupportedPlan
+from test_ragged import fake, nothing_is_launched  # noqa: F401  (a fixture that every test here uses)
+
+
+@pytest.mark.parametrize("total", [(1 << 31) - 1, (1 << 31) - 256, packed.MAX_ROWS + 1])
+def test_layouts_whose_tiles_do_not_fit_32_bits(total):
+    with pytest.raises(UnsupportedPlan):
+        packed.packed_layout(fake((3,), torch.int32), total)
+
+
+def test_rows_up_to_the_most_fit_32_bits_when_rounded_up():
+    # lf_packed_sort and lf_packed_plan add a tile's rows less one, the attention kernels walk three tiles of 64 behind the last one
+    assert packed.MAX_ROWS + max(packed.TILE_HEIGHTS) + 4 * 64 < 1 << 31
+
+
+def test_more_sequences_than_can_be_ranked():
+    with pytest.raises(UnsupportedPlan):
+        packed.packed_layout(fake((1,), torch.int32).expand(packed.MAX_SEQUENCES + 2), 1000)
+    # [3 + 4 heights][sequences + 2] numbers, indexed in 32 bits
+    assert 7 * (packed.MAX_SEQUENCES + 2) < 1 << 31
