@@ -24,6 +24,7 @@ from . import lowering
 from .lowering import AttnPlan, UnsupportedPlan
 
 _TABLE_DTYPES = (torch.int32, torch.int64)
+MAX_REQUESTS = 1 << 22      # of extend_tables, in which each forms its sums over all of them: a second or two for so many
 
 
 class _TablesParams(ctypes.Structure):
@@ -103,6 +104,8 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
     _on_gpu("free", free, (table.dtype,), 1, dev)
     if new.shape[0] != B or table.shape[0] != B:
         raise UnsupportedPlan(f"new and table must be of {B} requests")
+    if B > MAX_REQUESTS:
+        raise UnsupportedPlan(f"more than {MAX_REQUESTS} requests")
     if table.shape[1] and B and table.stride(1) != 1 or (B > 1 and table.stride(0) < table.shape[1]):
         raise UnsupportedPlan("rows of the table must be contiguous and apart")
     shift, total = _shift(page_size), _whole("total", total)
@@ -184,6 +187,10 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     shift = _shift(page)
     if T == 0 or pages == 0 or heads == 0 or D == 0:
         return
+    # (the kernel numbers rows in 32 bits, up to the end of the last block)
+    blocks = -(-T // max(256 // (heads * D // 8), 1))
+    if T > (1 << 31) - 256 or blocks * 256 >= 1 << 32:
+        raise UnsupportedPlan(f"a launch for {T} rows of {heads} heads of {D} is too large")
     with torch.cuda.device(k.device):
         if lowering._checks_tables():
             kept_slots = slots[slots >= 0]
@@ -192,8 +199,7 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
         packed = slots.contiguous()
         P = _StoreParams(0, 0, 0, 0, 0, *(x // 8 for x in (*k.stride()[:2], *v.stride()[:2], *ks, *vs)), pages * page, T, heads, D // 8, shift)
         spec = lowering._spec("store_kv", 0, 64)
-        grid = (-(-T // max(256 // (heads * D // 8), 1)), 1, 1)
-        repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), grid, 256)], {"kernels": [spec.entry()]})
+        repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (blocks, 1, 1), 256)], {"kernels": [spec.entry()]})
         _store(k, v, k_pool, v_pool, packed, repeat)
         if packed is slots:
             lowering._keep_call(lowering._call_key("s", (k, v, k_pool, v_pool), (slots,), None, ()), repeat, ())

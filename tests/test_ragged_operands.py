@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from loopfuse_amd import packed
+from loopfuse_amd import packed, paged
 from loopfuse_amd.lowering import UnsupportedPlan
 from test_ragged import fake, nothing_is_launched  # noqa: F401  (a fixture that every test here uses)
 
@@ -23,3 +23,16 @@ def test_more_sequences_than_can_be_ranked():
         packed.packed_layout(fake((1,), torch.int32).expand(packed.MAX_SEQUENCES + 2), 1000)
     # [3 + 4 heights][sequences + 2] numbers, indexed in 32 bits
     assert 7 * (packed.MAX_SEQUENCES + 2) < 1 << 31
+
+
+@pytest.mark.parametrize("T,heads,D", [((1 << 31) - 1, 1, 8), (1 << 31, 1, 8), ((1 << 31) - 255, 1, 8), (1 << 24, 32, 128)])
+def test_stores_whose_rows_pass_32_bits(T, heads, D):
+    k, pool = fake((1, heads, D)).expand(T, heads, D), fake((2, 4, heads, D))
+    with pytest.raises(UnsupportedPlan):
+        paged.store_kv(k, k, pool, pool, fake((1,), torch.int32).expand(T))
+
+
+def test_more_requests_than_can_be_summed():
+    many = fake((1,), torch.int32).expand(paged.MAX_REQUESTS + 1)
+    with pytest.raises(UnsupportedPlan):
+        paged.extend_tables(many, many, fake((paged.MAX_REQUESTS + 1, 1), torch.int32), fake((4,), torch.int32), 16, 10)
