@@ -5,13 +5,14 @@
 //   table[b, have + i] = free[first + i], i < need,
 //   offsets[b] = sum of `new` of the requests before it: the packed row of its first new token,
 //   positions[offsets[b] + t] = c + t, slots[...] = table[b, (c + t) / P] * P + (c + t) % P, t < n,
-//   lengths[b] = c + the number of its new tokens that fit.
+//   lengths[b] = c + the number of its new tokens in front of the first that has no slot.
 // A block has one request (and a share of its tokens): it forms the two sums itself from all B lengths, which are in L2 after the first
 // block, so that no block waits for another.  Slots of new pages come from the list of free ones, not from the table, so blocks of one
 // request do not wait for each other's entries either.  Bound by its chain of round trips (lengths, then the page, then the stores): 64 requests of one
 // new token 4.1 us, 256 of 2048 and fewer (2.2 MB) 6.1, as long as the call takes the host.
-// What does not fit -- no free page left, a row of the table too short, a token behind the last row -- gets page and slot -1 and is not
-// counted, so that nothing reads keys that are not there: of each kind it is the request's last tokens.
+// What does not fit -- no free page left, a row of the table too short, a token behind the last row -- gets page and slot -1.  A page id below 0 or
+// whose slots are no numbers in 32 bits is no page either: its tokens get slot -1.  lengths[b] ends in front of the first token without a slot,
+// so that nothing reads keys that are not there.
 
 struct LfTablesParams {
   const int* cached;          // [B]
@@ -31,6 +32,7 @@ struct LfTablesParams {
 #define LF_TABLES_NT 256
 extern "C" __global__ void __launch_bounds__(LF_TABLES_NT) lf_paged_tables(const LfTablesParams p) {
   __shared__ long long parts[4][LF_TABLES_NT / 64];
+  __shared__ int nones[LF_TABLES_NT / 64];
   const int tid = threadIdx.x, b = blockIdx.x, up = (1 << p.shift) - 1;
   auto cached = [&](int j) -> long long { return max(p.cached[j], 0); };
   auto fresh = [&](int j) -> long long { return max(p.fresh[j], 0); };
@@ -60,23 +62,40 @@ extern "C" __global__ void __launch_bounds__(LF_TABLES_NT) lf_paged_tables(const
   }
   const long long row = sum[0], rows = sum[1], first = sum[2];
   auto clamp32 = [](long long x) { return (int)min(x, 0x7fffffffll); };
-  auto page_at = [&](long long i) -> lf_table_t { return i < p.count ? p.free[i] : (lf_table_t)-1; };
   const int share = blockIdx.y * LF_TABLES_NT + tid, step = gridDim.y * LF_TABLES_NT;
   if (b < p.B) {
     const long long c = cached(b), n = fresh(b), have = pages(c), need = pages(c + n) - have;
     lf_table_t* mine = p.table + b * p.table_stride;
-    const long long end = min(n, p.T - row);
-    if (share == 0) {
-      const long long named = min((long long)p.width, have + min(need, max(p.count - first, 0ll)));      // entries of its row that name pages
-      p.offsets[b] = clamp32(row);
-      p.lengths[b] = clamp32(c + max(0ll, min(end, (named << p.shift) - c)));
+    const long long end = min(n, p.T - row);      // new tokens that have a row
+    auto new_page = [&](long long i) -> lf_table_t { return first + i < p.count ? p.free[first + i] : (lf_table_t)-1; };
+    // the page of entry `at` if a slot of it is a number in 32 bits, else -1
+    auto page_at = [&](long long at) -> lf_table_t {
+      const lf_table_t page = at >= p.width ? (lf_table_t)-1 : at < have ? mine[at] : new_page(at - have);
+      return page > (0x7fffffff >> p.shift) ? (lf_table_t)-1 : page;
+    };
+    if (blockIdx.y == 0) {
+      // the first of the new tokens' pages that is none ends the request
+      const long long from = c >> p.shift;
+      const int count = end > 0 ? (int)(((c + end - 1) >> p.shift) - from) + 1 : 0;
+      int none = count;
+      for (long long i = tid; i < none; i += LF_TABLES_NT)
+        if (page_at(from + i) < 0) none = (int)i;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) none = min(none, __shfl_xor(none, d, 64));
+      if (tid % 64 == 0) nones[tid / 64] = none;
+      __syncthreads();
+      if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < LF_TABLES_NT / 64; ++w) none = min(none, nones[w]);
+        p.offsets[b] = clamp32(row);
+        p.lengths[b] = clamp32(c + max(0ll, none < count ? ((from + none) << p.shift) - c : end));
+      }
     }
-    for (long long i = share; i < need && have + i < p.width; i += step) mine[have + i] = page_at(first + i);
+    for (long long i = share; i < need && have + i < p.width; i += step) mine[have + i] = new_page(i);
     for (long long t = share; t < end; t += step) {
-      const long long at = (c + t) >> p.shift;
-      const lf_table_t page = at >= p.width ? (lf_table_t)-1 : at < have ? mine[at] : page_at(first + at - have);
+      const lf_table_t page = page_at((c + t) >> p.shift);
       p.positions[row + t] = clamp32(c + t);
-      p.slots[row + t] = page < 0 || page > (0x7fffffff >> p.shift) ? -1 : (int)((page << p.shift) | ((c + t) & up));
+      p.slots[row + t] = page < 0 ? -1 : (int)((page << p.shift) | ((c + t) & up));
     }
   }
   if (b == 0 && share == 0) {

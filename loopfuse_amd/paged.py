@@ -93,7 +93,8 @@ def extend_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, 
 
     Nothing is raised for what only the GPU knows: where no free page is left, the row of the table is too short or a token lies behind
     ``total``, the token's slot (and the new entry) is -1, which ``store_kv`` leaves out, and ``lengths`` ends in front of it;
-    ``pages`` above ``len(free)`` says so.  Slots are numbers in 32 bits: a page behind those counts as none."""
+    ``pages`` above ``len(free)`` says so.  Slots are numbers in 32 bits: a page behind those counts as none, and so does one below 0
+    (``LOOPFUSE_CHECK_TABLES=1`` raises for all of these)."""
     done = _host.extend_tables(cached, new, table, free, page_size, total)
     if done is not None:
         return done
@@ -133,6 +134,8 @@ def _check_extension(cached, new, table, free, page_size, total) -> None:
     need, width, rows = int((pages - (c + page_size - 1) // page_size).sum()), int(pages.max()) if len(c) else 0, int(n.sum())
     if need > free.shape[0] or width > table.shape[1] or rows > total:
         raise ValueError(f"loopfuse_amd: {need} pages of {free.shape[0]} free ones, tables of {width} of {table.shape[1]} entries, {rows} of {total} rows")
+    if need and (int(free[:need].min()) < 0 or int(free[:need].max()) > ((1 << 31) - 1) // page_size):
+        raise ValueError(f"loopfuse_amd: free pages must be between 0 and {((1 << 31) - 1) // page_size}")
 
 
 def _tables(cached, new, table, free, total, repeat) -> PagedStep:

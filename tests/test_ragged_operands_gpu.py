@@ -3,7 +3,7 @@ pages that are none, the largest sizes."""
 import pytest
 import torch
 
-from loopfuse_amd import packed
+from loopfuse_amd import packed, paged
 from loopfuse_amd.lowering import AttnPlan
 from test_packed_gpu import check, inputs, layout_of, oracle
 
@@ -61,3 +61,61 @@ def test_operands_whose_rows_are_one(D, mask):
             a, b = ([x.detach().requires_grad_(True) for x in y] for y in (views, copies))
             a, b = (torch.autograd.grad(packed.attention_packed(*y, plan, layout), y, g) for y in (a, b))
             assert all(torch.equal(x, y) for x, y in zip(a, b)), (i, t.stride())
+
+
+# ---- pages that are none -----------------------------------------------------------------------------------------------------
+
+def plain_lengths(cached, new, table, free, page, total):
+    """Tokens of each request in front of the first new one that has no slot, from the slots of plain loops."""
+    taken, row, out, slots = 0, 0, [], []
+    for b, (c, n) in enumerate(zip(cached, new)):
+        pages = dict(enumerate(table[b]))
+        for i in range(-(-c // page), -(-(c + n) // page)):
+            pages[i] = free[taken] if taken < len(free) and i < len(table[b]) else -1
+            taken += 1
+        mine = []
+        for t in range(c, c + n):
+            id_ = pages[t // page] if t // page < len(table[b]) else -1
+            mine.append(id_ * page + t % page if 0 <= id_ <= (2 ** 31 - 1) // page else -1)
+        mine = mine[:max(0, total - row)]
+        out.append(c + (mine.index(-1) if -1 in mine else len(mine)))
+        row, slots = row + n, slots + mine
+    return out, slots
+
+
+NONE = [
+    # cached, new, table, free, page size, rows
+    ([0, 3, 20], [40, 20, 1], [[7] * 4] * 3, [5, -1, 9, -1, 11], 16, 61),
+    ([0] * 4, [16] * 4, [[0]] * 4, [2 ** 27 - 1, 2 ** 27, 2 ** 28, 2 ** 31 - 1], 16, 64),
+    ([5, 5], [3, 30], [[-1, 0, 0], [2 ** 27, 0, 0]], [4, 6], 16, 33),          # the page that a request's next token goes to
+    ([8], [500], [[0] * 600], list(range(1, 300)) + [-1] + list(range(300, 400)), 1, 508),
+    ([8], [5000], [[0] * 5100], list(range(1, 4700)) + [-7] + list(range(4700, 5200)), 1, 5000),
+    ([1, 16, 0], [40, 0, 40], [[3, 0, 0]] * 3, [9, 8, -1, -1, 5], 16, 70),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("case", range(len(NONE)))
+def test_lengths_end_in_front_of_a_token_without_a_slot(case, dtype):
+    cached, new, table, free, page, total = NONE[case]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    lengths, slots = plain_lengths(cached, new, table, free, page, total)
+    for _ in range(2):
+        step = paged.extend_tables(i32(cached), i32(new), torch.tensor(table, dtype=dtype, device=DEV), torch.tensor(free, dtype=dtype, device=DEV), page, total)
+        assert step.lengths.tolist() == lengths and step.slots.tolist() == slots + [-1] * (total - len(slots))
+
+
+def test_pages_beyond_64_bit_numbers_of_slots_are_none():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    step = paged.extend_tables(i32([0, 3]), i32([33, 2]), torch.tensor([[0] * 3, [2 ** 40] * 3], device=DEV), torch.tensor([4, 2 ** 33 + 1, 6], device=DEV), 16, 40)
+    assert step.lengths.tolist() == [16, 3] and step.slots.tolist() == list(range(64, 80)) + [-1] * 16 + [96] + [-1] * 7
+
+
+def test_checked_free_pages(monkeypatch):
+    monkeypatch.setenv("LOOPFUSE_CHECK_TABLES", "1")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    extend = lambda free: paged.extend_tables(i32([0]), i32([17]), i32([[0, 0]]), i32(free), 16, 17)
+    for free in ([1, -1], [1, 2 ** 27]):
+        with pytest.raises(ValueError):
+            extend(free)
+    assert extend([1, 2 ** 27 - 1, -1]).lengths.tolist() == [17]      # (one that is not taken)
