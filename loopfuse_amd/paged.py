@@ -263,6 +263,18 @@ def prefix_splits(units: int, keys: int, rows: int, D: int, prefix_bytes: int, o
     return best[1]
 
 
+def _checked_choice(choice: dict) -> dict:
+    """An override of the rules of the work split whose values the kernels serve: pieces begin at whole steps of 16 keys, in pairs, and are rounded up
+    in 32 bits; partial results are kept for every piece that the own keys are cut for."""
+    number = lambda lo, hi: lambda x: isinstance(x, int) and not isinstance(x, bool) and lo <= x <= hi
+    served = {"prefix": lambda x: x in ("tiles", "stream"), "splits": number(0, 1 << 30), "target_log2": number(0, 24), "coop": lambda x: number(0, 8)(x) and x % 4 == 0,
+              "least": lambda x: number(0, 1 << 30)(x) and x % 32 == 0, "near": lambda x: isinstance(x, bool)}
+    for name, x in choice.items():
+        if name not in served or not served[name](x):
+            raise UnsupportedPlan(f"choice {name!r}: {x!r} not served")
+    return choice
+
+
 def combine_grid(B: int, Hq: int, D: int) -> int:
     """Blocks of lf_shared_combine: 1024 / D rows of one request each, or one row whose parts the block's groups of threads share."""
     return B * Hq if B * Hq <= 1024 else B * -(-Hq // (1024 // D))
@@ -284,12 +296,13 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     The prefix is read once for all requests together: its keys meet the rows of the whole batch as a matrix product, the requests'
     own keys are streamed, and the partial results are joined in a second launch.  Page ids are trusted, as those of
     ``lowering.attention`` are (``LOOPFUSE_CHECK_TABLES=1`` looks at them).  ``choice`` overrides the rules of the work split: ``{"prefix": "tiles" | "stream", "splits": n,
-    "target_log2": n, "least": n, "coop": n, "near": bool}``."""
+    "target_log2": n, "least": n, "coop": n, "near": bool}``: splits 64 at most, target_log2 0 ... 24, least a multiple of 32, coop 0, or 4 or 8 heads where
+    ``own_loads`` could have its own."""
     if not choice:
         done = _host.attention_shared(q, k_pool, v_pool, out, table, lengths, prefix_table, v_table, prefix_v_table, plan, prefix_len)
         if done is not None:
             return done
-    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, _whole("prefix_len", prefix_len), v_table, prefix_v_table, out, choice or {})
+    return _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, _whole("prefix_len", prefix_len), v_table, prefix_v_table, out, _checked_choice(choice or {}))
 
 
 @lowering._on_device_of_first_argument
@@ -376,6 +389,8 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     if tiles and not choice.get("near", True) and page % 8 == 0:
         near = False
     coop = lowering._decode_coop_waves(3, page, 0, 0, Hkv, P, D)
+    if choice.get("coop") and (not coop or Hkv % choice["coop"] or choice["coop"] * D < 512 or (tiles and choice["coop"] != 4)):
+        raise UnsupportedPlan(f"choice 'coop': {choice['coop']} heads of {Hkv} of {D}")
     if coop:
         coop = choice.get("coop", own_loads(D, Hkv, tiles, B, B * P.room + (0 if tiles else prefix_len)))
     chunks = -(-group // lowering.DECODE_QROWS)

@@ -4,7 +4,7 @@ import torch
 
 from loopfuse_amd import packed, paged
 from loopfuse_amd.lowering import UnsupportedPlan
-from test_ragged import fake, nothing_is_launched  # noqa: F401  (a fixture that every test here uses)
+from test_ragged import fake, nothing_is_launched, pools, shared  # noqa: F401  (a fixture that every test here uses)
 
 
 @pytest.mark.parametrize("total", [(1 << 31) - 1, (1 << 31) - 256, packed.MAX_ROWS + 1])
@@ -36,3 +36,28 @@ def test_more_requests_than_can_be_summed():
     many = fake((1,), torch.int32).expand(paged.MAX_REQUESTS + 1)
     with pytest.raises(UnsupportedPlan):
         paged.extend_tables(many, many, fake((paged.MAX_REQUESTS + 1, 1), torch.int32), fake((4,), torch.int32), 16, 10)
+
+
+CHOICES = [{"prefix": "rows"}, {"splits": -1}, {"splits": 2.0}, {"target_log2": -1}, {"target_log2": 25}, {"least": -32}, {"least": 48}, {"least": (1 << 30) + 32},
+           {"coop": 3}, {"coop": True}, {"near": 1}, {"other": 1}, {"coop": 8}, {"coop": 4, "prefix": "tiles"}]
+
+
+@pytest.mark.parametrize("choice", CHOICES, ids=str)
+def test_choices_that_are_refused(choice):
+    # (2 heads of 64: no heads to load together)
+    with pytest.raises(UnsupportedPlan, match="choice"):
+        paged.attention_shared(**shared(choice=choice))
+
+
+@pytest.mark.parametrize("Hkv,D,choice", [(8, 128, {"coop": 8, "prefix": "tiles"}), (4, 128, {"coop": 8}), (6, 128, {"coop": 4}), (4, 64, {"coop": 4}), (4, 64, {"coop": 8})], ids=str)
+def test_heads_that_are_not_loaded_together(Hkv, D, choice):
+    kp, vp = pools(9, 4, Hkv, D)
+    with pytest.raises(UnsupportedPlan, match="coop"):
+        paged.attention_shared(**shared(q=fake((3, 2 * Hkv, 1, D)), k_pool=kp, v_pool=vp, choice=choice))
+
+
+@pytest.mark.parametrize("Hkv,D,choice", [(8, 128, {"coop": 8, "prefix": "stream"}), (4, 128, {"coop": 4, "prefix": "tiles"}), (8, 64, {"coop": 8, "prefix": "stream"}), (8, 128, {"coop": 0})], ids=str)
+def test_heads_that_are_loaded_together(Hkv, D, choice):
+    kp, vp = pools(9, 4, Hkv, D)
+    with pytest.raises(AssertionError, match="a launch"):
+        paged.attention_shared(**shared(q=fake((3, 2 * Hkv, 1, D)), k_pool=kp, v_pool=vp, choice=choice))
