@@ -93,13 +93,13 @@ bool put_plain(std::string& s, PyObject* o) {
   return true;
 }
 
-// a plain GPU tensor: no subclass, no wrapper of a transform, nothing pending
+// a plain GPU tensor: no subclass, no wrapper of a transform, nothing pending, no tangent
 const at::Tensor* plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.is_neg() || t.is_conj() ||
       t.unsafeGetTensorImpl()->is_python_dispatch() || t.unsafeGetTensorImpl()->has_symbolic_sizes_strides() ||
-      t.key_set().has(at::DispatchKey::Functionalize))
+      t.key_set().has(at::DispatchKey::Functionalize) || t._fw_grad(0).defined())
     return nullptr;
   return &t;
 }

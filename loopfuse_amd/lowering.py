@@ -864,6 +864,13 @@ def outside_graphs(fn):
     return call
 
 
+def _no_tangents(*tensors) -> None:
+    """Refuse forward-mode derivatives (``torch.autograd.forward_ad``), of which the result of an operator would say nothing."""
+    ad = torch.autograd.forward_ad
+    if getattr(ad, "_current_level", 0) >= 0 and any(isinstance(t, torch.Tensor) and ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise UnsupportedPlan("operands carry tangents: forward-mode derivatives are not formed")
+
+
 def _checks_tables() -> bool:
     """LOOPFUSE_CHECK_TABLES=1: index tensors are looked at before the launches (waits for the stream, which a capture forbids)."""
     return _env("LOOPFUSE_CHECK_TABLES", "0") == "1" and not torch.cuda.is_current_stream_capturing()

@@ -173,7 +173,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
 
     Inside ``torch.compile`` the call runs as it is, between two graphs.
 
-    Differentiable where gradients are recorded and neither ``out`` nor ``lse`` is given; gradients of rows of no sequence are zero.
+    Differentiable where gradients are recorded and neither ``out`` nor ``lse`` is given; gradients of rows of no sequence are zero.  Forward-mode
+    derivatives are refused.
     Under graph capture a leaf that another autograd graph holds is refused: capture forward and backward with no eager graph of them alive.
     Kept for the backward besides Q, K, V and O: lse, and what rounding takes from O, as large as O (it halves what delta is off by)."""
     if not isinstance(layout, PackedLayout):
@@ -191,6 +192,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
         q, k, v = (torch.nn.functional.pad(t, (0, (64 if D < 64 else 128) - D)) for t in (q, k, v))
         return attention_packed(q, k, v, plan, layout)[..., :D].contiguous()
     if grads:
+        lowering._no_tangents(q, k, v)      # (not to be seen inside)
         return _Packed.apply(q, k, v, plan, layout)
     done = _host.attention_packed(q, k, v, out, lse, layout.tiles, plan, layout.total, layout.caps[-1], False)
     return _forward(q, k, v, plan, layout, out, lse) if done is None else done
@@ -222,6 +224,7 @@ def _forward_again(q, k, v, layout, out, lse, low, repeat):
 
 @lowering._on_device_of_first_argument
 def _forward(q, k, v, plan, layout, out, lse, low=None):
+    lowering._no_tangents(q, k, v)
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
     mask, window, scale, cap = _constants(plan, layout.total)
     T = layout.total
@@ -333,6 +336,7 @@ def _backward_again(q, k, v, o, lse, dout, layout, low, repeat):
 
 @lowering._on_device_of_first_argument
 def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
+    lowering._no_tangents(q, k, v, o, dout)
     dtype, D, Hq, Hkv = _heads(q, k, v, layout)
     mask, window, scale, cap = _constants(plan, layout.total)
     T, dev = layout.total, q.device

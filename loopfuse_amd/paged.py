@@ -171,6 +171,7 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: tor
     of two rows with one slot, either may be found there afterwards, or a part of each."""
     if _host.store_kv(k, v, k_pool, v_pool, slots):
         return
+    lowering._no_tangents(k, v, k_pool, v_pool)
     if k.dtype not in lowering._DTYPE_CODE:
         raise UnsupportedPlan(f"dtype {k.dtype} not supported (bf16/fp16 only)")
     for name, t in (("K", k), ("V", v), ("K pool", k_pool), ("V pool", v_pool)):
@@ -291,7 +292,7 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
     the pages of each request's own keys, of which it has ``lengths[b]`` (int32 [B], on the GPU; what a row of the table has no room for is
     left out); entries behind the last page are not read.  prefix_table : [ceil(prefix_len / page)], the pages of the prefix, of
     the table's dtype.  ``v_table`` / ``prefix_v_table``: those of V where they differ from K's.  ``plan``: scale and softcap, no mask.
-    Returns O [B, Hq, 1, D]; a request without a key, e.g. an empty place of a padded batch, gets zeros.
+    Returns O [B, Hq, 1, D], of which no gradients are recorded; a request without a key, e.g. an empty place of a padded batch, gets zeros.
 
     The prefix is read once for all requests together: its keys meet the rows of the whole batch as a matrix product, the requests'
     own keys are streamed, and the partial results are joined in a second launch.  Page ids are trusted, as those of
@@ -308,6 +309,7 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
 @lowering._on_device_of_first_argument
 def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v_table, prefix_v_table, out, choice):
     given = (table, lengths, prefix_table, v_table, prefix_v_table)
+    lowering._no_tangents(q, k_pool, v_pool)
     dtype = q.dtype
     if dtype not in lowering._DTYPE_CODE:
         raise UnsupportedPlan(f"dtype {dtype} not supported by the MFMA kernels (bf16/fp16 only)")

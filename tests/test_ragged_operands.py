@@ -1,10 +1,11 @@
 """The largest sizes, overridden choices and derivatives that the operators for different lengths refuse; how they lay out what they keep; no GPU."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from loopfuse_amd import packed, paged
 from loopfuse_amd.lowering import UnsupportedPlan
-from test_ragged import fake, nothing_is_launched, pools, shared  # noqa: F401  (a fixture that every test here uses)
+from test_ragged import PLAN, fake, layout, nothing_is_launched, pools, qkv, shared  # noqa: F401  (a fixture that every test here uses)
 
 
 @pytest.mark.parametrize("total", [(1 << 31) - 1, (1 << 31) - 256, packed.MAX_ROWS + 1])
@@ -61,3 +62,21 @@ def test_heads_that_are_loaded_together(Hkv, D, choice):
     kp, vp = pools(9, 4, Hkv, D)
     with pytest.raises(AssertionError, match="a launch"):
         paged.attention_shared(**shared(q=fake((3, 2 * Hkv, 1, D)), k_pool=kp, v_pool=vp, choice=choice))
+
+
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(which, grad):
+    with forward_ad.dual_level():
+        a = list(qkv())
+        a[which] = forward_ad.make_dual(a[which], torch.ones_like(a[which]))
+        if grad:
+            a[0] = a[0].requires_grad_()
+        with pytest.raises(UnsupportedPlan, match="tangents"), pytest.MonkeyPatch.context() as m:
+            m.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+            packed.attention_packed(*a, PLAN, layout(10))
+        kp, vp = pools()
+        with pytest.raises(UnsupportedPlan, match="tangents"):
+            paged.store_kv(forward_ad.make_dual(fake((10, 2, 64)), fake((10, 2, 64))), fake((10, 2, 64)), kp, vp, fake((10,), torch.int32))
+        with pytest.raises(UnsupportedPlan, match="tangents"):
+            paged.attention_shared(**shared(q=forward_ad.make_dual(fake((3, 4, 1, 64)), fake((3, 4, 1, 64)))))

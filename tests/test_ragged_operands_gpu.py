@@ -2,9 +2,10 @@
 pages that are none, the largest sizes."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from loopfuse_amd import packed, paged
-from loopfuse_amd.lowering import AttnPlan
+from loopfuse_amd.lowering import AttnPlan, UnsupportedPlan
 from test_packed_gpu import check, inputs, layout_of, oracle
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +120,22 @@ def test_checked_free_pages(monkeypatch):
         with pytest.raises(ValueError):
             extend(free)
     assert extend([1, 2 ** 27 - 1, -1]).lengths.tolist() == [17]      # (one that is not taken)
+
+
+# ---- derivatives -------------------------------------------------------------------------------------------------------------
+
+def test_forward_mode_derivatives_are_refused_by_repeated_calls_too():
+    q, k, v, g, bounds = inputs([50, 30], 4, 2, 64, torch.bfloat16)
+    plan, layout = AttnPlan("causal", scale=0.1), layout_of(bounds, len(q))
+    want = packed.attention_packed(q, k, v, plan, layout)
+    kp, slots = torch.zeros((8, 16, 2, 64), dtype=q.dtype, device=DEV), torch.arange(len(q), dtype=torch.int32, device=DEV)
+    paged.store_kv(k, v, kp, torch.zeros_like(kp), slots)
+    with forward_ad.dual_level():
+        for i in range(3):
+            a = [forward_ad.make_dual(t, g[:, :t.shape[1]].contiguous()) if j == i else t for j, t in enumerate((q, k, v))]
+            with pytest.raises(UnsupportedPlan, match="tangents"):
+                packed.attention_packed(*a, plan, layout)
+        dual = forward_ad.make_dual(k, torch.ones_like(k))
+        with pytest.raises(UnsupportedPlan, match="tangents"):
+            paged.store_kv(dual, v, kp, torch.zeros_like(kp), slots)
+        assert torch.equal(packed.attention_packed(q, k, v, plan, layout), want)
