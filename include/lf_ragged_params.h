@@ -56,7 +56,7 @@ typedef struct LfSharedParamsHost {
   const int32_t* lengths;  /* [B] own keys of each request */
   const void* prefix_k;    /* page ids of the prefix, of the tables' type */
   const void* prefix_v;
-  float* pre_acc;          /* [Hkv, nsplit, B * rows, D] */
+  float* pre_acc;          /* [Hkv, nsplit, B * rows, D], 16-byte aligned as part_acc */
   float* pre_ml;           /* [Hkv, nsplit, B * rows, 2] */
   int32_t room;            /* own keys that a row of the tables has room for, 2^30 at most */
   int32_t units;           /* workgroups per piece of own keys */

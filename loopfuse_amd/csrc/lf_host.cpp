@@ -376,7 +376,7 @@ PyObject* store_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // attention_shared(q, k_pool, v_pool, out, table, lengths, prefix_table, v_table, prefix_v_table, plan, prefix_len) -> O;
-// more: floats of scratch, and the bytes in front of the second, third and fourth of its parts
+// more: floats of scratch, and the bytes in front of part_ml, pre_acc and pre_ml in it
 PyObject* attention_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!takes(n, 11)) return nullptr;

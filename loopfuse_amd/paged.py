@@ -276,6 +276,12 @@ def _checked_choice(choice: dict) -> dict:
     return choice
 
 
+def scratch_parts(own: int, pre: int, D: int) -> tuple:
+    """Floats of partial results, ``own`` rows of the requests' keys and ``pre`` of the prefix, and the bytes in front of part_ml, pre_acc and pre_ml: the sums
+    with V of both come first, whose rows of 4 D bytes stay on borders of 16, then the pairs of offset and sum."""
+    return (own + pre) * (D + 2), 4 * (own + pre) * D, 4 * own * D, 4 * (own + pre) * D + 8 * own
+
+
 def combine_grid(B: int, Hq: int, D: int) -> int:
     """Blocks of lf_shared_combine: 1024 / D rows of one request each, or one row whose parts the block's groups of threads share."""
     return B * Hq if B * Hq <= 1024 else B * -(-Hq // (1024 // D))
@@ -417,7 +423,6 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
         P.nsplit, P.pre_blocks = splits, splits * P.pre_units
     if (P.pre_blocks + items * P.units) * 64 * max(4, coop) >= 1 << 32:
         raise UnsupportedPlan(f"a launch for {B} requests of {Hq} heads is too large")
-    own, pre = items * Hq, splits * B * Hq            # rows of partial results
     args = dict(rows=lowering.DECODE_QROWS, waves=coop or 4, headwave=coop > 0, coop=coop > 0,
                 rowload=not coop and lowering._decode_rowload(3, page, 0, 0))
     steps, spec = [], lowering._spec("decode", lowering._DTYPE_CODE[dtype], D, lowering.MASK_NONE, softcap is not None, 3, page,
@@ -427,7 +432,7 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
     spec = lowering._spec("shared_combine", lowering._DTYPE_CODE[dtype], D)
     steps.append((lowering.get_kernel(spec, spec.entry()), (combine_grid(B, Hq, D), 1, 1), 256))
     repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps], "prefix": "tiles" if tiles else "stream", "splits": splits},
-                              ((own + pre) * (D + 2), 4 * own * D, 4 * own * (D + 2), 4 * own * (D + 2) + 4 * pre * D))
+                              scratch_parts(items * Hq, splits * B * Hq, D))
     res = _again(q, k_pool, v_pool, table, lengths, prefix_table if prefix_len else None, v_table, prefix_v_table, out, repeat)
     if not choice and all(a is b for a, b in zip(given[:3], (table, lengths, prefix_table))) and (given[3] is None or given[3] is v_table) \
             and (given[4] is None or given[4] is prefix_v_table):

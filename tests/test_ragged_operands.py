@@ -80,3 +80,12 @@ def test_forward_mode_derivatives_are_refused(which, grad):
             paged.store_kv(forward_ad.make_dual(fake((10, 2, 64)), fake((10, 2, 64))), fake((10, 2, 64)), kp, vp, fake((10,), torch.int32))
         with pytest.raises(UnsupportedPlan, match="tangents"):
             paged.attention_shared(**shared(q=forward_ad.make_dual(fake((3, 4, 1, 64)), fake((3, 4, 1, 64)))))
+
+
+@pytest.mark.parametrize("own,pre", [(513, 9), (0, 4), (171 * 3, 5 * 3), (1, 0), (7, 7)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_partial_results_lie_on_the_borders_they_are_read_at(own, pre, D):
+    floats, ml, pre_acc, pre_ml = paged.scratch_parts(own, pre, D)
+    spans = sorted([(0, 4 * own * D), (ml, 8 * own), (pre_acc, 4 * pre * D), (pre_ml, 8 * pre)])
+    assert all(a + n <= b for (a, n), (b, _) in zip(spans, spans[1:])) and spans[-1][0] + spans[-1][1] <= 4 * floats
+    assert pre_acc % 16 == 0 and ml % 8 == 0 and pre_ml % 8 == 0

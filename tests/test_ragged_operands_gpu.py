@@ -6,6 +6,7 @@ from torch.autograd import forward_ad
 
 from loopfuse_amd import packed, paged
 from loopfuse_amd.lowering import AttnPlan, UnsupportedPlan
+import test_paged_gpu as paged_tests
 from test_packed_gpu import check, inputs, layout_of, oracle
 
 pytestmark = pytest.mark.gpu
@@ -120,6 +121,20 @@ def test_checked_free_pages(monkeypatch):
         with pytest.raises(ValueError):
             extend(free)
     assert extend([1, 2 ** 27 - 1, -1]).lengths.tolist() == [17]      # (one that is not taken)
+
+
+# ---- partial results ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("prefix", ["tiles", "stream"])
+def test_an_odd_number_of_rows_of_own_keys(D, prefix):
+    # 1 request of 3 heads: 512 // 3 + 1 pieces of 3 rows each
+    q, kp, vp, table, n, pre = paged_tests.batch(1, [300], 200, 16, 3, 1, D, torch.bfloat16)
+    plan = AttnPlan(scale=D ** -0.5, k_paged=True, v_paged=True)
+    want = paged_tests.oracle(q, kp, vp, table, n, pre, 200, D ** -0.5, None)
+    for _ in range(2):
+        paged_tests.check(paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=200, choice={"prefix": prefix, "splits": 3}), want)
+        paged_tests.check(paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=200), want)
 
 
 # ---- derivatives -------------------------------------------------------------------------------------------------------------
