@@ -471,12 +471,13 @@ PyObject* attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // attention_packed_backward(q, k, v, o, dout, lse, tiles, low, plan, total, entries) -> (dq, dk, dv), False where dS has no room;
-// more: bytes in front of the two lists of tiles, elements of dS
+// more: bytes in front of the two lists of tiles, elements of dS, calls until room for dS is looked for again (-1: never)
 PyObject* attention_packed_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!takes(n, 11)) return nullptr;
   auto e = find('b', a, 8, 5, a[8], a + 9, 2);
-  if (!e) return none();
+  if (!e || e->more[3] == 0) return none();
+  if (e->more[3] > 0) --e->more[3];
   const at::Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &lse = THPVariable_Unpack(a[5]);
   const at::Tensor dq = made(q.sizes(), like(q)), dk = made(k.sizes(), like(k)), dv = made(k.sizes(), like(k)), delta = made(lse.sizes(), like(lse));
   Block block(*e);

@@ -368,7 +368,8 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
     if q_split:
         keys = 1
     blocks = ds_blocks(mask, window, T, layout.count)
-    keep_ds = room and bwd_keep_ds(D, cap is not None, Hq * blocks)
+    wants_ds = bwd_keep_ds(D, cap is not None, Hq * blocks)
+    keep_ds = room and wants_ds
     rows = 64 if q_split else 128 * keys
     both = bwd_both(D, nt, keep_ds)
     spec = bwd_spec(dtype, D, mask, cap is not None, keys, nt, q_split, lowering.bwd_grads_stay(2 * T * Hq * D), keep_ds, both)
@@ -388,9 +389,10 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
     res = _backward_again(q, k, v, o, lse, dout, layout, low, repeat)
     if res is None:
         return _backward_general(q, k, v, o, lse, dout, plan, layout, low, False)
-    if room:
-        key = lowering._call_key("b", (q, k, v, o, dout), (lse, layout.tiles, low), plan, (T, layout.caps[-1]))
-        lowering._keep_call(key, repeat, repeat.more)
+    key = lowering._call_key("b", (q, k, v, o, dout), (lse, layout.tiles, low), plan, (T, layout.caps[-1]))
+    # an allocation that fails makes the allocator give back what it holds and wait for the device: the form without dS is kept, and room for dS looked
+    # for again once in many calls
+    lowering._keep_call(key, repeat, (*repeat.more, -1 if keep_ds or not wants_ds else lowering._NO_ROOM_CALLS))
     return res
 
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from loopfuse_amd import packed, paged
+from loopfuse_amd import lowering, packed, paged
 from loopfuse_amd.lowering import AttnPlan, UnsupportedPlan
 import test_paged_gpu as paged_tests
 from test_packed_gpu import check, inputs, layout_of, oracle
@@ -154,3 +154,33 @@ def test_forward_mode_derivatives_are_refused_by_repeated_calls_too():
         with pytest.raises(UnsupportedPlan, match="tangents"):
             paged.store_kv(dual, v, kp, torch.zeros_like(kp), slots)
         assert torch.equal(packed.attention_packed(q, k, v, plan, layout), want)
+
+
+def test_a_backward_without_room_for_ds_looks_for_it_again_once_in_many_calls(monkeypatch):
+    q, k, v, g, bounds = inputs([3900], 16, 16, 128, torch.bfloat16)
+    plan, layout, lse = AttnPlan("causal", scale=0.1), layout_of(bounds, len(q)), torch.empty((16, len(q)), device=DEV)
+    o = packed.attention_packed(q, k, v, plan, layout, lse=lse)
+    asked, again = [], packed._backward_again
+
+    def tries(q, k, v, o, lse, dout, layout, low, repeat):
+        asked.append(repeat.more[2])
+        return None if repeat.more[2] else again(q, k, v, o, lse, dout, layout, low, repeat)       # (as where the allocation fails)
+
+    monkeypatch.setattr(packed, "_backward_again", tries)
+    monkeypatch.setattr(lowering, "_NO_ROOM_CALLS", 3)
+    paged._host.clear()
+    res = []
+    for _ in range(9):
+        res.append(packed.attention_packed_backward(q, k, v, o, lse, g, plan, layout))
+        assert lowering._last_launch["kernels"] == ["lf_attn_bwd_dq", "lf_attn_bwd_dkdv"]
+    size = asked[0]
+    assert size > 0 and asked == [size, 0] * 3          # calls 1, 5 and 9; three repeated ones behind each
+    assert all(torch.equal(x, y) for r in res for x, y in zip(r, res[0]))
+    # there is room again: found at the next look, and kept
+    monkeypatch.setattr(packed, "_backward_again", again)
+    for n in range(5):
+        got = packed.attention_packed_backward(q, k, v, o, lse, g, plan, layout)
+        assert ("lf_attn_bwd_delta" in lowering._last_launch["kernels"]) == (n >= 3)
+    monkeypatch.setattr(packed, "_backward_general", None)
+    assert all(torch.equal(x, y) for x, y in zip(packed.attention_packed_backward(q, k, v, o, lse, g, plan, layout), got))
+    paged._host.clear()
