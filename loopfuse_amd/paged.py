@@ -373,9 +373,11 @@ def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v
         return torch.empty(q.shape, dtype=dtype, device=q.device) if out is None else out
     if lowering._checks_tables():
         used = torch.arange(table.shape[1], device=q.device) < ((lengths.clamp(min=0).long() + page - 1) // page)[:, None]
-        named = [table[used], v_table[used]] + ([t[:-(-prefix_len // page)] for t in (prefix_table, prefix_v_table)] if prefix_len else [])
-        if any(len(t) and (int(t.min()) < 0 or int(t.max()) >= pages) for t in named) or (B and int(lengths.max()) > table.shape[1] * page):
-            raise ValueError(f"loopfuse_amd: page ids outside 0 ... {pages - 1}, or a length beyond its row of the table")
+        named = [(table[used], pages), (v_table[used], pages_v)]
+        if prefix_len:
+            named += [(t[:-(-prefix_len // page)], n) for t, n in ((prefix_table, pages), (prefix_v_table, pages_v))]
+        if any(len(t) and (int(t.min()) < 0 or int(t.max()) >= n) for t, n in named) or (B and int(lengths.max()) > table.shape[1] * page):
+            raise ValueError(f"loopfuse_amd: page ids outside 0 ... {pages - 1} (V: {pages_v - 1}), or a length beyond its row of the table")
     P = SharedParams()
     P.q_sb, P.q_sh, P.q_ss = q.stride(0), group * q.stride(1), q.stride(1)
     o_sb, o_sh = (Hq * D, D) if out is None else out.stride()[:2]

@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from loopfuse_amd import packed, paged
+from loopfuse_amd import lowering, packed, paged
 from loopfuse_amd.lowering import UnsupportedPlan
 from test_ragged import PLAN, fake, layout, nothing_is_launched, pools, qkv, shared  # noqa: F401  (a fixture that every test here uses)
 
@@ -89,3 +89,18 @@ def test_partial_results_lie_on_the_borders_they_are_read_at(own, pre, D):
     spans = sorted([(0, 4 * own * D), (ml, 8 * own), (pre_acc, 4 * pre * D), (pre_ml, 8 * pre)])
     assert all(a + n <= b for (a, n), (b, _) in zip(spans, spans[1:])) and spans[-1][0] + spans[-1][1] <= 4 * floats
     assert pre_acc % 16 == 0 and ml % 8 == 0 and pre_ml % 8 == 0
+
+
+@pytest.mark.parametrize("which", ["table", "prefix_table"])
+def test_checked_tables_look_at_the_pool_that_they_name_pages_of(which, monkeypatch):
+    """A V pool of fewer pages than K's: ids that K has and V has not."""
+    monkeypatch.setattr(lowering, "_checks_tables", lambda: True)
+    kp, vp = pools(9, 4, 2, 64)[0], pools(5, 4, 2, 64)[1]
+    a = shared(k_pool=kp, v_pool=vp, lengths=fake((3,), torch.int32) + 5)
+    with pytest.raises(AssertionError, match="a launch"):
+        paged.attention_shared(**a)
+    a[which] = a[which] + 7
+    with pytest.raises(ValueError, match="page ids"):
+        paged.attention_shared(**a)
+    with pytest.raises(AssertionError, match="a launch"):
+        paged.attention_shared(**a, **{{"table": "v_table", "prefix_table": "prefix_v_table"}[which]: a[which] - 7})
