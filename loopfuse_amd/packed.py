@@ -229,8 +229,8 @@ def _forward(q, k, v, plan, layout, out, lse, low=None):
     mask, window, scale, cap = _constants(plan, layout.total)
     T = layout.total
     for name, t in (("K", k), ("V", v)):
-        # direct-to-LDS loads address a sequence with 32-bit byte offsets, up to three tiles past its end
-        if t.stride(0) < 0 or 2 * (T + 192) * t.stride(0) + 2 * D >= 1 << 31:
+        # direct-to-LDS loads address a sequence, of whatever part of the rows, with unsigned 32-bit byte offsets, up to three tiles past its end
+        if t.stride(0) < 0 or 2 * (T + 192) * t.stride(0) + 2 * D >= 1 << 32:
             raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
     if out is not None:
         _rows("O", out, layout, dtype, D)

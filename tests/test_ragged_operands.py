@@ -104,3 +104,16 @@ def test_checked_tables_look_at_the_pool_that_they_name_pages_of(which, monkeypa
         paged.attention_shared(**a)
     with pytest.raises(AssertionError, match="a launch"):
         paged.attention_shared(**a, **{{"table": "v_table", "prefix_table": "prefix_v_table"}[which]: a[which] - 7})
+
+
+@pytest.mark.parametrize("stride,served", [(10_631_104, True), (10_631_112, False)])
+def test_rows_of_k_and_v_lie_within_32_bits(stride, served, monkeypatch):
+    """10 rows and three tiles behind them, 2 bytes per element: below 2**32 bytes in all."""
+    monkeypatch.setattr(lowering, "_check_tensor", lambda *a: None)
+    monkeypatch.setattr(packed, "_rows", lambda *a: None)
+    q, k, v = qkv()
+    far = torch.empty_strided((10, 2, 64), (stride, 64, 1), dtype=k.dtype, device="meta")
+    assert (2 * 202 * stride + 128 < 1 << 32) == served
+    for a in ((q, far, v), (q, k, far)):
+        with pytest.raises(AssertionError if served else UnsupportedPlan, match="a launch" if served else "reach"):
+            packed.attention_packed(*a, PLAN, layout(10))

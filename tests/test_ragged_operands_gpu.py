@@ -65,6 +65,25 @@ def test_operands_whose_rows_are_one(D, mask):
             assert all(torch.equal(x, y) for x, y in zip(a, b)), (i, t.stride())
 
 
+@pytest.mark.parametrize("D,mask,lengths", [(128, "causal", [1000]), (64, None, [300, 699, 1]), (128, "sliding", [999, 1])])
+def test_rows_of_one_sequence_beyond_2_gib(D, mask, lengths):
+    """K and V of 2 heads in rows 3 MB apart, the last ones nearly 3 GB behind their sequence's first."""
+    q, k, v, g, bounds = inputs(lengths, 4, 2, D, torch.bfloat16, 7)
+    plan, layout, row = AttnPlan(mask, window=70, scale=D ** -0.5), layout_of(bounds, len(q)), 3 << 19
+    wide = torch.empty(len(q) * row, dtype=torch.bfloat16, device=DEV)
+    far = []
+    for i, t in enumerate((k, v)):
+        far.append(wide.as_strided(t.shape, (row, D, 1), i * 2 * D))
+        far[-1].copy_(t)
+    assert 2 * row * (len(q) - 1) > 1 << 31
+    lse = torch.empty((4, len(q)), device=DEV)
+    want = packed.attention_packed(q, k, v, plan, layout, lse=lse)
+    for _ in range(2):
+        assert torch.equal(packed.attention_packed(q, *far, plan, layout), want)
+    grads = packed.attention_packed_backward(q, k, v, want, lse, g, plan, layout)
+    assert all(torch.equal(a, b) for a, b in zip(packed.attention_packed_backward(q, *far, want, lse, g, plan, layout), grads))
+
+
 # ---- pages that are none -----------------------------------------------------------------------------------------------------
 
 def plain_lengths(cached, new, table, free, page, total):
