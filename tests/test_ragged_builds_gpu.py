@@ -1,0 +1,218 @@
+"""Every build that the rules of the operators for different lengths can choose against the formulas in 64 bits: on small batches with the rules
+overridden, and on batches large enough that the rules choose the builds of real sizes by themselves, which is asserted.  Tolerances: those derived in
+test_packed_gpu.py and test_paged_gpu.py."""
+import pytest
+import torch
+
+import test_paged_gpu as paged_tests
+from loopfuse_amd import lowering, packed, paged
+from loopfuse_amd.lowering import AttnPlan
+from test_packed_gpu import check, inputs, layout_of, oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HALF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture
+def specs(monkeypatch):
+    """The builds that calls launch from now on, none of them kept from before or for later tests."""
+    seen, get = [], lowering.get_kernel
+
+    def record(spec, *a):
+        seen.append(spec)
+        return get(spec, *a)
+
+    monkeypatch.setattr(lowering, "get_kernel", record)
+    paged._host.clear()
+    yield seen
+    paged._host.clear()
+
+
+def options(specs, family):
+    """The -D options of the one build of a family among ``specs``."""
+    found = {s for s in specs if s.family in family}
+    assert len(found) == 1, found
+    return set(found.pop().options())
+
+
+# ---- packed: small batches, every build -----------------------------------------------------------------------------------------
+
+LENGTHS = [513, 1, 257, 0, 300, 64, 256]        # tails of one row behind tiles of 32 ... 256
+MASKS = [("causal", 0, None), (None, 0, None), ("sliding", 100, None), ("causal", 0, 20.0), ("sliding", 65, 30.0), (None, 0, 5.0)]
+
+
+@pytest.mark.parametrize("D,dtype", [(128, BF), (128, HALF), (64, BF), (64, HALF)])
+@pytest.mark.parametrize("mask,window,cap", MASKS)
+@pytest.mark.parametrize("Hq,Hkv", [(2, 2), (4, 2), (4, 1)])
+def test_builds_of_the_forward(D, dtype, mask, window, cap, Hq, Hkv, monkeypatch, specs):
+    """Key tiles of 64 and 32, plain and whole-row stores, 1, 2 and 4 heads per workgroup; with what rounding takes from O beside it."""
+    q, k, v, g, bounds = inputs(LENGTHS, Hq, Hkv, D, dtype, D + Hq, 3, 70)
+    plan, layout, T = AttnPlan(mask, window=window, scale=D ** -0.5, softcap=cap), layout_of(bounds, len(q)), len(q)
+    want = oracle(q, k, v, g, bounds, mask, window, D ** -0.5, cap)[0]["out"]
+    results = []
+    for bn in (0, 32) if D == 128 else (0,):
+        for stay in (False, True):
+            monkeypatch.setattr(lowering, "prefill_kv_tile", lambda *a: bn)
+            monkeypatch.setattr(lowering, "prefill_out_stays", lambda n: stay)
+            paged._host.clear()
+            specs.clear()
+            out = packed.attention_packed(q, k, v, plan, layout)
+            got = options(specs, ("prefill_swp",))
+            assert ("-DLF_STAY=1" in got) == stay and ("-DLF_BN=32" in got) == (bn == 32) and (f"-DLF_GQAPACK={Hq // Hkv}" in got) == (Hq > Hkv)
+            check(out, want, f"out {bn} {stay}")
+            lse, low = torch.empty(Hq, T, device=DEV), torch.zeros_like(q)
+            assert torch.equal(packed._forward(q, k, v, plan, layout, None, lse, low), out)
+            results.append((bn, out, low, lse))
+            into = torch.full((T, 2 * Hq, D), 3.0, dtype=dtype, device=DEV)
+            packed.attention_packed(q, k, v, plan, layout, out=into[:, ::2])
+            lo, hi = bounds[0], bounds[-1]
+            assert torch.equal(into[lo:hi, ::2], out[lo:hi]) and (into[:, 1::2] == 3).all() and (into[:lo] == 3).all() and (into[hi:] == 3).all()
+    # the stores move the same bits
+    for bn, out, low, lse in results:
+        first = next(r for r in results if r[0] == bn)
+        rows = slice(bounds[0], bounds[-1])
+        assert torch.equal(out, first[1]) and torch.equal(low, first[2]) and torch.equal(lse[:, rows], first[3][:, rows])
+
+
+@pytest.mark.parametrize("D,dtype", [(128, BF), (128, HALF), (64, BF), (64, HALF)])
+@pytest.mark.parametrize("mask,window,cap", MASKS)
+@pytest.mark.parametrize("Hq,Hkv", [(2, 2), (4, 1)])
+def test_builds_of_the_backward(D, dtype, mask, window, cap, Hq, Hkv, monkeypatch, specs):
+    """Whole keys, two blocks of them and queries shared by two waves, dQ of 256 and 512 threads, dS kept and formed again, whole-row and plain stores."""
+    q, k, v, g, bounds = inputs(LENGTHS, Hq, Hkv, D, dtype, D + Hq, 3, 70)
+    plan, layout, T = AttnPlan(mask, window=window, scale=D ** -0.5, softcap=cap), layout_of(bounds, len(q)), len(q)
+    want = oracle(q, k, v, g, bounds, mask, window, D ** -0.5, cap)[0]
+    lse, low = torch.empty(Hq, T, device=DEV), torch.zeros_like(q)
+    o = packed._forward(q, k, v, plan, layout, None, lse, low)
+    code = lowering._MASK_NAMES[mask]
+    for keys, q_split in ((1, False), (1, True)) + (((2, False),) if lowering.bwd_two_key_blocks(D, code, cap is not None) else ()):
+        for threads in (256, 512) if D == 128 else (256,):
+            for ds in (False, True) if D == 128 or cap else (False,):
+                for stay in (False, True):
+                    monkeypatch.setattr(lowering, "bwd_key_blocks", lambda *a: keys)
+                    monkeypatch.setattr(packed, "bwd_q_split", lambda *a: q_split)
+                    monkeypatch.setattr(packed, "bwd_dq_threads", lambda *a: threads)
+                    monkeypatch.setattr(packed, "bwd_keep_ds", lambda *a: ds)
+                    monkeypatch.setattr(lowering, "bwd_grads_stay", lambda n: stay)
+                    what = f"{keys} blocks, split {q_split}, {threads} threads, dS {ds}, stay {stay}"
+                    paged._host.clear()
+                    specs.clear()
+                    for with_low in (low, None):
+                        grads = packed._backward(q, k, v, o, lse, g, plan, layout, with_low)
+                        for name, t in zip(("dq", "dk", "dv"), grads):
+                            check(t, want[name], f"{name}: {what}")
+                    got = options(specs, ("bwd", "bwd_both"))
+                    assert {f"-DLF_BW_W={keys}", f"-DLF_BW_DQ_NT={threads}"} <= got
+                    assert ("-DLF_BW_QSPLIT=1" in got, "-DLF_BW_DS=1" in got, "-DLF_STAY=1" in got) == (q_split, ds, stay)
+                    assert ("-DLF_BW_BOTH=1" in got) == (D == 64 and not ds)
+
+
+# ---- packed: batches of real sizes, by the rules ------------------------------------------------------------------------------------
+
+LARGE = [
+    # lengths, Hq, Hkv, D, dtype, mask, window, softcap, options of the forward and of the backward that the rules choose
+    ([1048, 700, 900, 1500, 300, 333, 1, 1024, 257, 999], 32, 32, 128, HALF, "causal", 0, None, {"-DLF_BN=32"}, {"-DLF_BW_W=1", "-DLF_BW_DQ_NT=512", "-DLF_BW_DS=1"}),
+    ([2048, 1100, 900, 1500, 700, 333, 2000, 1025], 32, 32, 128, BF, "causal", 0, None, {"-DLF_BN=32"}, {"-DLF_BW_W=2", "-DLF_BW_DQ_NT=512", "-DLF_BW_DS=1"}),
+    ([2048, 1000, 37, 1500, 600, 1, 800, 2000, 99, 257, 1200, 500], 32, 8, 128, BF, "causal", 0, None, {"-DLF_BN=32", "-DLF_GQAPACK=4"}, {"-DLF_BW_DQ_NT=512", "-DLF_BW_DS=1"}),
+    ([4001, 1000, 2500, 333, 1], 32, 8, 128, HALF, "sliding", 256, 50.0, {"-DLF_BN=32", "-DLF_GQAPACK=4"}, {"-DLF_BW_W=1", "-DLF_BW_DQ_NT=512", "-DLF_BW_DS=1"}),
+    ([1025, 1500, 700, 2000], 32, 32, 128, BF, None, 0, None, {"-DLF_BN=32"}, {"-DLF_BW_W=2", "-DLF_BW_DQ_NT=512", "-DLF_BW_DS=1"}),
+    ([1000, 37, 500, 800, 250, 64, 1, 900, 333, 700, 600, 450, 100, 200, 999, 512, 31, 33, 800, 700, 650, 128, 129, 255], 16, 4, 64, HALF, "causal", 0, None,
+     {"-DLF_GQAPACK=4"}, {"-DLF_BW_BOTH=1", "-DLF_BW_DQ_NT=256", "-DLF_BW_QSPLIT=1"}),
+    ([1000, 37, 1500, 800, 1250, 64, 1, 1900], 16, 16, 64, BF, "causal", 0, None, set(), {"-DLF_BW_BOTH=1", "-DLF_BW_DQ_NT=256"}),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_batches_of_real_sizes(case, specs):
+    lengths, Hq, Hkv, D, dtype, mask, window, cap, forward, backward = LARGE[case]
+    q, k, v, g, bounds = inputs(lengths, Hq, Hkv, D, dtype, case, 0, 5)
+    plan, layout = AttnPlan(mask, window=window, scale=D ** -0.5, softcap=cap), layout_of(bounds, len(q))
+    specs.clear()
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = packed.attention_packed(*leaves, plan, layout)
+    grads = torch.autograd.grad(out, leaves, g)
+    got = options(specs, ("prefill_swp",)), options(specs, ("bwd", "bwd_both"))
+    # O, its residue and the gradients leave in whole rows at these sizes
+    assert forward <= got[0] and backward <= got[1], got
+    assert "-DLF_STAY=1" not in got[0] and "-DLF_STAY=1" not in got[1] and ("-DLF_BW_QSPLIT=1" in got[1]) == ("-DLF_BW_QSPLIT=1" in backward), got
+    want = oracle(q, k, v, g, bounds, mask, window, D ** -0.5, cap)[0]
+    for name, t in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads)):
+        check(t, want[name], name)
+    again = packed.attention_packed(*leaves, plan, layout)
+    assert torch.equal(again, out) and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, leaves, g), grads))
+
+
+@pytest.mark.parametrize("D,dtype", [(40, BF), (100, HALF), (8, HALF), (127, BF)])
+@pytest.mark.parametrize("mask,window,cap", [("causal", 0, None), ("sliding", 30, 15.0)])
+def test_gradients_of_other_head_dims(D, dtype, mask, window, cap):
+    q, k, v, g, bounds = inputs([70, 1, 200, 33], 4, 2, D, dtype, D, 0, 4)
+    plan, layout = AttnPlan(mask, window=window, scale=D ** -0.5, softcap=cap), layout_of(bounds, len(q))
+    want = oracle(q, k, v, g, bounds, mask, window, D ** -0.5, cap)[0]
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = packed.attention_packed(*leaves, plan, layout)
+    for name, t in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, g))):
+        check(t, want[name], name)
+
+
+# ---- a shared prefix and own keys: heads loaded together ------------------------------------------------------------------------------
+
+def shared_oracle(q, kp, vp, table, n, pre, prefix, scale, cap):
+    return paged_tests.oracle(q, kp, vp, table.cpu(), n.cpu(), pre.cpu(), prefix, scale, cap)
+
+
+COOP = [
+    # lengths, prefix, page, Hkv, group, D, dtype, softcap, choice
+    ([300, 0, 1, 45, 16, 700], 0, 16, 8, 4, 128, BF, None, {"coop": 4}),
+    ([300, 0, 1, 45, 16, 700], 0, 16, 8, 4, 128, HALF, 30.0, {"coop": 8}),
+    ([300, 0, 1, 45, 16, 700], 130, 16, 4, 2, 128, HALF, None, {"coop": 4, "prefix": "tiles"}),
+    ([300, 0, 1, 45, 16, 700], 130, 16, 8, 4, 128, BF, 20.0, {"coop": 4, "prefix": "tiles", "splits": 2}),
+    ([300, 0, 1, 45, 16, 700], 130, 8, 4, 1, 128, BF, None, {"coop": 4, "prefix": "tiles", "near": False}),
+    ([300, 0, 1, 45, 16, 700], 333, 16, 12, 2, 128, BF, None, {"coop": 4, "prefix": "stream", "splits": 3}),
+    ([300, 0, 1, 45, 16, 700], 333, 64, 8, 5, 128, BF, None, {"coop": 8, "prefix": "stream"}),
+    ([300, 0, 1, 45, 16, 700], 0, 1, 8, 4, 128, BF, None, {"coop": 4, "least": 32, "target_log2": 12}),
+    ([300, 0, 1, 45, 16, 700], 0, 16, 8, 4, 64, HALF, None, {"coop": 8}),
+    ([300, 0, 1, 45, 16, 700], 257, 8, 16, 1, 64, BF, 25.0, {"coop": 8, "prefix": "stream"}),
+    ([300, 0, 1, 45, 16, 700], 257, 64, 8, 17, 64, BF, None, {"coop": 8, "prefix": "stream", "least": 64, "target_log2": 12}),
+]
+
+
+@pytest.mark.parametrize("case", range(len(COOP)))
+def test_own_keys_whose_heads_are_loaded_together(case, specs):
+    lengths, prefix, page, Hkv, group, D, dtype, cap, choice = COOP[case]
+    q, kp, vp, table, n, pre = paged_tests.batch(len(lengths), lengths, prefix, page, Hkv, group, D, dtype, seed=case)
+    plan = AttnPlan(scale=D ** -0.5, softcap=cap, k_paged=True, v_paged=True)
+    want = shared_oracle(q, kp, vp, table, n, pre, prefix, D ** -0.5, cap)
+    for more in ({}, {"least": 256, "target_log2": 6}):
+        specs.clear()
+        out = paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=prefix, choice={**choice, **more})
+        got = options(specs, ("decode",))
+        assert {"-DLF_COOP=1", "-DLF_SHARED=1", f"-DLF_DW={choice['coop']}"} <= got
+        assert (f"-DLF_PREFIX={2 - choice.get('near', True)}" in got) == (choice.get("prefix") == "tiles")
+        paged_tests.check(out, want, str(more))
+
+
+SHARED_LARGE = [
+    # requests, most own keys, prefix, Hkv, group, D, dtype, softcap, options that the rules choose
+    (64, 1024, 2048, 8, 4, 128, BF, None, {"-DLF_COOP=1", "-DLF_DW=4", "-DLF_PREFIX=1"}),
+    (128, 300, 8208, 8, 4, 128, HALF, None, {"-DLF_COOP=1", "-DLF_DW=4", "-DLF_PREFIX=1"}),
+    (64, 900, 0, 8, 4, 128, BF, 30.0, {"-DLF_COOP=1", "-DLF_DW=4"}),
+    (160, 400, 0, 8, 4, 64, BF, None, {"-DLF_COOP=1", "-DLF_DW=8"}),
+    (120, 400, 100, 8, 1, 64, HALF, None, {"-DLF_PREFIX=1"}),
+    (40, 1900, 0, 8, 8, 64, HALF, None, {"-DLF_COOP=1", "-DLF_DW=8"}),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SHARED_LARGE)))
+def test_requests_of_real_numbers(case, specs):
+    B, most, prefix, Hkv, group, D, dtype, cap, chosen = SHARED_LARGE[case]
+    lengths = torch.randint(0, most + 1, (B,), generator=torch.Generator().manual_seed(case)).tolist()
+    lengths[:3] = [most, 0, 1]
+    q, kp, vp, table, n, pre = paged_tests.batch(B, lengths, prefix, 16, Hkv, group, D, dtype, seed=case)
+    plan = AttnPlan(scale=D ** -0.5, softcap=cap, k_paged=True, v_paged=True)
+    specs.clear()
+    out = paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=prefix)
+    assert chosen <= options(specs, ("decode",)), options(specs, ("decode",))
+    paged_tests.check(out, shared_oracle(q, kp, vp, table, n, pre, prefix, D ** -0.5, cap))
+    for _ in range(3):
+        assert torch.equal(paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=prefix), out)
