@@ -121,6 +121,12 @@ def _rows(name: str, t: torch.Tensor, layout: PackedLayout, dtype, D: Optional[i
         raise RuntimeError(f"loopfuse_amd: {name} is on {t.device}, the layout on {layout.tiles.device}")
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from a row to the next.  The stride of a dimension of one element can be any number: of one row its length, so that what is read
+    behind it lies outside."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
 def _constants(plan: AttnPlan, total: int) -> tuple:
     """(mask, window, scale, softcap or None) of a plan that the packed kernels serve."""
     if plan.k_paged or plan.v_paged or plan.denom_add != 0.0:
@@ -230,7 +236,7 @@ def _forward(q, k, v, plan, layout, out, lse, low=None):
     T = layout.total
     for name, t in (("K", k), ("V", v)):
         # direct-to-LDS loads address a sequence, of whatever part of the rows, with unsigned 32-bit byte offsets, up to three tiles past its end
-        if t.stride(0) < 0 or 2 * (T + 192) * t.stride(0) + 2 * D >= 1 << 32:
+        if _row_stride(t) < 0 or 2 * (T + 192) * _row_stride(t) + 2 * D >= 1 << 32:
             raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
     if out is not None:
         _rows("O", out, layout, dtype, D)
@@ -241,9 +247,9 @@ def _forward(q, k, v, plan, layout, out, lse, low=None):
     if T == 0:
         return torch.empty(q.shape, dtype=dtype, device=q.device) if out is None else out
     P = PackedAttnParams()
-    P.q_ss, P.q_sh = q.stride()[:2]
-    P.k_ss, P.k_sh = k.stride()[:2]
-    P.v_ss, P.v_sh = v.stride()[:2]
+    P.q_ss, P.q_sh = _row_stride(q), q.stride(1)
+    P.k_ss, P.k_sh = _row_stride(k), k.stride(1)
+    P.v_ss, P.v_sh = _row_stride(v), v.stride(1)
     P.o_ss, P.o_sh = (Hq * D, D) if out is None else out.stride()[:2]
     P.B, P.Hq, P.Hkv, P.Sq, P.Sk, P.window = 1, Hq, Hkv, T, T, window
     P.scale, P.softcap = scale, cap or 0.0
@@ -297,7 +303,7 @@ def attention_packed_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 def rows_apart(t):
     """``t`` or, where rows lie closer than a row is long (one row expanded over all), a copy.  The kernels take what lies behind a sequence's last
     row for zeros, which the ranges of their buffers make of it only where it lies behind that row's last element too."""
-    return t if t.dim() != 3 or t.stride(0) >= t.shape[2] else t.clone(memory_format=torch.contiguous_format)
+    return t if t.dim() != 3 or _row_stride(t) >= t.shape[2] else t.clone(memory_format=torch.contiguous_format)
 
 
 def _backward(q, k, v, o, lse, dout, plan, layout, low=None):
@@ -347,13 +353,13 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
     if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or not lse.is_contiguous() or lse.device != dev:
         raise UnsupportedPlan(f"lse must be a contiguous float32 [{Hq}, {T}] tensor on the device of Q")
     for name, t in (("Q", q), ("dO", dout), ("K", k), ("V", v)):
-        if t.stride(0) < D or 2 * (T + 64) * t.stride(0) + 2 * D >= 1 << 32:
+        if _row_stride(t) < D or 2 * (T + 64) * _row_stride(t) + 2 * D >= 1 << 32:
             raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
     if T == 0:
         return tuple(torch.empty(t.shape, dtype=dtype, device=dev) for t in (q, k, v))
     P = PackedBwdParams()
     for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("do", dout)):
-        setattr(P, name + "_ss", t.stride(0))
+        setattr(P, name + "_ss", _row_stride(t))
         setattr(P, name + "_sh", t.stride(1))
     for name, heads in (("dq", Hq), ("dk", Hkv), ("dv", Hkv)):
         setattr(P, name + "_ss", heads * D)

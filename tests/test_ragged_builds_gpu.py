@@ -108,6 +108,32 @@ def test_builds_of_the_backward(D, dtype, mask, window, cap, Hq, Hkv, monkeypatc
                     assert ("-DLF_BW_BOTH=1" in got) == (D == 64 and not ds)
 
 
+@pytest.mark.parametrize("mask", ["causal", None, "sliding"])
+@pytest.mark.parametrize("threads,q_split", [(256, False), (512, False), (256, True)])
+def test_kept_ds_of_a_sequence_of_nan_stays_apart(mask, threads, q_split, monkeypatch):
+    """Sequences of odd numbers of 32-row blocks, whose dS lie beside each other."""
+    monkeypatch.setattr(packed, "bwd_dq_threads", lambda *a: threads)
+    monkeypatch.setattr(packed, "bwd_q_split", lambda *a: q_split)
+    q, k, v, g, bounds = inputs([90, 33, 65, 1, 300], 2, 2, 128, BF)
+    plan, layout, lse = AttnPlan(mask, window=40, scale=0.1), layout_of(bounds, len(q)), torch.empty((2, len(q)), device=DEV)
+    res = []
+    for bad in (None, 1, 3):
+        a = [t.clone() for t in (q, k, v, g)]
+        if bad is not None:
+            for t in a:
+                t[bounds[bad]:bounds[bad + 1]] = float("nan")
+        paged._host.clear()
+        o = packed.attention_packed(*a[:3], plan, layout, lse=lse)
+        grads = packed.attention_packed_backward(*a[:3], o, lse, a[3], plan, layout)
+        assert "lf_attn_bwd_delta" in lowering._last_launch["kernels"]
+        res.append((bad, (o, *grads)))
+    paged._host.clear()
+    for bad, tensors in res[1:]:
+        keep = torch.ones(len(q), dtype=torch.bool, device=DEV)
+        keep[bounds[bad]:bounds[bad + 1]] = False
+        assert all(torch.equal(x[keep], y[keep]) for x, y in zip(tensors, res[0][1]))
+
+
 # ---- packed: batches of real sizes, by the rules ------------------------------------------------------------------------------------
 
 LARGE = [

@@ -117,3 +117,13 @@ def test_rows_of_k_and_v_lie_within_32_bits(stride, served, monkeypatch):
     for a in ((q, far, v), (q, k, far)):
         with pytest.raises(AssertionError if served else UnsupportedPlan, match="a launch" if served else "reach"):
             packed.attention_packed(*a, PLAN, layout(10))
+
+
+def test_one_row_may_have_any_stride(monkeypatch):
+    monkeypatch.setattr(lowering, "_kernels_of", lambda spec: None)
+    q, k, v = qkv(T=1)
+    far = [t.as_strided(t.shape, (1 << 40, 64, 1)) for t in (q, k, v)]
+    with pytest.raises(AssertionError, match="a launch"):
+        packed.attention_packed(*far, PLAN, layout(1))
+    with pytest.raises(AssertionError, match="a launch"):
+        packed.attention_packed_backward(*far, q, fake((4, 1), torch.float32), far[0], PLAN, layout(1))

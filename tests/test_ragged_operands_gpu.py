@@ -65,6 +65,20 @@ def test_operands_whose_rows_are_one(D, mask):
             assert all(torch.equal(x, y) for x, y in zip(a, b)), (i, t.stride())
 
 
+@pytest.mark.parametrize("stride", [0, 1, 8, 72, 1 << 40])
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 2, 2), (128, 4, 1)])
+def test_one_row_of_any_stride(stride, D, Hq, Hkv):
+    """The stride of a dimension of one element says nothing."""
+    q, k, v, g, bounds = inputs([1], Hq, Hkv, D, torch.bfloat16, 9)
+    plan, layout, lse = AttnPlan("causal", scale=D ** -0.5), layout_of(bounds, 1), torch.empty((Hq, 1), device=DEV)
+    want = packed.attention_packed(q, k, v, plan, layout, lse=lse)
+    grads = packed.attention_packed_backward(q, k, v, want, lse, g, plan, layout)
+    rows = [t.as_strided(t.shape, (stride, D, 1)) for t in (q, k, v, g)]
+    for _ in range(2):
+        assert torch.equal(packed.attention_packed(*rows[:3], plan, layout), want)
+        assert all(torch.equal(a, b) for a, b in zip(packed.attention_packed_backward(*rows[:3], want, lse, rows[3], plan, layout), grads))
+
+
 @pytest.mark.parametrize("D,mask,lengths", [(128, "causal", [1000]), (64, None, [300, 699, 1]), (128, "sliding", [999, 1])])
 def test_rows_of_one_sequence_beyond_2_gib(D, mask, lengths):
     """K and V of 2 heads in rows 3 MB apart, the last ones nearly 3 GB behind their sequence's first."""
