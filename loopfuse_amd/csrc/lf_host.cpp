@@ -470,15 +470,15 @@ PyObject* attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// attention_packed_backward(q, k, v, o, dout, lse, tiles, low, plan, total, entries) -> (dq, dk, dv), False where dS has no room;
+// attention_packed_backward(q, k, v, o, dout, low, lse, tiles, plan, total, entries) -> (dq, dk, dv), False where dS has no room;
 // more: bytes in front of the two lists of tiles, elements of dS, calls until room for dS is looked for again (-1: never)
 PyObject* attention_packed_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!takes(n, 11)) return nullptr;
-  auto e = find('b', a, 8, 5, a[8], a + 9, 2);
+  auto e = find('b', a, 8, 6, a[8], a + 9, 2);
   if (!e || e->more[3] == 0) return none();
   if (e->more[3] > 0) --e->more[3];
-  const at::Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &lse = THPVariable_Unpack(a[5]);
+  const at::Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &lse = THPVariable_Unpack(a[6]);
   const at::Tensor dq = made(q.sizes(), like(q)), dk = made(k.sizes(), like(k)), dv = made(k.sizes(), like(k)), delta = made(lse.sizes(), like(lse));
   Block block(*e);
   auto* p = block.as<LfPackedBwdParamsHost>();
@@ -487,14 +487,14 @@ PyObject* attention_packed_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
   p->bwd.v = at_(a[2]);
   p->bwd.o = at_(a[3]);
   p->bwd.dout = at_(a[4]);
-  p->bwd.lse = at_<float>(a[5]);
+  p->bwd.lse = at_<float>(a[6]);
   p->bwd.dq = dq.mutable_data_ptr();
   p->bwd.dk = dk.mutable_data_ptr();
   p->bwd.dv = dv.mutable_data_ptr();
   p->bwd.delta = delta.mutable_data_ptr<float>();
-  p->dkdv_tiles = reinterpret_cast<const LfPackedTileHost*>(at_<char>(a[6]) + e->more[0]);
-  p->dq_tiles = reinterpret_cast<const LfPackedTileHost*>(at_<char>(a[6]) + e->more[1]);
-  p->low = at_(a[7]);
+  p->dkdv_tiles = reinterpret_cast<const LfPackedTileHost*>(at_<char>(a[7]) + e->more[0]);
+  p->dq_tiles = reinterpret_cast<const LfPackedTileHost*>(at_<char>(a[7]) + e->more[1]);
+  p->low = at_(a[5]);
   at::Tensor ds;
   if (e->more[2]) {
     // last: it may take what room is left, which the results need and it does not

@@ -307,12 +307,12 @@ def rows_apart(t):
 
 
 def _backward(q, k, v, o, lse, dout, plan, layout, low=None):
-    done = _host.attention_packed_backward(q, k, v, o, dout, lse, layout.tiles, low, plan, layout.total, layout.caps[-1])
+    done = _host.attention_packed_backward(q, k, v, o, dout, low, lse, layout.tiles, plan, layout.total, layout.caps[-1])
     if done is None:      # (operands with rows that are not apart are of no signature that is kept)
         apart = [rows_apart(t) for t in (q, k, v, dout)]
         if any(a is not b for a, b in zip(apart, (q, k, v, dout))):
             q, k, v, dout = apart
-            done = _host.attention_packed_backward(q, k, v, o, dout, lse, layout.tiles, low, plan, layout.total, layout.caps[-1])
+            done = _host.attention_packed_backward(q, k, v, o, dout, low, lse, layout.tiles, plan, layout.total, layout.caps[-1])
     # (False: there was no room for dS)
     return done or _backward_general(q, k, v, o, lse, dout, plan, layout, low, done is None)
 
@@ -352,6 +352,10 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
             raise UnsupportedPlan(f"{name} must have the shape of Q")
     if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T) or not lse.is_contiguous() or lse.device != dev:
         raise UnsupportedPlan(f"lse must be a contiguous float32 [{Hq}, {T}] tensor on the device of Q")
+    if low is not None:
+        _rows("what rounding took from O", low, layout, dtype, D)
+        if low.shape != o.shape or low.stride() != o.stride():
+            raise UnsupportedPlan("what rounding took from O must have its shape and strides")
     for name, t in (("Q", q), ("dO", dout), ("K", k), ("V", v)):
         if _row_stride(t) < D or 2 * (T + 64) * _row_stride(t) + 2 * D >= 1 << 32:
             raise UnsupportedPlan(f"{name}: {T} rows of stride {t.stride(0)} are beyond the direct loads' reach")
@@ -395,7 +399,7 @@ def _backward_general(q, k, v, o, lse, dout, plan, layout, low, room=True):
     res = _backward_again(q, k, v, o, lse, dout, layout, low, repeat)
     if res is None:
         return _backward_general(q, k, v, o, lse, dout, plan, layout, low, False)
-    key = lowering._call_key("b", (q, k, v, o, dout), (lse, layout.tiles, low), plan, (T, layout.caps[-1]))
+    key = lowering._call_key("b", (q, k, v, o, dout, low), (lse, layout.tiles), plan, (T, layout.caps[-1]))
     # an allocation that fails makes the allocator give back what it holds and wait for the device: the form without dS is kept, and room for dS looked
     # for again once in many calls
     lowering._keep_call(key, repeat, (*repeat.more, -1 if keep_ds or not wants_ds else lowering._NO_ROOM_CALLS))
@@ -452,6 +456,8 @@ def bwd_keep_ds(D: int, softcap: bool, blocks: int) -> bool:
 
 def _gradients(ctx, dout):
     q, k, v, out, lse, low = ctx.saved_tensors
+    if low.stride() != out.stride():      # (hooks of saved tensors may give them back with strides of their own)
+        out, low = (t.clone(memory_format=torch.contiguous_format) for t in (out, low))
     if dout.stride(-1) != 1 or dout.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(dout.shape[:-1], dout.stride()[:-1])):
         dout = dout.contiguous()
     return (*_backward(q, k, v, out, lse, dout, ctx.plan, ctx.layout, low), None, None)

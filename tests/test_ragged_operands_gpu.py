@@ -217,3 +217,34 @@ def test_a_backward_without_room_for_ds_looks_for_it_again_once_in_many_calls(mo
     monkeypatch.setattr(packed, "_backward_general", None)
     assert all(torch.equal(x, y) for x, y in zip(packed.attention_packed_backward(q, k, v, o, lse, g, plan, layout), got))
     paged._host.clear()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("how", ["strides", "borders"])
+def test_saved_tensors_that_hooks_give_back_with_strides_of_their_own(D, how):
+    """What is kept beside O is read by O's strides, in pieces of 16 bytes."""
+    q, k, v, g, bounds = inputs([50, 1, 97], 4, 2, D, torch.bfloat16, 11)
+    plan, layout = AttnPlan("causal", scale=D ** -0.5), layout_of(bounds, len(q))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(packed.attention_packed(*leaves, plan, layout), leaves, g)
+    count = []
+
+    def unpack(t):
+        count.append(t)
+        if len(count) % 6:                 # Q, K, V, O and lse as they are, what is kept beside O last
+            return t
+        if how == "strides":
+            return t.transpose(0, 1).contiguous().transpose(0, 1)
+        flat = torch.empty(t.numel() + 8, dtype=t.dtype, device=DEV)
+        return flat[1:1 + t.numel()].view(t.shape).copy_(t)
+
+    for _ in range(2):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            out = packed.attention_packed(*leaves, plan, layout)
+            if how == "borders":
+                with pytest.raises(UnsupportedPlan, match="aligned"):
+                    torch.autograd.grad(out, leaves, g)
+            else:
+                got = torch.autograd.grad(out, leaves, g)
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert len(count) == 12
