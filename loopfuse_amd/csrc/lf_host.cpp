@@ -12,8 +12,10 @@
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -287,6 +289,28 @@ bool takes(Py_ssize_t n, Py_ssize_t want) {
   return n == want;
 }
 
+// Does the node that made the tensor, and that its gradient goes to, belong to a stream outside the capture?  A captured backward that reaches such
+// a node would have its stream wait inside the capture, which ends the process.
+bool node_elsewhere(const at::Tensor& t) {
+  const std::shared_ptr<torch::autograd::Node> node = t.requires_grad() ? t.grad_fn() : nullptr;
+  const auto stream = node ? node->stream() : std::nullopt;
+  if (!stream) return false;
+  // (torch's nodes name the device type CUDA, its HIP streams HIP)
+  const c10::hip::HIPStream its(c10::hip::HIPStream::UNCHECKED,
+                                c10::Stream(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, stream->device_index()), stream->id()));
+  if (its.stream() == nullptr) return true;            // (the default stream is never captured, and not to be asked while another is)
+  const c10::hip::HIPStreamGuard guard(its);
+  return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::Active;
+}
+
+// elsewhere(tensor) -> node_elsewhere
+PyObject* elsewhere(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 1)) return nullptr;
+  return PyBool_FromLong(THPVariable_Check(a[0]) && node_elsewhere(THPVariable_Unpack(a[0])));
+  END_HANDLE_TH_ERRORS
+}
+
 // extend_tables(cached, new, table, free, page_size, total) -> PagedStep; more: entries of the one allocation, then of its five parts
 PyObject* extend_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -516,7 +540,7 @@ PyObject* attention_packed_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
 
 #define LF_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LF_FAST(setup), LF_FAST(key), LF_FAST(keep), {"clear", clear, METH_NOARGS, nullptr}, {"size", size, METH_NOARGS, nullptr},
-                         LF_FAST(packed_layout), LF_FAST(extend_tables), LF_FAST(store_kv), LF_FAST(attention_shared), LF_FAST(attention_packed), LF_FAST(attention_packed_backward),
+                         LF_FAST(elsewhere), LF_FAST(packed_layout), LF_FAST(extend_tables), LF_FAST(store_kv), LF_FAST(attention_shared), LF_FAST(attention_packed), LF_FAST(attention_packed_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lf_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -181,16 +181,17 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
 
     Differentiable where gradients are recorded and neither ``out`` nor ``lse`` is given; gradients of rows of no sequence are zero.  Forward-mode
     derivatives are refused.
-    Under graph capture a leaf that another autograd graph holds is refused: capture forward and backward with no eager graph of them alive.
+    Under graph capture a leaf that another autograd graph holds is refused, and what a graph made outside the capture computed: capture forward and
+    backward with no eager graph of them alive.
     Kept for the backward besides Q, K, V and O: lse, and what rounding takes from O, as large as O (it halves what delta is off by)."""
     if not isinstance(layout, PackedLayout):
         raise UnsupportedPlan("layout must come from packed_layout")
     grads = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if grads and (out is not None or lse is not None):
         raise UnsupportedPlan("out and lse are for calls without gradients")
-    if grads and torch.cuda.is_current_stream_capturing() and any(t.requires_grad and t.is_leaf and in_a_graph(t) for t in (q, k, v)):
-        raise UnsupportedPlan("under capture, Q, K and V must not be leaves of an autograd graph that lives: its stream would be waited for. "
-                              "Drop what that graph computed, or take detached tensors")
+    if grads and torch.cuda.is_current_stream_capturing() and any(t.requires_grad and (in_a_graph(t) if t.is_leaf else _host.elsewhere(t)) for t in (q, k, v)):
+        raise UnsupportedPlan("under capture, Q, K and V must not be leaves of an autograd graph that lives, nor come from one that was made outside: its "
+                              "stream would be waited for. Drop what that graph computed, or take detached tensors")
     if q.dim() == 3 and q.shape[2] not in (64, 128) and 1 <= q.shape[2] < 128:
         if out is not None or lse is not None or k.dim() != 3 or v.dim() != 3 or k.shape[2] != q.shape[2] or v.shape[2] != q.shape[2]:
             raise UnsupportedPlan(f"head dim {q.shape[2]}: by zero-padding, without out and lse")

@@ -248,3 +248,53 @@ def test_saved_tensors_that_hooks_give_back_with_strides_of_their_own(D, how):
                 got = torch.autograd.grad(out, leaves, g)
                 assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert len(count) == 12
+
+
+def test_a_captured_call_refuses_what_an_eager_graph_computed():
+    q, k, v, g, bounds = inputs([50, 30], 4, 2, 64, torch.bfloat16)
+    plan, layout = AttnPlan("causal", scale=0.1), layout_of(bounds, len(q))
+    packed.attention_packed(q, k, v, plan, layout)
+    leaf = q.clone().requires_grad_(True)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        there = leaf * 2
+    outside = [leaf * 2, there, (leaf * 2).view(q.shape)]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        g.add_(0)
+        for x in outside:
+            with pytest.raises(UnsupportedPlan, match="under capture"):
+                packed.attention_packed(x, k, v, plan, layout)
+        packed.attention_packed(outside[0].detach(), k, v, plan, layout)
+        with torch.no_grad():
+            packed.attention_packed(outside[0], k, v, plan, layout)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_captured_calls_take_what_was_computed_in_the_capture(D):
+    q, k, v, g, bounds = inputs([50, 1, 130], 4, 2, D, torch.bfloat16)
+    plan, layout = AttnPlan("causal", scale=D ** -0.5), layout_of(bounds, len(q))
+
+    def step(leaves):
+        a, b, c = leaves
+        first = packed.attention_packed(a, b, c, plan, layout)
+        second = packed.attention_packed(first + a, b * 1, c * 2, plan, layout)
+        return (first.detach(), second.detach(), *torch.autograd.grad((first, second), leaves, (g, g)))
+
+    def fresh():
+        return [t.clone().requires_grad_(True) for t in (q, k, v)]
+
+    step(fresh())
+    want = step(fresh())
+    held = fresh()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(held)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        step(fresh())
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
