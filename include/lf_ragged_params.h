@@ -27,7 +27,7 @@ typedef struct LfPackedPlanParamsHost {
   const int32_t* offsets;  /* [N + 1] */
   LfPackedTileHost* tiles; /* [4 * (cap[0] + ... + cap[3])] */
   int32_t* sorted;         /* scratch, [7][N + 2] */
-  int32_t N, T;            /* sequences, rows */
+  int32_t N, T;            /* sequences, 2^22 at most; rows, 2^31 - 1024 at most */
   int32_t cap[4];          /* entries of a list: T / height + N + 2 */
 } LfPackedPlanParamsHost;
 
@@ -39,7 +39,8 @@ typedef struct LfPackedAttnParamsHost {
   int32_t clear;           /* 1: zeros into rows of no sequence */
 } LfPackedAttnParamsHost;
 
-/* The backward kernels with -DLF_PACKED=1: B = 1, Sq = Sk = T, lse and delta [Hq, T]. */
+/* The backward kernels with -DLF_PACKED=1: B = 1, Sq = Sk = T, lse and delta [Hq, T]; rows of Q, K, V and dO lie D elements apart or more
+ * (what is read behind a sequence's last row has to lie outside it). */
 typedef struct LfPackedBwdParamsHost {
   LfAttnBwdParamsHost bwd;
   const LfPackedTileHost* dkdv_tiles;      /* lists for tiles of as many keys, and queries, as a workgroup has */
@@ -92,7 +93,7 @@ typedef struct LfStoreParamsHost {
   int64_t k_ss, k_sh, v_ss, v_sh;                    /* strides in pieces of 16 bytes: rows, heads */
   int64_t kp_sb, kp_ss, kp_sh, vp_sb, vp_ss, vp_sh;  /* pages, tokens of a page, heads */
   int64_t last;            /* slots of a pool */
-  int32_t T, heads, per_head;
+  int32_t T, heads, per_head;      /* T: 2^31 - 256 at most */
   int32_t shift;           /* log2 of the tokens per page */
 } LfStoreParamsHost;
 

@@ -7,9 +7,13 @@
 //   Workgroup -> (entry, head): the heads of an entry are neighbours, so that with a multiple of 8 of them each XCD walks
 // its own heads over the entries in their order, and the tiles of a (sequence, head) share its K / V (or Q / dO) in one L2.  A list is
 // ordered by the tiles' work within groups of sequences; which list a launch takes: packed.group_size.
-//   MFMA- and exponential-bound as the dense kernels are, with the longest chain of tiles on top where sequences are few.  bf16 causal, head dim 128, 12
-// sequences up to 2048, 32/8 heads: 175 us (887 TFLOP/s); window 256 and softcap, fp16, 5 up to 4001: 87 us (2.8 TB/s of Q, K, V and O); forward
-// and backward, 8 up to 2048, 32/32 heads 142 + 452 us (646 TFLOP/s), 24 up to 1000, fp16, D 64, 16/4 heads 25 + 77 us (its longest key tile).
+//   MFMA- and exponential-bound as the dense kernels are, with the longest chain of tiles on top where sequences are few.  Kernels, bf16 causal, head
+// dim 128, 12 sequences up to 2048, 32/8 heads: 177 us (877 TFLOP/s); window 256 and softcap, fp16, 5 up to 4001: 94 us (2.6 TB/s of Q, K, V and O);
+// forward, delta, dK and dV, dQ, 8 up to 2048, 32/32 heads 142 + 41 + 322 + 102 us (631 TFLOP/s); forward, delta, all gradients, 24 up to 1000, fp16, D 64,
+// 16/4 heads 25 + 11 + 66 us (its longest key tile).
+//   P, and dS in the backward, are 16-bit operands of the second products, as in the dense kernels: matrix instructions take both operands in the
+// type of K, V, Q and dO, and dS kept in 32 bits would be twice the bytes that bound dQ.  Against 64 bits that is 1.25 ... 1.45 times the error of
+// rounding the results alone, a little over 1.5 where rows of dS cancel.
 #ifndef LF_PACKED_HIP_H
 #define LF_PACKED_HIP_H
 
@@ -47,7 +51,7 @@ struct LfPackedAttnParams : LfAttnParams {      // Sq = Sk = rows of the tensors
   const LfPackedTile* tiles;
   // Optional, strides of O: O in 32 bits minus O as stored, rounded.  The backward takes delta = rowsum(dO * O) from dP, often of its size:
   // of O as stored alone, dQ and dK are off by 1.8 times what rounding the formula's gradients costs, of both by 1.45 times.  The 2 bytes
-  // per element, written and read once, cost 594 -> 616 us at 8 sequences of 2048, 32/8 heads of 128.
+  // per element, written and read once, cost 572 -> 597 us (forward and backward) at 8 sequences up to 2048, 32/32 heads of 128.
   lf_elem* low;
   int clear;               // 1: rows of no sequence are set to zero, 0: they are left as they are
 };

@@ -8,8 +8,9 @@
 //   lengths[b] = c + the number of its new tokens in front of the first that has no slot.
 // A block has one request (and a share of its tokens): it forms the two sums itself from all B lengths, which are in L2 after the first
 // block, so that no block waits for another.  Slots of new pages come from the list of free ones, not from the table, so blocks of one
-// request do not wait for each other's entries either.  Bound by its chain of round trips (lengths, then the page, then the stores): 64 requests of one
-// new token 4.1 us, 256 of 2048 and fewer (2.2 MB) 6.1, as long as the call takes the host.
+// request do not wait for each other's entries either.  The first of them looks for the first page that is none, with all its threads.  Bound by its chain of
+// round trips (lengths, then the pages, then the stores): 64 requests of one new token 4.4 us, 256 of 2048 and fewer (2.2 MB) 6.4, as long as the
+// call takes the host.
 // What does not fit -- no free page left, a row of the table too short, a token behind the last row -- gets page and slot -1.  A page id below 0 or
 // whose slots are no numbers in 32 bits is no page either: its tokens get slot -1.  lengths[b] ends in front of the first token without a slot,
 // so that nothing reads keys that are not there.
