@@ -134,6 +134,35 @@ def test_kept_ds_of_a_sequence_of_nan_stays_apart(mask, threads, q_split, monkey
         assert all(torch.equal(x[keep], y[keep]) for x, y in zip(tensors, res[0][1]))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_windows_beyond_all_rows_and_batches_of_no_sequence(D):
+    q, k, v, g, bounds = inputs([200, 1, 90], 4, 2, D, BF, 0, 5, 3)
+    layout, T = layout_of(bounds, len(q)), len(q)
+    for window in (200, 1 << 20, 1 << 40):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        out = packed.attention_packed(*leaves, AttnPlan("sliding", window=window, scale=0.1), layout)
+        want = oracle(q, k, v, g, bounds, "causal", 0, 0.1, None)[0]
+        for name, t in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, g))):
+            check(t, want[name], f"{name} {window}")
+    none = packed.packed_layout(torch.tensor([7], dtype=torch.int32, device=DEV), T)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = packed.attention_packed(*leaves, AttnPlan("causal", scale=0.1), none)
+    assert not out.any() and not any(t.any() for t in torch.autograd.grad(out, leaves, g))
+
+
+@pytest.mark.parametrize("D,mask,cap", [(128, "causal", None), (64, None, None), (128, "sliding", 30.0)])
+def test_peaked_rows(D, mask, cap):
+    """Scores of +-100 and more: rows whose weight lies on one key, far from the first tile's maximum."""
+    q, k, v, g, bounds = inputs([400, 65, 130], 4, 2, D, BF, 2)
+    q, k = q * 4, k * 4
+    plan, layout = AttnPlan(mask, window=150, scale=0.5, softcap=cap), layout_of(bounds, len(q))
+    want = oracle(q, k, v, g, bounds, mask, 150, 0.5, cap)[0]
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = packed.attention_packed(*leaves, plan, layout)
+    for name, t in zip(("out", "dq", "dk", "dv"), (out.detach(), *torch.autograd.grad(out, leaves, g))):
+        check(t, want[name], name)
+
+
 # ---- packed: batches of real sizes, by the rules ------------------------------------------------------------------------------------
 
 LARGE = [
@@ -242,3 +271,33 @@ def test_requests_of_real_numbers(case, specs):
     paged_tests.check(out, shared_oracle(q, kp, vp, table, n, pre, prefix, D ** -0.5, cap))
     for _ in range(3):
         assert torch.equal(paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=prefix), out)
+
+
+@pytest.mark.parametrize("choice", [{"coop": 4, "prefix": "tiles"}, {"coop": 4, "prefix": "tiles", "near": False}, {"coop": 0, "prefix": "tiles", "near": False}, {"coop": 8, "prefix": "stream"}], ids=str)
+def test_builds_with_tables_in_64_bits(choice):
+    q, kp, vp, table, n, pre = paged_tests.batch(4, [90, 0, 300, 16], 150, 16, 8, 4, 128, BF, seed=3, table_dtype=torch.int64)
+    plan = AttnPlan(scale=0.1, k_paged=True, v_paged=True)
+    want = shared_oracle(q, kp, vp, table, n, pre, 150, 0.1, None)
+    paged_tests.check(paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=150, choice=choice), want)
+
+
+@pytest.mark.parametrize("page,D", [(2, 128), (4, 64), (32, 128), (128, 64), (512, 128)])
+def test_other_page_sizes(page, D):
+    q, kp, vp, table, n, pre = paged_tests.batch(4, [90, 0, 700, 33], 600, page, 8, 4, D, HALF, seed=page)
+    plan = AttnPlan(scale=0.1, k_paged=True, v_paged=True)
+    want = shared_oracle(q, kp, vp, table, n, pre, 600, 0.1, None)
+    for choice in (None, {"prefix": "stream", "splits": 3}, {"prefix": "tiles", "near": False}) + (({"coop": 4},) if D == 128 else ({"coop": 8, "prefix": "stream"},)):
+        paged_tests.check(paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=600, choice=choice), want, str(choice))
+
+
+@pytest.mark.parametrize("prefix", [0, 70])
+def test_thousands_of_requests(prefix):
+    """The lengths are scanned 64 at a time."""
+    lengths = [(i * 37) % 41 for i in range(3000)]
+    q, kp, vp, table, n, pre = paged_tests.batch(3000, lengths, prefix, 16, 2, 2, 64, BF, seed=1)
+    plan = AttnPlan(scale=0.1, k_paged=True, v_paged=True)
+    out = paged.attention_shared(q, kp, vp, plan, table, n, prefix_table=pre, prefix_len=prefix)
+    some = list(range(0, 3000, 43)) + [2998, 2999]
+    at = torch.tensor(some, device=DEV)
+    paged_tests.check(out[at], shared_oracle(q[at], kp, vp, table[at], n[at], pre, prefix, 0.1, None))
+    assert torch.isfinite(out).all() and (prefix or not out[n == 0].any())
