@@ -140,6 +140,23 @@ def test_lengths_end_in_front_of_a_token_without_a_slot(case, dtype):
         assert step.lengths.tolist() == lengths and step.slots.tolist() == slots + [-1] * (total - len(slots))
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("count", [64, 65, 68, 1023, 1025, 8193, 20000])
+def test_the_first_page_that_is_none_is_found_anywhere_in_a_long_list(count, dtype):
+    """One-token pages from lists that begin anywhere, two requests; the last id, the first, two of them, those beside the requests' own."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    for lead, bad in ((0, []), (1, [count - 1]), (2, [0]), (3, [count // 2, count // 3]), (5, [count]), (1, [count + 3, 2])):
+        store = torch.arange(lead + count + 10, dtype=dtype, device=DEV)
+        free = store[lead:]
+        free[torch.tensor(bad, dtype=torch.long, device=DEV)] = -1
+        store[:lead] = -1
+        free[count + 7:] = -1
+        table = torch.zeros((2, count + 9), dtype=dtype, device=DEV)
+        step = paged.extend_tables(i32([2, 0]), i32([count, 7]), table, free, 1, count + 7)
+        mine, other = [x for x in bad if x < count], [x - count for x in bad if x >= count]
+        assert step.lengths.tolist() == [2 + min(mine, default=count), min(other, default=7)], (lead, bad)
+
+
 def test_pages_beyond_64_bit_numbers_of_slots_are_none():
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
     step = paged.extend_tables(i32([0, 3]), i32([33, 2]), torch.tensor([[0] * 3, [2 ** 40] * 3], device=DEV), torch.tensor([4, 2 ** 33 + 1, 6], device=DEV), 16, 40)
