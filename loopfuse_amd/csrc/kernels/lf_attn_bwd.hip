@@ -118,6 +118,13 @@ __device__ __forceinline__ long long lf_bw_ds_before(int row0, int seq, int T, i
   return (long long)(row0 / 32 + seq) * per;
 }
 #endif
+// The factor of dS in dQ and dK, zero where all rows that it is for see one key (or row `row` does): P is 1 whatever the scores are, dP and delta are the same
+// sum, and what their two orders leave of it, 1e-7 of its terms, would be all that a batch of one-row sequences has of dQ and dK.
+#if LF_PACKED
+__device__ __forceinline__ float lf_bw_factor(float scale, int len, int window, int row) {
+  return len == 1 || (LF_MASK == 2 && window == 1) || (LF_MASK >= 1 && row == 0) ? 0.0f : scale;
+}
+#endif
 // A block holds what the lanes of lf_attn_bwd_dkdv hold as the B operand of dK^T += Q^T dS, 16-byte chunks (half h of the 32
 // queries, lane half g, key) of 8 queries, permuted so that the transposed reads of lf_attn_bwd_dq (4 keys, all 16 queries
 // of both halves at a time) touch every LDS bank once: byte offset of lane (g, key)'s chunk of half 0; half 1 is (it ^ 128) + 1024.
@@ -965,10 +972,11 @@ extern "C" __global__ void __launch_bounds__(LF_BW_NT, 1) lf_attn_bwd_dkdv(const
   // the parameters of the output are read only now: held over the loop they cost scalar registers it needs
   auto ep = (const LfAttnBwdParams __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(ep));
-  const float scale = ep->scale;
 #if LF_PACKED
+  const float scale = lf_bw_factor(ep->scale, p.Sk, ep->window, -1);
   const long long out0 = mine.row0;
 #else
+  const float scale = ep->scale;
   const long long out0 = 0;
 #endif
 #if LF_BW_QSPLIT
@@ -1154,10 +1162,15 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   }
 #pragma unroll
   for (int db = 0; db < LF_NDB; ++db) asm volatile(LF_BW_MFMA_DRAIN_LAST : "+a"(dq[db]));
+#if LF_PACKED
+  const float scale = lf_bw_factor(p.scale, p.Sk, p.window, wq0 + l32);
+#else
+  const float scale = p.scale;
+#endif
 #pragma unroll
   for (int db = 0; db < LF_NDB; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dq[db][i] *= p.scale;
+    for (int i = 0; i < 16; ++i) dq[db][i] *= scale;
   static_assert(kWaves * LF_BW_ROWS_LDS <= (int)sizeof(ds_tiles), "the rows fit the tiles");
 #if !LF_STAY
   __syncthreads();               // nobody reads the tiles any more
@@ -1534,10 +1547,15 @@ extern "C" __global__ void __launch_bounds__(LF_BW_DQ_NT, LF_BW_DQ_NT / 256) lf_
   }
 #pragma unroll
   for (int db = 0; db < LF_NDB; ++db) asm volatile(LF_BW_MFMA_DRAIN_LAST : "+a"(dq[db]));
+#if LF_PACKED
+  const float scale = lf_bw_factor(p.scale, p.Sk, p.window, wq0 + l32);
+#else
+  const float scale = p.scale;
+#endif
 #pragma unroll
   for (int db = 0; db < LF_NDB; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dq[db][i] *= p.scale;
+    for (int i = 0; i < 16; ++i) dq[db][i] *= scale;
   static_assert(LF_BW_DQ_NT / 64 * LF_BW_ROWS_LDS <= (int)sizeof(tiles), "the rows fit the tiles");
 #if !LF_STAY
   __syncthreads();               // nobody reads the tiles any more

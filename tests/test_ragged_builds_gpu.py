@@ -134,6 +134,34 @@ def test_kept_ds_of_a_sequence_of_nan_stays_apart(mask, threads, q_split, monkey
         assert all(torch.equal(x[keep], y[keep]) for x, y in zip(tensors, res[0][1]))
 
 
+@pytest.mark.parametrize("D,dtype", [(64, BF), (64, HALF), (128, BF), (128, HALF)])
+@pytest.mark.parametrize("mask,window,cap", [("causal", 0, None), (None, 0, None), ("sliding", 1, None), ("sliding", 9, 20.0), (None, 0, 5.0)])
+@pytest.mark.parametrize("threads,q_split,ds", [(256, True, True), (512, False, True), (256, False, False), (512, True, False)])
+def test_rows_that_see_one_key_have_no_gradient_of_scores(D, dtype, mask, window, cap, threads, q_split, ds, monkeypatch):
+    """Their softmax is 1 whatever Q and K are: dQ is zero, and dK of keys that nothing else sees; dV is dO."""
+    if D == 64 and (threads == 512 or (ds and not cap)):
+        pytest.skip("no such build")
+    monkeypatch.setattr(packed, "bwd_dq_threads", lambda *a: threads)
+    monkeypatch.setattr(packed, "bwd_q_split", lambda *a: q_split)
+    monkeypatch.setattr(packed, "bwd_keep_ds", lambda *a: ds)
+    plan = AttnPlan(mask, window=window, scale=D ** -0.5, softcap=cap)
+    for lengths in ([1] * 50, [1, 0, 0, 1], [1, 70, 1, 300]):
+        q, k, v, g, bounds = inputs(lengths, 4, 2, D, dtype, len(lengths))
+        layout = layout_of(bounds, len(q))
+        paged._host.clear()
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        dq, dk, dv = torch.autograd.grad(packed.attention_packed(*leaves, plan, layout), leaves, g)
+        want = oracle(q, k, v, g, bounds, mask, window, plan.scale, cap)[0]
+        for name, t in (("dq", dq), ("dk", dk), ("dv", dv)):
+            check(t, want[name], name)
+        for lo, hi in zip(bounds[:-1], bounds[1:]):
+            if hi - lo == 1 or (mask == "sliding" and window == 1):
+                assert not dq[lo:hi].any() and not dk[lo:hi].any()
+            elif hi > lo and mask is not None:
+                assert not dq[lo].any() and dq[lo + 1:hi].any()
+    paged._host.clear()
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_windows_beyond_all_rows_and_batches_of_no_sequence(D):
     q, k, v, g, bounds = inputs([200, 1, 90], 4, 2, D, BF, 0, 5, 3)
