@@ -134,13 +134,15 @@ def test_kept_ds_of_a_sequence_of_nan_stays_apart(mask, threads, q_split, monkey
         assert all(torch.equal(x[keep], y[keep]) for x, y in zip(tensors, res[0][1]))
 
 
-@pytest.mark.parametrize("D,dtype", [(64, BF), (64, HALF), (128, BF), (128, HALF)])
-@pytest.mark.parametrize("mask,window,cap", [("causal", 0, None), (None, 0, None), ("sliding", 1, None), ("sliding", 9, 20.0), (None, 0, 5.0)])
-@pytest.mark.parametrize("threads,q_split,ds", [(256, True, True), (512, False, True), (256, False, False), (512, True, False)])
+# masks, and the builds that there are: head dim 64 has small workgroups, and keeps dS with a softcap only
+ONE_KEY = [(D, *mask, *build) for D in (64, 128) for mask in (("causal", 0, None), (None, 0, None), ("sliding", 1, None), ("sliding", 9, 20.0), (None, 0, 5.0))
+           for build in ((256, True, True), (512, False, True), (256, False, False), (512, True, False)) if D == 128 or (build[0] == 256 and (mask[2] or not build[2]))]
+
+
+@pytest.mark.parametrize("dtype", [BF, HALF])
+@pytest.mark.parametrize("D,mask,window,cap,threads,q_split,ds", ONE_KEY)
 def test_rows_that_see_one_key_have_no_gradient_of_scores(D, dtype, mask, window, cap, threads, q_split, ds, monkeypatch):
     """Their softmax is 1 whatever Q and K are: dQ is zero, and dK of keys that nothing else sees; dV is dO."""
-    if D == 64 and (threads == 512 or (ds and not cap)):
-        pytest.skip("no such build")
     monkeypatch.setattr(packed, "bwd_dq_threads", lambda *a: threads)
     monkeypatch.setattr(packed, "bwd_q_split", lambda *a: q_split)
     monkeypatch.setattr(packed, "bwd_keep_ds", lambda *a: ds)
