@@ -189,9 +189,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
     grads = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if grads and (out is not None or lse is not None):
         raise UnsupportedPlan("out and lse are for calls without gradients")
-    if grads and torch.cuda.is_current_stream_capturing() and any(t.requires_grad and (in_a_graph(t) if t.is_leaf else _host.elsewhere(t)) for t in (q, k, v)):
-        raise UnsupportedPlan("under capture, Q, K and V must not be leaves of an autograd graph that lives, nor come from one that was made outside: its "
-                              "stream would be waited for. Drop what that graph computed, or take detached tensors")
+    if grads:
+        refuse_outside_capture((q, k, v), "Q, K and V")
     if q.dim() == 3 and q.shape[2] not in (64, 128) and 1 <= q.shape[2] < 128:
         if out is not None or lse is not None or k.dim() != 3 or v.dim() != 3 or k.shape[2] != q.shape[2] or v.shape[2] != q.shape[2]:
             raise UnsupportedPlan(f"head dim {q.shape[2]}: by zero-padding, without out and lse")
@@ -212,6 +211,12 @@ def in_a_graph(leaf: torch.Tensor) -> bool:
     edge = torch.autograd.graph.get_gradient_edge
     edge(leaf).node.metadata["loopfuse_amd"] = True
     return edge(leaf).node.metadata.pop("loopfuse_amd", False)
+
+
+def refuse_outside_capture(operands, names: str) -> None:
+    if torch.cuda.is_current_stream_capturing() and any(t.requires_grad and (in_a_graph(t) if t.is_leaf else _host.elsewhere(t)) for t in operands):
+        raise UnsupportedPlan(f"under capture, {names} must not be leaves of an autograd graph that lives, nor come from one that was made outside: its "
+                              "stream would be waited for. Drop what that graph computed, or take detached tensors")
 
 
 def _forward_again(q, k, v, layout, out, lse, low, repeat):

@@ -8,19 +8,27 @@ A serving step over a batch of requests, nothing of which waits for the lengths,
                          prefix_table=prefix, prefix_len=n)              # and over a prefix that all requests share
 
 Pools are ``[pages, page, Hkv, D]`` (or ``[pages, Hkv, D]`` for one-token pages), as ``lowering.attention`` takes them; a table
-row names a request's pages in the order of its tokens.  The reference reads caches of one length through
+row names a request's pages in the order of its tokens.  ``append_kv`` norms and rotates the new queries and keys on the way to the pools.
+
+Pools in 4 bits (``pool4``) hold nearly four times as many tokens and are read in a quarter of the time:
+
+    q = append_kv(q, k, v, k_pool, v_pool, step.slots, step.positions, table_of_angles)
+    o = attention_cached(q, k_pool, v_pool, plan, table, step.lengths, step.offsets, step.positions)      # one token per request or several
+
+The reference reads caches of one length through
 ``paged_load`` (reference loopfuse/torch_backend/__init__.py:46-56) and leaves tables and stores to its user.
 """
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 import math
 import operator
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Union
 
 import torch
 
-from . import lowering
+from . import lowering, rotary
 from .lowering import AttnPlan, UnsupportedPlan
 
 _TABLE_DTYPES = (torch.int32, torch.int64)
@@ -47,6 +55,33 @@ class SharedParams(lowering.AttnParams):
 
     _fields_ = ([(n, ctypes.c_void_p) for n in ("lengths", "prefix_k", "prefix_v", "pre_acc", "pre_ml")]
                 + [(n, ctypes.c_int) for n in ("room", "units", "pre_units", "pre_blocks", "target_log2", "least")])
+
+
+class _ReadParams(ctypes.Structure):
+    """Mirror of ``struct LfReadParams`` in csrc/kernels/lf_read_kv.hip."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k_pool", "v_pool", "k_scales", "v_scales", "k", "v", "slots")]
+                + [(n, ctypes.c_longlong) for n in ("kp_sb", "kp_ss", "kp_sh", "vp_sb", "vp_ss", "vp_sh", "last")]
+                + [(n, ctypes.c_int) for n in ("T", "heads", "per_head", "shift")])
+
+
+@dataclasses.dataclass(frozen=True, eq=False)
+class Pool4:
+    """A page pool of keys or values held in 4 bits (``pool4``)."""
+
+    codes: torch.Tensor        # uint8 [pages, heads, page / 16, 8 * D]
+    scales: torch.Tensor       # uint8 [pages, heads, page / 16, D / 2]
+    dtype: torch.dtype         # of the rows that it stands for
+
+    @property
+    def shape(self) -> tuple:
+        """(pages, page size, heads, D)"""
+        n, heads, tiles, row = self.codes.shape
+        return n, 16 * tiles, heads, row // 8
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
 
 
 class PagedStep(NamedTuple):
@@ -163,13 +198,199 @@ def _pool(name: str, t: torch.Tensor) -> tuple:
     raise UnsupportedPlan(f"{name} pool must be [N, Hkv, D] or [N, P, Hkv, D]")
 
 
+def pool4(pages: int, page_size: int, heads: int, D: int, dtype: torch.dtype, device=None) -> Pool4:
+    """A pool of ``pages`` pages of keys, or of values, in 4 bits, holding zeros.  page_size: a power of two, 16 at least; D 64 or 128; ``dtype``:
+    bf16 or fp16, of the rows that it stands for.
+
+    A value is 0 0.5 1 1.5 2 3 4 or 6 with a sign, times a power of two that 32 neighbours of a row share, the least one of which their largest size is below the
+    7-fold: 4.25 bits an element, off by a sixth of the largest size of its 32 at most.  Sizes beyond ``6 * 2 ** 125`` (fp16: ``6 * 2 ** 13``) count as that; 32
+    neighbours with a NaN or an infinity among them are NaN.  Keys and values lie in different orders: a pool of the one is not read as the other."""
+    shift = _shift(page_size)
+    if shift < 4 or D not in (64, 128) or heads < 1 or pages < 0 or dtype not in lowering._DTYPE_CODE:
+        raise UnsupportedPlan("a pool in 4 bits has pages of 16 tokens or more, head dim 64 or 128, and stands for bf16 or fp16 rows")
+    lead = (pages, heads, page_size // 16)
+    return Pool4(torch.zeros((*lead, 8 * D), dtype=torch.uint8, device=device), torch.zeros((*lead, D // 2), dtype=torch.uint8, device=device), dtype)
+
+
+def _pool4(name: str, pool: Pool4, dtype, device) -> tuple:
+    """(pages, page size, heads, D) of a pool in 4 bits that the kernels serve."""
+    if not isinstance(pool, Pool4):
+        raise UnsupportedPlan("pools of K and V must both be in 4 bits, or both not")
+    codes, scales = pool.codes, pool.scales
+    for t in (codes, scales):
+        _on_gpu(f"{name} pool", t, (torch.uint8,), 4, device)
+    n, heads, tiles, row = codes.shape
+    if pool.dtype != dtype:
+        raise UnsupportedPlan(f"{name} pool stands for {pool.dtype} rows, not for {dtype}")
+    if row not in (512, 1024) or tuple(scales.shape) != (n, heads, tiles, row // 16) or heads < 1 or tiles < 1 or tiles & (tiles - 1):
+        raise UnsupportedPlan(f"{name} pool: not the shapes that pool4 makes")
+    for t in (codes, scales):
+        if n and not t[0].is_contiguous() or t.data_ptr() % 16 or (n > 1 and (t.stride(0) % 16 or t.stride(0) < t[0].numel())):
+            raise UnsupportedPlan(f"{name} pool: pages must be contiguous and apart, on 16-byte borders")
+    return pool.shape
+
+
+def _two_pools4(k_pool, v_pool, dtype, device) -> tuple:
+    shape = _pool4("K", k_pool, dtype, device)
+    if _pool4("V", v_pool, dtype, device) != shape:
+        raise UnsupportedPlan("the pools must agree in pages, page size, heads and head dim")
+    return shape
+
+
+def _two_pools(k_pool, v_pool, dtype, device, heads: int, D: int, written=True) -> tuple:
+    """(pages, page size, strides of K's pages, tokens and heads, V's) of pools of 16-bit rows."""
+    for name, t in (("K pool", k_pool), ("V pool", v_pool)):
+        if not isinstance(t, torch.Tensor):
+            raise UnsupportedPlan("pools of K and V must both be in 4 bits, or both not")
+        lowering._check_tensor(name, t, dtype)
+        if t.device != device:
+            raise RuntimeError(f"loopfuse_amd: {name} is on {t.device}, not on {device}")
+    pages, page, hk, dk, *ks = _pool("K", k_pool)
+    pages_v, page_v, hv, dv, *vs = _pool("V", v_pool)
+    if (pages, page) != (pages_v, page_v) or (hk, dk) != (heads, D) or (hv, dv) != (heads, D):
+        raise UnsupportedPlan("the pools must agree in pages and page size with each other, in heads and head dim with K and V")
+    if written and any(n > 1 and s == 0 for p in (k_pool, v_pool) for n, s in zip(p.shape, p.stride())):
+        raise UnsupportedPlan("every element of a pool must have a place of its own")
+    return pages, page, ks, vs
+
+
+def _checked_slots(slots, last) -> None:
+    if lowering._checks_tables():
+        kept = slots[slots >= 0]
+        if len(kept) and (int(kept.max()) >= last or len(torch.unique(kept)) < len(kept)):
+            raise ValueError(f"loopfuse_amd: slots must be distinct and below {last}")
+
+
 @lowering.outside_graphs
-def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Tensor) -> None:
+def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pool: Union[torch.Tensor, Pool4], v_pool: Union[torch.Tensor, Pool4], slots: torch.Tensor,
+              positions: torch.Tensor, table: Optional[torch.Tensor], *, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+              eps: Optional[float] = None, pairs: bool = False) -> torch.Tensor:
+    """The new tokens' keys, normed and rotated, and their values into the page pools, and their queries, normed and rotated, as a new tensor: what
+    ``rotary.rotate_heads`` and ``store_kv`` do, in one pass.  No gradients are recorded.
+
+    q ``[rows, Hq, D]``, k and v ``[rows, Hkv, D]``, ``positions``, ``table``, weights, ``eps`` and ``pairs`` as ``rotate_heads`` takes them; slots int32 ``[rows]`` and
+    the pools as ``store_kv``: ``PagedStep.slots`` and ``.positions`` of ``extend_tables``.  A row whose position is below 0 or behind the table's last is one of no token:
+    zeros among the queries, left out of the pools whatever its slot.  Without a table and a norm rows stay as they are."""
+    if positions is None:
+        raise UnsupportedPlan("positions must be given")
+    return _append(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight, eps, bool(pairs))
+
+
+@lowering._on_device_of_first_argument
+def _append(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight, eps, pairs):
+    """``positions`` None: only keys and values, into pools in 4 bits; ``q`` then stands for nothing."""
+    lowering._no_tangents(q, k, v, q_weight, k_weight)
+    keys_only = positions is None
+    T, Hq, Hkv, D, R, wide = rotary.check_operands(q, k, positions, table, q_weight, k_weight, eps, (("V", v),), plain=True)
+    _on_gpu("slots", slots, (torch.int32,), 1, q.device)
+    if slots.shape[0] != T:
+        raise UnsupportedPlan(f"slots must be int32 [{T}]")
+    P, per = rotary.params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs)
+    P.v_ss, P.v_sh = v.stride()[:2]
+    if isinstance(k_pool, Pool4) or isinstance(v_pool, Pool4):
+        pages, page, heads, d = _two_pools4(k_pool, v_pool, q.dtype, q.device)
+        if (heads, d) != (Hkv, D):
+            raise UnsupportedPlan("the pools must have the heads and head dim of K and V")
+        P.kp_sb, P.kp_ss, P.vp_sb, P.vp_ss = k_pool.codes.stride(0), k_pool.scales.stride(0), v_pool.codes.stride(0), v_pool.scales.stride(0)
+        store = 2
+    else:
+        lowering._no_tangents(k_pool, v_pool)
+        pages, page, (P.kp_sb, P.kp_ss, P.kp_sh), (P.vp_sb, P.vp_ss, P.vp_sh) = _two_pools(k_pool, v_pool, q.dtype, q.device, Hkv, D)
+        store = 1
+    P.shift, P.last = _shift(page), pages * page
+    if P.q_blocks + 2 * P.k_blocks >= 1 << 24:
+        raise UnsupportedPlan(f"a launch for {T} rows of {Hq} and {Hkv} heads of {D} is too large")
+    if T == 0:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _checked_slots(slots, P.last)
+    if not keys_only:
+        rotary._checked_positions(positions, P.places)
+    if keys_only:
+        P.q_blocks = 0
+    spec = rotary.kernel_spec(q.dtype, D, per, store)
+    repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (P.q_blocks + 2 * P.k_blocks, 1, 1), 256)], {"kernels": [spec.entry()]})
+    return _append_again(q, k, v, k_pool, v_pool, slots.contiguous(), None if keys_only else positions.contiguous(), table, rotary.even_weight(q_weight),
+                         rotary.even_weight(k_weight), repeat)
+
+
+def _append_again(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight, repeat):
+    P = rotary.RotateParams.from_buffer_copy(repeat.block)
+    out = None if positions is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    P.q, P.k, P.v, P.slots = q.data_ptr(), k.data_ptr(), v.data_ptr(), slots.data_ptr()
+    if positions is not None:
+        P.q_out, P.positions = out.data_ptr(), positions.data_ptr()
+    _set_pools(P, "k_out", "v_out", k_pool, v_pool)
+    rotary.set_tables(P, table, q_weight, k_weight)
+    repeat.launches.launch(P)
+    lowering._last_launch.set(repeat.record)
+    return out
+
+
+def _set_pools(P, k_name, v_name, k_pool, v_pool) -> None:
+    for name, scales, pool in ((k_name, "k_scales", k_pool), (v_name, "v_scales", v_pool)):
+        if isinstance(pool, Pool4):
+            setattr(P, name, pool.codes.data_ptr())
+            setattr(P, scales, pool.scales.data_ptr())
+        else:
+            setattr(P, name, pool.data_ptr())
+
+
+@lowering.outside_graphs
+def read_kv(k_pool: Union[torch.Tensor, Pool4], v_pool: Union[torch.Tensor, Pool4], slots: torch.Tensor) -> tuple:
+    """Rows of keys and values out of the page pools, what ``store_kv`` and ``append_kv`` have put there: ``(k, v)``, each ``[rows, Hkv, D]``, row t of slot ``slots[t]``
+    (int32 ``[rows]`` on the GPU, any number of times), zeros where it is below 0 or behind the pool's last.  From pools in 4 bits the values that they stand for,
+    rounded to the type (those of fp16 have less than a bit below its least normal number).  For keys that go on elsewhere: into another cache, or beside
+    those of a prompt's next part."""
+    dtype = k_pool.dtype if isinstance(k_pool, (Pool4, torch.Tensor)) else None
+    if dtype not in lowering._DTYPE_CODE:
+        raise UnsupportedPlan("pools must be of bf16 or fp16 rows")
+    if k_pool.device.type != "cuda" and not getattr(k_pool, "is_cuda", False):
+        raise RuntimeError("loopfuse_amd: K pool is not on the GPU; the HIP path has no CPU fallback")
+    with torch.cuda.device(k_pool.device if k_pool.device.type == "cuda" else -1):
+        P = _ReadParams()
+        if isinstance(k_pool, Pool4):
+            pages, page, heads, D = _two_pools4(k_pool, v_pool, dtype, k_pool.device)
+            P.kp_sb, P.kp_ss, P.vp_sb, P.vp_ss = k_pool.codes.stride(0), k_pool.scales.stride(0), v_pool.codes.stride(0), v_pool.scales.stride(0)
+            spec = lowering._spec("read_kv", lowering._DTYPE_CODE[dtype], D, extra=("-DLF_READ4=1",))
+        else:
+            lowering._no_tangents(k_pool, v_pool)
+            _, _, heads, D, *_ = _pool("K", k_pool)
+            if D % 8:
+                raise UnsupportedPlan("head dim must be a multiple of 8")
+            pages, page, (P.kp_sb, P.kp_ss, P.kp_sh), (P.vp_sb, P.vp_ss, P.vp_sh) = _two_pools(k_pool, v_pool, dtype, k_pool.device, heads, D, False)
+            spec = lowering._spec("read_kv", lowering._DTYPE_CODE[dtype], 64)
+        _on_gpu("slots", slots, (torch.int32,), 1, k_pool.device)
+        T = slots.shape[0]
+        P.last, P.T, P.heads, P.per_head, P.shift = pages * page, T, heads, D // 8, _shift(page)
+        pieces = T * heads * (D // 8)
+        if pieces + 256 >= 1 << 32:
+            raise UnsupportedPlan(f"a launch for {T} rows of {heads} heads of {D} is too large")
+        if pieces == 0:
+            return tuple(torch.empty((T, heads, D), dtype=dtype, device=k_pool.device) for _ in range(2))
+        repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (-(-pieces // 256), 1, 1), 256)], {"kernels": [spec.entry()]}, (T, heads, D))
+        return _read_again(k_pool, v_pool, slots.contiguous(), repeat)
+
+
+def _read_again(k_pool, v_pool, slots, repeat):
+    P = _ReadParams.from_buffer_copy(repeat.block)
+    k, v = (torch.empty(repeat.more, dtype=k_pool.dtype, device=slots.device) for _ in range(2))
+    P.k, P.v, P.slots = k.data_ptr(), v.data_ptr(), slots.data_ptr()
+    _set_pools(P, "k_pool", "v_pool", k_pool, v_pool)
+    repeat.launches.launch(P)
+    lowering._last_launch.set(repeat.record)
+    return k, v
+
+
+@lowering.outside_graphs
+def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: Union[torch.Tensor, Pool4], v_pool: Union[torch.Tensor, Pool4], slots: torch.Tensor) -> None:
     """Write rows of new keys and values, k and v ``[rows, Hkv, D]``, into the page pools: row t into token ``slots[t] % page`` of page
-    ``slots[t] // page``.  bf16 / fp16, D a multiple of 8; views will do.  ``slots``: int32 [rows] (``PagedStep.slots``); rows whose slot is below 0 or
+    ``slots[t] // page``, in pools in 4 bits (``pool4``) rounded as those say.  bf16 / fp16, D a multiple of 8; views will do.  ``slots``: int32 [rows] (``PagedStep.slots``); rows whose slot is below 0 or
     behind the pool's last are left out.  Slots that are not left out are distinct, as those of ``extend_tables`` are:
     of two rows with one slot, either may be found there afterwards, or a part of each."""
     if _host.store_kv(k, v, k_pool, v_pool, slots):
+        return
+    if isinstance(k_pool, Pool4) or isinstance(v_pool, Pool4):
+        _append(k, k, v, k_pool, v_pool, slots, None, None, None, None, None, False)
         return
     lowering._no_tangents(k, v, k_pool, v_pool)
     if k.dtype not in lowering._DTYPE_CODE:
