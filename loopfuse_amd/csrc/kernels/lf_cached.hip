@@ -1,0 +1,561 @@
+// lf_cached.hip — attention of the new tokens of requests of different lengths over their keys and values in page pools held in 4 bits
+// (lf_pool4.hip.h), those of the new tokens among them.
+//
+// Request b has n = offsets[b + 1] - offsets[b] rows of q and lengths[b] keys; a row at position p sees the keys j <= p (and p - j < window), or all.
+// A kv head's n * group rows are taken LF_CACHED_ROWS at a time (a chunk), its keys in pieces of one length for all requests, so that about 2^target_log2
+// workgroups have one; (chunk, piece) pairs are numbered request by request, and every wave finds its own from the lengths, as nothing of them is known
+// to the host.  A piece leaves, per row, an exponent offset, the sum of the exponentials and their sum with V, which lf_cached_combine joins; a
+// chunk of one piece is written at once.
+//
+// A wave takes 32 keys at a time for LF_CACHED_CB * 16 rows, its operands straight from memory:
+//   S^T = K Q^T   : 16 keys' codes and scales are, as loaded, the first operand of the 16x16x128 product of scaled 4- and 8-bit numbers.  Q^T is
+//                   split beforehand into 8-bit numbers of 4 significant bits each whose sum it is (two of them hold bf16's 8, three fp16's 11, down
+//                   to 2^-21 of a row's largest element), with a power of two per row: the products are those of the unrounded q, and no key is
+//                   converted.  Lane (q = c, g) receives S^T[keys 4 g ... 4 g + 3][q].
+//   softmax       : one exponent offset per row, which may lag the running maximum by 2^LF_CACHED_LAZY.
+//   O^T += V^T P^T: a lane holds 4 keys' D / 16 neighbouring elements; two conversions and two byte permutations make the two lanes' worth of
+//                   operand of two elements out of them, and the product number i has the elements D / 16 * row + i, so that a lane ends up with
+//                   D / 4 neighbouring elements of O.
+// No LDS and no barrier in the loop.  Four waves share a chunk's keys and merge through LDS, or (LF_CACHED_ROWWAVES) have a chunk's rows one each.
+#ifndef LF_CACHED_CB
+#define LF_CACHED_CB 1
+#endif
+#ifndef LF_CACHED_ROWWAVES
+#define LF_CACHED_ROWWAVES 0
+#endif
+#define LF_CACHED_LAZY 8
+#define LF_CACHED_ROWS (16 * LF_CACHED_CB * (LF_CACHED_ROWWAVES ? 4 : 1))     /* of a workgroup */
+#define LF_CACHED_D LF_HEAD_DIM
+#define LF_CACHED_NV (LF_HEAD_DIM / 16)    /* products of O^T */
+#define LF_CACHED_QN (LF_DTYPE == 0 ? 2 : 3)
+#define LF_CACHED_OSTRIDE (LF_HEAD_DIM + 4)
+
+typedef int lf_i32x8 __attribute__((ext_vector_type(8)));
+
+struct LfCachedParams {
+  const lf_elem* q;            // [T, Hq, D], strides below
+  lf_elem* o;
+  const unsigned char* k;      // codes and scales of the pools
+  const unsigned char* v;
+  const unsigned char* k_scales;
+  const unsigned char* v_scales;
+  const void* table;           // [B, ...], rows table_stride apart
+  const int* lengths;          // [B]
+  const int* offsets;          // [B + 1]; none: a row each
+  const int* positions;        // [T]; none: the last key's
+  float* part_acc;             // [items, Hkv, LF_CACHED_ROWS, D]
+  float* part_ml;              // [items, Hkv, LF_CACHED_ROWS, 2]
+  long long q_ss, q_sh, o_ss, o_sh;
+  long long k_sb, v_sb, ks_sb, vs_sb, table_stride;    // bytes of a page; entries
+  int T, B, Hkv, group;
+  int room;                    // keys that a row of the table has room for
+  int shift;                   // log2 of the tokens per page
+  int window;
+  int items;                   // (chunk, piece) pairs that there are workgroups for, one more than there can be
+  int target_log2, least;      // workgroups that the keys are cut for; least length of a piece, a multiple of 32
+  int clear;                   // 1: zeros into rows of no request
+  float scale, softcap;
+};
+
+// What a lane knows of its request.
+struct LfCachedRequest {
+  int first, n;                // its rows
+  int start, end;              // its keys: the first that any row can see, a multiple of 32
+  int chunks;
+};
+__device__ __forceinline__ LfCachedRequest lf_cached_request(const LfCachedParams& p, int b) {
+  LfCachedRequest r = {0, 0, 0, 0, 0};
+  if (b >= p.B) return r;
+  r.first = p.offsets ? min(max(p.offsets[b], 0), p.T) : b;
+  r.n = p.offsets ? max(min(p.offsets[b + 1], p.T) - r.first, 0) : 1;
+  r.end = min(max(p.lengths[b], 0), p.room);
+#if LF_MASK == 2
+  if (r.n > 0) r.start = max((p.positions ? p.positions[r.first] : r.end - 1) - p.window + 1, 0) & ~31;
+  r.start = min(r.start, r.end & ~31);
+#endif
+  r.chunks = (int)(((long long)r.n * p.group + LF_CACHED_ROWS - 1) / LF_CACHED_ROWS);
+  return r;
+}
+__device__ __forceinline__ float lf_cached_sum(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
+  return x;
+}
+// Length of a piece.  `mine`: the first 64 requests, one per lane.  (Whole pairs of tiles; the sum's rounding is below the 2^-10 that are added.)
+__device__ __forceinline__ int lf_cached_split(const LfCachedParams& p, const LfCachedRequest& mine) {
+  float sum = 0.0f;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const LfCachedRequest r = b0 ? lf_cached_request(p, b0 + __lane_id()) : mine;
+    sum += (float)(r.end - r.start) * (float)r.chunks;
+  }
+  const float even = lf_cached_sum(sum) * (float)p.Hkv * (1.0f + 0x1p-10f) * __builtin_bit_cast(float, (127 - p.target_log2) << 23);
+  const int split = even < 0x1p30f ? ((int)even + 32) & ~31 : 1 << 30;
+  return __builtin_amdgcn_readfirstlane(max(p.least, split));
+}
+__device__ __forceinline__ int lf_cached_pieces(const LfCachedRequest& r, int split) { return max((r.end - r.start + split - 1) / split, 1); }
+
+struct LfCachedUnit {
+  int b, chunk, piece, pieces;
+  LfCachedRequest r;
+  int before;                  // (chunk, piece) pairs of the requests before
+};
+// The request that `item` is of, or of whose rows `row` is one where `item` is below 0; false: of none (`before` = all pairs then).
+__device__ __forceinline__ bool lf_cached_find(const LfCachedParams& p, const LfCachedRequest& mine, int split, int item, int row, LfCachedUnit& u) {
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const LfCachedRequest r = b0 ? lf_cached_request(p, b0 + __lane_id()) : mine;
+    const int count = r.chunks * lf_cached_pieces(r, split), upto = lf_wave_scan(count);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(item >= 0 ? before + upto > item : r.n > 0 && row >= r.first && row < r.first + r.n);
+    if (hit != 0ull) {
+      const int l = (int)__builtin_ctzll(hit);
+      u.b = b0 + l;
+      u.r.first = __builtin_amdgcn_readlane(r.first, l);
+      u.r.n = __builtin_amdgcn_readlane(r.n, l);
+      u.r.start = __builtin_amdgcn_readlane(r.start, l);
+      u.r.end = __builtin_amdgcn_readlane(r.end, l);
+      u.r.chunks = __builtin_amdgcn_readlane(r.chunks, l);
+      u.pieces = lf_cached_pieces(u.r, split);
+      u.before = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l);
+      if (item >= 0) {
+        const int within = item - u.before;
+        u.chunk = u.r.chunks - 1 - within / u.pieces;      // (under a causal mask the last rows have the most keys: first)
+        u.piece = within - within / u.pieces * u.pieces;
+      }
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  u.before = before;
+  return false;
+}
+
+// 32 keys of a head as loaded
+struct LfCachedStage {
+  lf_u32x4 k[2];
+  unsigned v[2][LF_HEAD_DIM / 32];     // D 64: 4 keys of 2 bytes, 128: of 4
+  unsigned ks[2], vs[2];
+};
+
+extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedParams p) {
+  constexpr int D = LF_CACHED_D, CB = LF_CACHED_CB;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int item = blockIdx.x / p.Hkv, h = blockIdx.x - item * p.Hkv;
+  const LfCachedRequest mine = lf_cached_request(p, lane);
+  const int split = lf_cached_split(p, mine);
+  LfCachedUnit u;
+  if (!lf_cached_find(p, mine, split, item, 0, u)) {
+    // rows of no request, shared by the workgroups without a pair
+    if (!p.clear || !p.offsets) return;
+    const int lo = min(max(p.offsets[0], 0), p.T), hi = max(min(max(p.offsets[p.B], 0), p.T), lo);
+    const int Hq = p.Hkv * p.group, pieces = Hq * (D / 8);
+    const long long all = (long long)(lo + p.T - hi) * pieces;
+    for (long long i = (long long)((item - u.before) * p.Hkv + h) * 256 + tid; i < all; i += (long long)(p.items - u.before) * p.Hkv * 256) {
+      const long long row = i / pieces;
+      const int at = (int)(i - row * pieces), head = at / (D / 8);
+      *reinterpret_cast<lf_u32x4*>(p.o + (row < lo ? row : row - lo + hi) * p.o_ss + head * p.o_sh + 8 * (at - head * (D / 8))) = lf_u32x4{0u, 0u, 0u, 0u};
+    }
+    return;
+  }
+  const int rows = u.r.n * p.group;      // of a kv head
+  const int row0 = u.chunk * LF_CACHED_ROWS + (LF_CACHED_ROWWAVES ? wave * 16 * CB : 0);
+  const int piece_begin = u.r.start + u.piece * split, piece_end = min(piece_begin + split, u.r.end);
+
+  // ---- rows of this lane, one per column block: their bounds and Q^T in 8-bit parts
+  lf_i32x8 qp[CB][LF_CACHED_QN];
+  int qscale[CB];                        // exponent of the first part, as the product takes it
+  int lo[CB], hi[CB];
+  int least_hi = 0x7fffffff, most_hi = 0, least_lo = 0x7fffffff, most_lo = 0;
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    const int row = row0 + 16 * cb + c;
+    const bool real = row < rows;
+    const int t = u.r.first + (real ? row / p.group : 0), head = h * p.group + (real ? row % p.group : 0);
+    const int pos = p.positions ? p.positions[t] : u.r.end - 1;
+    lo[cb] = 0;
+    hi[cb] = 0;
+    if (real && pos >= 0) {
+#if LF_MASK == 0
+      hi[cb] = u.r.end;
+#else
+      hi[cb] = min(pos, u.r.end - 1) + 1;
+#endif
+#if LF_MASK == 2
+      lo[cb] = max(pos - p.window + 1, 0);
+#endif
+      least_hi = min(least_hi, hi[cb]);
+      most_hi = max(most_hi, hi[cb]);
+      least_lo = min(least_lo, lo[cb]);
+      most_lo = max(most_lo, lo[cb]);
+    }
+    // bytes 0 ... 15 of a lane are k = 16 g ..., bytes 16 ... 31 k = 64 + 16 g ... (D 64: zeros)
+    const lf_elem* qrow = p.q + (long long)t * p.q_ss + head * p.q_sh;
+    float x[32];
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lf_elem8 raw = {};
+      if (D == 128 || i < 2) raw = *reinterpret_cast<const lf_elem8*>(qrow + 16 * g + (i < 2 ? 8 * i : 48 + 8 * i));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[8 * i + e] = real ? lf_to_float(raw[e]) : 0.0f;
+        top = max(top, __builtin_bit_cast(unsigned, x[8 * i + e]) & 0x7fffffffu);
+      }
+    }
+    top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
+    top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+    // the largest in [128, 256); an infinity or NaN makes all of the row's scores NaN
+    const int up = top >= 0x7f800000u ? 255 : max((int)(top >> 23) - 7, 20);
+    qscale[cb] = up;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = up == 255 ? 0.0f : __builtin_amdgcn_ldexpf(x[i], 127 - up);
+#pragma unroll
+    for (int n = 0; n < LF_CACHED_QN; ++n)
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        int packed = 0;
+        packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w], x[4 * w + 1], packed, false);
+        packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2], x[4 * w + 3], packed, true);
+        qp[cb][n][w] = packed;
+        const lf_f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(packed, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(packed, true);
+        // what is left of it, 2^5 times
+        x[4 * w] = (x[4 * w] - a[0]) * 32.0f;
+        x[4 * w + 1] = (x[4 * w + 1] - a[1]) * 32.0f;
+        x[4 * w + 2] = (x[4 * w + 2] - b[0]) * 32.0f;
+        x[4 * w + 3] = (x[4 * w + 3] - b[1]) * 32.0f;
+      }
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    least_hi = min(least_hi, __shfl_xor(least_hi, d, 64));
+    most_hi = max(most_hi, __shfl_xor(most_hi, d, 64));
+    least_lo = min(least_lo, __shfl_xor(least_lo, d, 64));
+    most_lo = max(most_lo, __shfl_xor(most_lo, d, 64));
+  }
+  least_hi = __builtin_amdgcn_readfirstlane(least_hi);
+  most_lo = __builtin_amdgcn_readfirstlane(most_lo);
+  const int begin = max(piece_begin, __builtin_amdgcn_readfirstlane(least_lo) & ~31), end = min(piece_end, __builtin_amdgcn_readfirstlane(most_hi));
+  const int pairs = end > begin ? (end - begin + 31) >> 5 : 0;
+
+#if LF_SOFTCAP
+  const float sc_in = p.scale / p.softcap;
+  const float cexp = LF_LOG2E;
+#else
+  const float cexp = p.scale * LF_LOG2E;
+#endif
+  lf_f32x4 o[CB][LF_CACHED_NV];
+  float mc[CB], l_part[CB];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    mc[cb] = LF_NEG_INF;
+    l_part[cb] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] = lf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // ---- loads
+  const int last_tile = (u.r.end - 1) & ~15;
+  const long long head_tiles = (long long)h << (p.shift - 4);
+  const int in_page = (1 << p.shift) - 1;
+#if LF_TABLE_I64
+  const lf_cu64* ids = reinterpret_cast<const lf_cu64*>(reinterpret_cast<unsigned long long>(p.table)) + (long long)u.b * p.table_stride;
+#else
+  const lf_cint* ids = reinterpret_cast<const lf_cint*>(reinterpret_cast<unsigned long long>(p.table)) + (long long)u.b * p.table_stride;
+#endif
+  struct Ids {
+    long long a, b;
+  };
+  auto tile_of = [&](int pair, int which) { return min(begin + 32 * min(pair, pairs - 1) + 16 * which, last_tile); };
+  auto fetch = [&](int pair) -> Ids { return {(long long)ids[tile_of(pair, 0) >> p.shift], (long long)ids[tile_of(pair, 1) >> p.shift]}; };
+  auto issue = [&](LfCachedStage& s, int pair, const Ids& id) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const long long page = w ? id.b : id.a, tile = head_tiles + ((tile_of(pair, w) & in_page) >> 4);
+      const unsigned char* kt = p.k + page * p.k_sb + tile * (8 * D);
+      const unsigned char* vt = p.v + page * p.v_sb + tile * (8 * D);
+      const unsigned char* kst = p.k_scales + page * p.ks_sb + tile * (D / 2);
+      const unsigned char* vst = p.v_scales + page * p.vs_sb + tile * (D / 2);
+      // (D 64: lanes of g 2 and 3, whose part of Q^T is zeros, read what those of 0 and 1 do)
+      s.k[w] = *reinterpret_cast<const lf_u32x4*>(kt + c * (D / 2) + 16 * (g % (D / 32)));
+      s.ks[w] = kst[c * (D / 32) + g % (D / 32)];
+      if (D == 128) {
+        const lf_u32x4 x = *reinterpret_cast<const lf_u32x4*>(vt + 16 * lane);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) s.v[w][i] = x[i];
+      } else {
+        const lf_u32x2 x = *reinterpret_cast<const lf_u32x2*>(vt + 8 * lane);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) s.v[w][i] = x[i];
+      }
+      s.vs[w] = *reinterpret_cast<const unsigned*>(vst + (g * (D / 32) + c / (512 / D)) * 4);
+    }
+  };
+
+  // ---- 32 keys
+  auto consume = [&](LfCachedStage& s, int pair) {
+    const int t0 = begin + 32 * pair;
+    const bool partly = t0 < most_lo || t0 + 32 > least_hi;      // some row does not see all of them
+    if (t0 + 32 > u.r.end) {
+      // what lies behind the last key may be anything: nothing, with weights of zero
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (t0 + 16 * w + 4 * g + e >= u.r.end) s.vs[w] &= ~(0xffu << (8 * e));
+    }
+    lf_elem8 va[LF_CACHED_NV];           // V^T: lane (row c, g) has keys 4 g ... of either tile, element D / 16 * c + i
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float by[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) by[e] = __builtin_bit_cast(float, ((s.vs[w] >> (8 * e)) & 0xffu) << 23);
+#pragma unroll
+      for (int m = 0; m < LF_CACHED_NV / 2; ++m) {
+        // byte m of each key: elements 2 m and 2 m + 1
+        lf_pool4_two y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned word = D == 128 ? s.v[w][e % (D / 32)] : s.v[w][e / 2];
+          switch (D == 128 ? m : 2 * (e % 2) + m) {
+            case 0: y[e] = lf_pool4_pair<0>(word, by[e]); break;
+            case 1: y[e] = lf_pool4_pair<1>(word, by[e]); break;
+            case 2: y[e] = lf_pool4_pair<2>(word, by[e]); break;
+            default: y[e] = lf_pool4_pair<3>(word, by[e]);
+          }
+          va[2 * m][4 * w + e] = y[e][0];
+          va[2 * m + 1][4 * w + e] = y[e][1];
+        }
+      }
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      float x[8], mx = LF_NEG_INF;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const lf_i32x8 a = {(int)s.k[w][0], (int)s.k[w][1], (int)s.k[w][2], (int)s.k[w][3], 0, 0, 0, 0};
+        lf_f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int n = LF_CACHED_QN - 1; n >= 0; --n)
+          r = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qp[cb][n], r, 4, 0, 0, (int)s.ks[w], 0, qscale[cb] == 255 ? 255 : qscale[cb] - 5 * n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float y = r[e];
+#if LF_SOFTCAP
+          y = p.softcap * lf_tanh(y * sc_in);
+#endif
+          x[4 * w + e] = y * cexp;
+        }
+      }
+      if (partly) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = t0 + 16 * (i / 4) + 4 * g + i % 4;
+          if (j < lo[cb] || j >= hi[cb]) x[i] = LF_NEG_INF;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
+      if (__builtin_amdgcn_ballot_w64(mx > mc[cb] + (float)LF_CACHED_LAZY) != 0ull) {
+        float mq = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mq = fmaxf(mq, __shfl_xor(mq, 32, 64));
+        const float m_new = fmaxf(mc[cb], mq);
+        const float r = (m_new == LF_NEG_INF) ? 1.0f : lf_exp2(mc[cb] - m_new);
+        mc[cb] = m_new;
+        l_part[cb] *= r;
+#pragma unroll
+        for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] *= r;
+      }
+      const float m_sub = (mc[cb] == LF_NEG_INF) ? 0.0f : mc[cb];
+      lf_elem8 pb;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = lf_exp2(x[i] - m_sub);
+        l_part[cb] += e;
+        pb[i] = lf_from_float(e);
+      }
+#pragma unroll
+      for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] = lf_mfma16(va[i], pb, o[cb][i]);
+    }
+  };
+
+  // ---- this wave's pairs: three stages rotate; loads past the end repeat the last pair, so that the loop has no condition on them
+  {
+    constexpr int kStep = LF_CACHED_ROWWAVES ? 1 : 4;
+    const int first = LF_CACHED_ROWWAVES ? 0 : wave;
+    if (first < pairs) {
+      LfCachedStage s0, s1, s2;
+      Ids i0 = fetch(first), i1 = fetch(first + kStep), i2 = fetch(first + 2 * kStep);
+      issue(s0, first, i0);
+      issue(s1, first + kStep, i1);
+      issue(s2, first + 2 * kStep, i2);
+      i0 = fetch(first + 3 * kStep);
+      i1 = fetch(first + 4 * kStep);
+      i2 = fetch(first + 5 * kStep);
+      for (int pr = first; pr < pairs; pr += 3 * kStep) {
+        consume(s0, pr);
+        issue(s0, pr + 3 * kStep, i0);
+        i0 = fetch(pr + 6 * kStep);
+        if (pr + kStep >= pairs) break;
+        consume(s1, pr + kStep);
+        issue(s1, pr + 4 * kStep, i1);
+        i1 = fetch(pr + 7 * kStep);
+        if (pr + 2 * kStep >= pairs) break;
+        consume(s2, pr + 2 * kStep);
+        issue(s2, pr + 5 * kStep, i2);
+        i2 = fetch(pr + 8 * kStep);
+      }
+    }
+  }
+
+  // ---- results: lane (q = c, g) has elements D / 4 * g ... of its row, 4 groups of D / 16
+  float l_wave[CB];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    l_wave[cb] = l_part[cb] + __shfl_xor(l_part[cb], 16, 64);
+    l_wave[cb] += __shfl_xor(l_wave[cb], 32, 64);
+  }
+  const bool whole = u.pieces == 1;
+  const long long slot0 = ((long long)item * p.Hkv + h) * LF_CACHED_ROWS;
+  auto inverse = [](float l) { return l == 0.0f ? 0.0f : 1.0f / l; };      // a row without a key: zeros; NaN stays
+  auto out_row = [&](int row) { return p.o + (long long)(u.r.first + row / p.group) * p.o_ss + (h * p.group + row % p.group) * p.o_sh; };
+#if LF_CACHED_ROWWAVES
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    const int row = row0 + 16 * cb + c;
+    if (row >= rows) continue;
+    if (whole) {
+      lf_elem* to = out_row(row) + D / 4 * g;
+      const float inv = inverse(l_wave[cb]);
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n) {
+        lf_elem8 y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = lf_from_float(o[cb][(8 * n + i) % LF_CACHED_NV][(8 * n + i) / LF_CACHED_NV] * inv);
+        *reinterpret_cast<lf_elem8*>(to + 8 * n) = y;
+      }
+    } else {
+      const long long slot = slot0 + (row - u.chunk * LF_CACHED_ROWS);
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        lf_f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = o[cb][(4 * n + i) % LF_CACHED_NV][(4 * n + i) / LF_CACHED_NV];
+        *reinterpret_cast<lf_f32x4*>(&p.part_acc[slot * D + D / 4 * g + 4 * n]) = y;
+      }
+      if (g == 0) {
+        p.part_ml[slot * 2] = mc[cb];
+        p.part_ml[slot * 2 + 1] = l_wave[cb];
+      }
+    }
+  }
+#else
+  __shared__ float red_o[4 * 16 * LF_CACHED_OSTRIDE];
+  __shared__ float red_m[4][16], red_l[4][16];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    if (cb) __syncthreads();
+    if (g == 0) {
+      red_m[wave][c] = mc[cb];
+      red_l[wave][c] = l_wave[cb];
+    }
+    __syncthreads();
+    {
+      const float m_all = fmaxf(fmaxf(red_m[0][c], red_m[1][c]), fmaxf(red_m[2][c], red_m[3][c]));
+      const float f = lf_exp2(mc[cb] - (m_all == LF_NEG_INF ? 0.0f : m_all));
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        lf_f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = o[cb][(4 * n + i) % LF_CACHED_NV][(4 * n + i) / LF_CACHED_NV] * f;
+        *reinterpret_cast<lf_f32x4*>(&red_o[(wave * 16 + c) * LF_CACHED_OSTRIDE + D / 4 * g + 4 * n]) = y;
+      }
+    }
+    __syncthreads();
+    // thread -> (row, 8 elements)
+    for (int at = tid; at < 16 * D / 8; at += 256) {
+      const int r = at / (D / 8), d0 = at % (D / 8) * 8, row = row0 + 16 * cb + r;
+      if (row >= rows) continue;
+      const float m_all = fmaxf(fmaxf(red_m[0][r], red_m[1][r]), fmaxf(red_m[2][r], red_m[3][r])), m_sub = m_all == LF_NEG_INF ? 0.0f : m_all;
+      float l = 0.0f, sum[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        l += red_l[w][r] * lf_exp2(red_m[w][r] - m_sub);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += red_o[(w * 16 + r) * LF_CACHED_OSTRIDE + d0 + i];
+      }
+      if (whole) {
+        const float inv = inverse(l);
+        lf_elem8 y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = lf_from_float(sum[i] * inv);
+        *reinterpret_cast<lf_elem8*>(out_row(row) + d0) = y;
+      } else {
+        const long long slot = slot0 + 16 * cb + r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<lf_f32x4*>(&p.part_acc[slot * D + d0 + 4 * i]) = lf_f32x4{sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]};
+        if (d0 == 0) {
+          p.part_ml[slot * 2] = m_all;
+          p.part_ml[slot * 2 + 1] = l;
+        }
+      }
+    }
+  }
+#endif
+}
+
+// Joins a row's pieces.  D / 4 threads have a row, 4 elements each; a block of 256 has 1024 / D heads of one token, or, in grids of a block per
+// (token, head), one row whose pieces its groups of threads share and merge through LDS.
+extern "C" __global__ void __launch_bounds__(256) lf_cached_combine(const LfCachedParams p) {
+  constexpr int kTPR = LF_HEAD_DIM / 4, kRPB = 256 / kTPR;
+  const int Hq = p.Hkv * p.group;
+  const bool row_per_block = (long long)gridDim.x == (long long)p.T * Hq;
+  const int part = threadIdx.x / kTPR, per = row_per_block ? Hq : (Hq + kRPB - 1) / kRPB;
+  const int t = blockIdx.x / per, head = row_per_block ? blockIdx.x - t * per : (blockIdx.x - t * per) * kRPB + part;
+  const int d0 = 4 * (threadIdx.x % kTPR);
+  const LfCachedRequest mine = lf_cached_request(p, __lane_id());
+  const int split = lf_cached_split(p, mine);
+  LfCachedUnit u;
+  if (!lf_cached_find(p, mine, split, -1, t, u) || u.pieces == 1) return;       // (written already)
+  if (head >= Hq) return;
+  const int h = head / p.group, row = (t - u.r.first) * p.group + head - h * p.group, chunk = row / LF_CACHED_ROWS;
+  const long long first = u.before + (long long)(u.r.chunks - 1 - chunk) * u.pieces;
+  float m = LF_NEG_INF, l = 0.0f;
+  lf_f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto join = [&](float m2, float l2, const lf_f32x4& a2) {
+    if (l2 == 0.0f) return;
+    const float mj = fmaxf(m, m2), ms = mj == LF_NEG_INF ? 0.0f : mj, r = lf_exp2(m - ms), f = lf_exp2(m2 - ms);
+    l = l * r + l2 * f;
+    a = a * r + a2 * f;
+    m = mj;
+  };
+  for (int z0 = row_per_block ? 4 * part : 0; z0 < u.pieces; z0 += row_per_block ? 4 * kRPB : 4) {
+    lf_f32x2 ml[4];
+    lf_f32x4 ac[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long slot = ((first + min(z0 + i, u.pieces - 1)) * p.Hkv + h) * LF_CACHED_ROWS + row - chunk * LF_CACHED_ROWS;
+      ml[i] = *reinterpret_cast<const lf_f32x2*>(&p.part_ml[slot * 2]);
+      ac[i] = *reinterpret_cast<const lf_f32x4*>(&p.part_acc[slot * LF_HEAD_DIM + d0]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (z0 + i < u.pieces) join(ml[i][0], ml[i][1], ac[i]);
+  }
+  if (row_per_block) {
+    __shared__ lf_f32x4 acc[kRPB][kTPR];
+    __shared__ lf_f32x2 ml[kRPB];
+    acc[part][d0 / 4] = a;
+    if (d0 == 0) ml[part] = lf_f32x2{m, l};
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int i = 1; i < kRPB; ++i) join(ml[i][0], ml[i][1], acc[i][d0 / 4]);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  lf_elem4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = lf_from_float(a[i] * inv);
+  *reinterpret_cast<lf_elem4*>(p.o + (long long)t * p.o_ss + head * p.o_sh + d0) = y;
+}

@@ -225,6 +225,17 @@ __device__ __forceinline__ void lf_wave_exchange() {
 // name: hipRTC's compiler knows no builtin for it yet.
 extern "C" __device__ bool lf_lane_bit(unsigned long long word) __asm("llvm.amdgcn.inverse.ballot.i64");
 
+// sum of x over lanes 0 ... this one: within rows of 16 lanes, then across them
+__device__ __forceinline__ int lf_wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);      // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 __device__ __forceinline__ float lf_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1); exact limits at +-inf.

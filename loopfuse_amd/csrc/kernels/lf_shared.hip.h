@@ -31,16 +31,6 @@ struct LfSharedParams : LfAttnParams {       // q_sb, q_sh, q_ss: request, kv he
 __device__ __forceinline__ int lf_shared_length(const LfSharedParams& p, int b) {
   return b < p.B ? min(max(p.lengths[b], 0), p.room) : 0;
 }
-// sum of x over lanes 0 ... this one: within rows of 16 lanes, then across them
-__device__ __forceinline__ int lf_wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);      // row_shr:1, 2, 4, 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // row_bcast:31 into rows 2 and 3
-  return x;
-}
 // length of a piece: whole pairs of 16-key steps.  `mine` = lengths of the first 64 requests, one per lane (read once for all scans)
 __device__ __forceinline__ int lf_shared_split(const LfSharedParams& p, int mine) {
   const int lane = __lane_id();

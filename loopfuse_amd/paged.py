@@ -65,6 +65,15 @@ class _ReadParams(ctypes.Structure):
                 + [(n, ctypes.c_int) for n in ("T", "heads", "per_head", "shift")])
 
 
+class CachedParams(ctypes.Structure):
+    """Mirror of ``struct LfCachedParams`` in csrc/kernels/lf_cached.hip."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "o", "k", "v", "k_scales", "v_scales", "table", "lengths", "offsets", "positions", "part_acc", "part_ml")]
+                + [(n, ctypes.c_longlong) for n in ("q_ss", "q_sh", "o_ss", "o_sh", "k_sb", "v_sb", "ks_sb", "vs_sb", "table_stride")]
+                + [(n, ctypes.c_int) for n in ("T", "B", "Hkv", "group", "room", "shift", "window", "items", "target_log2", "least", "clear")]
+                + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)])
+
+
 @dataclasses.dataclass(frozen=True, eq=False)
 class Pool4:
     """A page pool of keys or values held in 4 bits (``pool4``)."""
@@ -679,6 +688,154 @@ def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_ta
         scratch = lowering._get_scratch(q.device, floats)
         at = scratch.data_ptr()
         P.part_acc, P.part_ml, P.pre_acc, P.pre_ml = at, at + ml, at + pre_acc, at + pre_ml
+        repeat.launches.launch(P)
+    lowering._last_launch.set(repeat.record)
+    return out
+
+
+def cached_build(rows: float) -> tuple:
+    """(blocks of 16 rows of a wave, do a workgroup's waves have rows of their own) for so many rows of a kv head per request: up to 16, and up to 32, the four waves
+    share the keys."""
+    return (1, False) if rows <= 16 else (2, False) if rows <= 32 else (2, True)
+
+
+def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64: bool, blocks: int, rowwaves: bool) -> lowering.KernelSpec:
+    return lowering._spec("cached", lowering._DTYPE_CODE[dtype], D, mask, softcap, table_i64=table_i64,
+                          extra=(f"-DLF_CACHED_CB={blocks}",) + (("-DLF_CACHED_ROWWAVES=1",) if rowwaves else ()))
+
+
+def cached_split(room: int, chunks: int, Hkv: int) -> tuple:
+    """(log2 of the workgroups that the keys are cut for, least length of a piece).  ``chunks`` = of rows, at most."""
+    if room <= 128 or chunks * Hkv >= 2048:
+        return 0, 1 << 30
+    return 10, 128
+
+
+@lowering.outside_graphs
+def attention_cached(q: torch.Tensor, k_pool: Pool4, v_pool: Pool4, plan: AttnPlan, table: torch.Tensor, lengths: torch.Tensor,
+                     offsets: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens of requests of different lengths, one each or several, over their keys and values in page pools held in 4 bits.
+
+    q : [rows, Hq, D], bf16 / fp16, Hq a multiple of the pools' heads, D 64 or 128 (views will do).  table : [B, width], int32 or int64, each request's pages, of which it
+    has ``lengths[b]`` keys (int32 [B], on the GPU; what a row of the table has no room for is left out), those of its new tokens among them; entries behind the last
+    page are not read.  ``offsets``: int32 [B + 1], request b's new tokens are rows offsets[b] ... offsets[b + 1]; ``positions``: int32 [rows], of each in its request, not
+    descending within it; below 0: a row of no token.  Both as ``extend_tables`` leaves them (``PagedStep``); without offsets row b is request b's, without
+    positions (for one row per request at most) its last key's.  ``plan``: scale and softcap, and the mask: causal (a token sees the keys up to its own position), sliding, or
+    none (all keys of its request).
+
+    Returns O [rows, Hq, D], of which no gradients are recorded.  Rows of no token, and those without a key, are zeros; rows of no request are zeros too, or stay as they
+    are in an ``out`` that is given.  A prompt's next part, behind what the cache has of it, is such a call; a prompt of which the cache has nothing attends over
+    its own unrounded keys by ``packed.attention_packed``.  Page ids are trusted, as those of ``lowering.attention`` are (``LOOPFUSE_CHECK_TABLES=1`` looks at them)."""
+    return _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out)
+
+
+@lowering._on_device_of_first_argument
+def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
+    given = (table, lengths, offsets, positions)
+    lowering._no_tangents(q)
+    dtype = q.dtype
+    if dtype not in lowering._DTYPE_CODE:
+        raise UnsupportedPlan(f"dtype {dtype} not supported by the MFMA kernels (bf16/fp16 only)")
+    if q.dim() != 3 or q.shape[2] not in (64, 128):
+        raise UnsupportedPlan("Q must be [rows, Hq, D] with head dim 64 or 128")
+    lowering._check_tensor("Q", q, dtype)
+    T, Hq, D = q.shape
+    pages, page, Hkv, Dk = _two_pools4(k_pool, v_pool, dtype, q.device)
+    if Dk != D or Hq < 1 or Hq % Hkv:
+        raise UnsupportedPlan("the pools must have Q's head dim, Hq a multiple of their heads")
+    if plan.mask not in lowering._MASK_NAMES or plan.denom_add != 0.0:
+        raise UnsupportedPlan("attention over a cache in 4 bits takes no mask, a causal or a sliding one, and the plain softmax denominator")
+    mask = lowering._MASK_NAMES[plan.mask]
+    if mask == lowering.MASK_SLIDING and plan.window < 1:
+        raise UnsupportedPlan("sliding mask needs window >= 1")
+    if not (plan.scale > 0.0) or not math.isfinite(plan.scale):
+        raise UnsupportedPlan("score scale must be positive and finite")
+    softcap = None
+    if plan.softcap is not None:
+        softcap = abs(float(plan.softcap))
+        if not (softcap > 0.0) or not math.isfinite(softcap):
+            raise UnsupportedPlan("softcap must be finite and non-zero")
+    _on_gpu("table", table, _TABLE_DTYPES, 2, q.device)
+    _on_gpu("lengths", lengths, (torch.int32,), 1, q.device)
+    B = table.shape[0]
+    if lengths.shape[0] != B:
+        raise UnsupportedPlan(f"table and lengths must be of as many requests, not {B} and {lengths.shape[0]}")
+    if offsets is not None:
+        _on_gpu("offsets", offsets, (torch.int32,), 1, q.device)
+        if offsets.shape[0] != B + 1:
+            raise UnsupportedPlan(f"offsets must be int32 [{B + 1}]")
+    elif T != B:
+        raise UnsupportedPlan(f"without offsets there is a row for each of the {B} requests, not {T}")
+    if positions is not None:
+        _on_gpu("positions", positions, (torch.int32,), 1, q.device)
+        if positions.shape[0] != T:
+            raise UnsupportedPlan(f"positions must be int32 [{T}]")
+    elif offsets is not None and T > B:
+        raise UnsupportedPlan("requests with several rows need positions")
+    room = table.shape[1] * page
+    if room > 1 << 30:
+        raise UnsupportedPlan("a request has room for more than 2**30 keys")
+    if out is not None:
+        lowering._check_tensor("O", out, dtype)
+        if tuple(out.shape) != (T, Hq, D) or out.device != q.device or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+            raise UnsupportedPlan(f"O must be [{T}, {Hq}, {D}] on the device of Q, every element with a place of its own")
+    if T == 0 or B == 0:
+        return torch.zeros(q.shape, dtype=dtype, device=q.device) if out is None else out
+    if lowering._checks_tables():
+        used = torch.arange(table.shape[1], device=q.device) < ((lengths.clamp(min=0).long() + page - 1) // page)[:, None]
+        ids = table[used]
+        if len(ids) and (int(ids.min()) < 0 or int(ids.max()) >= pages) or int(lengths.max()) > room:
+            raise ValueError(f"loopfuse_amd: page ids outside 0 ... {pages - 1}, or a length beyond its row of the table")
+        if offsets is not None and (bool((offsets[1:] < offsets[:-1]).any()) or int(offsets[0]) < 0 or int(offsets[-1]) > T):
+            raise ValueError(f"loopfuse_amd: offsets must not descend, within 0 ... {T}")
+    table = table if table.shape[1] == 0 or table.stride(1) == 1 else table.contiguous()
+    lengths, offsets, positions = (t if t is None else t.contiguous() for t in (lengths, offsets, positions))
+    P = CachedParams()
+    P.q_ss, P.q_sh = q.stride()[:2]
+    P.o_ss, P.o_sh = (Hq * D, D) if out is None else out.stride()[:2]
+    P.k_sb, P.v_sb, P.ks_sb, P.vs_sb = k_pool.codes.stride(0), v_pool.codes.stride(0), k_pool.scales.stride(0), v_pool.scales.stride(0)
+    P.table_stride, P.T, P.B, P.Hkv, P.group = table.stride(0), T, B, Hkv, Hq // Hkv
+    P.room, P.shift, P.clear = room, _shift(page), int(out is None)
+    P.window = min(int(plan.window), 1 << 30) if mask == lowering.MASK_SLIDING else 0
+    P.scale, P.softcap = plan.scale, softcap or 0.0
+    blocks, rowwaves = cached_build(T * P.group / B)
+    rows = 16 * blocks * (4 if rowwaves else 1)
+    chunks = T * P.group // rows + min(T, B)
+    P.target_log2, P.least = cached_split(room, chunks, Hkv)
+    # (at most so many pairs of a chunk and a piece; one place more, for rows of no request, and one for the sums' rounding)
+    split = P.least < room
+    P.items = chunks + 2 + ((1 << P.target_log2) // Hkv if split else 0)
+    if P.items * Hkv * 256 >= 1 << 32 or T * P.group >= 1 << 30:
+        raise UnsupportedPlan(f"a launch for {T} rows of {Hq} heads is too large")
+    spec = cached_spec(dtype, D, mask, softcap is not None, table.dtype == torch.int64, blocks, rowwaves)
+    steps = [(lowering.get_kernel(spec, "lf_cached"), (P.items * Hkv, 1, 1), 256)]
+    if split:
+        per = 1024 // D
+        grid = T * Hq if T * Hq <= 1024 else T * -(-Hq // per)
+        if grid * 256 >= 1 << 32:
+            raise UnsupportedPlan(f"a launch for {T} rows of {Hq} heads is too large")
+        steps.append((lowering.get_kernel(spec, "lf_cached_combine"), (grid, 1, 1), 256))
+    slots = P.items * Hkv * rows if split else 0
+    repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps]}, (slots * (D + 2), 4 * slots * D))
+    return _cached_again(q, k_pool, v_pool, table, lengths, offsets, positions, out, repeat)
+
+
+def _cached_again(q, k_pool, v_pool, table, lengths, offsets, positions, out, repeat):
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    P = CachedParams.from_buffer_copy(repeat.block)
+    P.q, P.o, P.table, P.lengths = q.data_ptr(), out.data_ptr(), table.data_ptr(), lengths.data_ptr()
+    for name, t in (("offsets", offsets), ("positions", positions)):
+        if t is not None:
+            setattr(P, name, t.data_ptr())
+    _set_pools(P, "k", "v", k_pool, v_pool)
+    floats, ml = repeat.more
+    if floats:
+        with lowering._scratch_lock:        # no other thread's step on this stream between the launches
+            at = lowering._get_scratch(q.device, floats).data_ptr()
+            P.part_acc, P.part_ml = at, at + ml
+            repeat.launches.launch(P)
+    else:
         repeat.launches.launch(P)
     lowering._last_launch.set(repeat.record)
     return out
