@@ -97,6 +97,92 @@ typedef struct LfStoreParamsHost {
   int32_t shift;           /* log2 of the tokens per page */
 } LfStoreParamsHost;
 
+/* lf_rotate: 256 / slots items per workgroup, an item being -DLF_ROT_HP heads of a token, slots = D / 16 rounded up to a power of two; the workgroups of the
+ * queries come first, then those of the keys and, with -DLF_ROT_STORE=1 or 2, as many of the values.  -DLF_HEAD_DIM=(16 * slots). */
+typedef struct LfRotateParamsHost {
+  const void* q;           /* [T, Hq, D] */
+  const void* k;           /* [T, Hkv, D] */
+  const void* v;
+  void* q_out;             /* [T, Hq, D], contiguous */
+  void* k_out;             /* [T, Hkv, D], or the pool (its codes) */
+  void* v_out;
+  uint8_t* k_scales;       /* of pools in 4 bits */
+  uint8_t* v_scales;
+  const float* table;      /* [places, R] */
+  const void* q_weight;    /* [D], optional */
+  const void* k_weight;
+  const int32_t* positions;        /* [T]; null: all rows live */
+  const int32_t* slots;    /* [T] */
+  int64_t q_ss, q_sh, k_ss, k_sh, v_ss, v_sh;
+  int64_t kp_sb, kp_ss, kp_sh, vp_sb, vp_ss, vp_sh;  /* pools; in 4 bits bytes of a page's codes, of its scales, unused; without a pool the first and the last unused */
+  int64_t table_stride, last;      /* last: slots of a pool */
+  int32_t T, Hq, Hkv, D, R, places;
+  int32_t q_chunks, k_chunks;      /* items of a token */
+  int32_t q_blocks, k_blocks;
+  int32_t shift;           /* log2 of the tokens per page */
+  int32_t pairs, norm, wide;       /* neighbours are partners; with norms; weights are floats */
+  float eps;
+} LfRotateParamsHost;
+
+/* lf_rotate_bwd, then with `parts` lf_rotate_dw on a (D / 16, 2) grid. */
+typedef struct LfRotateBwdParamsHost {
+  const void* q;           /* null without norms */
+  const void* k;
+  const void* dq_out;
+  const void* dk_out;
+  void* dq;                /* [T, Hq, D], contiguous */
+  void* dk;
+  const float* table;
+  const void* q_weight;
+  const void* k_weight;
+  void* dq_weight;         /* [D], optional */
+  void* dk_weight;
+  float* parts;            /* [q_blocks + k_blocks, D] */
+  const int32_t* positions;
+  int64_t q_ss, q_sh, k_ss, k_sh, dqo_ss, dqo_sh, dko_ss, dko_sh, table_stride;
+  int32_t T, Hq, Hkv, D, R, places;
+  int32_t q_chunks, k_chunks, q_blocks, k_blocks;
+  int32_t pairs, norm, wide;
+  float eps;
+} LfRotateBwdParamsHost;
+
+/* lf_read_kv */
+typedef struct LfReadParamsHost {
+  const void* k_pool;
+  const void* v_pool;
+  const uint8_t* k_scales;
+  const uint8_t* v_scales;
+  void* k;                 /* [T, heads, 8 * per_head], contiguous */
+  void* v;
+  const int32_t* slots;
+  int64_t kp_sb, kp_ss, kp_sh, vp_sb, vp_ss, vp_sh, last;
+  int32_t T, heads, per_head, shift;
+} LfReadParamsHost;
+
+/* lf_cached on items * Hkv workgroups, then, where a chunk can have several pieces (least < room), lf_cached_combine.  A workgroup has
+ * rows = 16 * LF_CACHED_CB of a kv head's, four times as many with -DLF_CACHED_ROWWAVES=1. */
+typedef struct LfCachedParamsHost {
+  const void* q;           /* [T, Hkv * group, D] */
+  void* o;
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* k_scales;
+  const uint8_t* v_scales;
+  const void* table;       /* int32 or int64 (LF_TABLE_I64) */
+  const int32_t* lengths;
+  const int32_t* offsets;  /* optional */
+  const int32_t* positions;        /* optional */
+  float* part_acc;         /* [items, Hkv, rows, D] */
+  float* part_ml;          /* [items, Hkv, rows, 2] */
+  int64_t q_ss, q_sh, o_ss, o_sh;
+  int64_t k_sb, v_sb, ks_sb, vs_sb, table_stride;    /* bytes; entries */
+  int32_t T, B, Hkv, group, room, shift, window;
+  int32_t items;           /* T * group / rows + min(T, B) + 2, and 2^target_log2 / Hkv more where there can be several pieces */
+  int32_t target_log2, least;
+  int32_t clear;
+  float scale, softcap;
+} LfCachedParamsHost;
+
 #ifdef __cplusplus
 }
 #endif

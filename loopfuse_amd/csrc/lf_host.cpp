@@ -213,6 +213,17 @@ bool launch(const Entry& e, Block& block, void* stream, bool told = true) {
   return !told || PyObject_SetAttr(env.last, name_record, e.record) == 0;
 }
 
+// Room for partial results, under scratch_lock: a captured call has its own, the graph's.
+at::Tensor partial_results(long long floats, const at::Tensor& q, void* stream) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return made({floats}, like(q).dtype(at::kFloat));
+  std::string where;
+  put(where, q.get_device());
+  put(where, stream);
+  at::Tensor& t = scratch[where];
+  if (!t.defined() || t.numel() < floats) t = made({std::max<int64_t>(floats, 1 << 20)}, like(q).dtype(at::kFloat));
+  return t;
+}
+
 // ---- module functions ------------------------------------------------------------------------------------------
 
 // setup(os, environ, variables, switches, checks, last, fail, step, launch)
@@ -425,17 +436,7 @@ PyObject* attention_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
     // (without the GIL: whoever holds the lock needs nothing of Python's)
     pybind11::gil_scoped_release without;
     std::lock_guard<std::mutex> lock(scratch_lock);
-    at::Tensor room;
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
-      room = made({e->more[0]}, like(q).dtype(at::kFloat));      // the graph's own
-    } else {
-      std::string where;
-      put(where, q.get_device());
-      put(where, stream);
-      at::Tensor& t = scratch[where];
-      if (!t.defined() || t.numel() < e->more[0]) t = made({std::max<int64_t>(e->more[0], 1 << 20)}, like(q).dtype(at::kFloat));
-      room = t;
-    }
+    const at::Tensor room = partial_results(e->more[0], q, stream);
     char* at = static_cast<char*>(room.mutable_data_ptr());
     p->attn.part_acc = reinterpret_cast<float*>(at);
     p->attn.part_ml = reinterpret_cast<float*>(at + e->more[1]);
@@ -538,9 +539,181 @@ PyObject* attention_packed_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
   END_HANDLE_TH_ERRORS
 }
 
+// tensors as a tuple, None in the place of one that is not defined
+PyObject* tuple_of(std::initializer_list<const at::Tensor*> parts) {
+  PyObject* r = PyTuple_New(parts.size());
+  Py_ssize_t i = 0;
+  if (r)
+    for (const at::Tensor* t : parts) PyTuple_SET_ITEM(r, i++, t->defined() ? THPVariable_Wrap(*t) : none());
+  return r;
+}
+
+// rotate_heads(q, k, table, q_weight, k_weight, positions, eps, pairs) -> (q, k)
+PyObject* rotate_heads(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 8)) return nullptr;
+  auto e = find('r', a, 6, 5, nullptr, a + 6, 2);
+  if (!e) return none();
+  const at::Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]);
+  const at::Tensor q_out = made(q.sizes(), like(q)), k_out = made(k.sizes(), like(k));
+  Block block(*e);
+  auto* p = block.as<LfRotateParamsHost>();
+  p->q = at_(a[0]);
+  p->k = at_(a[1]);
+  p->table = at_<float>(a[2]);
+  p->q_weight = at_(a[3]);
+  p->k_weight = at_(a[4]);
+  p->positions = at_<int32_t>(a[5]);
+  p->q_out = q_out.mutable_data_ptr();
+  p->k_out = k_out.mutable_data_ptr();
+  if (!launch(*e, block, stream_of(q))) return nullptr;
+  return tuple_of({&q_out, &k_out});
+  END_HANDLE_TH_ERRORS
+}
+
+// rotate_backward(dq_out, dk_out, q, k, table, q_weight, k_weight, positions, eps, pairs, of q_weight, of k_weight) -> (dq, dk, dq_weight, dk_weight);
+// more: floats of the weights' partial sums
+PyObject* rotate_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 12)) return nullptr;
+  auto e = find('R', a, 8, 7, nullptr, a + 8, 4);
+  if (!e) return none();
+  const at::Tensor &dq_out = THPVariable_Unpack(a[0]), &dk_out = THPVariable_Unpack(a[1]);
+  const at::Tensor dq = made(dq_out.sizes(), like(dq_out)), dk = made(dk_out.sizes(), like(dk_out));
+  at::Tensor parts, dw[2];
+  Block block(*e);
+  auto* p = block.as<LfRotateBwdParamsHost>();
+  p->dq_out = at_(a[0]);
+  p->dk_out = at_(a[1]);
+  p->q = at_(a[2]);
+  p->k = at_(a[3]);
+  p->table = at_<float>(a[4]);
+  p->q_weight = at_(a[5]);
+  p->k_weight = at_(a[6]);
+  p->positions = at_<int32_t>(a[7]);
+  p->dq = dq.mutable_data_ptr();
+  p->dk = dk.mutable_data_ptr();
+  for (int i = 0; i < 2; ++i)
+    if (a[10 + i] == Py_True) {
+      const at::Tensor& w = THPVariable_Unpack(a[5 + i]);
+      dw[i] = made(w.sizes(), like(w));
+      (i ? p->dk_weight : p->dq_weight) = dw[i].mutable_data_ptr();
+    }
+  if (e->more[0]) {
+    parts = made({e->more[0]}, like(dq_out).dtype(at::kFloat));
+    p->parts = parts.mutable_data_ptr<float>();
+  }
+  if (!launch(*e, block, stream_of(dq_out))) return nullptr;
+  return tuple_of({&dq, &dk, &dw[0], &dw[1]});
+  END_HANDLE_TH_ERRORS
+}
+
+// append_kv(q, k, v, k_pool, v_pool, k_scales, v_scales, table, q_weight, k_weight, slots, positions, eps, pairs) -> q, without positions True; the pools are those
+// of 16-bit rows, or the codes with their scales
+PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 14)) return nullptr;
+  auto e = find('a', a, 12, 10, nullptr, a + 12, 2);
+  if (!e) return none();
+  const at::Tensor& q = THPVariable_Unpack(a[0]);
+  at::Tensor out;
+  Block block(*e);
+  auto* p = block.as<LfRotateParamsHost>();
+  p->q = at_(a[0]);
+  p->k = at_(a[1]);
+  p->v = at_(a[2]);
+  p->k_out = at_(a[3]);
+  p->v_out = at_(a[4]);
+  p->k_scales = at_<uint8_t>(a[5]);
+  p->v_scales = at_<uint8_t>(a[6]);
+  p->table = at_<float>(a[7]);
+  p->q_weight = at_(a[8]);
+  p->k_weight = at_(a[9]);
+  p->slots = at_<int32_t>(a[10]);
+  p->positions = at_<int32_t>(a[11]);
+  if (a[11] != Py_None) {
+    out = made(q.sizes(), like(q));
+    p->q_out = out.mutable_data_ptr();
+  }
+  if (!launch(*e, block, stream_of(q))) return nullptr;
+  if (out.defined()) return THPVariable_Wrap(out);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// read_kv(k_pool, v_pool, k_scales, v_scales, slots, fp16) -> (k, v); more: the shape of either
+PyObject* read_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 6)) return nullptr;
+  auto e = find('g', a, 5, 4, nullptr, a + 5, 1);
+  if (!e) return none();
+  const auto options = like(THPVariable_Unpack(a[0])).dtype(a[5] == Py_True ? at::kHalf : at::kBFloat16);
+  const at::Tensor k = made({e->more[0], e->more[1], e->more[2]}, options), v = made(k.sizes(), options);
+  Block block(*e);
+  auto* p = block.as<LfReadParamsHost>();
+  p->k_pool = at_(a[0]);
+  p->v_pool = at_(a[1]);
+  p->k_scales = at_<uint8_t>(a[2]);
+  p->v_scales = at_<uint8_t>(a[3]);
+  p->slots = at_<int32_t>(a[4]);
+  p->k = k.mutable_data_ptr();
+  p->v = v.mutable_data_ptr();
+  if (!launch(*e, block, stream_of(k))) return nullptr;
+  return tuple_of({&k, &v});
+  END_HANDLE_TH_ERRORS
+}
+
+// attention_cached(q, k_codes, v_codes, k_scales, v_scales, out, table, lengths, offsets, positions, plan) -> O; more: floats of scratch, and the bytes in front of
+// part_ml in it
+PyObject* attention_cached(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 11)) return nullptr;
+  auto e = find('c', a, 10, 6, a[10], nullptr, 0);
+  if (!e) return none();
+  const at::Tensor& q = THPVariable_Unpack(a[0]);
+  const at::Tensor out = a[5] == Py_None ? made(q.sizes(), like(q)) : THPVariable_Unpack(a[5]);
+  Block block(*e);
+  auto* p = block.as<LfCachedParamsHost>();
+  p->q = at_(a[0]);
+  p->k = at_<uint8_t>(a[1]);
+  p->v = at_<uint8_t>(a[2]);
+  p->k_scales = at_<uint8_t>(a[3]);
+  p->v_scales = at_<uint8_t>(a[4]);
+  p->o = out.mutable_data_ptr();
+  p->table = at_(a[6]);
+  p->lengths = at_<int32_t>(a[7]);
+  p->offsets = at_<int32_t>(a[8]);
+  p->positions = at_<int32_t>(a[9]);
+  void* stream = stream_of(q);
+  if (e->more[0]) {
+    int rc;
+    {
+      // (without the GIL: whoever holds the lock needs nothing of Python's)
+      pybind11::gil_scoped_release without;
+      std::lock_guard<std::mutex> lock(scratch_lock);
+      const at::Tensor room = partial_results(e->more[0], q, stream);
+      p->part_acc = room.mutable_data_ptr<float>();
+      p->part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(p->part_acc) + e->more[1]);
+      rc = env.launch(reinterpret_cast<const lf_launch_item*>(e->items.data()), e->count, block.bytes, stream);
+    }
+    if (rc) {
+      Py_XDECREF(PyObject_CallFunction(env.fail, "i", rc));
+      return nullptr;
+    }
+    if (PyObject_SetAttr(env.last, name_record, e->record)) return nullptr;
+  } else if (!launch(*e, block, stream)) {
+    return nullptr;
+  }
+  if (a[5] == Py_None) return THPVariable_Wrap(out);
+  Py_INCREF(a[5]);
+  return a[5];
+  END_HANDLE_TH_ERRORS
+}
+
 #define LF_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LF_FAST(setup), LF_FAST(key), LF_FAST(keep), {"clear", clear, METH_NOARGS, nullptr}, {"size", size, METH_NOARGS, nullptr},
                          LF_FAST(elsewhere), LF_FAST(packed_layout), LF_FAST(extend_tables), LF_FAST(store_kv), LF_FAST(attention_shared), LF_FAST(attention_packed), LF_FAST(attention_packed_backward),
+                         LF_FAST(rotate_heads), LF_FAST(rotate_backward), LF_FAST(append_kv), LF_FAST(read_kv), LF_FAST(attention_cached),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lf_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

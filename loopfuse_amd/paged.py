@@ -28,7 +28,7 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 
-from . import lowering, rotary
+from . import lowering
 from .lowering import AttnPlan, UnsupportedPlan
 
 _TABLE_DTYPES = (torch.int32, torch.int64)
@@ -246,6 +246,15 @@ def _two_pools4(k_pool, v_pool, dtype, device) -> tuple:
     return shape
 
 
+def _parts(k_pool, v_pool, dtype):
+    """Pools as the host module takes them: K, V, scales of K, of V; None: not for it."""
+    if isinstance(k_pool, Pool4):
+        if not isinstance(v_pool, Pool4) or k_pool.dtype is not dtype or v_pool.dtype is not dtype:
+            return None
+        return k_pool.codes, v_pool.codes, k_pool.scales, v_pool.scales
+    return k_pool, v_pool, None, None
+
+
 def _two_pools(k_pool, v_pool, dtype, device, heads: int, D: int, written=True) -> tuple:
     """(pages, page size, strides of K's pages, tokens and heads, V's) of pools of 16-bit rows."""
     for name, t in (("K pool", k_pool), ("V pool", v_pool)):
@@ -282,6 +291,10 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pool: Union[t
     zeros among the queries, left out of the pools whatever its slot.  Without a table and a norm rows stay as they are."""
     if positions is None:
         raise UnsupportedPlan("positions must be given")
+    parts = _parts(k_pool, v_pool, getattr(q, "dtype", None))
+    done = None if parts is None else _host.append_kv(q, k, v, *parts, table, q_weight, k_weight, slots, positions, eps, bool(pairs))
+    if done is not None:
+        return done
     return _append(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight, eps, bool(pairs))
 
 
@@ -318,8 +331,12 @@ def _append(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight
         P.q_blocks = 0
     spec = rotary.kernel_spec(q.dtype, D, per, store)
     repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (P.q_blocks + 2 * P.k_blocks, 1, 1), 256)], {"kernels": [spec.entry()]})
-    return _append_again(q, k, v, k_pool, v_pool, slots.contiguous(), None if keys_only else positions.contiguous(), table, rotary.even_weight(q_weight),
-                         rotary.even_weight(k_weight), repeat)
+    given = slots, positions, q_weight, k_weight
+    even = slots.contiguous(), None if keys_only else positions.contiguous(), rotary.even_weight(q_weight), rotary.even_weight(k_weight)
+    res = _append_again(q, k, v, k_pool, v_pool, even[0], even[1], table, even[2], even[3], repeat)
+    if all(a is b for a, b in zip(even, given)):
+        lowering._keep_call(lowering._call_key("a", (q, k, v, *_parts(k_pool, v_pool, q.dtype), table, q_weight, k_weight), (slots, positions), None, (eps, pairs)), repeat, ())
+    return res
 
 
 def _append_again(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight, repeat):
@@ -351,6 +368,10 @@ def read_kv(k_pool: Union[torch.Tensor, Pool4], v_pool: Union[torch.Tensor, Pool
     rounded to the type (those of fp16 have less than a bit below its least normal number).  For keys that go on elsewhere: into another cache, or beside
     those of a prompt's next part."""
     dtype = k_pool.dtype if isinstance(k_pool, (Pool4, torch.Tensor)) else None
+    parts = _parts(k_pool, v_pool, dtype)
+    done = None if parts is None else _host.read_kv(*parts, slots, dtype is torch.float16)
+    if done is not None:
+        return done
     if dtype not in lowering._DTYPE_CODE:
         raise UnsupportedPlan("pools must be of bf16 or fp16 rows")
     if k_pool.device.type != "cuda" and not getattr(k_pool, "is_cuda", False):
@@ -377,7 +398,11 @@ def read_kv(k_pool: Union[torch.Tensor, Pool4], v_pool: Union[torch.Tensor, Pool
         if pieces == 0:
             return tuple(torch.empty((T, heads, D), dtype=dtype, device=k_pool.device) for _ in range(2))
         repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (-(-pieces // 256), 1, 1), 256)], {"kernels": [spec.entry()]}, (T, heads, D))
-        return _read_again(k_pool, v_pool, slots.contiguous(), repeat)
+        even = slots.contiguous()
+        res = _read_again(k_pool, v_pool, even, repeat)
+        if even is slots:
+            lowering._keep_call(lowering._call_key("g", parts, (slots,), None, (dtype is torch.float16,)), repeat, (T, heads, D))
+        return res
 
 
 def _read_again(k_pool, v_pool, slots, repeat):
@@ -399,7 +424,9 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, k_pool: Union[torch.Tensor, Pool4
     if _host.store_kv(k, v, k_pool, v_pool, slots):
         return
     if isinstance(k_pool, Pool4) or isinstance(v_pool, Pool4):
-        _append(k, k, v, k_pool, v_pool, slots, None, None, None, None, None, False)
+        parts = _parts(k_pool, v_pool, k.dtype)
+        if parts is None or _host.append_kv(k, k, v, *parts, None, None, None, slots, None, None, False) is None:
+            _append(k, k, v, k_pool, v_pool, slots, None, None, None, None, None, False)
         return
     lowering._no_tangents(k, v, k_pool, v_pool)
     if k.dtype not in lowering._DTYPE_CODE:
@@ -726,6 +753,11 @@ def attention_cached(q: torch.Tensor, k_pool: Pool4, v_pool: Pool4, plan: AttnPl
     Returns O [rows, Hq, D], of which no gradients are recorded.  Rows of no token, and those without a key, are zeros; rows of no request are zeros too, or stay as they
     are in an ``out`` that is given.  A prompt's next part, behind what the cache has of it, is such a call; a prompt of which the cache has nothing attends over
     its own unrounded keys by ``packed.attention_packed``.  Page ids are trusted, as those of ``lowering.attention`` are (``LOOPFUSE_CHECK_TABLES=1`` looks at them)."""
+    parts = _parts(k_pool, v_pool, q.dtype)
+    if parts is not None and parts[2] is not None:
+        done = _host.attention_cached(q, *parts, out, table, lengths, offsets, positions, plan)
+        if done is not None:
+            return done
     return _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out)
 
 
@@ -817,7 +849,10 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
         steps.append((lowering.get_kernel(spec, "lf_cached_combine"), (grid, 1, 1), 256))
     slots = P.items * Hkv * rows if split else 0
     repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps]}, (slots * (D + 2), 4 * slots * D))
-    return _cached_again(q, k_pool, v_pool, table, lengths, offsets, positions, out, repeat)
+    res = _cached_again(q, k_pool, v_pool, table, lengths, offsets, positions, out, repeat)
+    if all(a is b for a, b in zip(given, (table, lengths, offsets, positions))):
+        lowering._keep_call(lowering._call_key("c", (q, *_parts(k_pool, v_pool, dtype), out), given, plan, ()), repeat, repeat.more)
+    return res
 
 
 def _cached_again(q, k_pool, v_pool, table, lengths, offsets, positions, out, repeat):
@@ -840,5 +875,7 @@ def _cached_again(q, k_pool, v_pool, table, lengths, offsets, positions, out, re
     lowering._last_launch.set(repeat.record)
     return out
 
+
+from . import rotary  # noqa: E402  (either module's host module knows PagedStep)
 
 _host = lowering._host()

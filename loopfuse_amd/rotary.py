@@ -102,8 +102,6 @@ def check_operands(q, k, positions, table, q_weight, k_weight, eps, extra=(), pl
             raise UnsupportedPlan("rows of the table: a multiple of 16 rotated elements, head dim at most, contiguous and apart, on 16-byte borders")
         if table.shape[0] > _ALL:
             raise UnsupportedPlan(f"a table of more than {_ALL} positions")
-        if torch.is_grad_enabled() and table.requires_grad:
-            raise UnsupportedPlan("no gradient of the table is formed")
     weights = [(n, w) for n, w in (("q_weight", q_weight), ("k_weight", k_weight)) if w is not None]
     if eps is None:
         if weights:
@@ -164,12 +162,18 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     autograd graph holds, nor for what a graph made outside the capture computed.  Kept for the backward: q and k as given where there is a norm."""
     operands = [t for t in (q, k, q_weight, k_weight) if isinstance(t, torch.Tensor)]
     if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
-        check_operands(q, k, _given(positions), table, q_weight, k_weight, eps)
+        if isinstance(table, torch.Tensor) and table.requires_grad:
+            raise UnsupportedPlan("no gradient of the table is formed")
         from . import packed
         packed.refuse_outside_capture(operands, "Q, K and the weights")
         lowering._no_tangents(*operands)      # (not to be seen inside)
-        return _Rotate.apply(q, k, positions, table, q_weight, k_weight, eps, bool(pairs))
+        return _Rotate.apply(q, k, _given(positions), table, q_weight, k_weight, eps, bool(pairs))
     return _forward(q, k, positions, table, q_weight, k_weight, eps, bool(pairs))
+
+
+def _forward(q, k, positions, table, q_weight, k_weight, eps, pairs):
+    done = _host.rotate_heads(q, k, table, q_weight, k_weight, positions, eps, pairs)
+    return _general(q, k, positions, table, q_weight, k_weight, eps, pairs) if done is None else done
 
 
 def _given(positions):
@@ -179,7 +183,7 @@ def _given(positions):
 
 
 @lowering._on_device_of_first_argument
-def _forward(q, k, positions, table, q_weight, k_weight, eps, pairs):
+def _general(q, k, positions, table, q_weight, k_weight, eps, pairs):
     lowering._no_tangents(q, k, q_weight, k_weight)
     T, Hq, Hkv, D, R, wide = check_operands(q, k, _given(positions), table, q_weight, k_weight, eps)
     if T:
@@ -190,7 +194,11 @@ def _forward(q, k, positions, table, q_weight, k_weight, eps, pairs):
     P.kp_ss, P.kp_sh = Hkv * D, D
     spec = kernel_spec(q.dtype, D, per)
     repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (P.q_blocks + P.k_blocks, 1, 1), 256)], {"kernels": [spec.entry()]})
-    return _forward_again(q, k, positions.contiguous(), table, even_weight(q_weight), even_weight(k_weight), repeat)
+    even = positions.contiguous(), even_weight(q_weight), even_weight(k_weight)
+    res = _forward_again(q, k, even[0], table, *even[1:], repeat)
+    if all(a is b for a, b in zip(even, (positions, q_weight, k_weight))):
+        lowering._keep_call(lowering._call_key("r", (q, k, table, q_weight, k_weight), (positions,), None, (eps, pairs)), repeat, ())
+    return res
 
 
 def params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs) -> tuple:
@@ -222,23 +230,27 @@ def set_tables(P, table, q_weight, k_weight) -> None:
             setattr(P, name, t.data_ptr())
 
 
+def _backward(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, pairs, sums):
+    """Gradients of q and k, and where the ``sums`` say so of q_weight and k_weight; q and k none without a norm."""
+    done = _host.rotate_backward(dq_out, dk_out, q, k, table, q_weight, k_weight, positions, eps, pairs, *sums)
+    return _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, pairs, sums) if done is None else done
+
+
 @lowering._on_device_of_first_argument
-def _backward(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, pairs, wanted):
-    """Gradients of the ``wanted`` ones of q, k, q_weight and k_weight; q and k none without a norm."""
+def _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, pairs, sums):
     lowering._no_tangents(dq_out, dk_out)
+    given = dq_out, dk_out
     dq_out, dk_out = (t if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(n > 1 and s % 8 for n, s in zip(t.shape[:-1], t.stride()[:-1])) else t.contiguous()
-                      for t in (dq_out, dk_out))
+                      for t in given)
     T, Hq, D = dq_out.shape
     Hkv, dev, dtype = dk_out.shape[1], dq_out.device, dq_out.dtype
     weights = [w for w in (q_weight, k_weight) if w is not None]
-    sums = [w is not None and x for w, x in zip((q_weight, k_weight), wanted[2:])]
     dq, dk = (torch.empty(t.shape, dtype=dtype, device=dev) for t in (dq_out, dk_out))
     dw = [torch.empty(D, dtype=weights[0].dtype, device=dev) if x else None for x in sums]
     if T == 0:
         return dq, dk, *(None if w is None else w.zero_() for w in dw)
     P = RotateBwdParams()
     if eps is not None:
-        P.q, P.k = q.data_ptr(), k.data_ptr()
         P.q_ss, P.q_sh, P.k_ss, P.k_sh = *q.stride()[:2], *k.stride()[:2]
     P.dqo_ss, P.dqo_sh, P.dko_ss, P.dko_sh = *dq_out.stride()[:2], *dk_out.stride()[:2]
     P.T, P.Hq, P.Hkv, P.D, P.R, P.pairs, P.norm = T, Hq, Hkv, D, 0 if table is None else table.shape[1], int(pairs), int(eps is not None)
@@ -250,19 +262,25 @@ def _backward(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, p
     if any(sums):
         P.q_blocks, P.k_blocks = min(P.q_blocks, BWD_BLOCKS), min(P.k_blocks, BWD_BLOCKS)
     spec = kernel_spec(dtype, D, per)
+    floats = (P.q_blocks + P.k_blocks) * D if any(sums) else 0
     steps = [(lowering.get_kernel(spec, "lf_rotate_bwd"), (P.q_blocks + P.k_blocks, 1, 1), 256)]
     if any(sums):
         steps.append((lowering.get_kernel(spec, "lf_rotate_dw"), (D // 16, 2, 1), 256))
-        parts = torch.empty((P.q_blocks + P.k_blocks) * D, dtype=torch.float32, device=dev)
+    repeat = lowering._Repeat(P, steps, {"kernels": [x.symbol for x, _, _ in steps]})
+    if floats:
+        parts = torch.empty(floats, dtype=torch.float32, device=dev)
         P.parts = parts.data_ptr()
-    repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps]})
     P.dq_out, P.dk_out, P.dq, P.dk, P.positions = dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), positions.data_ptr()
+    if eps is not None:
+        P.q, P.k = q.data_ptr(), k.data_ptr()
     set_tables(P, table, q_weight, k_weight)
     for name, w in zip(("dq_weight", "dk_weight"), dw):
         if w is not None:
             setattr(P, name, w.data_ptr())
     repeat.launches.launch(P)
     lowering._last_launch.set(repeat.record)
+    if dq_out is given[0] and dk_out is given[1]:
+        lowering._keep_call(lowering._call_key("R", (dq_out, dk_out, q, k, table, q_weight, k_weight), (positions,), None, (eps, pairs, *sums)), repeat, (floats,))
     return dq, dk, *dw
 
 
@@ -271,7 +289,7 @@ BWD_BLOCKS = 1024       # workgroups that sum the weights' gradients, of the que
 
 def _gradients(ctx, dq_out, dk_out):
     q, k, positions, table, q_weight, k_weight = ctx.saved_tensors
-    dq, dk, dqw, dkw = _backward(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, ctx.eps, ctx.pairs, [ctx.needs_input_grad[i] for i in (0, 1, 4, 5)])
+    dq, dk, dqw, dkw = _backward(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, ctx.eps, ctx.pairs, (q_weight is not None and ctx.needs_input_grad[4], k_weight is not None and ctx.needs_input_grad[5]))
     return dq, dk, None, None, dqw, dkw, None, None
 
 
@@ -293,3 +311,6 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq_out, dk_out):
         return (_gradients_once if torch.is_grad_enabled() else _gradients)(ctx, dq_out, dk_out)
+
+
+_host = lowering._host()
