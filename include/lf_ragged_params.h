@@ -159,8 +159,8 @@ typedef struct LfReadParamsHost {
   int32_t T, heads, per_head, shift;
 } LfReadParamsHost;
 
-/* lf_cached on items * Hkv workgroups, then, where a chunk can have several pieces (least < room), lf_cached_combine.  A workgroup has
- * rows = 16 * LF_CACHED_CB of a kv head's, four times as many with -DLF_CACHED_ROWWAVES=1. */
+/* lf_cached, then, where fixed is 0 or more, lf_cached_combine on T * Hkv * group workgroups (or T * ceil(Hkv * group / (1024 / D))).  A unit is rows =
+ * 16 * LF_CACHED_CB rows of a kv head of a request, four times as many with -DLF_CACHED_ROWWAVES=1: T * group / rows + min(T, B) units per kv head at most. */
 typedef struct LfCachedParamsHost {
   const void* q;           /* [T, Hkv * group, D] */
   void* o;
@@ -172,13 +172,16 @@ typedef struct LfCachedParamsHost {
   const int32_t* lengths;
   const int32_t* offsets;  /* optional */
   const int32_t* positions;        /* optional */
-  float* part_acc;         /* [items, Hkv, rows, D] */
-  float* part_ml;          /* [items, Hkv, rows, 2] */
+  float* part_acc;         /* [units + workgroups, rows, D] */
+  float* part_ml;          /* [units + workgroups, rows, 2] */
   int64_t q_ss, q_sh, o_ss, o_sh;
   int64_t k_sb, v_sb, ks_sb, vs_sb, table_stride;    /* bytes; entries */
-  int32_t T, B, Hkv, group, room, shift, window;
-  int32_t items;           /* T * group / rows + min(T, B) + 2, and 2^target_log2 / Hkv more where there can be several pieces */
-  int32_t target_log2, least;
+  int32_t T, B, Hkv, group;
+  uint32_t per_group;      /* 2^32 / group, rounded up */
+  int32_t room, shift, window;
+  int32_t fixed;           /* what a unit costs besides its pairs of tiles of 16 keys; -1: each workgroup has a unit */
+  int32_t least;           /* least share of a workgroup */
+  int32_t workgroups;      /* of lf_cached; with fixed -1 the most units that there can be */
   int32_t clear;
   float scale, softcap;
 } LfCachedParamsHost;

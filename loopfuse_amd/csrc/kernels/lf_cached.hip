@@ -2,10 +2,10 @@
 // (lf_pool4.hip.h), those of the new tokens among them.
 //
 // Request b has n = offsets[b + 1] - offsets[b] rows of q and lengths[b] keys; a row at position p sees the keys j <= p (and p - j < window), or all.
-// A kv head's n * group rows are taken LF_CACHED_ROWS at a time (a chunk), its keys in pieces of one length for all requests, so that about 2^target_log2
-// workgroups have one; (chunk, piece) pairs are numbered request by request, and every wave finds its own from the lengths, as nothing of them is known
-// to the host.  A piece leaves, per row, an exponent offset, the sum of the exponentials and their sum with V, which lf_cached_combine joins; a
-// chunk of one piece is written at once.
+// A unit of work is a kv head's LF_CACHED_ROWS rows of a request over its keys, 32 at a time.  Lengths are on the GPU only: every wave sums what the units
+// cost, each its pairs of tiles of 16 keys and something for its begin, and finds the share of its workgroup, the same for all, by itself.  So no workgroup
+// waits for a longer one.  A unit that several workgroups have leaves, from each, an exponent offset, the sum of the exponentials and their sum with V per
+// row, which lf_cached_combine joins; one that a workgroup has alone is written at once.  Where units are many each workgroup takes one.
 //
 // A wave takes 32 keys at a time for LF_CACHED_CB * 16 rows, its operands straight from memory:
 //   S^T = K Q^T   : 16 keys' codes and scales are, as loaded, the first operand of the 16x16x128 product of scaled 4- and 8-bit numbers.  Q^T is
@@ -31,6 +31,7 @@
 #define LF_CACHED_OSTRIDE (LF_HEAD_DIM + 4)
 
 typedef int lf_i32x8 __attribute__((ext_vector_type(8)));
+typedef short lf_i16x2 __attribute__((ext_vector_type(2)));
 
 struct LfCachedParams {
   const lf_elem* q;            // [T, Hq, D], strides below
@@ -43,69 +44,76 @@ struct LfCachedParams {
   const int* lengths;          // [B]
   const int* offsets;          // [B + 1]; none: a row each
   const int* positions;        // [T]; none: the last key's
-  float* part_acc;             // [items, Hkv, LF_CACHED_ROWS, D]
-  float* part_ml;              // [items, Hkv, LF_CACHED_ROWS, 2]
+  float* part_acc;             // [slots, LF_CACHED_ROWS, D]
+  float* part_ml;              // [slots, LF_CACHED_ROWS, 2]
   long long q_ss, q_sh, o_ss, o_sh;
   long long k_sb, v_sb, ks_sb, vs_sb, table_stride;    // bytes of a page; entries
   int T, B, Hkv, group;
+  unsigned per_group;          // 2^32 / group, rounded up
   int room;                    // keys that a row of the table has room for
   int shift;                   // log2 of the tokens per page
   int window;
-  int items;                   // (chunk, piece) pairs that there are workgroups for, one more than there can be
-  int target_log2, least;      // workgroups that the keys are cut for; least length of a piece, a multiple of 32
+  int fixed;                   // what a unit costs besides its pairs of tiles, in pairs; below 0: each workgroup has a unit, whatever it costs
+  int least;                   // least share of a workgroup
+  int workgroups;
   int clear;                   // 1: zeros into rows of no request
   float scale, softcap;
 };
 
-// What a lane knows of its request.
+// A request: its rows and its keys.
 struct LfCachedRequest {
-  int first, n;                // its rows
-  int start, end;              // its keys: the first that any row can see, a multiple of 32
-  int chunks;
+  int first, n;
+  int start, end;              // the first key that any row can see, a multiple of 32; the last one's successor
+  int chunks;                  // LF_CACHED_ROWS rows of a kv head each
+  int pairs;                   // of tiles of 16 keys, 1 at least: a unit without a key has its zeros to write
 };
 __device__ __forceinline__ LfCachedRequest lf_cached_request(const LfCachedParams& p, int b) {
-  LfCachedRequest r = {0, 0, 0, 0, 0};
-  if (b >= p.B) return r;
-  r.first = p.offsets ? min(max(p.offsets[b], 0), p.T) : b;
-  r.n = p.offsets ? max(min(p.offsets[b + 1], p.T) - r.first, 0) : 1;
-  r.end = min(max(p.lengths[b], 0), p.room);
+  LfCachedRequest r;
+  const int at = min(b, p.B - 1);
+  int end = p.lengths[at], lo = at, hi = at + 1;
+  if (p.offsets) {
+    lo = p.offsets[at];
+    hi = p.offsets[at + 1];
+  }
+  r.first = min(max(lo, 0), p.T);
+  r.n = b < p.B ? max(min(hi, p.T) - r.first, 0) : 0;
+  r.end = min(max(end, 0), p.room);
+  r.start = 0;
 #if LF_MASK == 2
-  if (r.n > 0) r.start = max((p.positions ? p.positions[r.first] : r.end - 1) - p.window + 1, 0) & ~31;
-  r.start = min(r.start, r.end & ~31);
+  const int from = p.positions && r.n > 0 ? p.positions[r.first] : r.end - 1;
+  r.start = min(max(from - p.window + 1, 0), max(r.end - 1, 0)) & ~31;
 #endif
   r.chunks = (int)(((long long)r.n * p.group + LF_CACHED_ROWS - 1) / LF_CACHED_ROWS);
+  r.pairs = max((r.end - r.start + 31) >> 5, 1);
   return r;
 }
-__device__ __forceinline__ float lf_cached_sum(float x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
-  return x;
-}
-// Length of a piece.  `mine`: the first 64 requests, one per lane.  (Whole pairs of tiles; the sum's rounding is below the 2^-10 that are added.)
-__device__ __forceinline__ int lf_cached_split(const LfCachedParams& p, const LfCachedRequest& mine) {
-  float sum = 0.0f;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const LfCachedRequest r = b0 ? lf_cached_request(p, b0 + __lane_id()) : mine;
-    sum += (float)(r.end - r.start) * (float)r.chunks;
-  }
-  const float even = lf_cached_sum(sum) * (float)p.Hkv * (1.0f + 0x1p-10f) * __builtin_bit_cast(float, (127 - p.target_log2) << 23);
-  const int split = even < 0x1p30f ? ((int)even + 32) & ~31 : 1 << 30;
-  return __builtin_amdgcn_readfirstlane(max(p.least, split));
-}
-__device__ __forceinline__ int lf_cached_pieces(const LfCachedRequest& r, int split) { return max((r.end - r.start + split - 1) / split, 1); }
 
-struct LfCachedUnit {
-  int b, chunk, piece, pieces;
-  LfCachedRequest r;
-  int before;                  // (chunk, piece) pairs of the requests before
-};
-// The request that `item` is of, or of whose rows `row` is one where `item` is below 0; false: of none (`before` = all pairs then).
-__device__ __forceinline__ bool lf_cached_find(const LfCachedParams& p, const LfCachedRequest& mine, int split, int item, int row, LfCachedUnit& u) {
-  int before = 0;
+// The units (request, chunk, kv head), heads innermost, lie one behind the other on a line, each as long as `fixed` and its pairs (or all of length 1);
+// workgroup i has the line from i * share on.  (The host sees to it that the line is shorter than 2^31.)
+__device__ __forceinline__ int lf_cached_size(const LfCachedParams& p, const LfCachedRequest& r) { return p.fixed < 0 ? 1 : r.pairs + p.fixed; }
+__device__ __forceinline__ int lf_cached_line(const LfCachedParams& p, const LfCachedRequest& mine) {
+  int line = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     const LfCachedRequest r = b0 ? lf_cached_request(p, b0 + __lane_id()) : mine;
-    const int count = r.chunks * lf_cached_pieces(r, split), upto = lf_wave_scan(count);
-    const unsigned long long hit = __builtin_amdgcn_ballot_w64(item >= 0 ? before + upto > item : r.n > 0 && row >= r.first && row < r.first + r.n);
+    line += __builtin_amdgcn_readlane(lf_wave_scan(r.chunks * p.Hkv * lf_cached_size(p, r)), 63);
+  }
+  return line;
+}
+__device__ __forceinline__ int lf_cached_share(const LfCachedParams& p, int line, int workgroups) { return max(p.least, (line + workgroups - 1) / workgroups); }
+
+struct LfCachedPlace {
+  int b;
+  LfCachedRequest r;
+  int before;                  // on the line, in front of the request's units
+  int units;                   // of the requests in front of it
+};
+// The request that has place `place` of the line, or where that is below 0 row `row`; false: none has.
+__device__ __forceinline__ bool lf_cached_find(const LfCachedParams& p, const LfCachedRequest& mine, int place, int row, LfCachedPlace& u) {
+  int before = 0, units = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const LfCachedRequest r = b0 ? lf_cached_request(p, b0 + __lane_id()) : mine;
+    const int count = r.chunks * p.Hkv, cost = count * lf_cached_size(p, r), upto = lf_wave_scan(cost), units_upto = lf_wave_scan(count);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(place >= 0 ? before + upto > place : r.n > 0 && row >= r.first && row < r.first + r.n);
     if (hit != 0ull) {
       const int l = (int)__builtin_ctzll(hit);
       u.b = b0 + l;
@@ -114,19 +122,26 @@ __device__ __forceinline__ bool lf_cached_find(const LfCachedParams& p, const Lf
       u.r.start = __builtin_amdgcn_readlane(r.start, l);
       u.r.end = __builtin_amdgcn_readlane(r.end, l);
       u.r.chunks = __builtin_amdgcn_readlane(r.chunks, l);
-      u.pieces = lf_cached_pieces(u.r, split);
-      u.before = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l);
-      if (item >= 0) {
-        const int within = item - u.before;
-        u.chunk = u.r.chunks - 1 - within / u.pieces;      // (under a causal mask the last rows have the most keys: first)
-        u.piece = within - within / u.pieces * u.pieces;
-      }
+      u.r.pairs = __builtin_amdgcn_readlane(r.pairs, l);
+      u.before = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(cost, l);
+      u.units = units + __builtin_amdgcn_readlane(units_upto, l) - __builtin_amdgcn_readlane(count, l);
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
+    units += __builtin_amdgcn_readlane(units_upto, 63);
   }
-  u.before = before;
   return false;
+}
+
+// Largest, or least, over the 16 lanes of a row, the same in all four rows of the wave.
+template <bool kMost>
+__device__ __forceinline__ int lf_cached_of_rows(int x) {
+  auto take = [](int a, int b) { return kMost ? max(a, b) : min(a, b); };
+  x = take(x, __builtin_amdgcn_update_dpp(x, x, 0xb1, 0xf, 0xf, false));       // quad_perm [1,0,3,2]
+  x = take(x, __builtin_amdgcn_update_dpp(x, x, 0x4e, 0xf, 0xf, false));       // quad_perm [2,3,0,1]
+  x = take(x, __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, false));      // row_half_mirror
+  x = take(x, __builtin_amdgcn_update_dpp(x, x, 0x140, 0xf, 0xf, false));      // row_mirror
+  return __builtin_amdgcn_readfirstlane(x);
 }
 
 // 32 keys of a head as loaded
@@ -139,121 +154,49 @@ struct LfCachedStage {
 extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedParams p) {
   constexpr int D = LF_CACHED_D, CB = LF_CACHED_CB;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-  const int item = blockIdx.x / p.Hkv, h = blockIdx.x - item * p.Hkv;
   const LfCachedRequest mine = lf_cached_request(p, lane);
-  const int split = lf_cached_split(p, mine);
-  LfCachedUnit u;
-  if (!lf_cached_find(p, mine, split, item, 0, u)) {
-    // rows of no request, shared by the workgroups without a pair
-    if (!p.clear || !p.offsets) return;
-    const int lo = min(max(p.offsets[0], 0), p.T), hi = max(min(max(p.offsets[p.B], 0), p.T), lo);
-    const int Hq = p.Hkv * p.group, pieces = Hq * (D / 8);
-    const long long all = (long long)(lo + p.T - hi) * pieces;
-    for (long long i = (long long)((item - u.before) * p.Hkv + h) * 256 + tid; i < all; i += (long long)(p.items - u.before) * p.Hkv * 256) {
-      const long long row = i / pieces;
-      const int at = (int)(i - row * pieces), head = at / (D / 8);
-      *reinterpret_cast<lf_u32x4*>(p.o + (row < lo ? row : row - lo + hi) * p.o_ss + head * p.o_sh + 8 * (at - head * (D / 8))) = lf_u32x4{0u, 0u, 0u, 0u};
-    }
-    return;
-  }
+  const int line = lf_cached_line(p, mine), share = lf_cached_share(p, line, p.workgroups);
+  auto inverse = [](float l) { return l == 0.0f ? 0.0f : 1.0f / l; };      // a row without a key: zeros; NaN stays
+#if !LF_CACHED_ROWWAVES
+  __shared__ float red_o[4 * 16 * LF_CACHED_OSTRIDE];
+  __shared__ float red_m[4][16], red_l[4][16];
+#endif
+  int place = min((long long)blockIdx.x * share, (long long)line);
+  const int place_end = min((long long)place + share, (long long)line);
+  while (place < place_end) {
+  LfCachedPlace u;
+  if (!lf_cached_find(p, mine, place, 0, u)) break;
+  const int size = lf_cached_size(p, u.r), unit = (place - u.before) / size, from = place - u.before - unit * size, upto = min(size, from + place_end - place);
+  // (under a causal mask the last rows have the most keys: first)
+  const int chunk = u.r.chunks - 1 - unit / p.Hkv, h = unit % p.Hkv;
+  const int slot = u.units + unit + (int)blockIdx.x;       // (either grows along the line)
+  place += upto - from;
+  if (upto <= p.fixed) continue;
+  const int pair0 = p.fixed < 0 ? 0 : max(from - p.fixed, 0), pair1 = p.fixed < 0 ? u.r.pairs : upto - p.fixed;
   const int rows = u.r.n * p.group;      // of a kv head
-  const int row0 = u.chunk * LF_CACHED_ROWS + (LF_CACHED_ROWWAVES ? wave * 16 * CB : 0);
-  const int piece_begin = u.r.start + u.piece * split, piece_end = min(piece_begin + split, u.r.end);
+  const int row0 = chunk * LF_CACHED_ROWS + (LF_CACHED_ROWWAVES ? wave * 16 * CB : 0);
+  const bool whole = pair0 == 0 && pair1 == u.r.pairs;
 
-  // ---- rows of this lane, one per column block: their bounds and Q^T in 8-bit parts
-  lf_i32x8 qp[CB][LF_CACHED_QN];
-  int qscale[CB];                        // exponent of the first part, as the product takes it
-  int lo[CB], hi[CB];
-  int least_hi = 0x7fffffff, most_hi = 0, least_lo = 0x7fffffff, most_lo = 0;
+  // ---- loads: rows of this lane, one per column block, and their positions; then the first keys
+  constexpr int kHeld = D == 128 ? 4 : 2;      // 16-byte pieces of a row
+  lf_elem8 raw[CB][kHeld];
+  int pos[CB];
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
-    const int row = row0 + 16 * cb + c;
-    const bool real = row < rows;
-    const int t = u.r.first + (real ? row / p.group : 0), head = h * p.group + (real ? row % p.group : 0);
-    const int pos = p.positions ? p.positions[t] : u.r.end - 1;
-    lo[cb] = 0;
-    hi[cb] = 0;
-    if (real && pos >= 0) {
-#if LF_MASK == 0
-      hi[cb] = u.r.end;
-#else
-      hi[cb] = min(pos, u.r.end - 1) + 1;
-#endif
-#if LF_MASK == 2
-      lo[cb] = max(pos - p.window + 1, 0);
-#endif
-      least_hi = min(least_hi, hi[cb]);
-      most_hi = max(most_hi, hi[cb]);
-      least_lo = min(least_lo, lo[cb]);
-      most_lo = max(most_lo, lo[cb]);
-    }
-    // bytes 0 ... 15 of a lane are k = 16 g ..., bytes 16 ... 31 k = 64 + 16 g ... (D 64: zeros)
-    const lf_elem* qrow = p.q + (long long)t * p.q_ss + head * p.q_sh;
-    float x[32];
-    unsigned top = 0;
+    // (rows behind the last repeat the chunk's first; their results are dropped)
+    const int row = row0 + 16 * cb + c, at = row < rows ? row : min(row0, rows - 1);
+    const int t_of = p.group == 1 ? at : (int)__umulhi((unsigned)at, p.per_group);
+    const int t = u.r.first + t_of, head = h * p.group + at - t_of * p.group;
+    pos[cb] = p.positions ? p.positions[t] : u.r.end - 1;
+    // bytes 0 ... 15 of a lane's 8-bit operand are k = 16 g ..., bytes 16 ... 31 k = 64 + 16 g ... (D 64: zeros)
+    const lf_elem* qrow = p.q + (long long)t * p.q_ss + head * p.q_sh + 16 * g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lf_elem8 raw = {};
-      if (D == 128 || i < 2) raw = *reinterpret_cast<const lf_elem8*>(qrow + 16 * g + (i < 2 ? 8 * i : 48 + 8 * i));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[8 * i + e] = real ? lf_to_float(raw[e]) : 0.0f;
-        top = max(top, __builtin_bit_cast(unsigned, x[8 * i + e]) & 0x7fffffffu);
-      }
-    }
-    top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
-    top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
-    // the largest in [128, 256); an infinity or NaN makes all of the row's scores NaN
-    const int up = top >= 0x7f800000u ? 255 : max((int)(top >> 23) - 7, 20);
-    qscale[cb] = up;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = up == 255 ? 0.0f : __builtin_amdgcn_ldexpf(x[i], 127 - up);
-#pragma unroll
-    for (int n = 0; n < LF_CACHED_QN; ++n)
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        int packed = 0;
-        packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w], x[4 * w + 1], packed, false);
-        packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2], x[4 * w + 3], packed, true);
-        qp[cb][n][w] = packed;
-        const lf_f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(packed, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(packed, true);
-        // what is left of it, 2^5 times
-        x[4 * w] = (x[4 * w] - a[0]) * 32.0f;
-        x[4 * w + 1] = (x[4 * w + 1] - a[1]) * 32.0f;
-        x[4 * w + 2] = (x[4 * w + 2] - b[0]) * 32.0f;
-        x[4 * w + 3] = (x[4 * w + 3] - b[1]) * 32.0f;
-      }
+    for (int i = 0; i < kHeld; ++i) raw[cb][i] = *reinterpret_cast<const lf_elem8*>(qrow + (i < 2 ? 8 * i : 48 + 8 * i));
   }
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
-    least_hi = min(least_hi, __shfl_xor(least_hi, d, 64));
-    most_hi = max(most_hi, __shfl_xor(most_hi, d, 64));
-    least_lo = min(least_lo, __shfl_xor(least_lo, d, 64));
-    most_lo = max(most_lo, __shfl_xor(most_lo, d, 64));
-  }
-  least_hi = __builtin_amdgcn_readfirstlane(least_hi);
-  most_lo = __builtin_amdgcn_readfirstlane(most_lo);
-  const int begin = max(piece_begin, __builtin_amdgcn_readfirstlane(least_lo) & ~31), end = min(piece_end, __builtin_amdgcn_readfirstlane(most_hi));
-  const int pairs = end > begin ? (end - begin + 31) >> 5 : 0;
-
-#if LF_SOFTCAP
-  const float sc_in = p.scale / p.softcap;
-  const float cexp = LF_LOG2E;
-#else
-  const float cexp = p.scale * LF_LOG2E;
-#endif
-  lf_f32x4 o[CB][LF_CACHED_NV];
-  float mc[CB], l_part[CB];
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    mc[cb] = LF_NEG_INF;
-    l_part[cb] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] = lf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  // ---- loads
-  const int last_tile = (u.r.end - 1) & ~15;
+  int begin = u.r.start + 32 * pair0, pairs = u.r.end > 0 ? pair1 - pair0 : 0;
+  constexpr int kStep = LF_CACHED_ROWWAVES ? 1 : 4;
+  const int first = LF_CACHED_ROWWAVES ? 0 : wave;
+  const int last_tile = max(u.r.end - 1, 0) & ~15;
   const long long head_tiles = (long long)h << (p.shift - 4);
   const int in_page = (1 << p.shift) - 1;
 #if LF_TABLE_I64
@@ -289,6 +232,102 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
       s.vs[w] = *reinterpret_cast<const unsigned*>(vst + (g * (D / 32) + c / (512 / D)) * 4);
     }
   };
+  // three stages rotate; loads past the end repeat the last pair, so that there is no condition on them
+  LfCachedStage s0, s1, s2;
+  Ids i0, i1, i2;
+  auto issue_first = [&]() {
+    if (first >= pairs) return;
+    i0 = fetch(first);
+    i1 = fetch(first + kStep);
+    i2 = fetch(first + 2 * kStep);
+    issue(s0, first, i0);
+    issue(s1, first + kStep, i1);
+    issue(s2, first + 2 * kStep, i2);
+    i0 = fetch(first + 3 * kStep);
+    i1 = fetch(first + 4 * kStep);
+    i2 = fetch(first + 5 * kStep);
+  };
+  if (!LF_CACHED_ROWWAVES) issue_first();
+  // bounds of the rows
+  int lo[CB], hi[CB];
+  int least_hi = 0x7fffffff, most_hi = 0, least_lo = 0x7fffffff, most_lo = 0;
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    hi[cb] = pos[cb] < 0 ? 0 : LF_MASK == 0 ? u.r.end : min(pos[cb], u.r.end - 1) + 1;
+    lo[cb] = LF_MASK == 2 ? max(pos[cb] - p.window + 1, 0) : 0;
+    least_hi = min(least_hi, hi[cb]);
+    most_hi = max(most_hi, hi[cb]);
+    least_lo = min(least_lo, lo[cb]);
+    most_lo = max(most_lo, lo[cb]);
+  }
+  least_hi = lf_cached_of_rows<false>(least_hi);
+  if (LF_MASK == 2) most_lo = lf_cached_of_rows<true>(most_lo);
+#if LF_CACHED_ROWWAVES
+  // (where a chunk's rows differ a wave leaves out what none of its own sees)
+  {
+    const int end = min(begin + 32 * pairs, lf_cached_of_rows<true>(most_hi));
+    if (LF_MASK == 2) begin = max(begin, lf_cached_of_rows<false>(least_lo) & ~31);
+    pairs = end > begin ? (end - begin + 31) >> 5 : 0;
+  }
+  issue_first();
+#endif
+
+  // ---- Q^T in 8-bit parts
+  lf_i32x8 qp[CB][LF_CACHED_QN];
+  int qscale[CB];                        // exponent of the first part, as the product takes it
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    float x[8 * kHeld], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * kHeld; ++i) {
+      x[i] = lf_to_float(raw[cb][i / 8][i % 8]);
+      top = fmaxf(top, fabsf(x[i]));
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    // the largest in [128, 256); an infinity makes all of the row's scores NaN (a NaN is one in 8 bits too)
+    const int exponent = (int)(__builtin_bit_cast(unsigned, top) >> 23), up = max(exponent - 7, 20);
+    qscale[cb] = exponent == 255 ? 255 : up;
+#pragma unroll
+    for (int n = 0; n < LF_CACHED_QN; ++n) {
+      const float by = __builtin_bit_cast(float, (up - 5 * n) << 23);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        if (w >= 2 * kHeld) {
+          qp[cb][n][w] = 0;
+          continue;
+        }
+        lf_i16x2 packed = {0, 0};
+        packed = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(packed, x[4 * w], x[4 * w + 1], by, false);
+        packed = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(packed, x[4 * w + 2], x[4 * w + 3], by, true);
+        qp[cb][n][w] = __builtin_bit_cast(int, packed);
+        if (n + 1 == LF_CACHED_QN) continue;
+        // what is left of it: less than a 2^-4 th, for the next part, whose power is 2^5 times less
+        const lf_f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(__builtin_bit_cast(unsigned, packed), by, false);
+        const lf_f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(__builtin_bit_cast(unsigned, packed), by, true);
+        x[4 * w] -= a[0];
+        x[4 * w + 1] -= a[1];
+        x[4 * w + 2] -= b[0];
+        x[4 * w + 3] -= b[1];
+      }
+    }
+  }
+
+#if LF_SOFTCAP
+  const float sc_in = p.scale / p.softcap;
+  const float cexp = LF_LOG2E;
+#else
+  const float cexp = p.scale * LF_LOG2E;
+#endif
+  lf_f32x4 o[CB][LF_CACHED_NV];
+  float mc[CB], l_part[CB];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    mc[cb] = LF_NEG_INF;
+    l_part[cb] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] = lf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
 
   // ---- 32 keys
   auto consume = [&](LfCachedStage& s, int pair) {
@@ -342,7 +381,7 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
 #if LF_SOFTCAP
           y = p.softcap * lf_tanh(y * sc_in);
 #endif
-          x[4 * w + e] = y * cexp;
+          x[4 * w + e] = y;
         }
       }
       if (partly) {
@@ -354,6 +393,7 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
+      mx *= cexp;
       if (__builtin_amdgcn_ballot_w64(mx > mc[cb] + (float)LF_CACHED_LAZY) != 0ull) {
         float mq = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mq = fmaxf(mq, __shfl_xor(mq, 32, 64));
@@ -368,7 +408,7 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
       lf_elem8 pb;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = lf_exp2(x[i] - m_sub);
+        const float e = lf_exp2(__builtin_fmaf(x[i], cexp, -m_sub));
         l_part[cb] += e;
         pb[i] = lf_from_float(e);
       }
@@ -377,33 +417,19 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
     }
   };
 
-  // ---- this wave's pairs: three stages rotate; loads past the end repeat the last pair, so that the loop has no condition on them
-  {
-    constexpr int kStep = LF_CACHED_ROWWAVES ? 1 : 4;
-    const int first = LF_CACHED_ROWWAVES ? 0 : wave;
-    if (first < pairs) {
-      LfCachedStage s0, s1, s2;
-      Ids i0 = fetch(first), i1 = fetch(first + kStep), i2 = fetch(first + 2 * kStep);
-      issue(s0, first, i0);
-      issue(s1, first + kStep, i1);
-      issue(s2, first + 2 * kStep, i2);
-      i0 = fetch(first + 3 * kStep);
-      i1 = fetch(first + 4 * kStep);
-      i2 = fetch(first + 5 * kStep);
-      for (int pr = first; pr < pairs; pr += 3 * kStep) {
-        consume(s0, pr);
-        issue(s0, pr + 3 * kStep, i0);
-        i0 = fetch(pr + 6 * kStep);
-        if (pr + kStep >= pairs) break;
-        consume(s1, pr + kStep);
-        issue(s1, pr + 4 * kStep, i1);
-        i1 = fetch(pr + 7 * kStep);
-        if (pr + 2 * kStep >= pairs) break;
-        consume(s2, pr + 2 * kStep);
-        issue(s2, pr + 5 * kStep, i2);
-        i2 = fetch(pr + 8 * kStep);
-      }
-    }
+  // ---- this wave's pairs
+  for (int pr = first; pr < pairs; pr += 3 * kStep) {
+    consume(s0, pr);
+    issue(s0, pr + 3 * kStep, i0);
+    i0 = fetch(pr + 6 * kStep);
+    if (pr + kStep >= pairs) break;
+    consume(s1, pr + kStep);
+    issue(s1, pr + 4 * kStep, i1);
+    i1 = fetch(pr + 7 * kStep);
+    if (pr + 2 * kStep >= pairs) break;
+    consume(s2, pr + 2 * kStep);
+    issue(s2, pr + 5 * kStep, i2);
+    i2 = fetch(pr + 8 * kStep);
   }
 
   // ---- results: lane (q = c, g) has elements D / 4 * g ... of its row, 4 groups of D / 16
@@ -413,10 +439,11 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
     l_wave[cb] = l_part[cb] + __shfl_xor(l_part[cb], 16, 64);
     l_wave[cb] += __shfl_xor(l_wave[cb], 32, 64);
   }
-  const bool whole = u.pieces == 1;
-  const long long slot0 = ((long long)item * p.Hkv + h) * LF_CACHED_ROWS;
-  auto inverse = [](float l) { return l == 0.0f ? 0.0f : 1.0f / l; };      // a row without a key: zeros; NaN stays
-  auto out_row = [&](int row) { return p.o + (long long)(u.r.first + row / p.group) * p.o_ss + (h * p.group + row % p.group) * p.o_sh; };
+  const long long slot0 = (long long)slot * LF_CACHED_ROWS;
+  auto out_row = [&](int row) {
+    const unsigned t = p.group == 1 ? row : __umulhi(row, p.per_group);
+    return p.o + (long long)(u.r.first + (int)t) * p.o_ss + (h * p.group + row - (int)t * p.group) * p.o_sh;
+  };
 #if LF_CACHED_ROWWAVES
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
@@ -433,26 +460,24 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
         *reinterpret_cast<lf_elem8*>(to + 8 * n) = y;
       }
     } else {
-      const long long slot = slot0 + (row - u.chunk * LF_CACHED_ROWS);
+      const long long at = slot0 + (row - chunk * LF_CACHED_ROWS);
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {
         lf_f32x4 y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = o[cb][(4 * n + i) % LF_CACHED_NV][(4 * n + i) / LF_CACHED_NV];
-        *reinterpret_cast<lf_f32x4*>(&p.part_acc[slot * D + D / 4 * g + 4 * n]) = y;
+        *reinterpret_cast<lf_f32x4*>(&p.part_acc[at * D + D / 4 * g + 4 * n]) = y;
       }
       if (g == 0) {
-        p.part_ml[slot * 2] = mc[cb];
-        p.part_ml[slot * 2 + 1] = l_wave[cb];
+        p.part_ml[at * 2] = mc[cb];
+        p.part_ml[at * 2 + 1] = l_wave[cb];
       }
     }
   }
 #else
-  __shared__ float red_o[4 * 16 * LF_CACHED_OSTRIDE];
-  __shared__ float red_m[4][16], red_l[4][16];
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
-    if (cb) __syncthreads();
+    __syncthreads();       // (a block of rows, or a unit, before)
     if (g == 0) {
       red_m[wave][c] = mc[cb];
       red_l[wave][c] = l_wave[cb];
@@ -491,36 +516,51 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
         for (int i = 0; i < 8; ++i) y[i] = lf_from_float(sum[i] * inv);
         *reinterpret_cast<lf_elem8*>(out_row(row) + d0) = y;
       } else {
-        const long long slot = slot0 + 16 * cb + r;
+        const long long to = slot0 + 16 * cb + r;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          *reinterpret_cast<lf_f32x4*>(&p.part_acc[slot * D + d0 + 4 * i]) = lf_f32x4{sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]};
+          *reinterpret_cast<lf_f32x4*>(&p.part_acc[to * D + d0 + 4 * i]) = lf_f32x4{sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]};
         if (d0 == 0) {
-          p.part_ml[slot * 2] = m_all;
-          p.part_ml[slot * 2 + 1] = l;
+          p.part_ml[to * 2] = m_all;
+          p.part_ml[to * 2 + 1] = l;
         }
       }
     }
   }
 #endif
+  }
+  if (p.clear && p.offsets) {
+    // rows of no request, dealt to all workgroups
+    const int lo = min(max(p.offsets[0], 0), p.T), hi = max(min(max(p.offsets[p.B], 0), p.T), lo);
+    const int pieces = p.Hkv * p.group * (D / 8);
+    const long long all = (long long)(lo + p.T - hi) * pieces;
+    for (long long i = (long long)blockIdx.x * 256 + tid; i < all; i += (long long)gridDim.x * 256) {
+      const long long row = i / pieces;
+      const int at = (int)(i - row * pieces), head = at / (D / 8);
+      *reinterpret_cast<lf_u32x4*>(p.o + (row < lo ? row : row - lo + hi) * p.o_ss + head * p.o_sh + 8 * (at - head * (D / 8))) = lf_u32x4{0u, 0u, 0u, 0u};
+    }
+  }
 }
 
-// Joins a row's pieces.  D / 4 threads have a row, 4 elements each; a block of 256 has 1024 / D heads of one token, or, in grids of a block per
-// (token, head), one row whose pieces its groups of threads share and merge through LDS.
+// Joins the parts of rows whose unit several workgroups have.  D / 4 threads have a row, 4 elements each; a block of 256 has 1024 / D heads of one token,
+// or, in grids of a block per (token, head), one row whose parts its groups of threads share and merge through LDS.
 extern "C" __global__ void __launch_bounds__(256) lf_cached_combine(const LfCachedParams p) {
   constexpr int kTPR = LF_HEAD_DIM / 4, kRPB = 256 / kTPR;
   const int Hq = p.Hkv * p.group;
   const bool row_per_block = (long long)gridDim.x == (long long)p.T * Hq;
-  const int part = threadIdx.x / kTPR, per = row_per_block ? Hq : (Hq + kRPB - 1) / kRPB;
-  const int t = blockIdx.x / per, head = row_per_block ? blockIdx.x - t * per : (blockIdx.x - t * per) * kRPB + part;
+  const int group = threadIdx.x / kTPR, per = row_per_block ? Hq : (Hq + kRPB - 1) / kRPB;
+  const int t = blockIdx.x / per, head = row_per_block ? blockIdx.x - t * per : (blockIdx.x - t * per) * kRPB + group;
   const int d0 = 4 * (threadIdx.x % kTPR);
   const LfCachedRequest mine = lf_cached_request(p, __lane_id());
-  const int split = lf_cached_split(p, mine);
-  LfCachedUnit u;
-  if (!lf_cached_find(p, mine, split, -1, t, u) || u.pieces == 1) return;       // (written already)
-  if (head >= Hq) return;
+  const int share = lf_cached_share(p, lf_cached_line(p, mine), p.workgroups);
+  LfCachedPlace u;
+  if (!lf_cached_find(p, mine, -1, t, u) || head >= Hq) return;
   const int h = head / p.group, row = (t - u.r.first) * p.group + head - h * p.group, chunk = row / LF_CACHED_ROWS;
-  const long long first = u.before + (long long)(u.r.chunks - 1 - chunk) * u.pieces;
+  const int unit = (u.r.chunks - 1 - chunk) * p.Hkv + h, size = u.r.pairs + p.fixed, place = u.before + unit * size;
+  // the workgroups that have a pair of the unit
+  const int first = (place + p.fixed) / share, parts = (place + size - 1) / share - first + 1;
+  if (parts == 1) return;        // (written already)
+  const long long slot0 = ((long long)u.units + unit + first) * LF_CACHED_ROWS + row - chunk * LF_CACHED_ROWS;
   float m = LF_NEG_INF, l = 0.0f;
   lf_f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
   auto join = [&](float m2, float l2, const lf_f32x4& a2) {
@@ -530,26 +570,26 @@ extern "C" __global__ void __launch_bounds__(256) lf_cached_combine(const LfCach
     a = a * r + a2 * f;
     m = mj;
   };
-  for (int z0 = row_per_block ? 4 * part : 0; z0 < u.pieces; z0 += row_per_block ? 4 * kRPB : 4) {
+  for (int z0 = row_per_block ? 4 * group : 0; z0 < parts; z0 += row_per_block ? 4 * kRPB : 4) {
     lf_f32x2 ml[4];
     lf_f32x4 ac[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const long long slot = ((first + min(z0 + i, u.pieces - 1)) * p.Hkv + h) * LF_CACHED_ROWS + row - chunk * LF_CACHED_ROWS;
+      const long long slot = slot0 + (long long)min(z0 + i, parts - 1) * LF_CACHED_ROWS;
       ml[i] = *reinterpret_cast<const lf_f32x2*>(&p.part_ml[slot * 2]);
       ac[i] = *reinterpret_cast<const lf_f32x4*>(&p.part_acc[slot * LF_HEAD_DIM + d0]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (z0 + i < u.pieces) join(ml[i][0], ml[i][1], ac[i]);
+      if (z0 + i < parts) join(ml[i][0], ml[i][1], ac[i]);
   }
   if (row_per_block) {
     __shared__ lf_f32x4 acc[kRPB][kTPR];
     __shared__ lf_f32x2 ml[kRPB];
-    acc[part][d0 / 4] = a;
-    if (d0 == 0) ml[part] = lf_f32x2{m, l};
+    acc[group][d0 / 4] = a;
+    if (d0 == 0) ml[group] = lf_f32x2{m, l};
     __syncthreads();
-    if (part) return;
+    if (group) return;
 #pragma unroll
     for (int i = 1; i < kRPB; ++i) join(ml[i][0], ml[i][1], acc[i][d0 / 4]);
   }

@@ -331,23 +331,39 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate_bwd(const LfRo
   }
 }
 
-// dw of the parts: a workgroup has 16 columns of the queries' weight (blockIdx.y 0) or the keys', 16 threads to a column.
+// dw of the parts: a workgroup has 16 columns of the queries' weight (blockIdx.y 0) or the keys', 4 to a thread, 64 threads to a column, which take every 64th
+// part, eight loads under way at a time.  Bound by its chain of round trips: 2048 parts of 128 columns 24 us one part at a time.
 extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate_dw(const LfRotateBwdParams p) {
-  const int d = 16 * blockIdx.x + threadIdx.x % 16, part = threadIdx.x / 16;
+  constexpr int kSplit = LF_ROT_NT / 4, kLook = 8;
+  const int d = 16 * blockIdx.x + 4 * (threadIdx.x % 4), part = threadIdx.x / 4;
   const int first = blockIdx.y ? p.q_blocks : 0, count = blockIdx.y ? p.k_blocks : p.q_blocks;
-  float sum = 0.0f;
-  for (int i = part; i < count; i += 16) sum += p.parts[(long long)(first + i) * p.D + d];
-  __shared__ float sums[16][16];
-  sums[part][threadIdx.x % 16] = sum;
-  __syncthreads();
-  if (part) return;
-#pragma unroll
-  for (int i = 1; i < 16; ++i) sum += sums[i][threadIdx.x];
   void* out = blockIdx.y ? p.dk_weight : p.dq_weight;
   if (!out) return;
-  if (p.wide)
-    reinterpret_cast<float*>(out)[d] = sum;
-  else
-    reinterpret_cast<lf_elem*>(out)[d] = lf_from_float(sum);
+  lf_f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = part; i < count; i += kLook * kSplit) {
+    lf_f32x4 x[kLook];
+#pragma unroll
+    for (int u = 0; u < kLook; ++u) x[u] = *reinterpret_cast<const lf_f32x4*>(p.parts + (long long)(first + min(i + u * kSplit, count - 1)) * p.D + d);
+#pragma unroll
+    for (int u = 0; u < kLook; ++u)
+      if (i + u * kSplit < count) sum += x[u];
+  }
+  __shared__ lf_f32x4 sums[kSplit][4];
+  sums[part][threadIdx.x % 4] = sum;
+  __syncthreads();
+#pragma unroll
+  for (int n = kSplit / 2; n >= 1; n /= 2) {
+    if (part < n) sums[part][threadIdx.x % 4] += sums[part + n][threadIdx.x % 4];
+    __syncthreads();
+  }
+  if (part) return;
+  sum = sums[0][threadIdx.x];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (p.wide)
+      reinterpret_cast<float*>(out)[d + e] = sum[e];
+    else
+      reinterpret_cast<lf_elem*>(out)[d + e] = lf_from_float(sum[e]);
+  }
 }
 #endif

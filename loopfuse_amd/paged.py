@@ -70,8 +70,8 @@ class CachedParams(ctypes.Structure):
 
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "o", "k", "v", "k_scales", "v_scales", "table", "lengths", "offsets", "positions", "part_acc", "part_ml")]
                 + [(n, ctypes.c_longlong) for n in ("q_ss", "q_sh", "o_ss", "o_sh", "k_sb", "v_sb", "ks_sb", "vs_sb", "table_stride")]
-                + [(n, ctypes.c_int) for n in ("T", "B", "Hkv", "group", "room", "shift", "window", "items", "target_log2", "least", "clear")]
-                + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)])
+                + [(n, ctypes.c_int) for n in ("T", "B", "Hkv", "group")] + [("per_group", ctypes.c_uint)]
+                + [(n, ctypes.c_int) for n in ("room", "shift", "window", "fixed", "least", "workgroups", "clear")] + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)])
 
 
 @dataclasses.dataclass(frozen=True, eq=False)
@@ -721,9 +721,9 @@ def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_ta
 
 
 def cached_build(rows: float) -> tuple:
-    """(blocks of 16 rows of a wave, do a workgroup's waves have rows of their own) for so many rows of a kv head per request: up to 16, and up to 32, the four waves
-    share the keys."""
-    return (1, False) if rows <= 16 else (2, False) if rows <= 32 else (2, True)
+    """(blocks of 16 rows of a wave, do a workgroup's waves have rows of their own) for so many rows of a kv head per request: few rows by 16, the four waves sharing their
+    keys."""
+    return (1, False) if rows <= 64 else (2, True)
 
 
 def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64: bool, blocks: int, rowwaves: bool) -> lowering.KernelSpec:
@@ -731,11 +731,12 @@ def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64:
                           extra=(f"-DLF_CACHED_CB={blocks}",) + (("-DLF_CACHED_ROWWAVES=1",) if rowwaves else ()))
 
 
-def cached_split(room: int, chunks: int, Hkv: int) -> tuple:
-    """(log2 of the workgroups that the keys are cut for, least length of a piece).  ``chunks`` = of rows, at most."""
-    if room <= 128 or chunks * Hkv >= 2048:
-        return 0, 1 << 30
-    return 10, 128
+def cached_shares(units: int, keys: int, rowwaves: bool) -> tuple:
+    """(workgroups, what a unit costs besides its pairs of tiles or -1, least share of a workgroup) for at most so many units of up to ``keys`` keys that a row can see; -1:
+    each workgroup has a unit."""
+    if keys <= 1536 or (units >= 512 and (rowwaves or keys <= 3000)):
+        return units, -1, 1
+    return 512, 16, 20
 
 
 @lowering.outside_graphs
@@ -832,22 +833,21 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     P.scale, P.softcap = plan.scale, softcap or 0.0
     blocks, rowwaves = cached_build(T * P.group / B)
     rows = 16 * blocks * (4 if rowwaves else 1)
-    chunks = T * P.group // rows + min(T, B)
-    P.target_log2, P.least = cached_split(room, chunks, Hkv)
-    # (at most so many pairs of a chunk and a piece; one place more, for rows of no request, and one for the sums' rounding)
-    split = P.least < room
-    P.items = chunks + 2 + ((1 << P.target_log2) // Hkv if split else 0)
-    if P.items * Hkv * 256 >= 1 << 32 or T * P.group >= 1 << 30:
-        raise UnsupportedPlan(f"a launch for {T} rows of {Hq} heads is too large")
+    units = (T * P.group // rows + min(T, B)) * Hkv       # (at most: a chunk that is not full for each request)
+    P.workgroups, P.fixed, P.least = cached_shares(units, min(room, P.window + T) if P.window else room, rowwaves)
+    P.per_group = (-(-(1 << 32) // P.group)) & 0xffffffff
+    # (the line of all units, and rows times their division's error, are numbers in 32 bits)
+    if units * (-(-room // 32) + 64) >= 1 << 31 or T * P.group ** 2 >= 1 << 32 or T * P.group >= 1 << 30:
+        raise UnsupportedPlan(f"a launch for {T} rows of {Hq} heads, of {B} requests of up to {room} keys, is too large")
     spec = cached_spec(dtype, D, mask, softcap is not None, table.dtype == torch.int64, blocks, rowwaves)
-    steps = [(lowering.get_kernel(spec, "lf_cached"), (P.items * Hkv, 1, 1), 256)]
-    if split:
+    steps = [(lowering.get_kernel(spec, "lf_cached"), (P.workgroups, 1, 1), 256)]
+    if P.fixed >= 0:
         per = 1024 // D
         grid = T * Hq if T * Hq <= 1024 else T * -(-Hq // per)
         if grid * 256 >= 1 << 32:
             raise UnsupportedPlan(f"a launch for {T} rows of {Hq} heads is too large")
         steps.append((lowering.get_kernel(spec, "lf_cached_combine"), (grid, 1, 1), 256))
-    slots = P.items * Hkv * rows if split else 0
+    slots = (units + P.workgroups) * rows if P.fixed >= 0 else 0
     repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps]}, (slots * (D + 2), 4 * slots * D))
     res = _cached_again(q, k_pool, v_pool, table, lengths, offsets, positions, out, repeat)
     if all(a is b for a, b in zip(given, (table, lengths, offsets, positions))):
