@@ -8,10 +8,11 @@
 // row, which lf_cached_combine joins; one that a workgroup has alone is written at once.  Where units are many each workgroup takes one.
 //
 // A wave takes 32 keys at a time for LF_CACHED_CB * 16 rows, its operands straight from memory:
-//   S^T = K Q^T   : 16 keys' codes and scales are, as loaded, the first operand of the 16x16x128 product of scaled 4- and 8-bit numbers.  Q^T is
-//                   split beforehand into 8-bit numbers of 4 significant bits each whose sum it is (two of them hold bf16's 8, three fp16's 11, down
-//                   to 2^-21 of a row's largest element), with a power of two per row: the products are those of the unrounded q, and no key is
-//                   converted.  Lane (q = c, g) receives S^T[keys 4 g ... 4 g + 3][q].
+//   S^T = K Q^T   : lane (key c, g) holds the codes of the key's elements D / 4 * g ..., and their power of two: conversions of two codes at a time, exact in
+//                   the rows' type, make first operands of the 16x16x32 products of them, eight elements a step; lane (q = c, g) has the same elements
+//                   of Q.  (The products of 4- with 8-bit numbers that take powers of two along would save these conversions, q in two 8-bit parts, but
+//                   what they sum is cut off 2^-12 below the largest product, where keys with a few large elements need it.)
+//                   Lane (q = c, g) receives S^T[keys 4 g ... 4 g + 3][q].
 //   softmax       : one exponent offset per row, which may lag the running maximum by 2^LF_CACHED_LAZY.
 //   O^T += V^T P^T: a lane holds 4 keys' D / 16 neighbouring elements; two conversions and two byte permutations make the two lanes' worth of
 //                   operand of two elements out of them, and the product number i has the elements D / 16 * row + i, so that a lane ends up with
@@ -25,13 +26,9 @@
 #endif
 #define LF_CACHED_LAZY 8
 #define LF_CACHED_ROWS (16 * LF_CACHED_CB * (LF_CACHED_ROWWAVES ? 4 : 1))     /* of a workgroup */
-#define LF_CACHED_D LF_HEAD_DIM
 #define LF_CACHED_NV (LF_HEAD_DIM / 16)    /* products of O^T */
-#define LF_CACHED_QN (LF_DTYPE == 0 ? 2 : 3)
 #define LF_CACHED_OSTRIDE (LF_HEAD_DIM + 4)
 
-typedef int lf_i32x8 __attribute__((ext_vector_type(8)));
-typedef short lf_i16x2 __attribute__((ext_vector_type(2)));
 
 struct LfCachedParams {
   const lf_elem* q;            // [T, Hq, D], strides below
@@ -145,14 +142,15 @@ __device__ __forceinline__ int lf_cached_of_rows(int x) {
 }
 
 // 32 keys of a head as loaded
+typedef unsigned lf_cached_codes __attribute__((ext_vector_type(LF_HEAD_DIM / 32)));
 struct LfCachedStage {
-  lf_u32x4 k[2];
-  unsigned v[2][LF_HEAD_DIM / 32];     // D 64: 4 keys of 2 bytes, 128: of 4
+  lf_cached_codes k[2];        // of a key D / 4 neighbours
+  lf_cached_codes v[2];        // of four keys D / 16 neighbours each
   unsigned ks[2], vs[2];
 };
 
 extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedParams p) {
-  constexpr int D = LF_CACHED_D, CB = LF_CACHED_CB;
+  constexpr int D = LF_HEAD_DIM, CB = LF_CACHED_CB, NJ = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const LfCachedRequest mine = lf_cached_request(p, lane);
   const int line = lf_cached_line(p, mine), share = lf_cached_share(p, line, p.workgroups);
@@ -178,8 +176,7 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
   const bool whole = pair0 == 0 && pair1 == u.r.pairs;
 
   // ---- loads: rows of this lane, one per column block, and their positions; then the first keys
-  constexpr int kHeld = D == 128 ? 4 : 2;      // 16-byte pieces of a row
-  lf_elem8 raw[CB][kHeld];
+  lf_elem8 qb[CB][NJ];
   int pos[CB];
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
@@ -188,10 +185,9 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
     const int t_of = p.group == 1 ? at : (int)__umulhi((unsigned)at, p.per_group);
     const int t = u.r.first + t_of, head = h * p.group + at - t_of * p.group;
     pos[cb] = p.positions ? p.positions[t] : u.r.end - 1;
-    // bytes 0 ... 15 of a lane's 8-bit operand are k = 16 g ..., bytes 16 ... 31 k = 64 + 16 g ... (D 64: zeros)
-    const lf_elem* qrow = p.q + (long long)t * p.q_ss + head * p.q_sh + 16 * g;
+    const lf_elem* qrow = p.q + (long long)t * p.q_ss + head * p.q_sh + D / 4 * g;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) raw[cb][i] = *reinterpret_cast<const lf_elem8*>(qrow + (i < 2 ? 8 * i : 48 + 8 * i));
+    for (int j = 0; j < NJ; ++j) qb[cb][j] = *reinterpret_cast<const lf_elem8*>(qrow + 8 * j);
   }
   int begin = u.r.start + 32 * pair0, pairs = u.r.end > 0 ? pair1 - pair0 : 0;
   constexpr int kStep = LF_CACHED_ROWWAVES ? 1 : 4;
@@ -217,18 +213,9 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
       const unsigned char* vt = p.v + page * p.v_sb + tile * (8 * D);
       const unsigned char* kst = p.k_scales + page * p.ks_sb + tile * (D / 2);
       const unsigned char* vst = p.v_scales + page * p.vs_sb + tile * (D / 2);
-      // (D 64: lanes of g 2 and 3, whose part of Q^T is zeros, read what those of 0 and 1 do)
-      s.k[w] = *reinterpret_cast<const lf_u32x4*>(kt + c * (D / 2) + 16 * (g % (D / 32)));
-      s.ks[w] = kst[c * (D / 32) + g % (D / 32)];
-      if (D == 128) {
-        const lf_u32x4 x = *reinterpret_cast<const lf_u32x4*>(vt + 16 * lane);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) s.v[w][i] = x[i];
-      } else {
-        const lf_u32x2 x = *reinterpret_cast<const lf_u32x2*>(vt + 8 * lane);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) s.v[w][i] = x[i];
-      }
+      s.k[w] = *reinterpret_cast<const lf_cached_codes*>(kt + c * (D / 2) + D / 8 * g);
+      s.ks[w] = kst[(c * D + D / 4 * g) / 32];
+      s.v[w] = *reinterpret_cast<const lf_cached_codes*>(vt + D / 8 * lane);
       s.vs[w] = *reinterpret_cast<const unsigned*>(vst + (g * (D / 32) + c / (512 / D)) * 4);
     }
   };
@@ -272,47 +259,6 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
   issue_first();
 #endif
 
-  // ---- Q^T in 8-bit parts
-  lf_i32x8 qp[CB][LF_CACHED_QN];
-  int qscale[CB];                        // exponent of the first part, as the product takes it
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    float x[8 * kHeld], top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8 * kHeld; ++i) {
-      x[i] = lf_to_float(raw[cb][i / 8][i % 8]);
-      top = fmaxf(top, fabsf(x[i]));
-    }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    // the largest in [128, 256); an infinity makes all of the row's scores NaN (a NaN is one in 8 bits too)
-    const int exponent = (int)(__builtin_bit_cast(unsigned, top) >> 23), up = max(exponent - 7, 20);
-    qscale[cb] = exponent == 255 ? 255 : up;
-#pragma unroll
-    for (int n = 0; n < LF_CACHED_QN; ++n) {
-      const float by = __builtin_bit_cast(float, (up - 5 * n) << 23);
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        if (w >= 2 * kHeld) {
-          qp[cb][n][w] = 0;
-          continue;
-        }
-        lf_i16x2 packed = {0, 0};
-        packed = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(packed, x[4 * w], x[4 * w + 1], by, false);
-        packed = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(packed, x[4 * w + 2], x[4 * w + 3], by, true);
-        qp[cb][n][w] = __builtin_bit_cast(int, packed);
-        if (n + 1 == LF_CACHED_QN) continue;
-        // what is left of it: less than a 2^-4 th, for the next part, whose power is 2^5 times less
-        const lf_f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(__builtin_bit_cast(unsigned, packed), by, false);
-        const lf_f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(__builtin_bit_cast(unsigned, packed), by, true);
-        x[4 * w] -= a[0];
-        x[4 * w + 1] -= a[1];
-        x[4 * w + 2] -= b[0];
-        x[4 * w + 3] -= b[1];
-      }
-    }
-  }
-
 #if LF_SOFTCAP
   const float sc_in = p.scale / p.softcap;
   const float cexp = LF_LOG2E;
@@ -341,6 +287,19 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
         for (int e = 0; e < 4; ++e)
           if (t0 + 16 * w + 4 * g + e >= u.r.end) s.vs[w] &= ~(0xffu << (8 * e));
     }
+    lf_f32x4 r[CB][2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float by = __builtin_bit_cast(float, s.ks[w] << 23);
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) r[cb][w] = lf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const lf_elem8 a = lf_pool4_values(s.k[w][j], by);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) r[cb][w] = lf_mfma16(a, qb[cb][j], r[cb][w]);
+      }
+    }
     lf_elem8 va[LF_CACHED_NV];           // V^T: lane (row c, g) has keys 4 g ... of either tile, element D / 16 * c + i
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -353,7 +312,7 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
         lf_pool4_two y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const unsigned word = D == 128 ? s.v[w][e % (D / 32)] : s.v[w][e / 2];
+          const unsigned word = s.v[w][D == 128 ? e : e / 2];
           switch (D == 128 ? m : 2 * (e % 2) + m) {
             case 0: y[e] = lf_pool4_pair<0>(word, by[e]); break;
             case 1: y[e] = lf_pool4_pair<1>(word, by[e]); break;
@@ -369,20 +328,11 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
     for (int cb = 0; cb < CB; ++cb) {
       float x[8], mx = LF_NEG_INF;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const lf_i32x8 a = {(int)s.k[w][0], (int)s.k[w][1], (int)s.k[w][2], (int)s.k[w][3], 0, 0, 0, 0};
-        lf_f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int n = LF_CACHED_QN - 1; n >= 0; --n)
-          r = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qp[cb][n], r, 4, 0, 0, (int)s.ks[w], 0, qscale[cb] == 255 ? 255 : qscale[cb] - 5 * n);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float y = r[e];
+      for (int i = 0; i < 8; ++i) {
+        x[i] = r[cb][i / 4][i % 4];
 #if LF_SOFTCAP
-          y = p.softcap * lf_tanh(y * sc_in);
+        x[i] = p.softcap * lf_tanh(x[i] * sc_in);
 #endif
-          x[4 * w + e] = y;
-        }
       }
       if (partly) {
 #pragma unroll

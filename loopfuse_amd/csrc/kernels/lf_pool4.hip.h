@@ -3,10 +3,10 @@
 // A value is a code (bit 3 the sign, bits 0 ... 2 one of 0 0.5 1 1.5 2 3 4 6) times 2^(scale - 127), the scale a byte that 32 neighbours of a row
 // share, 255 for NaN.  A pool has, page by page, its heads, each with its tokens in tiles of 16: 8 D bytes of codes and D / 2 of scales a tile.
 // Within a tile the codes lie as the wave reads them that takes the tile, 64 threads (c = lane % 16, g = lane / 16):
-//   keys   : row after row, D / 2 bytes of token c; two neighbours to a byte, the first in its lower half.  Thread (c, g) reads block g of token c
-//            at 16 bytes, an operand of the matrix product with scales as it stands.  Scales: [token][block].
+//   keys   : row after row, D / 2 bytes of token c; two neighbours to a byte, the first in its lower half.  Thread (c, g) reads elements D / 4 * g ... of
+//            token c at once, 8 bytes at D 64 and 16 at 128, which share a scale.  Scales: [token][block].
 //   values : [token / 4][c][token % 4][D / 32 bytes], the bytes being elements D / 16 * c ... of the token.  Thread (c, g) reads its elements of tokens
-//            4 g ... 4 g + 3 at once, 8 bytes at D 64 and 16 at 128: a column of the transposed operand.  Scales: [token / 4][block][token % 4].
+//            4 g ... 4 g + 3 at once, as many bytes: a column of the transposed operand.  Scales: [token / 4][block][token % 4].
 #ifndef LF_POOL4_HIP_H
 #define LF_POOL4_HIP_H
 
@@ -81,8 +81,7 @@ __device__ __forceinline__ lf_pool4_two lf_pool4_pair(unsigned codes, float by) 
   return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, by, m);
 #endif
 }
-__device__ __forceinline__ lf_elem8 lf_pool4_values(unsigned codes, unsigned scale) {
-  const float by = __builtin_bit_cast(float, scale << 23);
+__device__ __forceinline__ lf_elem8 lf_pool4_values(unsigned codes, float by) {
   const lf_pool4_two a = lf_pool4_pair<0>(codes, by), b = lf_pool4_pair<1>(codes, by), c = lf_pool4_pair<2>(codes, by), d = lf_pool4_pair<3>(codes, by);
   return lf_elem8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }

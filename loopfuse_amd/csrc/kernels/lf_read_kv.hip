@@ -33,8 +33,8 @@ extern "C" __global__ void __launch_bounds__(256) lf_read_kv(const LfReadParams 
     unsigned sk, sv;
     const unsigned ck = lf_pool4_get(false, reinterpret_cast<const unsigned char*>(p.k_pool), p.k_scales, p.kp_sb, p.kp_ss, slot, p.shift, h, r8, sk);
     const unsigned cv = lf_pool4_get(true, reinterpret_cast<const unsigned char*>(p.v_pool), p.v_scales, p.vp_sb, p.vp_ss, slot, p.shift, h, r8, sv);
-    k = lf_pool4_values(ck, sk);
-    v = lf_pool4_values(cv, sv);
+    k = lf_pool4_values(ck, __builtin_bit_cast(float, sk << 23));
+    v = lf_pool4_values(cv, __builtin_bit_cast(float, sv << 23));
 #else
     const long long page = slot >> p.shift, at = slot & ((1 << p.shift) - 1);
     k = *reinterpret_cast<const lf_elem8*>(reinterpret_cast<const lf_elem*>(p.k_pool) + page * p.kp_sb + at * p.kp_ss + h * p.kp_sh + 8 * r8);
