@@ -31,6 +31,13 @@ typedef struct LfPackedPlanParamsHost {
   int32_t cap[4];          /* entries of a list: T / height + N + 2 */
 } LfPackedPlanParamsHost;
 
+/* lf_packed_positions, a thread per row */
+typedef struct LfPackedPositionsParamsHost {
+  const int32_t* offsets;  /* [N + 1] */
+  int32_t* positions;      /* [T] */
+  int32_t N, T;
+} LfPackedPositionsParamsHost;
+
 /* lf_attn_prefill_swp -DLF_PACKED=1: B = 1, Sq = Sk = T, *_sb unused, part_ml optional [Hq, T]. */
 typedef struct LfPackedAttnParamsHost {
   LfAttnParamsHost attn;

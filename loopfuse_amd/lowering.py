@@ -156,14 +156,14 @@ class KernelSpec:
         kernel = {"prefill": "lf_attn_prefill.hip", "prefill_swp": "lf_attn_prefill_swp.hip",
                   "decode": "lf_attn_decode.hip", "bwd": "lf_attn_bwd.hip", "bwd_both": "lf_attn_bwd.hip", "packed_plan": "lf_packed_plan.hip",
                   "shared_combine": "lf_shared_combine.hip", "paged_tables": "lf_paged_tables.hip", "store_kv": "lf_store_kv.hip",
-                  "rotate": "lf_rotate.hip", "read_kv": "lf_read_kv.hip", "cached": "lf_cached.hip"}[self.family]
+                  "packed_positions": "lf_packed_positions.hip", "rotate": "lf_rotate.hip", "read_kv": "lf_read_kv.hip", "cached": "lf_cached.hip"}[self.family]
         if self.family == "packed_plan":
             return ("lf_common.hip.h", "lf_packed.hip.h", kernel)
         if self.shared > 1:
             return ("lf_common.hip.h", "lf_shared.hip.h", "lf_prefill_blocks.hip.h", "lf_attn_prefill_swp.hip", kernel)
         if self.shared or self.family == "shared_combine":
             return ("lf_common.hip.h", "lf_shared.hip.h", kernel)
-        if self.family in ("paged_tables", "store_kv"):
+        if self.family in ("paged_tables", "store_kv", "packed_positions"):
             return ("lf_common.hip.h", kernel)
         if self.family in ("rotate", "read_kv", "cached"):
             return ("lf_common.hip.h", "lf_pool4.hip.h", kernel)
@@ -181,7 +181,7 @@ class KernelSpec:
     def entry(self) -> str:
         return {"prefill": "lf_attn_prefill", "prefill_swp": "lf_attn_prefill_swp", "decode": "lf_attn_decode",
                 "bwd": "lf_attn_bwd_dq", "bwd_both": "lf_attn_bwd_both", "packed_plan": "lf_packed_plan", "shared_combine": "lf_shared_combine",
-                "paged_tables": "lf_paged_tables", "store_kv": "lf_store_kv", "rotate": "lf_rotate", "read_kv": "lf_read_kv",
+                "paged_tables": "lf_paged_tables", "store_kv": "lf_store_kv", "packed_positions": "lf_packed_positions", "rotate": "lf_rotate", "read_kv": "lf_read_kv",
                 "cached": "lf_cached"}[self.family]
 
     def name(self) -> str:

@@ -37,6 +37,12 @@ class _PlanParams(ctypes.Structure):
                 ("cap", ctypes.c_int * 4)]
 
 
+class _PositionsParams(ctypes.Structure):
+    """Mirror of ``struct LfPackedPositionsParams`` in csrc/kernels/lf_packed_positions.hip."""
+
+    _fields_ = [("offsets", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("N", ctypes.c_int), ("T", ctypes.c_int)]
+
+
 class PackedAttnParams(lowering.AttnParams):
     """Mirror of ``struct LfPackedAttnParams`` in csrc/kernels/lf_packed.hip.h."""
 
@@ -109,6 +115,20 @@ def packed_layout(offsets: torch.Tensor, total: int) -> PackedLayout:
         if given is offsets:
             lowering._keep_call(lowering._call_key("l", (), (offsets,), None, (total,)), repeat, (tiles.shape[0], made.shape[0]), (repeat, caps))
     return PackedLayout(offsets, total, tiles, caps)
+
+
+@lowering.outside_graphs
+def packed_positions(layout: PackedLayout) -> torch.Tensor:
+    """int32 ``[total]``: the place of each row in its sequence, -1 for rows of none, as ``rotary.rotate_heads`` takes it.  One launch, once per batch."""
+    if not isinstance(layout, PackedLayout):
+        raise UnsupportedPlan("layout must come from packed_layout")
+    with torch.cuda.device(layout.tiles.device):
+        positions = torch.empty(layout.total, dtype=torch.int32, device=layout.tiles.device)
+        if layout.total:
+            P = _PositionsParams(layout.offsets.data_ptr(), positions.data_ptr(), layout.count, layout.total)
+            spec = lowering._spec("packed_positions", 0, 64)
+            runtime.LaunchList([(lowering.get_kernel(spec, spec.entry()), (-(-layout.total // 256), 1, 1), 256)]).launch(P)
+    return positions
 
 
 def _rows(name: str, t: torch.Tensor, layout: PackedLayout, dtype, D: Optional[int] = None) -> None:
