@@ -287,6 +287,32 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
         for (int e = 0; e < 4; ++e)
           if (t0 + 16 * w + 4 * g + e >= u.r.end) s.vs[w] &= ~(0xffu << (8 * e));
     }
+    if (partly) {
+      // values that are NaN must not meet a row that does not see them, whose weight of zero would make NaN of them: they count as zeros, and what a lane
+      // has of the rows that do see them, neighbours of one block, becomes NaN
+      unsigned long long nan[2][4], any = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) any |= nan[i / 4][i % 4] = __builtin_amdgcn_ballot_w64(((s.vs[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu);
+      if (any != 0ull) {
+        const int from = D / 4 * g / 32 * (512 / D);       // a lane that reads the scales of this one's block
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (((s.vs[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu) s.vs[i / 4] &= ~(0xffu << (8 * (i % 4)));
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+          bool sees = false;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int t = t0 + 16 * (i / 16) + i % 16;
+            sees |= ((nan[i / 16][i % 4] >> (i % 16 / 4 * 16 + from)) & 1) != 0 && t >= lo[cb] && t < hi[cb];
+          }
+          if (sees) {
+#pragma unroll
+            for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] = lf_f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+          }
+        }
+      }
+    }
     lf_f32x4 r[CB][2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {

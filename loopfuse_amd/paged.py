@@ -212,7 +212,7 @@ def pool4(pages: int, page_size: int, heads: int, D: int, dtype: torch.dtype, de
     bf16 or fp16, of the rows that it stands for.
 
     A value is 0 0.5 1 1.5 2 3 4 or 6 with a sign, times a power of two that 32 neighbours of a row share, the least one of which their largest size is below the
-    7-fold: 4.25 bits an element, off by a sixth of the largest size of its 32 at most.  Sizes beyond ``6 * 2 ** 125`` (fp16: ``6 * 2 ** 13``) count as that; 32
+    7-fold: 4.25 bits an element, off by a fifth of the largest size of its 32 at most.  Sizes beyond ``6 * 2 ** 125`` (fp16: ``6 * 2 ** 13``) count as that; 32
     neighbours with a NaN or an infinity among them are NaN.  Keys and values lie in different orders: a pool of the one is not read as the other."""
     shift = _shift(page_size)
     if shift < 4 or D not in (64, 128) or heads < 1 or pages < 0 or dtype not in lowering._DTYPE_CODE:
@@ -374,35 +374,37 @@ def read_kv(k_pool: Union[torch.Tensor, Pool4], v_pool: Union[torch.Tensor, Pool
         return done
     if dtype not in lowering._DTYPE_CODE:
         raise UnsupportedPlan("pools must be of bf16 or fp16 rows")
-    if k_pool.device.type != "cuda" and not getattr(k_pool, "is_cuda", False):
-        raise RuntimeError("loopfuse_amd: K pool is not on the GPU; the HIP path has no CPU fallback")
-    with torch.cuda.device(k_pool.device if k_pool.device.type == "cuda" else -1):
-        P = _ReadParams()
-        if isinstance(k_pool, Pool4):
-            pages, page, heads, D = _two_pools4(k_pool, v_pool, dtype, k_pool.device)
-            P.kp_sb, P.kp_ss, P.vp_sb, P.vp_ss = k_pool.codes.stride(0), k_pool.scales.stride(0), v_pool.codes.stride(0), v_pool.scales.stride(0)
-            spec = lowering._spec("read_kv", lowering._DTYPE_CODE[dtype], D, extra=("-DLF_READ4=1",))
-        else:
-            lowering._no_tangents(k_pool, v_pool)
-            _, _, heads, D, *_ = _pool("K", k_pool)
-            if D % 8:
-                raise UnsupportedPlan("head dim must be a multiple of 8")
-            pages, page, (P.kp_sb, P.kp_ss, P.kp_sh), (P.vp_sb, P.vp_ss, P.vp_sh) = _two_pools(k_pool, v_pool, dtype, k_pool.device, heads, D, False)
-            spec = lowering._spec("read_kv", lowering._DTYPE_CODE[dtype], 64)
-        _on_gpu("slots", slots, (torch.int32,), 1, k_pool.device)
-        T = slots.shape[0]
-        P.last, P.T, P.heads, P.per_head, P.shift = pages * page, T, heads, D // 8, _shift(page)
-        pieces = T * heads * (D // 8)
-        if pieces + 256 >= 1 << 32:
-            raise UnsupportedPlan(f"a launch for {T} rows of {heads} heads of {D} is too large")
-        if pieces == 0:
-            return tuple(torch.empty((T, heads, D), dtype=dtype, device=k_pool.device) for _ in range(2))
-        repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (-(-pieces // 256), 1, 1), 256)], {"kernels": [spec.entry()]}, (T, heads, D))
-        even = slots.contiguous()
-        res = _read_again(k_pool, v_pool, even, repeat)
-        if even is slots:
-            lowering._keep_call(lowering._call_key("g", parts, (slots,), None, (dtype is torch.float16,)), repeat, (T, heads, D))
-        return res
+    return _read(slots, k_pool, v_pool, parts)
+
+
+@lowering._on_device_of_first_argument
+def _read(slots, k_pool, v_pool, parts):
+    _on_gpu("slots", slots, (torch.int32,), 1)
+    P, dtype = _ReadParams(), k_pool.dtype
+    if isinstance(k_pool, Pool4):
+        pages, page, heads, D = _two_pools4(k_pool, v_pool, dtype, slots.device)
+        P.kp_sb, P.kp_ss, P.vp_sb, P.vp_ss = k_pool.codes.stride(0), k_pool.scales.stride(0), v_pool.codes.stride(0), v_pool.scales.stride(0)
+        spec = lowering._spec("read_kv", lowering._DTYPE_CODE[dtype], D, extra=("-DLF_READ4=1",))
+    else:
+        lowering._no_tangents(k_pool, v_pool)
+        _, _, heads, D, *_ = _pool("K", k_pool)
+        if D % 8:
+            raise UnsupportedPlan("head dim must be a multiple of 8")
+        pages, page, (P.kp_sb, P.kp_ss, P.kp_sh), (P.vp_sb, P.vp_ss, P.vp_sh) = _two_pools(k_pool, v_pool, dtype, slots.device, heads, D, False)
+        spec = lowering._spec("read_kv", lowering._DTYPE_CODE[dtype], 64)
+    T = slots.shape[0]
+    P.last, P.T, P.heads, P.per_head, P.shift = pages * page, T, heads, D // 8, _shift(page)
+    pieces = T * heads * (D // 8)
+    if pieces + 256 >= 1 << 32:
+        raise UnsupportedPlan(f"a launch for {T} rows of {heads} heads of {D} is too large")
+    if pieces == 0:
+        return tuple(torch.empty((T, heads, D), dtype=dtype, device=slots.device) for _ in range(2))
+    repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (-(-pieces // 256), 1, 1), 256)], {"kernels": [spec.entry()]}, (T, heads, D))
+    even = slots.contiguous()
+    res = _read_again(k_pool, v_pool, even, repeat)
+    if even is slots:
+        lowering._keep_call(lowering._call_key("g", parts, (slots,), None, (dtype is torch.float16,)), repeat, (T, heads, D))
+    return res
 
 
 def _read_again(k_pool, v_pool, slots, repeat):
@@ -821,13 +823,11 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
             raise ValueError(f"loopfuse_amd: page ids outside 0 ... {pages - 1}, or a length beyond its row of the table")
         if offsets is not None and (bool((offsets[1:] < offsets[:-1]).any()) or int(offsets[0]) < 0 or int(offsets[-1]) > T):
             raise ValueError(f"loopfuse_amd: offsets must not descend, within 0 ... {T}")
-    table = table if table.shape[1] == 0 or table.stride(1) == 1 else table.contiguous()
-    lengths, offsets, positions = (t if t is None else t.contiguous() for t in (lengths, offsets, positions))
     P = CachedParams()
     P.q_ss, P.q_sh = q.stride()[:2]
     P.o_ss, P.o_sh = (Hq * D, D) if out is None else out.stride()[:2]
     P.k_sb, P.v_sb, P.ks_sb, P.vs_sb = k_pool.codes.stride(0), v_pool.codes.stride(0), k_pool.scales.stride(0), v_pool.scales.stride(0)
-    P.table_stride, P.T, P.B, P.Hkv, P.group = table.stride(0), T, B, Hkv, Hq // Hkv
+    P.T, P.B, P.Hkv, P.group = T, B, Hkv, Hq // Hkv
     P.room, P.shift, P.clear = room, _shift(page), int(out is None)
     P.window = min(int(plan.window), 1 << 30) if mask == lowering.MASK_SLIDING else 0
     P.scale, P.softcap = plan.scale, softcap or 0.0
@@ -839,6 +839,9 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     # (the line of all units, and rows times their division's error, are numbers in 32 bits)
     if units * (-(-room // 32) + 64) >= 1 << 31 or T * P.group ** 2 >= 1 << 32 or T * P.group >= 1 << 30:
         raise UnsupportedPlan(f"a launch for {T} rows of {Hq} heads, of {B} requests of up to {room} keys, is too large")
+    table = table if table.shape[1] == 0 or table.stride(1) == 1 else table.contiguous()
+    lengths, offsets, positions = (t if t is None else t.contiguous() for t in (lengths, offsets, positions))
+    P.table_stride = table.stride(0)
     spec = cached_spec(dtype, D, mask, softcap is not None, table.dtype == torch.int64, blocks, rowwaves)
     steps = [(lowering.get_kernel(spec, "lf_cached"), (P.workgroups, 1, 1), 256)]
     if P.fixed >= 0:
