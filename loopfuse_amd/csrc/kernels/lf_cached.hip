@@ -44,7 +44,7 @@ struct LfCachedParams {
   float* part_acc;             // [slots, LF_CACHED_ROWS, D]
   float* part_ml;              // [slots, LF_CACHED_ROWS, 2]
   long long q_ss, q_sh, o_ss, o_sh;
-  long long k_sb, v_sb, ks_sb, vs_sb, table_stride;    // bytes of a page; entries
+  long long codes_sb, scales_sb, table_stride;         // bytes of a page, the same for keys and values; entries
   int T, B, Hkv, group;
   unsigned per_group;          // 2^32 / group, rounded up
   int room;                    // keys that a row of the table has room for
@@ -104,8 +104,34 @@ struct LfCachedPlace {
   int before;                  // on the line, in front of the request's units
   int units;                   // of the requests in front of it
 };
+__device__ __forceinline__ void lf_cached_take(const LfCachedRequest& r, int lane, LfCachedPlace& u) {
+  u.r.first = __builtin_amdgcn_readlane(r.first, lane);
+  u.r.n = __builtin_amdgcn_readlane(r.n, lane);
+  u.r.start = __builtin_amdgcn_readlane(r.start, lane);
+  u.r.end = __builtin_amdgcn_readlane(r.end, lane);
+  u.r.chunks = __builtin_amdgcn_readlane(r.chunks, lane);
+  u.r.pairs = __builtin_amdgcn_readlane(r.pairs, lane);
+}
 // The request that has place `place` of the line, or where that is below 0 row `row`; false: none has.
 __device__ __forceinline__ bool lf_cached_find(const LfCachedParams& p, const LfCachedRequest& mine, int place, int row, LfCachedPlace& u) {
+#if LF_CACHED_ROWWAVES
+  if (p.fixed < 0 && p.B <= 64) {
+    // a unit each: those of the request with the most keys first, as what begins last should be short
+    const int count = mine.chunks * p.Hkv, lane = __lane_id();
+    int before = 0;
+    for (int i = 0; i < p.B; ++i) {
+      const int pairs = __builtin_amdgcn_readlane(mine.pairs, i), its = __builtin_amdgcn_readlane(count, i);
+      if (pairs > mine.pairs || (pairs == mine.pairs && i < lane)) before += its;
+    }
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(place >= before && place < before + count);
+    if (hit == 0ull) return false;
+    lf_cached_take(mine, (int)__builtin_ctzll(hit), u);
+    u.b = (int)__builtin_ctzll(hit);
+    u.before = __builtin_amdgcn_readlane(before, u.b);
+    u.units = 0;
+    return true;
+  }
+#endif
   int before = 0, units = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     const LfCachedRequest r = b0 ? lf_cached_request(p, b0 + __lane_id()) : mine;
@@ -114,12 +140,7 @@ __device__ __forceinline__ bool lf_cached_find(const LfCachedParams& p, const Lf
     if (hit != 0ull) {
       const int l = (int)__builtin_ctzll(hit);
       u.b = b0 + l;
-      u.r.first = __builtin_amdgcn_readlane(r.first, l);
-      u.r.n = __builtin_amdgcn_readlane(r.n, l);
-      u.r.start = __builtin_amdgcn_readlane(r.start, l);
-      u.r.end = __builtin_amdgcn_readlane(r.end, l);
-      u.r.chunks = __builtin_amdgcn_readlane(r.chunks, l);
-      u.r.pairs = __builtin_amdgcn_readlane(r.pairs, l);
+      lf_cached_take(r, l, u);
       u.before = before + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(cost, l);
       u.units = units + __builtin_amdgcn_readlane(units_upto, l) - __builtin_amdgcn_readlane(count, l);
       return true;
@@ -149,7 +170,7 @@ struct LfCachedStage {
   unsigned ks[2], vs[2];
 };
 
-extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedParams p) {
+extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf_cached(const LfCachedParams p) {
   constexpr int D = LF_HEAD_DIM, CB = LF_CACHED_CB, NJ = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const LfCachedRequest mine = lf_cached_request(p, lane);
@@ -201,38 +222,33 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
   const lf_cint* ids = reinterpret_cast<const lf_cint*>(reinterpret_cast<unsigned long long>(p.table)) + (long long)u.b * p.table_stride;
 #endif
   struct Ids {
-    long long a, b;
+    int a, b;                  // (a pool has less than 2^31 pages)
   };
   auto tile_of = [&](int pair, int which) { return min(begin + 32 * min(pair, pairs - 1) + 16 * which, last_tile); };
-  auto fetch = [&](int pair) -> Ids { return {(long long)ids[tile_of(pair, 0) >> p.shift], (long long)ids[tile_of(pair, 1) >> p.shift]}; };
+  auto fetch = [&](int pair) -> Ids { return {(int)ids[tile_of(pair, 0) >> p.shift], (int)ids[tile_of(pair, 1) >> p.shift]}; };
+  const int k_at = c * (D / 2) + D / 8 * g, ks_at = (c * D + D / 4 * g) / 32, v_at = D / 8 * lane, vs_at = (g * (D / 32) + c / (512 / D)) * 4;
   auto issue = [&](LfCachedStage& s, int pair, const Ids& id) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const long long page = w ? id.b : id.a, tile = head_tiles + ((tile_of(pair, w) & in_page) >> 4);
-      const unsigned char* kt = p.k + page * p.k_sb + tile * (8 * D);
-      const unsigned char* vt = p.v + page * p.v_sb + tile * (8 * D);
-      const unsigned char* kst = p.k_scales + page * p.ks_sb + tile * (D / 2);
-      const unsigned char* vst = p.v_scales + page * p.vs_sb + tile * (D / 2);
-      s.k[w] = *reinterpret_cast<const lf_cached_codes*>(kt + c * (D / 2) + D / 8 * g);
-      s.ks[w] = kst[(c * D + D / 4 * g) / 32];
-      s.v[w] = *reinterpret_cast<const lf_cached_codes*>(vt + D / 8 * lane);
-      s.vs[w] = *reinterpret_cast<const unsigned*>(vst + (g * (D / 32) + c / (512 / D)) * 4);
+      const long long codes = page * p.codes_sb + tile * (8 * D), scales = page * p.scales_sb + tile * (D / 2);
+      s.k[w] = *reinterpret_cast<const lf_cached_codes*>(p.k + codes + k_at);
+      s.ks[w] = p.k_scales[scales + ks_at];
+      s.v[w] = *reinterpret_cast<const lf_cached_codes*>(p.v + codes + v_at);
+      s.vs[w] = *reinterpret_cast<const unsigned*>(p.v_scales + scales + vs_at);
     }
   };
-  // three stages rotate; loads past the end repeat the last pair, so that there is no condition on them
-  LfCachedStage s0, s1, s2;
-  Ids i0, i1, i2;
+  // two stages take turns; loads past the end repeat the last pair, so that there is no condition on them
+  LfCachedStage s0, s1;
+  Ids i0, i1;
   auto issue_first = [&]() {
     if (first >= pairs) return;
     i0 = fetch(first);
     i1 = fetch(first + kStep);
-    i2 = fetch(first + 2 * kStep);
     issue(s0, first, i0);
     issue(s1, first + kStep, i1);
-    issue(s2, first + 2 * kStep, i2);
-    i0 = fetch(first + 3 * kStep);
-    i1 = fetch(first + 4 * kStep);
-    i2 = fetch(first + 5 * kStep);
+    i0 = fetch(first + 2 * kStep);
+    i1 = fetch(first + 3 * kStep);
   };
   if (!LF_CACHED_ROWWAVES) issue_first();
   // bounds of the rows
@@ -266,11 +282,11 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
   const float cexp = p.scale * LF_LOG2E;
 #endif
   lf_f32x4 o[CB][LF_CACHED_NV];
-  float mc[CB], l_part[CB];
+  float mc[CB], l_part[CB], bad[CB];
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     mc[cb] = LF_NEG_INF;
-    l_part[cb] = 0.0f;
+    l_part[cb] = bad[cb] = 0.0f;
 #pragma unroll
     for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] = lf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -289,26 +305,23 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
     }
     if (partly) {
       // values that are NaN must not meet a row that does not see them, whose weight of zero would make NaN of them: they count as zeros, and what a lane
-      // has of the rows that do see them, neighbours of one block, becomes NaN
-      unsigned long long nan[2][4], any = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) any |= nan[i / 4][i % 4] = __builtin_amdgcn_ballot_w64(((s.vs[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu);
-      if (any != 0ull) {
+      // has of the rows that do see them, neighbours of one block, becomes NaN in the end
+      auto none = [](unsigned x) { return (~x - 0x01010101u) & x & 0x80808080u; };       // is a byte of it 255?
+      if (__builtin_amdgcn_ballot_w64((none(s.vs[0]) | none(s.vs[1])) != 0u) != 0ull) {
         const int from = D / 4 * g / 32 * (512 / D);       // a lane that reads the scales of this one's block
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const unsigned byte = 0xffu << (8 * (i & 3));
+          const bool mine = ((i < 4 ? s.vs[0] : s.vs[1]) & byte) == byte;
+          const unsigned long long all = __builtin_amdgcn_ballot_w64(mine);
+          if (mine) (i < 4 ? s.vs[0] : s.vs[1]) &= ~byte;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (((s.vs[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu) s.vs[i / 4] &= ~(0xffu << (8 * (i % 4)));
+          for (int at = 0; at < 4; ++at) {
+            const int t = t0 + 16 * (i >> 2) + 4 * at + (i & 3);
+            const bool is = ((all >> (16 * at + from)) & 1) != 0;
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-          bool sees = false;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int t = t0 + 16 * (i / 16) + i % 16;
-            sees |= ((nan[i / 16][i % 4] >> (i % 16 / 4 * 16 + from)) & 1) != 0 && t >= lo[cb] && t < hi[cb];
-          }
-          if (sees) {
-#pragma unroll
-            for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] = lf_f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            for (int cb = 0; cb < CB; ++cb)
+              if (is && t >= lo[cb] && t < hi[cb]) bad[cb] = __builtin_nanf("");
           }
         }
       }
@@ -326,30 +339,7 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
         for (int cb = 0; cb < CB; ++cb) r[cb][w] = lf_mfma16(a, qb[cb][j], r[cb][w]);
       }
     }
-    lf_elem8 va[LF_CACHED_NV];           // V^T: lane (row c, g) has keys 4 g ... of either tile, element D / 16 * c + i
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float by[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) by[e] = __builtin_bit_cast(float, ((s.vs[w] >> (8 * e)) & 0xffu) << 23);
-#pragma unroll
-      for (int m = 0; m < LF_CACHED_NV / 2; ++m) {
-        // byte m of each key: elements 2 m and 2 m + 1
-        lf_pool4_two y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned word = s.v[w][D == 128 ? e : e / 2];
-          switch (D == 128 ? m : 2 * (e % 2) + m) {
-            case 0: y[e] = lf_pool4_pair<0>(word, by[e]); break;
-            case 1: y[e] = lf_pool4_pair<1>(word, by[e]); break;
-            case 2: y[e] = lf_pool4_pair<2>(word, by[e]); break;
-            default: y[e] = lf_pool4_pair<3>(word, by[e]);
-          }
-          va[2 * m][4 * w + e] = y[e][0];
-          va[2 * m + 1][4 * w + e] = y[e][1];
-        }
-      }
-    }
+    lf_elem8 pb[CB];
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       float x[8], mx = LF_NEG_INF;
@@ -381,32 +371,54 @@ extern "C" __global__ void __launch_bounds__(256, 2) lf_cached(const LfCachedPar
         for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] *= r;
       }
       const float m_sub = (mc[cb] == LF_NEG_INF) ? 0.0f : mc[cb];
-      lf_elem8 pb;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float e = lf_exp2(__builtin_fmaf(x[i], cexp, -m_sub));
         l_part[cb] += e;
-        pb[i] = lf_from_float(e);
+        pb[cb][i] = lf_from_float(e);
+      }
+    }
+    // V^T: lane (row c, g) has keys 4 g ... of either tile, elements D / 16 * c + 2 m and + 1 of byte m of each key
+    float by[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) by[e] = __builtin_bit_cast(float, ((s.vs[e / 4] >> (8 * (e % 4))) & 0xffu) << 23);
+#pragma unroll
+    for (int m = 0; m < LF_CACHED_NV / 2; ++m) {
+      lf_elem8 va[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const unsigned word = s.v[e / 4][D == 128 ? e % 4 : e % 4 / 2];
+        lf_pool4_two y;
+        switch (D == 128 ? m : 2 * (e % 2) + m) {
+          case 0: y = lf_pool4_pair<0>(word, by[e]); break;
+          case 1: y = lf_pool4_pair<1>(word, by[e]); break;
+          case 2: y = lf_pool4_pair<2>(word, by[e]); break;
+          default: y = lf_pool4_pair<3>(word, by[e]);
+        }
+        va[0][e] = y[0];
+        va[1][e] = y[1];
       }
 #pragma unroll
-      for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] = lf_mfma16(va[i], pb, o[cb][i]);
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) o[cb][2 * m + n] = lf_mfma16(va[n], pb[cb], o[cb][2 * m + n]);
     }
   };
 
   // ---- this wave's pairs
-  for (int pr = first; pr < pairs; pr += 3 * kStep) {
+  for (int pr = first; pr < pairs; pr += 2 * kStep) {
     consume(s0, pr);
-    issue(s0, pr + 3 * kStep, i0);
-    i0 = fetch(pr + 6 * kStep);
+    issue(s0, pr + 2 * kStep, i0);
+    i0 = fetch(pr + 4 * kStep);
     if (pr + kStep >= pairs) break;
     consume(s1, pr + kStep);
-    issue(s1, pr + 4 * kStep, i1);
-    i1 = fetch(pr + 7 * kStep);
-    if (pr + 2 * kStep >= pairs) break;
-    consume(s2, pr + 2 * kStep);
-    issue(s2, pr + 5 * kStep, i2);
-    i2 = fetch(pr + 8 * kStep);
+    issue(s1, pr + 3 * kStep, i1);
+    i1 = fetch(pr + 5 * kStep);
   }
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+    for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] += bad[cb];
 
   // ---- results: lane (q = c, g) has elements D / 4 * g ... of its row, 4 groups of D / 16
   float l_wave[CB];

@@ -69,7 +69,7 @@ class CachedParams(ctypes.Structure):
     """Mirror of ``struct LfCachedParams`` in csrc/kernels/lf_cached.hip."""
 
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "o", "k", "v", "k_scales", "v_scales", "table", "lengths", "offsets", "positions", "part_acc", "part_ml")]
-                + [(n, ctypes.c_longlong) for n in ("q_ss", "q_sh", "o_ss", "o_sh", "k_sb", "v_sb", "ks_sb", "vs_sb", "table_stride")]
+                + [(n, ctypes.c_longlong) for n in ("q_ss", "q_sh", "o_ss", "o_sh", "codes_sb", "scales_sb", "table_stride")]
                 + [(n, ctypes.c_int) for n in ("T", "B", "Hkv", "group")] + [("per_group", ctypes.c_uint)]
                 + [(n, ctypes.c_int) for n in ("room", "shift", "window", "fixed", "least", "workgroups", "clear")] + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)])
 
@@ -722,10 +722,12 @@ def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_ta
     return out
 
 
-def cached_build(rows: float) -> tuple:
-    """(blocks of 16 rows of a wave, do a workgroup's waves have rows of their own) for so many rows of a kv head per request: few rows by 16, the four waves sharing their
-    keys."""
-    return (1, False) if rows <= 64 else (2, True)
+def cached_build(rows: float, all_rows: int, keys: int) -> tuple:
+    """(blocks of 16 rows of a wave, do a workgroup's waves have rows of their own) for so many rows of a kv head per request, ``all_rows`` of all heads and up to ``keys`` keys.
+    Few rows are taken 16 at a time by four waves that share their keys, many 128 at a time, where a wave converts keys and values for two blocks of rows, once there are workgroups
+    enough.  us, 16 / 128, 32/8 heads of 128: 16 requests of 2048 keys, 8 new tokens 18 / 40, 32 40 / 52, 64 73 / 65, 512 491 / 307; 4 of 8192, 32 46 / 49, 128 123 / 111; 1 of 4096,
+    128 30 / 36, 512 69 / 71; 32 of 1024, 16/16 heads of 64, 64 new 31 / 37, 128 57 / 37."""
+    return (2, True) if rows > 64 and all_rows >= (12288 if keys >= 4096 else 24576) else (1, False)
 
 
 def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64: bool, blocks: int, rowwaves: bool) -> lowering.KernelSpec:
@@ -733,12 +735,16 @@ def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64:
                           extra=(f"-DLF_CACHED_CB={blocks}",) + (("-DLF_CACHED_ROWWAVES=1",) if rowwaves else ()))
 
 
-def cached_shares(units: int, keys: int, rowwaves: bool) -> tuple:
-    """(workgroups, what a unit costs besides its pairs of tiles or -1, least share of a workgroup) for at most so many units of up to ``keys`` keys that a row can see; -1:
-    each workgroup has a unit."""
-    if keys <= 1536 or (units >= 512 and (rowwaves or keys <= 3000)):
+def cached_shares(units: int, keys: int, rows: float, rowwaves: bool, D: int) -> tuple:
+    """(workgroups, what a unit costs besides its pairs of tiles or -1, least share of a workgroup) for at most so many units of up to ``keys`` keys that a row can see, ``rows`` as
+    above; -1: each workgroup has a unit.  Shares cost a second launch, 4 us, and the begin of every part of a unit; a unit of its own the chain of its pairs, 0.6 us a
+    pair of each wave, and what the longest lasts longer than the others, which differ less where a request has many.  As many workgroups as run at once (two, or at head
+    dimension 64 three on a CU).  us, shares / units: 2 requests up to 1000, 32/8 heads of 128, 12.5 / 10.8, 64 up to 8192 65 / 76, 4 up to 100 000 58 / 620, 75 up to 2063, 8/8, 32 / 30,
+    48 up to 1029 in a window, 16/4 of 64, 21 / 17, 53 of 1681 with 75 new tokens each, 4/4, 54 / 40; in tiles of 128 rows 16 of 2048 with 64 new each, 32/8, 78 / 65, 4 of 8192 with 256
+    new each 194 / 228.  Workgroups, 512 / 768 / 1024: 64 up to 8192 64 / 66 / 73, 48 up to 12 341, 32/8 of 64, 57 / 52 / 50."""
+    if keys <= 1536 or (units >= 512 and (rows >= 64 or keys <= 2100)) or (rowwaves and units >= 256 and keys <= 4096):
         return units, -1, 1
-    return 512, 16, 20
+    return 512 if D == 128 else 768, 16, 20
 
 
 @lowering.outside_graphs
@@ -776,6 +782,8 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     lowering._check_tensor("Q", q, dtype)
     T, Hq, D = q.shape
     pages, page, Hkv, Dk = _two_pools4(k_pool, v_pool, dtype, q.device)
+    if pages > 1 and (k_pool.codes.stride(0), k_pool.scales.stride(0)) != (v_pool.codes.stride(0), v_pool.scales.stride(0)):
+        raise UnsupportedPlan("pages must be as far apart in V's pool as in K's")
     if Dk != D or Hq < 1 or Hq % Hkv:
         raise UnsupportedPlan("the pools must have Q's head dim, Hq a multiple of their heads")
     if plan.mask not in lowering._MASK_NAMES or plan.denom_add != 0.0:
@@ -826,15 +834,16 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     P = CachedParams()
     P.q_ss, P.q_sh = q.stride()[:2]
     P.o_ss, P.o_sh = (Hq * D, D) if out is None else out.stride()[:2]
-    P.k_sb, P.v_sb, P.ks_sb, P.vs_sb = k_pool.codes.stride(0), v_pool.codes.stride(0), k_pool.scales.stride(0), v_pool.scales.stride(0)
+    P.codes_sb, P.scales_sb = k_pool.codes.stride(0), k_pool.scales.stride(0)
     P.T, P.B, P.Hkv, P.group = T, B, Hkv, Hq // Hkv
     P.room, P.shift, P.clear = room, _shift(page), int(out is None)
     P.window = min(int(plan.window), 1 << 30) if mask == lowering.MASK_SLIDING else 0
     P.scale, P.softcap = plan.scale, softcap or 0.0
-    blocks, rowwaves = cached_build(T * P.group / B)
+    keys, per = min(room, P.window + T) if P.window else room, T * P.group / B
+    blocks, rowwaves = cached_build(per, T * Hq, keys)
     rows = 16 * blocks * (4 if rowwaves else 1)
     units = (T * P.group // rows + min(T, B)) * Hkv       # (at most: a chunk that is not full for each request)
-    P.workgroups, P.fixed, P.least = cached_shares(units, min(room, P.window + T) if P.window else room, rowwaves)
+    P.workgroups, P.fixed, P.least = cached_shares(units, keys, per, rowwaves, D)
     P.per_group = (-(-(1 << 32) // P.group)) & 0xffffffff
     # (the line of all units, and rows times their division's error, are numbers in 32 bits)
     if units * (-(-room // 32) + 64) >= 1 << 31 or T * P.group ** 2 >= 1 << 32 or T * P.group >= 1 << 30:

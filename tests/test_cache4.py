@@ -206,7 +206,7 @@ def test_every_pair_has_one_workgroup_and_every_part_a_place(lengths, new, windo
         rows = 16 * blocks * (4 if rowwaves else 1)
         most = (T * group // rows + min(T, B)) * Hkv
         keys = max(lengths)
-        workgroups, fixed, least = choice or paged.cached_shares(most, keys, rowwaves)
+        workgroups, fixed, least = choice or paged.cached_shares(most, keys, T * group / B, rowwaves, 128)
         requests = line_of(lengths, new, window, group, Hkv, rows, fixed)
         units = [(b, u) for b, (chunks, _, _) in enumerate(requests) for u in range(chunks * Hkv)]
         assert len(units) <= most
@@ -268,7 +268,7 @@ def test_builds_that_the_rules_choose_are_built_ahead():
             for mask in (0, 1, 2):
                 for cap in (False, True):
                     for rows in (1, 4, 16, 40, 64, 65, 500, 10000):
-                        assert paged.cached_spec(dtype, D, mask, cap, False, *paged.cached_build(rows)) in built
+                        assert paged.cached_spec(dtype, D, mask, cap, False, *paged.cached_build(rows, 32 * rows, 5000)) in built
         for D in (16, 48, 64, 96, 128, 256):
             for T in (1, 100, 100000):
                 assert rotary.kernel_spec(dtype, D, rotary.heads_per_thread(T, D)) in built

@@ -292,8 +292,8 @@ def test_attention_over_a_cache_is_the_formula(lengths, new, page, Hkv, group, D
     # other shares, and other builds
     for choice in ((97, 3, 5), (1, 0, 1), None):
         for build in ((1, False), (2, True)):
-            monkeypatch.setattr(paged, "cached_build", lambda rows: build)
-            monkeypatch.setattr(paged, "cached_shares", lambda units, keys, rowwaves: choice or (units, -1, 1))
+            monkeypatch.setattr(paged, "cached_build", lambda *a: build)
+            monkeypatch.setattr(paged, "cached_shares", lambda units, *a: choice or (units, -1, 1))
             paged._host.clear()
             check(paged.attention_cached(q, *pools, plan, table, n, offsets, positions), want, f"{choice} {build}")
     monkeypatch.undo()
@@ -318,7 +318,7 @@ def test_lengths_that_tables_have_no_room_for_and_rows_of_no_token():
 @pytest.mark.parametrize("build", [(1, False), (2, True)])
 def test_nan_in_places_that_a_row_does_not_see_stays_there(D, dtype, build, monkeypatch):
     """A key and a value that are NaN, each in one block of a token, over rows some of which see the token: causal, behind a window, and alone."""
-    monkeypatch.setattr(paged, "cached_build", lambda rows: build)
+    monkeypatch.setattr(paged, "cached_build", lambda *a: build)
     paged._host.clear()
     for mask, window in (("causal", 0), ("sliding", 20)):
         for bad in (3, 30, 58, 61):
