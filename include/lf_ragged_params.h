@@ -182,7 +182,7 @@ typedef struct LfCachedParamsHost {
   float* part_acc;         /* [units + workgroups, rows, D] */
   float* part_ml;          /* [units + workgroups, rows, 2] */
   int64_t q_ss, q_sh, o_ss, o_sh;
-  int64_t codes_sb, scales_sb, table_stride;         /* bytes of a page, of keys and values alike; entries */
+  int64_t page_bytes, table_stride;                  /* of codes, for keys and values alike, 16 times those of scales; entries */
   int32_t T, B, Hkv, group;
   uint32_t per_group;      /* 2^32 / group, rounded up */
   int32_t room, shift, window;

@@ -44,7 +44,7 @@ struct LfCachedParams {
   float* part_acc;             // [slots, LF_CACHED_ROWS, D]
   float* part_ml;              // [slots, LF_CACHED_ROWS, 2]
   long long q_ss, q_sh, o_ss, o_sh;
-  long long codes_sb, scales_sb, table_stride;         // bytes of a page, the same for keys and values; entries
+  long long page_bytes, table_stride;                  // of codes, for keys and values alike, 16 times those of scales; entries
   int T, B, Hkv, group;
   unsigned per_group;          // 2^32 / group, rounded up
   int room;                    // keys that a row of the table has room for
@@ -214,7 +214,7 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
   constexpr int kStep = LF_CACHED_ROWWAVES ? 1 : 4;
   const int first = LF_CACHED_ROWWAVES ? 0 : wave;
   const int last_tile = max(u.r.end - 1, 0) & ~15;
-  const long long head_tiles = (long long)h << (p.shift - 4);
+  const int head_tiles = h << (p.shift - 4);
   const int in_page = (1 << p.shift) - 1;
 #if LF_TABLE_I64
   const lf_cu64* ids = reinterpret_cast<const lf_cu64*>(reinterpret_cast<unsigned long long>(p.table)) + (long long)u.b * p.table_stride;
@@ -230,8 +230,7 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
   auto issue = [&](LfCachedStage& s, int pair, const Ids& id) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      const long long page = w ? id.b : id.a, tile = head_tiles + ((tile_of(pair, w) & in_page) >> 4);
-      const long long codes = page * p.codes_sb + tile * (8 * D), scales = page * p.scales_sb + tile * (D / 2);
+      const long long codes = (w ? id.b : id.a) * p.page_bytes + (head_tiles + ((tile_of(pair, w) & in_page) >> 4)) * (8 * D), scales = codes >> 4;
       s.k[w] = *reinterpret_cast<const lf_cached_codes*>(p.k + codes + k_at);
       s.ks[w] = p.k_scales[scales + ks_at];
       s.v[w] = *reinterpret_cast<const lf_cached_codes*>(p.v + codes + v_at);
@@ -381,7 +380,7 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
     // V^T: lane (row c, g) has keys 4 g ... of either tile, elements D / 16 * c + 2 m and + 1 of byte m of each key
     float by[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) by[e] = __builtin_bit_cast(float, ((s.vs[e / 4] >> (8 * (e % 4))) & 0xffu) << 23);
+    for (int e = 0; e < 8; ++e) by[e] = __builtin_bit_cast(float, e % 4 == 3 ? s.vs[e / 4] >> 1 : s.vs[e / 4] << (23 - 8 * (e % 4)));       // (only a power's exponent is looked at)
 #pragma unroll
     for (int m = 0; m < LF_CACHED_NV / 2; ++m) {
       lf_elem8 va[2];

@@ -69,7 +69,7 @@ class CachedParams(ctypes.Structure):
     """Mirror of ``struct LfCachedParams`` in csrc/kernels/lf_cached.hip."""
 
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "o", "k", "v", "k_scales", "v_scales", "table", "lengths", "offsets", "positions", "part_acc", "part_ml")]
-                + [(n, ctypes.c_longlong) for n in ("q_ss", "q_sh", "o_ss", "o_sh", "codes_sb", "scales_sb", "table_stride")]
+                + [(n, ctypes.c_longlong) for n in ("q_ss", "q_sh", "o_ss", "o_sh", "page_bytes", "table_stride")]
                 + [(n, ctypes.c_int) for n in ("T", "B", "Hkv", "group")] + [("per_group", ctypes.c_uint)]
                 + [(n, ctypes.c_int) for n in ("room", "shift", "window", "fixed", "least", "workgroups", "clear")] + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)])
 
@@ -782,8 +782,8 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     lowering._check_tensor("Q", q, dtype)
     T, Hq, D = q.shape
     pages, page, Hkv, Dk = _two_pools4(k_pool, v_pool, dtype, q.device)
-    if pages > 1 and (k_pool.codes.stride(0), k_pool.scales.stride(0)) != (v_pool.codes.stride(0), v_pool.scales.stride(0)):
-        raise UnsupportedPlan("pages must be as far apart in V's pool as in K's")
+    if pages > 1 and not k_pool.codes.stride(0) == v_pool.codes.stride(0) == 16 * k_pool.scales.stride(0) == 16 * v_pool.scales.stride(0):
+        raise UnsupportedPlan("pages must be as far apart in V's pool as in K's, those of codes 16 times as far as those of scales")
     if Dk != D or Hq < 1 or Hq % Hkv:
         raise UnsupportedPlan("the pools must have Q's head dim, Hq a multiple of their heads")
     if plan.mask not in lowering._MASK_NAMES or plan.denom_add != 0.0:
@@ -834,7 +834,7 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     P = CachedParams()
     P.q_ss, P.q_sh = q.stride()[:2]
     P.o_ss, P.o_sh = (Hq * D, D) if out is None else out.stride()[:2]
-    P.codes_sb, P.scales_sb = k_pool.codes.stride(0), k_pool.scales.stride(0)
+    P.page_bytes = k_pool.codes.stride(0)
     P.T, P.B, P.Hkv, P.group = T, B, Hkv, Hq // Hkv
     P.room, P.shift, P.clear = room, _shift(page), int(out is None)
     P.window = min(int(plan.window), 1 << 30) if mask == lowering.MASK_SLIDING else 0

@@ -151,6 +151,8 @@ CACHED = {
     "positions": dict(positions=fake((6,), I32)), "several rows without positions": dict(positions=None), "no offsets": dict(offsets=None), "out": dict(out=fake((7, 4, 128))),
     "out of one row": dict(out=fake((1, 4, 64)).expand(7, 4, 64)), "type of out": dict(out=fake((7, 4, 64), HF)), "strides": dict(q=fake((7, 4, 68))[..., :64]),
     "room beyond 2**30 keys": dict(table=fake((3, 1), I32).expand(3, (1 << 26) + 1)), "groups of 2**20 heads": dict(q=fake((1, 1, 64)).expand(7, 1 << 20, 64), k_pool=pool(9, heads=1), v_pool=pool(9, heads=1)),
+    "pages of V further apart": dict(v_pool=Pool4(fake((9, 4, 1, 512), U8)[:, :2], fake((9, 4, 1, 32), U8)[:, :2], BF)),
+    "pages of codes further apart": dict(k_pool=Pool4(fake((9, 4, 1, 512), U8)[:, :2], pool(9).scales, BF), v_pool=Pool4(fake((9, 4, 1, 512), U8)[:, :2], pool(9).scales, BF)),
     "more than can lie on a line": dict(q=fake((1, 4, 64)).expand(1 << 16, 4, 64), positions=fake((1,), I32).expand(1 << 16), table=fake((1, 1), I32).expand(1 << 16, 1 << 20), lengths=fake((1,), I32).expand(1 << 16), offsets=fake((1,), I32).expand((1 << 16) + 1)),
 }
 
@@ -162,7 +164,8 @@ def test_cached_calls_that_are_refused(case):
 
 
 def test_cached_calls_that_are_served_reach_a_launch():
-    for a in (cached(), cached(plan=AttnPlan(None, scale=0.1)), cached(plan=AttnPlan("sliding", 3, scale=0.1, softcap=-5.0)), cached(q=fake((3, 2, 64)), offsets=None, positions=None),
+    parts = Pool4(fake((9, 4, 1, 512), U8)[:, :2], fake((9, 4, 1, 32), U8)[:, :2], BF)
+    for a in (cached(), cached(k_pool=parts, v_pool=parts), cached(plan=AttnPlan(None, scale=0.1)), cached(plan=AttnPlan("sliding", 3, scale=0.1, softcap=-5.0)), cached(q=fake((3, 2, 64)), offsets=None, positions=None),
               cached(q=fake((2, 2, 64)), positions=None), cached(out=fake((7, 8, 64))[:, ::2]), cached(table=fake((3, 5), torch.int64))):
         with pytest.raises(AssertionError, match="a launch"):
             paged.attention_cached(**a)
