@@ -189,6 +189,7 @@ typedef struct LfCachedParamsHost {
   int32_t fixed;           /* what a unit costs besides its pairs of tiles of 16 keys; -1: each workgroup has a unit */
   int32_t least;           /* least share of a workgroup */
   int32_t workgroups;      /* of lf_cached; with fixed -1 the most units that there can be */
+  int32_t slots;           /* of part_acc and part_ml */
   int32_t clear;
   float scale, softcap;
 } LfCachedParamsHost;

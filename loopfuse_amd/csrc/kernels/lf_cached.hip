@@ -53,6 +53,7 @@ struct LfCachedParams {
   int fixed;                   // what a unit costs besides its pairs of tiles, in pairs; below 0: each workgroup has a unit, whatever it costs
   int least;                   // least share of a workgroup
   int workgroups;
+  int slots;                   // that there is room for, as many as the units and workgroups; offsets that descend would ask for more: those stay away
   int clear;                   // 1: zeros into rows of no request
   float scale, softcap;
 };
@@ -195,6 +196,7 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
   const int rows = u.r.n * p.group;      // of a kv head
   const int row0 = chunk * LF_CACHED_ROWS + (LF_CACHED_ROWWAVES ? wave * 16 * CB : 0);
   const bool whole = pair0 == 0 && pair1 == u.r.pairs;
+  if (!whole && (unsigned)slot >= (unsigned)p.slots) break;
 
   // ---- loads: rows of this lane, one per column block, and their positions; then the first keys
   lf_elem8 qb[CB][NJ];
@@ -546,8 +548,10 @@ extern "C" __global__ void __launch_bounds__(256) lf_cached_combine(const LfCach
   const int unit = (u.r.chunks - 1 - chunk) * p.Hkv + h, size = u.r.pairs + p.fixed, place = u.before + unit * size;
   // the workgroups that have a pair of the unit
   const int first = (place + p.fixed) / share, parts = (place + size - 1) / share - first + 1;
-  if (parts == 1) return;        // (written already)
-  const long long slot0 = ((long long)u.units + unit + first) * LF_CACHED_ROWS + row - chunk * LF_CACHED_ROWS;
+  if (parts <= 1) return;        // (written already)
+  const unsigned begin = u.units + unit + first;
+  if (begin >= (unsigned)p.slots || (unsigned)parts > (unsigned)p.slots - begin) return;
+  const long long slot0 = (long long)begin * LF_CACHED_ROWS + row - chunk * LF_CACHED_ROWS;
   float m = LF_NEG_INF, l = 0.0f;
   lf_f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
   auto join = [&](float m2, float l2, const lf_f32x4& a2) {

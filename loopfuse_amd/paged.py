@@ -71,7 +71,7 @@ class CachedParams(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "o", "k", "v", "k_scales", "v_scales", "table", "lengths", "offsets", "positions", "part_acc", "part_ml")]
                 + [(n, ctypes.c_longlong) for n in ("q_ss", "q_sh", "o_ss", "o_sh", "page_bytes", "table_stride")]
                 + [(n, ctypes.c_int) for n in ("T", "B", "Hkv", "group")] + [("per_group", ctypes.c_uint)]
-                + [(n, ctypes.c_int) for n in ("room", "shift", "window", "fixed", "least", "workgroups", "clear")] + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)])
+                + [(n, ctypes.c_int) for n in ("room", "shift", "window", "fixed", "least", "workgroups", "slots", "clear")] + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)])
 
 
 @dataclasses.dataclass(frozen=True, eq=False)
@@ -859,7 +859,8 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
         if grid * 256 >= 1 << 32:
             raise UnsupportedPlan(f"a launch for {T} rows of {Hq} heads is too large")
         steps.append((lowering.get_kernel(spec, "lf_cached_combine"), (grid, 1, 1), 256))
-    slots = (units + P.workgroups) * rows if P.fixed >= 0 else 0
+    P.slots = units + P.workgroups if P.fixed >= 0 else 0
+    slots = P.slots * rows
     repeat = lowering._Repeat(P, steps, {"kernels": [k.symbol for k, _, _ in steps]}, (slots * (D + 2), 4 * slots * D))
     res = _cached_again(q, k_pool, v_pool, table, lengths, offsets, positions, out, repeat)
     if all(a is b for a, b in zip(given, (table, lengths, offsets, positions))):

@@ -314,6 +314,17 @@ def test_lengths_that_tables_have_no_room_for_and_rows_of_no_token():
     assert int(torch.count_nonzero(paged.attention_cached(q, *pools, plan, table[:, :0], n, offsets, positions))) == 0
 
 
+def test_offsets_that_descend_stay_within_the_rows_and_the_room():
+    """Offsets that are none (they say of more rows than there are): numbers come out, and nothing beside O and the parts is written."""
+    pools, table, n, _, _ = batch([5000] * 6, [1] * 6, 16, 2, 64, BF, 1)
+    T, plan = 40, AttnPlan("causal", 0, 0.1, None, True, True)
+    q, positions = rnd((T, 4, 64), 1), torch.full((T,), 4999, dtype=torch.int32, device=DEV)
+    for offsets in ([0, 40, 0, 40, 0, 40, 0], [-5, 60, 20, 10, 50, 30, 20], [40, 30, 20, 10, 5, 3, 0], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 0, 2 ** 31 - 1, -1, 40]):
+        out = torch.zeros((T + 2, 4, 64), dtype=BF, device=DEV)
+        paged.attention_cached(q, *pools, plan, table, n, i32(offsets), positions, out=out[1:-1])
+        assert int(torch.count_nonzero(out[0])) == 0 and int(torch.count_nonzero(out[-1])) == 0
+
+
 @pytest.mark.parametrize("D,dtype", [(64, HF), (128, BF)])
 @pytest.mark.parametrize("build", [(1, False), (2, True)])
 def test_nan_in_places_that_a_row_does_not_see_stays_there(D, dtype, build, monkeypatch):
