@@ -784,6 +784,8 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     pages, page, Hkv, Dk = _two_pools4(k_pool, v_pool, dtype, q.device)
     if pages > 1 and not k_pool.codes.stride(0) == v_pool.codes.stride(0) == 16 * k_pool.scales.stride(0) == 16 * v_pool.scales.stride(0):
         raise UnsupportedPlan("pages must be as far apart in V's pool as in K's, those of codes 16 times as far as those of scales")
+    if page * Hkv * Dk >= 1 << 32:
+        raise UnsupportedPlan("a page of 2 GiB of codes or more")
     if Dk != D or Hq < 1 or Hq % Hkv:
         raise UnsupportedPlan("the pools must have Q's head dim, Hq a multiple of their heads")
     if plan.mask not in lowering._MASK_NAMES or plan.denom_add != 0.0:

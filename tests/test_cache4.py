@@ -142,6 +142,7 @@ def cached(**change):
     return a
 
 
+HUGE = Pool4(*(torch.empty((1, 2, 1 << 21, n), dtype=U8).as_subclass(OnGpu) for n in (512, 32)), BF)       # (never touched: it takes no memory)
 CACHED = {
     "fp32": dict(q=fake((7, 4, 64), F32)), "type": dict(q=fake((7, 4, 64), HF)), "dims": dict(q=fake((7, 4, 1, 64))), "head dim": dict(q=fake((7, 4, 96))), "another head dim": dict(q=fake((7, 4, 128))),
     "heads": dict(q=fake((7, 3, 64))), "mask": dict(plan=AttnPlan("other", scale=0.1)), "window": dict(plan=AttnPlan("sliding", scale=0.1)), "denominator": dict(plan=AttnPlan("causal", scale=0.1, denom_add=1.0)),
@@ -153,6 +154,7 @@ CACHED = {
     "room beyond 2**30 keys": dict(table=fake((3, 1), I32).expand(3, (1 << 26) + 1)), "groups of 2**20 heads": dict(q=fake((1, 1, 64)).expand(7, 1 << 20, 64), k_pool=pool(9, heads=1), v_pool=pool(9, heads=1)),
     "pages of V further apart": dict(v_pool=Pool4(fake((9, 4, 1, 512), U8)[:, :2], fake((9, 4, 1, 32), U8)[:, :2], BF)),
     "pages of codes further apart": dict(k_pool=Pool4(fake((9, 4, 1, 512), U8)[:, :2], pool(9).scales, BF), v_pool=Pool4(fake((9, 4, 1, 512), U8)[:, :2], pool(9).scales, BF)),
+    "a page of 2 GiB": dict(k_pool=HUGE, v_pool=HUGE, table=fake((3, 1), I32)),
     "more than can lie on a line": dict(q=fake((1, 4, 64)).expand(1 << 16, 4, 64), positions=fake((1,), I32).expand(1 << 16), table=fake((1, 1), I32).expand(1 << 16, 1 << 20), lengths=fake((1,), I32).expand(1 << 16), offsets=fake((1,), I32).expand((1 << 16) + 1)),
 }
 
