@@ -131,6 +131,14 @@ def even_weight(w):
     return w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.clone(memory_format=torch.contiguous_format)
 
 
+def even_rows(t):
+    """Rows that are read 16 bytes at a time."""
+    unit = 16 // t.element_size() if t is not None else 0
+    if t is None or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(n > 1 and s % unit for n, s in zip(t.shape[:-1], t.stride()[:-1]))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def grid(T: int, heads: int, D: int, per: int) -> tuple:
     """(groups of ``per`` heads of a token, workgroups for all tokens')."""
     chunks, groups = -(-heads // per), 256 // slots_of(D)
@@ -239,9 +247,10 @@ def _backward(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, p
 @lowering._on_device_of_first_argument
 def _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, pairs, sums):
     lowering._no_tangents(dq_out, dk_out)
-    given = dq_out, dk_out
-    dq_out, dk_out = (t if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(n > 1 and s % 8 for n, s in zip(t.shape[:-1], t.stride()[:-1])) else t.contiguous()
-                      for t in given)
+    given = dq_out, dk_out, q, k, table, q_weight, k_weight, positions
+    # (hooks of saved tensors may give them back laid out otherwise)
+    dq_out, dk_out, q, k = (even_rows(t) for t in given[:4])
+    table, q_weight, k_weight, positions = even_rows(table), even_weight(q_weight), even_weight(k_weight), positions.contiguous()
     T, Hq, D = dq_out.shape
     Hkv, dev, dtype = dk_out.shape[1], dq_out.device, dq_out.dtype
     weights = [w for w in (q_weight, k_weight) if w is not None]
@@ -279,7 +288,7 @@ def _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight
             setattr(P, name, w.data_ptr())
     repeat.launches.launch(P)
     lowering._last_launch.set(repeat.record)
-    if dq_out is given[0] and dk_out is given[1]:
+    if all(a is b for a, b in zip(given, (dq_out, dk_out, q, k, table, q_weight, k_weight, positions))):
         lowering._keep_call(lowering._call_key("R", (dq_out, dk_out, q, k, table, q_weight, k_weight), (positions,), None, (eps, pairs, *sums)), repeat, (floats,))
     return dq, dk, *dw
 

@@ -180,6 +180,24 @@ def test_gradients_of_broadcast_rows_and_of_a_sum():
     assert torch.equal(got[0], dq.sum(0, keepdim=True)) and torch.equal(got[1], dk.sum(1, keepdim=True))
 
 
+def test_saved_tensors_that_hooks_lay_out_otherwise():
+    q, k, positions, table, norm = operands(70, 4, 2, 64, 64, BF, BF, 8)
+    leaves = [t.requires_grad_() for t in (q, k, norm["q_weight"], norm["k_weight"])]
+    grads = [rnd(t.shape, 30 + i) for i, t in enumerate((q, k))]
+    y = rotary.rotate_heads(q, k, positions, table, **norm)
+    want = torch.autograd.grad(y, leaves, grads)
+
+    def apart(t):       # columns of a wider tensor that begins off the borders of 16 bytes
+        wide = torch.empty((*t.shape, 3), dtype=t.dtype, device=t.device)
+        wide[..., 1] = t.detach()
+        return wide[..., 1]
+
+    for unpack in (apart, lambda t: torch.cat((t.detach().flatten()[:1], t.detach().flatten()))[1:].view(t.shape)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = rotary.rotate_heads(q, k, positions, table, **norm)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, grads), want))
+
+
 def test_results_do_not_change_from_call_to_call():
     q, k, positions, table, norm = operands(3000, 16, 4, 128, 128, BF, F32, 9)
     leaves = [t.requires_grad_() for t in (q, k, norm["q_weight"], norm["k_weight"])]
