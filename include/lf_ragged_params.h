@@ -104,7 +104,7 @@ typedef struct LfStoreParamsHost {
   int32_t shift;           /* log2 of the tokens per page */
 } LfStoreParamsHost;
 
-/* lf_rotate: 256 / slots items per workgroup, an item being -DLF_ROT_HP heads of a token, slots = D / 16 rounded up to a power of two; the workgroups of the
+/* lf_rotate: 256 / slots items per workgroup, an item being two heads of a token, slots = D / 16 rounded up to a power of two; the workgroups of the
  * queries come first, then those of the keys and, with -DLF_ROT_STORE=1 or 2, as many of the values.  -DLF_HEAD_DIM=(16 * slots). */
 typedef struct LfRotateParamsHost {
   const void* q;           /* [T, Hq, D] */

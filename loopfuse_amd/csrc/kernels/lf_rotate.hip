@@ -8,7 +8,12 @@
 // 4 bits takes for a row does not depend on who rotated it.
 //
 // LF_ROT_SLOTS threads have a row, 16 elements each: in rotated rows 8 of either half, the partners of each other, so that no value changes threads
-// but in the norm's sum (row permutations of 16 lanes).  A group of threads takes LF_ROT_HP heads of a token, whose row of the table it reads once.
+// but in the norm's sum (row permutations of 16 lanes).  A group of threads takes two heads of a token, whose row of the table it reads once: one, two and four
+// at a time take 134 / 129 / 133 us forwards and backwards together, 75 / 75 / 79 into pages and 50 / 48 / 50 into 4 bits and back, at the sizes below.
+//
+// Bound by memory: 8192 rows of 32 and 32 heads of 128 in bf16 with norms 44 us forwards (268 MB, 6.1 TB/s) and 78 backwards with the weights' gradients (403 MB,
+// 5.2); 16384 rows of 32 and 8 heads into pages 74 (407 MB, 5.5); 8192 such rows into 4 bits 35 (177 MB, 5.1).
+// One new token each for up to 64 requests: 3.5 to 4 us, a launch and two round trips to memory.
 //
 // In 4 bits: 32 neighbours of a row share a power of two, 2^e with the least e of which their largest size is below 7 * 2^e (what lies between
 // 6 and 7 of them rounds to 6, an error no larger than that of the step from 4 to 6), and each has a sign, two bits of exponent and one of mantissa
@@ -17,9 +22,7 @@
 #ifndef LF_ROT_STORE
 #define LF_ROT_STORE 0
 #endif
-#ifndef LF_ROT_HP
-#define LF_ROT_HP 1
-#endif
+#define LF_ROT_HEADS 2
 #define LF_ROT_SLOTS (LF_HEAD_DIM / 16)    /* 1, 2, 4, 8, 16: D rounded up to a power of two */
 #define LF_ROT_NT 256
 #define LF_ROT_GROUPS (LF_ROT_NT / LF_ROT_SLOTS)
@@ -42,7 +45,7 @@ struct LfRotateParams {
   long long kp_sb, kp_ss, kp_sh, vp_sb, vp_ss, vp_sh;  // pages, tokens of a page, heads of the pools (LF_ROT_STORE 2: bytes of a page's codes, of its scales, unused)
   long long table_stride, last;                        // last: slots of a pool
   int T, Hq, Hkv, D, R, places;
-  int q_chunks, k_chunks;      // groups of LF_ROT_HP heads
+  int q_chunks, k_chunks;      // groups of LF_ROT_HEADS heads
   int q_blocks, k_blocks;      // workgroups of the queries, of the keys; the others have values
   int shift;                   // log2 of the tokens per page
   int pairs, norm, wide;       // neighbours are partners; with norms; weights in 32 bits
@@ -155,7 +158,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate(const LfRotate
   const int H = which ? p.Hkv : p.Hq, chunks = which ? p.k_chunks : p.q_chunks, R = which == 2 ? 0 : p.R;
   const unsigned item = (unsigned)block * LF_ROT_GROUPS + tid / LF_ROT_SLOTS;
   const unsigned t = item / (unsigned)chunks;
-  const int h0 = (int)(item - t * chunks) * LF_ROT_HP;
+  const int h0 = (int)(item - t * chunks) * LF_ROT_HEADS;
   const bool in = t < (unsigned)p.T && 16 * slot_of_row < p.D;
   const int position = t < (unsigned)p.T && p.positions ? p.positions[t] : 0;
   const bool live = in && position >= 0 && position < p.places;
@@ -168,9 +171,9 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate(const LfRotate
   const lf_elem* x0 = which == 0 ? p.q + (long long)t * p.q_ss : which == 1 ? p.k + (long long)t * p.k_ss : p.v + (long long)t * p.v_ss;
   const long long x_sh = which == 0 ? p.q_sh : which == 1 ? p.k_sh : p.v_sh;
   const bool wanted = live && (!LF_ROT_STORE || which == 0 || slot >= 0);
-  lf_elem8 raw[LF_ROT_HP][2];
+  lf_elem8 raw[LF_ROT_HEADS][2];
 #pragma unroll
-  for (int u = 0; u < LF_ROT_HP; ++u) {
+  for (int u = 0; u < LF_ROT_HEADS; ++u) {
     raw[u][0] = raw[u][1] = lf_elem8{};
     if (wanted && h0 + u < H) lf_rot_load(x0 + (h0 + u) * x_sh, at, raw[u]);
   }
@@ -182,7 +185,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate(const LfRotate
   __shared__ __attribute__((aligned(16))) lf_elem rows[LF_ROT_GROUPS][LF_HEAD_DIM + 8];
 #endif
 #pragma unroll
-  for (int u = 0; u < LF_ROT_HP; ++u) {
+  for (int u = 0; u < LF_ROT_HEADS; ++u) {
     float x[16];
     lf_rot_floats(raw[u], x);
     if (norm) {
@@ -258,13 +261,13 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate_bwd(const LfRo
   for (long long first = (long long)block * LF_ROT_GROUPS; first < items; first += (long long)blocks * LF_ROT_GROUPS) {
     const unsigned item = (unsigned)(first + tid / LF_ROT_SLOTS);
     const unsigned t = item / (unsigned)chunks;
-    const int h0 = (int)(item - t * chunks) * LF_ROT_HP;
+    const int h0 = (int)(item - t * chunks) * LF_ROT_HEADS;
     const bool in = inside && t < (unsigned)p.T;
     const int position = in ? p.positions[t] : -1;
     const bool live = position >= 0 && position < p.places;
-    lf_elem8 gr[LF_ROT_HP][2], xr[LF_ROT_HP][2];
+    lf_elem8 gr[LF_ROT_HEADS][2], xr[LF_ROT_HEADS][2];
 #pragma unroll
-    for (int u = 0; u < LF_ROT_HP; ++u) {
+    for (int u = 0; u < LF_ROT_HEADS; ++u) {
       gr[u][0] = gr[u][1] = xr[u][0] = xr[u][1] = lf_elem8{};
       if (live && h0 + u < H) {
         lf_rot_load(g0 + (long long)t * g_ss + (h0 + u) * g_sh, at, gr[u]);
@@ -274,7 +277,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate_bwd(const LfRo
     float c[8], s[8];
     if (live && at.turns) lf_rot_angles(p.table + (long long)position * p.table_stride, p.R, slot_of_row, c, s);
 #pragma unroll
-    for (int u = 0; u < LF_ROT_HP; ++u) {
+    for (int u = 0; u < LF_ROT_HEADS; ++u) {
       float g[16];
       lf_rot_floats(gr[u], g);
       if (live && at.turns) {

@@ -307,7 +307,7 @@ def _append(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight
     _on_gpu("slots", slots, (torch.int32,), 1, q.device)
     if slots.shape[0] != T:
         raise UnsupportedPlan(f"slots must be int32 [{T}]")
-    P, per = rotary.params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs)
+    P = rotary.params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs)
     P.v_ss, P.v_sh = v.stride()[:2]
     if isinstance(k_pool, Pool4) or isinstance(v_pool, Pool4):
         pages, page, heads, d = _two_pools4(k_pool, v_pool, q.dtype, q.device)
@@ -329,7 +329,7 @@ def _append(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight
         rotary._checked_positions(positions, P.places)
     if keys_only:
         P.q_blocks = 0
-    spec = rotary.kernel_spec(q.dtype, D, per, store)
+    spec = rotary.kernel_spec(q.dtype, D, store)
     repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (P.q_blocks + 2 * P.k_blocks, 1, 1), 256)], {"kernels": [spec.entry()]})
     given = slots, positions, q_weight, k_weight
     even = slots.contiguous(), None if keys_only else positions.contiguous(), rotary.even_weight(q_weight), rotary.even_weight(k_weight)

@@ -62,13 +62,8 @@ def slots_of(D: int) -> int:
     return 1 << (D // 16 - 1).bit_length()
 
 
-def heads_per_thread(rows: int, D: int) -> int:
-    """Heads of a token that a group of threads takes, one after the other, ``rows`` = (token, head) pairs of a launch."""
-    return 4 if rows * slots_of(D) >= 1 << 20 else 1
-
-
-def kernel_spec(dtype: torch.dtype, D: int, heads: int, store: int = 0) -> lowering.KernelSpec:
-    return lowering._spec("rotate", lowering._DTYPE_CODE[dtype], 16 * slots_of(D), extra=(f"-DLF_ROT_HP={heads}",) + ((f"-DLF_ROT_STORE={store}",) if store else ()))
+def kernel_spec(dtype: torch.dtype, D: int, store: int = 0) -> lowering.KernelSpec:
+    return lowering._spec("rotate", lowering._DTYPE_CODE[dtype], 16 * slots_of(D), extra=(f"-DLF_ROT_STORE={store}",) if store else ())
 
 
 def check_operands(q, k, positions, table, q_weight, k_weight, eps, extra=(), plain=False) -> tuple:
@@ -139,9 +134,9 @@ def even_rows(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def grid(T: int, heads: int, D: int, per: int) -> tuple:
-    """(groups of ``per`` heads of a token, workgroups for all tokens')."""
-    chunks, groups = -(-heads // per), 256 // slots_of(D)
+def grid(T: int, heads: int, D: int) -> tuple:
+    """(groups of two heads of a token, workgroups for all tokens')."""
+    chunks, groups = -(-heads // 2), 256 // slots_of(D)
     blocks = -(-T * chunks // groups)
     # (the kernels number items, up to the end of the last workgroup, in 32 bits)
     if blocks * groups >= 1 << 32 or blocks * 256 >= 1 << 32:
@@ -196,11 +191,11 @@ def _general(q, k, positions, table, q_weight, k_weight, eps, pairs):
     T, Hq, Hkv, D, R, wide = check_operands(q, k, _given(positions), table, q_weight, k_weight, eps)
     if T:
         _checked_positions(positions, table.shape[0] if table is not None else _ALL)
-    P, per = params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs)
+    P = params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs)
     if T == 0:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
     P.kp_ss, P.kp_sh = Hkv * D, D
-    spec = kernel_spec(q.dtype, D, per)
+    spec = kernel_spec(q.dtype, D)
     repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (P.q_blocks + P.k_blocks, 1, 1), 256)], {"kernels": [spec.entry()]})
     even = positions.contiguous(), even_weight(q_weight), even_weight(k_weight)
     res = _forward_again(q, k, even[0], table, *even[1:], repeat)
@@ -209,17 +204,16 @@ def _general(q, k, positions, table, q_weight, k_weight, eps, pairs):
     return res
 
 
-def params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs) -> tuple:
-    """The parameter block of a call, its pointers and what it stores still to be set, and the heads of a group of threads."""
+def params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs) -> RotateParams:
+    """The parameter block of a call, its pointers and what it stores still to be set."""
     P = RotateParams()
     P.q_ss, P.q_sh, P.k_ss, P.k_sh = *q.stride()[:2], *k.stride()[:2]
     P.T, P.Hq, P.Hkv, P.D, P.R, P.pairs, P.norm, P.wide = T, Hq, Hkv, D, R, int(pairs), int(eps is not None), int(wide)
     P.eps = 0.0 if eps is None else float(eps)
     P.places, P.table_stride = (table.shape[0], table.stride(0)) if table is not None else (_ALL, 0)
-    per = heads_per_thread(T * (Hq + Hkv), D)
-    P.q_chunks, P.q_blocks = grid(T, Hq, D, per)
-    P.k_chunks, P.k_blocks = grid(T, Hkv, D, per)
-    return P, per
+    P.q_chunks, P.q_blocks = grid(T, Hq, D)
+    P.k_chunks, P.k_blocks = grid(T, Hkv, D)
+    return P
 
 
 def _forward_again(q, k, positions, table, q_weight, k_weight, repeat):
@@ -265,12 +259,11 @@ def _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight
     P.T, P.Hq, P.Hkv, P.D, P.R, P.pairs, P.norm = T, Hq, Hkv, D, 0 if table is None else table.shape[1], int(pairs), int(eps is not None)
     P.wide, P.eps = int(bool(weights) and weights[0].dtype == torch.float32), 0.0 if eps is None else float(eps)
     P.places, P.table_stride = (table.shape[0], table.stride(0)) if table is not None else (_ALL, 0)
-    per = min(heads_per_thread(T * (Hq + Hkv), D), 2)
-    P.q_chunks, P.q_blocks = grid(T, Hq, D, per)
-    P.k_chunks, P.k_blocks = grid(T, Hkv, D, per)
+    P.q_chunks, P.q_blocks = grid(T, Hq, D)
+    P.k_chunks, P.k_blocks = grid(T, Hkv, D)
     if any(sums):
         P.q_blocks, P.k_blocks = min(P.q_blocks, BWD_BLOCKS), min(P.k_blocks, BWD_BLOCKS)
-    spec = kernel_spec(dtype, D, per)
+    spec = kernel_spec(dtype, D)
     floats = (P.q_blocks + P.k_blocks) * D if any(sums) else 0
     steps = [(lowering.get_kernel(spec, "lf_rotate_bwd"), (P.q_blocks + P.k_blocks, 1, 1), 256)]
     if any(sums):
@@ -293,7 +286,9 @@ def _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight
     return dq, dk, *dw
 
 
-BWD_BLOCKS = 1024       # workgroups that sum the weights' gradients, of the queries and of the keys
+# Workgroups that sum the weights' gradients, of the queries and of the keys: few leave some memory idle, many more parts to add.  us, 256 / 512 / 1024 / 2048, 32/8 heads of 128, both
+# launches: 4096 rows 33 / 28 / 29 / 32, 8192 58 / 47 / 48 / 51, 16384 111 / 98 / 98 / 96; 8192 of 32/32, 512 / 1024, 90 / 82.
+BWD_BLOCKS = 1024
 
 
 def _gradients(ctx, dq_out, dk_out):

@@ -275,8 +275,5 @@ def test_builds_that_the_rules_choose_are_built_ahead():
                     for rows in (1, 4, 16, 40, 64, 65, 500, 10000):
                         assert paged.cached_spec(dtype, D, mask, cap, False, *paged.cached_build(rows, 32 * rows, 5000)) in built
         for D in (16, 48, 64, 96, 128, 256):
-            for T in (1, 100, 100000):
-                assert rotary.kernel_spec(dtype, D, rotary.heads_per_thread(T, D)) in built
-                assert rotary.kernel_spec(dtype, D, min(2, rotary.heads_per_thread(T, D))) in built
-                assert rotary.kernel_spec(dtype, D, rotary.heads_per_thread(T, D), 1) in built
-                assert D not in (64, 128) or rotary.kernel_spec(dtype, D, rotary.heads_per_thread(T, D), 2) in built
+            assert rotary.kernel_spec(dtype, D) in built and rotary.kernel_spec(dtype, D, 1) in built
+            assert D not in (64, 128) or rotary.kernel_spec(dtype, D, 2) in built

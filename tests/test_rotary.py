@@ -127,17 +127,16 @@ def test_launches_beyond_32_bits(monkeypatch):
         rotary.rotate_heads(q, k, fake((1,), I32).expand(1 << 28), fake((4, 256), F32))
 
 
-def test_threads_of_a_row_and_heads_of_a_thread():
+def test_threads_of_a_row_and_groups_of_heads():
     for D in range(16, 257, 16):
         n = rotary.slots_of(D)
         assert n in (1, 2, 4, 8, 16) and 16 * n >= D > 8 * n or D == 16
     for T in (1, 7, 1000, 20000):
         for H in (1, 3, 32):
             for D in (16, 80, 128, 256):
-                for per in (1, 2, 4):
-                    chunks, blocks = rotary.grid(T, H, D, per)
-                    groups = 256 // rotary.slots_of(D)
-                    assert chunks * per >= H > (chunks - 1) * per and blocks * groups >= T * chunks > (blocks - 1) * groups
+                chunks, blocks = rotary.grid(T, H, D)
+                groups = 256 // rotary.slots_of(D)
+                assert 2 * chunks >= H > 2 * (chunks - 1) and blocks * groups >= T * chunks > (blocks - 1) * groups
 
 
 def test_the_host_module_leaves_other_operands_to_the_general_path():
