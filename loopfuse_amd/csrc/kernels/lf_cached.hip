@@ -7,17 +7,21 @@
 // waits for a longer one.  A unit that several workgroups have leaves, from each, an exponent offset, the sum of the exponentials and their sum with V per
 // row, which lf_cached_combine joins; one that a workgroup has alone is written at once.  Where units are many each workgroup takes one.
 //
-// A wave takes 32 keys at a time for LF_CACHED_CB * 16 rows, its operands straight from memory:
-//   S^T = K Q^T   : lane (key c, g) holds the codes of the key's elements D / 4 * g ..., and their power of two: conversions of two codes at a time, exact in
-//                   the rows' type, make first operands of the 16x16x32 products of them, eight elements a step; lane (q = c, g) has the same elements
-//                   of Q.  (The products of 4- with 8-bit numbers that take powers of two along would save these conversions, q in two 8-bit parts, but
-//                   what they sum is cut off 2^-12 below the largest product, where keys with a few large elements need it.)
+// A wave takes 32 keys at a time for LF_CACHED_CB * 16 rows:
+//   S^T = K Q^T   : lane (key c, g) has elements D / 4 * g ... of its key, which share a power of two: conversions of two codes at a time, exact in the rows' type, make first operands
+//                   of the 16x16x32 products of them, eight elements a step; lane (q = c, g) has the same elements of Q.  (The products of 4- with 8-bit numbers that take powers of two
+//                   along would save these conversions, q in two 8-bit parts, but what they sum is cut off 2^-12 below the largest product, where keys with a few large elements need it.)
 //                   Lane (q = c, g) receives S^T[keys 4 g ... 4 g + 3][q].
 //   softmax       : one exponent offset per row, which may lag the running maximum by 2^LF_CACHED_LAZY.
-//   O^T += V^T P^T: a lane holds 4 keys' D / 16 neighbouring elements; two conversions and two byte permutations make the two lanes' worth of
-//                   operand of two elements out of them, and the product number i has the elements D / 16 * row + i, so that a lane ends up with
-//                   D / 4 neighbouring elements of O.
-// No LDS and no barrier in the loop.  Four waves share a chunk's keys and merge through LDS, or (LF_CACHED_ROWWAVES) have a chunk's rows one each.
+//   O^T += V^T P^T: a lane holds 4 keys' D / 16 neighbouring elements; two conversions and two byte permutations make the two lanes' worth of operand of two elements out of them, and the
+//                   product number i has the elements D / 16 * row + i, so that a lane ends up with D / 4 neighbouring elements of O.
+//
+// Few rows: 16 of a kv head, a workgroup's four waves have a fourth of the pairs of tiles each and merge through LDS in the end; operands straight from memory, two pairs under way, no LDS
+// and no barrier in the loop.  Bound by memory where keys are many: 64 requests of one token up to 8192 keys, 32/8 heads of 128, 59 us and 5 for the joining (291 MB, 4.6 TB/s both); 4 up to
+// 100 000 53 and 5 (272 MB, 4.7); by one wave's chain where they are few: 2 up to 1000 10 us, of which lengths and shares 1.2, the first loads 0.9, eight pairs 4.2, the merge 0.8.
+// Many rows (LF_CACHED_ROWWAVES): 128, each wave has 32 of them over all pairs.  Of a pair two waves convert a tile of keys each, two one of values, into LDS, where all four find the operands as the
+// products take them: a fourth of the conversions, and fewer registers, so that three waves run on a SIMD.  Bound by the softmax and the products: 4 requests up to 6001 keys with up to 1000
+// new tokens 235 us (213 GFLOP, 905 TFLOP/s; each wave with keys and values of its own 257), 2 of 8192 with 4096 805 us (1025; 897).
 #ifndef LF_CACHED_CB
 #define LF_CACHED_CB 1
 #endif
@@ -165,19 +169,32 @@ __device__ __forceinline__ int lf_cached_of_rows(int x) {
 
 // 32 keys of a head as loaded
 typedef unsigned lf_cached_codes __attribute__((ext_vector_type(LF_HEAD_DIM / 32)));
+#if LF_CACHED_ROWWAVES
+struct LfCachedStage {
+  lf_cached_codes x;           // of this wave's tile: of a key D / 4 neighbours, or of four keys' values D / 16 neighbours each
+  unsigned scales;
+};
+#else
 struct LfCachedStage {
   lf_cached_codes k[2];        // of a key D / 4 neighbours
   lf_cached_codes v[2];        // of four keys D / 16 neighbours each
   unsigned ks[2], vs[2];
 };
+#endif
 
-extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf_cached(const LfCachedParams p) {
+extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES && LF_HEAD_DIM == 64 ? 4 : 3) lf_cached(const LfCachedParams p) {
   constexpr int D = LF_HEAD_DIM, CB = LF_CACHED_CB, NJ = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const LfCachedRequest mine = lf_cached_request(p, lane);
   const int line = lf_cached_line(p, mine), share = lf_cached_share(p, line, p.workgroups);
   auto inverse = [](float l) { return l == 0.0f ? 0.0f : 1.0f / l; };      // a row without a key: zeros; NaN stays
-#if !LF_CACHED_ROWWAVES
+#if LF_CACHED_ROWWAVES
+  // 32 keys as operands of the products, twice
+  __shared__ lf_elem8 kt[2][2][NJ][64];                    // [tile, step][lane]
+  __shared__ lf_elem4 vt[2][LF_CACHED_NV][2][64];          // [product][tile][lane]
+  __shared__ unsigned v_scales_of[2][2][64];               // where a value is NaN
+  __shared__ int v_nan[2][2], chunk_end[4], chunk_begin[4];
+#else
   __shared__ float red_o[4 * 16 * LF_CACHED_OSTRIDE];
   __shared__ float red_m[4][16], red_l[4][16];
 #endif
@@ -213,8 +230,6 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
     for (int j = 0; j < NJ; ++j) qb[cb][j] = *reinterpret_cast<const lf_elem8*>(qrow + 8 * j);
   }
   int begin = u.r.start + 32 * pair0, pairs = u.r.end > 0 ? pair1 - pair0 : 0;
-  constexpr int kStep = LF_CACHED_ROWWAVES ? 1 : 4;
-  const int first = LF_CACHED_ROWWAVES ? 0 : wave;
   const int last_tile = max(u.r.end - 1, 0) & ~15;
   const int head_tiles = h << (p.shift - 4);
   const int in_page = (1 << p.shift) - 1;
@@ -223,12 +238,77 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
 #else
   const lf_cint* ids = reinterpret_cast<const lf_cint*>(reinterpret_cast<unsigned long long>(p.table)) + (long long)u.b * p.table_stride;
 #endif
+  auto tile_of = [&](int pair, int which) { return min(begin + 32 * min(pair, pairs - 1) + 16 * which, last_tile); };
+  const int k_at = c * (D / 2) + D / 8 * g, ks_at = (c * D + D / 4 * g) / 32, v_at = D / 8 * lane, vs_at = (g * (D / 32) + c / (512 / D)) * 4;
+#if LF_CACHED_ROWWAVES
+  // two waves have the keys' tiles, two the values'
+  const int tile_w = wave & 1;
+  const bool has_values = wave >= 2;
+  const unsigned char* codes_of = has_values ? p.v : p.k;
+  const unsigned char* scales_of = has_values ? p.v_scales : p.k_scales;
+  const unsigned x_at = has_values ? v_at : k_at, scales_at = has_values ? vs_at : ks_at;
+  auto issue = [&](LfCachedStage& s, int pair) {
+    const int tile = tile_of(pair, tile_w);
+    const long long codes = (int)ids[tile >> p.shift] * p.page_bytes + (head_tiles + ((tile & in_page) >> 4)) * (8 * D);
+    s.x = *reinterpret_cast<const lf_cached_codes*>(codes_of + codes + x_at);
+    if (has_values)
+      s.scales = *reinterpret_cast<const unsigned*>(scales_of + (codes >> 4) + scales_at);
+    else
+      s.scales = scales_of[(codes >> 4) + scales_at];
+  };
+  // what was loaded into the operands' places
+  auto convert = [&](LfCachedStage& s, int pair, int buf) {
+    if (!has_values) {
+      const float by = __builtin_bit_cast(float, s.scales << 23);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) kt[buf][tile_w][j][lane] = lf_pool4_values(s.x[j], by);
+      return;
+    }
+    const int t0 = begin + 32 * pair + 16 * tile_w;
+    if (t0 + 16 > u.r.end) {
+      // what lies behind the last key may be anything: nothing, with weights of zero
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e >= u.r.end - t0 - 4 * g) s.scales &= ~(0xffu << (8 * e));
+    }
+    const bool nan = ((~s.scales - 0x01010101u) & s.scales & 0x80808080u) != 0u, any = __builtin_amdgcn_ballot_w64(nan) != 0ull;
+    if (any) {
+      v_scales_of[buf][tile_w][lane] = s.scales;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (((s.scales >> (8 * e)) & 0xffu) == 0xffu) s.scales &= ~(0xffu << (8 * e));
+    }
+    if (lane == 0) v_nan[buf][tile_w] = any;
+    float by[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) by[e] = __builtin_bit_cast(float, e == 3 ? s.scales >> 1 : s.scales << (23 - 8 * e));       // (only a power's exponent is looked at)
+#pragma unroll
+    for (int m = 0; m < LF_CACHED_NV / 2; ++m) {
+      lf_elem4 va[2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned word = s.x[D == 128 ? e : e / 2];
+        lf_pool4_two y;
+        switch (D == 128 ? m : 2 * (e % 2) + m) {
+          case 0: y = lf_pool4_pair<0>(word, by[e]); break;
+          case 1: y = lf_pool4_pair<1>(word, by[e]); break;
+          case 2: y = lf_pool4_pair<2>(word, by[e]); break;
+          default: y = lf_pool4_pair<3>(word, by[e]);
+        }
+        va[0][e] = y[0];
+        va[1][e] = y[1];
+      }
+      vt[buf][2 * m][tile_w][lane] = va[0];
+      vt[buf][2 * m + 1][tile_w][lane] = va[1];
+    }
+  };
+#else
+  constexpr int kStep = 4;
+  const int first = wave;
   struct Ids {
     int a, b;                  // (a pool has less than 2^31 pages)
   };
-  auto tile_of = [&](int pair, int which) { return min(begin + 32 * min(pair, pairs - 1) + 16 * which, last_tile); };
   auto fetch = [&](int pair) -> Ids { return {(int)ids[tile_of(pair, 0) >> p.shift], (int)ids[tile_of(pair, 1) >> p.shift]}; };
-  const int k_at = c * (D / 2) + D / 8 * g, ks_at = (c * D + D / 4 * g) / 32, v_at = D / 8 * lane, vs_at = (g * (D / 32) + c / (512 / D)) * 4;
   auto issue = [&](LfCachedStage& s, int pair, const Ids& id) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -239,7 +319,12 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
       s.vs[w] = *reinterpret_cast<const unsigned*>(p.v_scales + scales + vs_at);
     }
   };
-  // two stages take turns; loads past the end repeat the last pair, so that there is no condition on them
+#endif
+  // loads past the end repeat the last pair, so that there is no condition on them
+#if LF_CACHED_ROWWAVES
+  LfCachedStage s;
+#else
+  // (two stages take turns)
   LfCachedStage s0, s1;
   Ids i0, i1;
   auto issue_first = [&]() {
@@ -251,7 +336,8 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
     i0 = fetch(first + 2 * kStep);
     i1 = fetch(first + 3 * kStep);
   };
-  if (!LF_CACHED_ROWWAVES) issue_first();
+  issue_first();
+#endif
   // bounds of the rows
   int lo[CB], hi[CB];
   int least_hi = 0x7fffffff, most_hi = 0, least_lo = 0x7fffffff, most_lo = 0;
@@ -267,13 +353,21 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
   least_hi = lf_cached_of_rows<false>(least_hi);
   if (LF_MASK == 2) most_lo = lf_cached_of_rows<true>(most_lo);
 #if LF_CACHED_ROWWAVES
-  // (where a chunk's rows differ a wave leaves out what none of its own sees)
-  {
-    const int end = min(begin + 32 * pairs, lf_cached_of_rows<true>(most_hi));
-    if (LF_MASK == 2) begin = max(begin, lf_cached_of_rows<false>(least_lo) & ~31);
-    pairs = end > begin ? (end - begin + 31) >> 5 : 0;
+  // (what no row of the chunk sees is left out)
+  const int wave_end = lf_cached_of_rows<true>(most_hi), wave_begin = LF_MASK == 2 ? lf_cached_of_rows<false>(least_lo) : 0;
+  if (lane == 0) {
+    chunk_end[wave] = wave_end;
+    chunk_begin[wave] = wave_begin;
   }
-  issue_first();
+  __syncthreads();
+  {
+    const int ends = min(begin + 32 * pairs, max(max(chunk_end[0], chunk_end[1]), max(chunk_end[2], chunk_end[3])));
+    if (LF_MASK == 2) begin = max(begin, min(min(chunk_begin[0], chunk_begin[1]), min(chunk_begin[2], chunk_begin[3])) & ~31);
+    pairs = ends > begin ? (ends - begin + 31) >> 5 : 0;
+    pairs = __builtin_amdgcn_readfirstlane(pairs);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+  }
+  if (pairs > 0) issue(s, 0);
 #endif
 
 #if LF_SOFTCAP
@@ -293,9 +387,16 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
   }
 
   // ---- 32 keys
+#if LF_CACHED_ROWWAVES
+  auto consume = [&](int buf, int pair) {
+#else
   auto consume = [&](LfCachedStage& s, int pair) {
+#endif
     const int t0 = begin + 32 * pair;
     const bool partly = t0 < most_lo || t0 + 32 > least_hi;      // some row does not see all of them
+#if LF_CACHED_ROWWAVES
+    const int nan0 = v_nan[buf][0], nan1 = v_nan[buf][1];
+#else
     if (t0 + 32 > u.r.end) {
       // what lies behind the last key may be anything: nothing, with weights of zero
 #pragma unroll
@@ -327,58 +428,93 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
         }
       }
     }
+#endif
     lf_f32x4 r[CB][2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
+#if !LF_CACHED_ROWWAVES
       const float by = __builtin_bit_cast(float, s.ks[w] << 23);
+#endif
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) r[cb][w] = lf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
+#if LF_CACHED_ROWWAVES
+        const lf_elem8 a = kt[buf][w][j][lane];
+#else
         const lf_elem8 a = lf_pool4_values(s.k[w][j], by);
+#endif
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) r[cb][w] = lf_mfma16(a, qb[cb][j], r[cb][w]);
+      }
+    }
+    float top[CB];
+    bool grows = false;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+#if LF_SOFTCAP
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[cb][i / 4][i % 4] = p.softcap * lf_tanh(r[cb][i / 4][i % 4] * sc_in);
+#endif
+      if (partly) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = 16 * (i / 4) + i % 4;       // from t0 + 4 g on
+          if (j >= hi[cb] - t0 - 4 * g || (LF_MASK == 2 && j < lo[cb] - t0 - 4 * g)) r[cb][i / 4][i % 4] = LF_NEG_INF;
+        }
+      }
+      float mx = LF_NEG_INF;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, r[cb][i / 4][i % 4]);
+      top[cb] = mx * cexp;
+      grows = grows || top[cb] > mc[cb] + (float)LF_CACHED_LAZY;
+    }
+    if (__builtin_amdgcn_ballot_w64(grows) != 0ull) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        float mq = fmaxf(top[cb], __shfl_xor(top[cb], 16, 64));
+        mq = fmaxf(mq, __shfl_xor(mq, 32, 64));
+        const float m_new = fmaxf(mc[cb], mq);
+        const float f = (m_new == LF_NEG_INF) ? 1.0f : lf_exp2(mc[cb] - m_new);
+        mc[cb] = m_new;
+        l_part[cb] *= f;
+#pragma unroll
+        for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] *= f;
       }
     }
     lf_elem8 pb[CB];
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
-      float x[8], mx = LF_NEG_INF;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = r[cb][i / 4][i % 4];
-#if LF_SOFTCAP
-        x[i] = p.softcap * lf_tanh(x[i] * sc_in);
-#endif
-      }
-      if (partly) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = t0 + 16 * (i / 4) + 4 * g + i % 4;
-          if (j < lo[cb] || j >= hi[cb]) x[i] = LF_NEG_INF;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
-      mx *= cexp;
-      if (__builtin_amdgcn_ballot_w64(mx > mc[cb] + (float)LF_CACHED_LAZY) != 0ull) {
-        float mq = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mq = fmaxf(mq, __shfl_xor(mq, 32, 64));
-        const float m_new = fmaxf(mc[cb], mq);
-        const float r = (m_new == LF_NEG_INF) ? 1.0f : lf_exp2(mc[cb] - m_new);
-        mc[cb] = m_new;
-        l_part[cb] *= r;
-#pragma unroll
-        for (int i = 0; i < LF_CACHED_NV; ++i) o[cb][i] *= r;
-      }
       const float m_sub = (mc[cb] == LF_NEG_INF) ? 0.0f : mc[cb];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = lf_exp2(__builtin_fmaf(x[i], cexp, -m_sub));
+        const float e = lf_exp2(__builtin_fmaf(r[cb][i / 4][i % 4], cexp, -m_sub));
         l_part[cb] += e;
         pb[cb][i] = lf_from_float(e);
       }
     }
+#if LF_CACHED_ROWWAVES
+#pragma unroll
+    for (int i = 0; i < LF_CACHED_NV; ++i) {
+      const lf_elem4 a = vt[buf][i][0][lane], b = vt[buf][i][1][lane];
+      const lf_elem8 va = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) o[cb][i] = lf_mfma16(va, pb[cb], o[cb][i]);
+    }
+    if ((__builtin_amdgcn_readfirstlane(nan0 | nan1)) != 0) {
+      // values that are NaN must not meet a row that does not see them, whose weight of zero would make NaN of them: they count as zeros, and what a lane
+      // has of the rows that do see them, neighbours of one block, becomes NaN in the end
+      const int from = D / 4 * g / 32 * (512 / D);       // a lane that reads the scales of this one's block
+#pragma unroll 1
+      for (int i = 0; i < 32; ++i) {
+        const int w = i >> 4, at = i & 15, t = t0 + i;
+        const bool is = v_nan[buf][w] != 0 && ((v_scales_of[buf][w][16 * (at >> 2) + from] >> (8 * (at & 3))) & 0xffu) == 0xffu;
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+          if (is && t >= lo[cb] && t < hi[cb]) bad[cb] = __builtin_nanf("");
+      }
+    }
+#else
     // V^T: lane (row c, g) has keys 4 g ... of either tile, elements D / 16 * c + 2 m and + 1 of byte m of each key
     float by[8];
 #pragma unroll
@@ -404,8 +540,32 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) o[cb][2 * m + n] = lf_mfma16(va[n], pb[cb], o[cb][2 * m + n]);
     }
+#endif
   };
 
+#if LF_CACHED_ROWWAVES
+  // ---- the workgroup's pairs: while a pair's products are formed the next one's operands go into the other places, and the one's after that are under way
+  auto meet = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  auto step = [&](int buf, int pr) {
+    convert(s, pr + 1, buf ^ 1);
+    issue(s, pr + 2);
+    const int t0 = begin + 32 * pr;
+    if (t0 < wave_end && (LF_MASK != 2 || t0 + 32 > wave_begin)) consume(buf, pr);
+    meet();
+  };
+  if (pairs > 0) {
+    convert(s, 0, 0);
+    issue(s, 1);
+    meet();
+    for (int pr = 0; pr < pairs; pr += 2) {
+      step(0, pr);
+      if (pr + 1 >= pairs) break;
+      step(1, pr + 1);
+    }
+  } else {
+    __syncthreads();       // (the chunk's bounds are read)
+  }
+#else
   // ---- this wave's pairs
   for (int pr = first; pr < pairs; pr += 2 * kStep) {
     consume(s0, pr);
@@ -416,6 +576,7 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES ? 2 : 3) lf
     issue(s1, pr + 3 * kStep, i1);
     i1 = fetch(pr + 5 * kStep);
   }
+#endif
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb)
 #pragma unroll

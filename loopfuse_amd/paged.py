@@ -724,10 +724,11 @@ def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_ta
 
 def cached_build(rows: float, all_rows: int, keys: int) -> tuple:
     """(blocks of 16 rows of a wave, do a workgroup's waves have rows of their own) for so many rows of a kv head per request, ``all_rows`` of all heads and up to ``keys`` keys.
-    Few rows are taken 16 at a time by four waves that share their keys, many 128 at a time, where a wave converts keys and values for two blocks of rows, once there are workgroups
-    enough.  us, 16 / 128, 32/8 heads of 128: 16 requests of 2048 keys, 8 new tokens 18 / 40, 32 40 / 52, 64 73 / 65, 512 491 / 307; 4 of 8192, 32 46 / 49, 128 123 / 111; 1 of 4096,
-    128 30 / 36, 512 69 / 71; 32 of 1024, 16/16 heads of 64, 64 new 31 / 37, 128 57 / 37."""
-    return (2, True) if rows > 64 and all_rows >= (12288 if keys >= 4096 else 24576) else (1, False)
+    Few rows are taken 16 at a time by four waves that share their keys, many 128 at a time, whose keys and values are converted once, where there are workgroups or keys enough
+    for that.  us, 16 / 128: 32/8 heads of 128, 16 requests of 2048 keys, 64 new tokens each 66 / 70, 96 94 / 90, 512 476 / 276; 4 of 8192, 64 67 / 73, 96 89 / 90, 128 115 / 97; 1 of 32 768,
+    256 233 / 182; 8 of 4096, 64 63 / 71, 128 115 / 108; 16 of 4001, 33 53 / 67; 1 of 1000, all 45 / 42; 32 of 700, 64 67 / 44; 16/16 of 64, 32 of 1024, 64 31 / 40, 128 59 / 41."""
+    many = all_rows >= (32768 if keys <= 1536 else 49152) or all_rows * keys >= 10 ** 8
+    return (2, True) if rows > 64 and many else (1, False)
 
 
 def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64: bool, blocks: int, rowwaves: bool) -> lowering.KernelSpec:
@@ -738,11 +739,17 @@ def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64:
 def cached_shares(units: int, keys: int, rows: float, rowwaves: bool, D: int) -> tuple:
     """(workgroups, what a unit costs besides its pairs of tiles or -1, least share of a workgroup) for at most so many units of up to ``keys`` keys that a row can see, ``rows`` as
     above; -1: each workgroup has a unit.  Shares cost a second launch, 4 us, and the begin of every part of a unit; a unit of its own the chain of its pairs, 0.6 us a
-    pair of each wave, and what the longest lasts longer than the others, which differ less where a request has many.  As many workgroups as run at once (two, or at head
-    dimension 64 three on a CU).  us, shares / units: 2 requests up to 1000, 32/8 heads of 128, 12.5 / 10.8, 64 up to 8192 65 / 76, 4 up to 100 000 58 / 620, 75 up to 2063, 8/8, 32 / 30,
-    48 up to 1029 in a window, 16/4 of 64, 21 / 17, 53 of 1681 with 75 new tokens each, 4/4, 54 / 40; in tiles of 128 rows 16 of 2048 with 64 new each, 32/8, 78 / 65, 4 of 8192 with 256
-    new each 194 / 228.  Workgroups, 512 / 768 / 1024: 64 up to 8192 64 / 66 / 73, 48 up to 12 341, 32/8 of 64, 57 / 52 / 50."""
-    if keys <= 1536 or (units >= 512 and (rows >= 64 or keys <= 2100)) or (rowwaves and units >= 256 and keys <= 4096):
+    pair of each wave (1.2 us in 128 rows), and what the longest lasts longer than the others, which differ less where a request has many; under a causal mask the first of a request's new tokens
+    have fewer keys than shares are cut for.  As many workgroups as run at once: two on a CU (16 rows, head dimension 128), three (its 128 rows; 16 rows of 64), four.
+    us, shares / units: 16 rows, 2 requests up to 1000, 32/8 heads of 128, 12.5 / 10.8, 64 up to 8192 65 / 76, 4 up to 100 000 58 / 620, 75 up to 2063, 8/8, 32 / 30, 48 up to 1029 in a window,
+    16/4 of 64, 21 / 17, 53 of 1681 with 75 new tokens each, 4/4, 54 / 40; workgroups, 512 / 768 / 1024: 64 up to 8192 64 / 66 / 73, 48 up to 12 341, 32/8 of 64, 57 / 52 / 50.  128 rows, 32/8 of
+    128: 16 of 2048 with 128 new each 108 / 92, 8 of 4096 with 128 108 / 147, 4 up to 6001 with up to 1000 286 / 235, 1 of 12 000 with 1000 231 / 407, 1 of 32 768 with 3500 1820 / 2341, with 6144
+    2965 / 2854; workgroups, 512 / 768 / 1024: 4 of 8192 with 256 new each 195 / 161 / 199."""
+    if rowwaves:
+        if units >= (256 if keys <= 1536 else 512 if keys <= 4096 else 768 if keys <= 12288 else 1536):
+            return units, -1, 1
+        return 768 if D == 128 else 1024, 8, 20
+    if keys <= 1536 or (units >= 512 and (rows >= 64 or keys <= 2100)):
         return units, -1, 1
     return 512 if D == 128 else 768, 16, 20
 
