@@ -16,6 +16,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -608,6 +610,90 @@ PyObject* rotate_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The gradients of rotate_heads as a node of the graph: a node in Python takes 19 us more of the host (6001 rows of 16 and 4 heads of 64 with gradients 95 / 76 us, 26 of them the kernels; the rest is torch's
+// engine).  Where its launches are not kept, or what it returns
+// is to be part of a graph, it calls `differentiate` (rotary._differentiate).
+PyObject* differentiate = nullptr;
+struct RotateNode : torch::autograd::Node {
+  torch::autograd::SavedVariable q, k, table, q_weight, k_weight, positions;
+  bool norm = false, pairs = false;
+  double eps = 0.0;
+
+  std::string name() const override { return "RotateHeadsBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (torch::autograd::SavedVariable* v : {&q, &k, &table, &q_weight, &k_weight, &positions}) v->reset_data();
+  }
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    at::Tensor saved[6];
+    {
+      std::lock_guard<std::mutex> lock(mutex_);
+      const torch::autograd::SavedVariable* from[] = {&q, &k, &table, &q_weight, &k_weight, &positions};
+      for (int i = 0; i < 6; ++i) saved[i] = from[i]->unpack();
+    }
+    for (int i = 0; i < 2; ++i)
+      if (!grads[i].defined()) grads[i] = input_metadata(i).zeros_like();
+    pybind11::gil_scoped_acquire gil;
+    auto wrap = [](const at::Tensor& t) { return t.defined() ? THPVariable_Wrap(t) : none(); };
+    PyObject* a[12] = {wrap(grads[0]), wrap(grads[1]), wrap(saved[0]), wrap(saved[1]), wrap(saved[2]), wrap(saved[3]), wrap(saved[4]), wrap(saved[5]),
+                       norm ? PyFloat_FromDouble(eps) : none(), PyBool_FromLong(pairs), PyBool_FromLong(saved[3].defined() && task_should_compute_output(2)),
+                       PyBool_FromLong(saved[4].defined() && task_should_compute_output(3))};
+    PyObject* r = nullptr;
+    bool made_all = true;
+    for (PyObject* x : a) made_all = made_all && x;
+    if (made_all) {
+      if (c10::GradMode::is_enabled())
+        r = none();
+      else
+        r = rotate_backward(nullptr, a, 12);
+      if (r == Py_None) {
+        Py_DECREF(r);
+        r = PyObject_Vectorcall(differentiate, a, 12, nullptr);
+      }
+    }
+    for (PyObject* x : a) Py_XDECREF(x);
+    torch::autograd::variable_list res(4);
+    if (r)
+      for (int i = 0; i < 4; ++i) {
+        PyObject* x = PyTuple_GET_ITEM(r, i);
+        if (x != Py_None) res[i] = THPVariable_Unpack(x);
+      }
+    Py_XDECREF(r);
+    if (!r) {
+      python_error e;
+      e.persist();
+      throw std::move(e);
+    }
+    return res;
+  }
+};
+
+// rotate_train(q, k, table, q_weight, k_weight, positions, eps, pairs, differentiate) -> (q, k), with gradients
+PyObject* rotate_train(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!takes(n, 9)) return nullptr;
+  if (!plain(a[0]) || (a[6] != Py_None && !PyFloat_CheckExact(a[6])) || !PyBool_Check(a[7]) || c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return none();
+  PyObject* out = rotate_heads(nullptr, a, 8);
+  if (!out || out == Py_None) return out;
+  pybind11::object owned = pybind11::reinterpret_steal<pybind11::object>(out);
+  if (!differentiate) Py_INCREF(differentiate = a[8]);
+  at::Tensor in[6];
+  for (int i = 0; i < 6; ++i)
+    if (a[i] != Py_None) in[i] = THPVariable_Unpack(a[i]);
+  const std::shared_ptr<RotateNode> node(new RotateNode(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(in[0], in[1], in[3], in[4]));
+  node->norm = a[6] != Py_None;
+  node->eps = node->norm ? PyFloat_AS_DOUBLE(a[6]) : 0.0;
+  node->pairs = a[7] == Py_True;
+  torch::autograd::SavedVariable* to[] = {&node->q, &node->k, &node->table, &node->q_weight, &node->k_weight, &node->positions};
+  for (int i = node->norm ? 0 : 2; i < 6; ++i) *to[i] = torch::autograd::SavedVariable(in[i], false);
+  for (int i = 0; i < 2; ++i) torch::autograd::set_history(THPVariable_Unpack(PyTuple_GET_ITEM(out, i)), node);
+  return owned.release().ptr();
+  END_HANDLE_TH_ERRORS
+}
+
 // append_kv(q, k, v, k_pool, v_pool, k_scales, v_scales, table, q_weight, k_weight, slots, positions, eps, pairs) -> q, without positions True; the pools are those
 // of 16-bit rows, or the codes with their scales
 PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -713,7 +799,7 @@ PyObject* attention_cached(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define LF_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LF_FAST(setup), LF_FAST(key), LF_FAST(keep), {"clear", clear, METH_NOARGS, nullptr}, {"size", size, METH_NOARGS, nullptr},
                          LF_FAST(elsewhere), LF_FAST(packed_layout), LF_FAST(extend_tables), LF_FAST(store_kv), LF_FAST(attention_shared), LF_FAST(attention_packed), LF_FAST(attention_packed_backward),
-                         LF_FAST(rotate_heads), LF_FAST(rotate_backward), LF_FAST(append_kv), LF_FAST(read_kv), LF_FAST(attention_cached),
+                         LF_FAST(rotate_heads), LF_FAST(rotate_backward), LF_FAST(rotate_train), LF_FAST(append_kv), LF_FAST(read_kv), LF_FAST(attention_cached),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lf_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -167,6 +167,9 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
         if isinstance(table, torch.Tensor) and table.requires_grad:
             raise UnsupportedPlan("no gradient of the table is formed")
+        done = _host.rotate_train(q, k, table, q_weight, k_weight, positions, eps, bool(pairs), _differentiate)      # (neither under capture nor with tangents)
+        if done is not None:
+            return done
         from . import packed
         packed.refuse_outside_capture(operands, "Q, K and the weights")
         lowering._no_tangents(*operands)      # (not to be seen inside)
@@ -298,6 +301,12 @@ def _gradients(ctx, dq_out, dk_out):
 
 
 _gradients_once = torch.autograd.function.once_differentiable(_gradients)
+_backward_once = torch.autograd.function.once_differentiable(lambda ctx, dq_out, dk_out, rest: _backward(dq_out, dk_out, *rest))
+
+
+def _differentiate(dq_out, dk_out, q, k, table, q_weight, k_weight, positions, eps, pairs, of_q_weight, of_k_weight):
+    """As ``_gradients``, for the host module's own node."""
+    return _backward_once(None, dq_out, dk_out, (q, k, positions, table, q_weight, k_weight, eps, pairs, (of_q_weight, of_k_weight)))
 
 
 class _Rotate(torch.autograd.Function):

@@ -217,6 +217,78 @@ def test_gradients_are_not_differentiated_again():
         torch.autograd.grad(dq.float().sum(), q)
 
 
+def test_gradients_of_repeated_calls():
+    """The graph's node that repeated calls make gives what the first call's does, and behaves as it in what autograd asks of a node."""
+    q, k, positions, table, norm = operands(70, 4, 2, 64, 32, BF, BF, 8)
+    leaves = [t.requires_grad_() for t in (q, k, norm["q_weight"], norm["k_weight"])]
+    grads = [rnd(t.shape, 30 + i) for i, t in enumerate((q, k))]
+
+    def call(first=False, **change):
+        if first:
+            rotary._host.clear()
+        return rotary.rotate_heads(q, k, positions, table, **{**norm, **change})
+
+    first = call(True)
+    want = torch.autograd.grad(first, leaves, grads)
+    call(), torch.autograd.grad(call(), leaves, grads)
+    y = call()
+    assert y[0].grad_fn is y[1].grad_fn and y[0].grad_fn.name() == "RotateHeadsBackward" != first[0].grad_fn.name() and torch.equal(y[0], first[0]) and torch.equal(y[1], first[1])
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, grads, retain_graph=True), want))
+    torch.autograd.grad(y, leaves, grads)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, leaves, grads)
+    # one result alone, some of the leaves
+    for i in range(2):
+        want_i = torch.autograd.grad(call(True)[i], leaves, grads[i], allow_unused=True)
+        call(), torch.autograd.grad(call(), leaves, grads)
+        got = torch.autograd.grad(call()[i], leaves, grads[i], allow_unused=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want_i))
+        got, = torch.autograd.grad(call()[i], leaves[2 + i], grads[i])
+        assert torch.equal(got, want[2 + i])
+    # without norms nothing of q and k is kept
+    want_plain = torch.autograd.grad(rotary.rotate_heads(q, k, positions, table), leaves[:2], grads)
+    y = rotary.rotate_heads(q, k, positions, table)
+    assert y[0].grad_fn.name() == "RotateHeadsBackward" and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves[:2], grads), want_plain))
+    # not differentiated again, though a graph may be asked for
+    y = call()
+    dq, = torch.autograd.grad(y[0].float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.float().sum(), q)
+    # written to meanwhile
+    y = call()
+    with torch.no_grad():
+        q.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y, leaves, grads)
+    # what hooks give back, in the order of 16 bytes or off it
+    for unpack in (lambda t: t.detach().clone(), lambda t: torch.cat((t.detach().flatten()[:1], t.detach().flatten()))[1:].view(t.shape)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = call()
+        assert y[0].grad_fn.name() == "RotateHeadsBackward" and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, grads), want))
+    # into leaves, on a stream of their own, from threads
+    wrong = []
+
+    def run():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = torch.autograd.grad(call(), leaves, grads)
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(got)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=run) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    torch.autograd.backward(call(), grads)
+    assert all(torch.equal(t.grad, g) for t, g in zip(leaves, want))
+
+
 def test_repeated_calls_follow_their_operands():
     """Calls of one signature, each with its own operands, on streams of their own and in threads."""
     sets = [operands(64, 8, 2, 128, 128, BF, BF, seed) for seed in range(6)]
