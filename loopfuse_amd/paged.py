@@ -573,6 +573,8 @@ def attention_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor
 
 @lowering._on_device_of_first_argument
 def _shared(q, k_pool, v_pool, plan, table, lengths, prefix_table, prefix_len, v_table, prefix_v_table, out, choice):
+    if isinstance(k_pool, Pool4) or isinstance(v_pool, Pool4):
+        raise UnsupportedPlan("pools in 4 bits are attended over by attention_cached")
     given = (table, lengths, prefix_table, v_table, prefix_v_table)
     lowering._no_tangents(q, k_pool, v_pool)
     dtype = q.dtype
@@ -824,7 +826,7 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
             raise UnsupportedPlan(f"positions must be int32 [{T}]")
     elif offsets is not None and T > B:
         raise UnsupportedPlan("requests with several rows need positions")
-    room = table.shape[1] * page
+    room = table.shape[1] * page if pages else 0
     if room > 1 << 30:
         raise UnsupportedPlan("a request has room for more than 2**30 keys")
     if out is not None:

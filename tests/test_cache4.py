@@ -60,6 +60,11 @@ def test_calls_refuse_pools_that_are_none(case, which):
             call()
 
 
+def test_attention_over_a_prefix_refuses_pools_in_4_bits():
+    with pytest.raises(UnsupportedPlan, match="4 bits"):
+        paged.attention_shared(fake((3, 4, 1, 64)), pool(), pool(), AttnPlan(scale=0.1, k_paged=True, v_paged=True), fake((3, 4), I32), fake((3,), I32))
+
+
 def test_pools_on_the_cpu_are_refused():
     p, rows, i = paged.pool4(3, 16, 2, 64, BF), fake((10, 2, 64)), fake((10,), I32)
     for call in (lambda: paged.store_kv(rows, rows, p, p, i), lambda: paged.read_kv(p, p, i), lambda: paged.read_kv(rows.as_subclass(torch.Tensor)[None], rows[None], i),

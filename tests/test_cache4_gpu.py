@@ -312,6 +312,9 @@ def test_lengths_that_tables_have_no_room_for_and_rows_of_no_token():
     check(out, want)
     assert int(torch.count_nonzero(out[1])) == 0 and int(torch.count_nonzero(out[3:5])) == 0
     assert int(torch.count_nonzero(paged.attention_cached(q, *pools, plan, table[:, :0], n, offsets, positions))) == 0
+    # a pool without a page has none
+    empty = [Pool4(p.codes[:0], p.scales[:0], p.dtype) for p in pools]
+    assert int(torch.count_nonzero(paged.attention_cached(q, *empty, plan, table, n, offsets, positions))) == 0
 
 
 def test_offsets_that_descend_stay_within_the_rows_and_the_room():
