@@ -245,11 +245,16 @@ def _backward(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, p
 def _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight, eps, pairs, sums):
     lowering._no_tangents(dq_out, dk_out)
     given = dq_out, dk_out, q, k, table, q_weight, k_weight, positions
-    # (hooks of saved tensors may give them back laid out otherwise)
+    # (hooks of saved tensors may give them back laid out otherwise, or as something else)
     dq_out, dk_out, q, k = (even_rows(t) for t in given[:4])
     table, q_weight, k_weight, positions = even_rows(table), even_weight(q_weight), even_weight(k_weight), positions.contiguous()
+    saved = (q, k) if eps is not None else (dq_out, dk_out)
+    check_operands(*saved, positions, table, q_weight, k_weight, eps)
     T, Hq, D = dq_out.shape
     Hkv, dev, dtype = dk_out.shape[1], dq_out.device, dq_out.dtype
+    for t, g in zip(saved, (dq_out, dk_out)):
+        if t.shape != g.shape or t.dtype != g.dtype or t.device != g.device:
+            raise UnsupportedPlan("gradients must be of the results' shape and dtype, with Q and K")
     weights = [w for w in (q_weight, k_weight) if w is not None]
     dq, dk = (torch.empty(t.shape, dtype=dtype, device=dev) for t in (dq_out, dk_out))
     dw = [torch.empty(D, dtype=weights[0].dtype, device=dev) if x else None for x in sums]

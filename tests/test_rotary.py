@@ -127,6 +127,20 @@ def test_launches_beyond_32_bits(monkeypatch):
         rotary.rotate_heads(q, k, fake((1,), I32).expand(1 << 28), fake((4, 256), F32))
 
 
+def test_gradients_refuse_saved_tensors_that_are_others():
+    """What hooks of saved tensors give back in their place."""
+    a = operands()
+    right = dict(dq_out=fake((10, 4, 64)), dk_out=fake((10, 2, 64)), **a, q_weight=None, k_weight=None, eps=1e-6, pairs=False, sums=(False, False))
+    elsewhere = torch.zeros((10, 4, 64), dtype=torch.bfloat16)
+    for change in (dict(q=fake((10, 4, 64), F32)), dict(q=fake((9, 4, 64))), dict(k=fake((10, 3, 64))), dict(q=elsewhere), dict(q=fake((10, 4, 128)), k=fake((10, 2, 128))), dict(positions=fake((9,), I32)),
+                   dict(positions=fake((10,), torch.int64)), dict(table=fake((50, 64))), dict(table=torch.zeros(50, 64)), dict(q_weight=fake((32,))), dict(dq_out=fake((10, 4, 64), torch.float16)),
+                   dict(dq_out=fake((10, 5, 64))), dict(eps=None, dk_out=fake((9, 2, 64)))):
+        with pytest.raises((UnsupportedPlan, RuntimeError)):
+            rotary._backward(**{**right, **change})
+    with pytest.raises(AssertionError, match="a launch"):
+        rotary._backward(**right)
+
+
 def test_threads_of_a_row_and_groups_of_heads():
     for D in range(16, 257, 16):
         n = rotary.slots_of(D)

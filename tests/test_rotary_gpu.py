@@ -266,6 +266,16 @@ def test_gradients_of_repeated_calls():
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
             y = call()
         assert y[0].grad_fn.name() == "RotateHeadsBackward" and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, grads), want))
+    # or that are none of them: elsewhere, of another type or shape
+    for unpack in (lambda t: t.detach().cpu(), lambda t: t.detach().double(), lambda t: t.detach()[:1], lambda t: t.detach()[None]):
+        for again in (False, True):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                y = call(not again)
+            rotary._host.clear()
+            with pytest.raises((UnsupportedPlan, RuntimeError)):
+                torch.autograd.grad(y, leaves, grads)
+            call(True), torch.autograd.grad(call(True), leaves, grads)
+    assert call()[0].grad_fn.name() == "RotateHeadsBackward"
     # into leaves, on a stream of their own, from threads
     wrong = []
 
