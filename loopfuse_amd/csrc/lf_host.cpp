@@ -670,10 +670,15 @@ struct RotateNode : torch::autograd::Node {
   }
 };
 
-// rotate_train(q, k, table, q_weight, k_weight, positions, eps, pairs, differentiate) -> (q, k), with gradients
-PyObject* rotate_train(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// rotate(q, k, table, q_weight, k_weight, positions, eps, pairs, differentiate) -> (q, k), with gradients where they are asked for
+PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!takes(n, 9)) return nullptr;
+  bool train = false;
+  if (c10::GradMode::is_enabled())
+    for (int i : {0, 1, 3, 4}) train = train || (THPVariable_Check(a[i]) && THPVariable_Unpack(a[i]).requires_grad());
+  if (!train) return rotate_heads(nullptr, a, 8);
+  if (THPVariable_Check(a[2]) && THPVariable_Unpack(a[2]).requires_grad()) return none();      // (refused)
   if (!plain(a[0]) || (a[6] != Py_None && !PyFloat_CheckExact(a[6])) || !PyBool_Check(a[7]) || c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return none();
   PyObject* out = rotate_heads(nullptr, a, 8);
   if (!out || out == Py_None) return out;
@@ -799,7 +804,7 @@ PyObject* attention_cached(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define LF_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {LF_FAST(setup), LF_FAST(key), LF_FAST(keep), {"clear", clear, METH_NOARGS, nullptr}, {"size", size, METH_NOARGS, nullptr},
                          LF_FAST(elsewhere), LF_FAST(packed_layout), LF_FAST(extend_tables), LF_FAST(store_kv), LF_FAST(attention_shared), LF_FAST(attention_packed), LF_FAST(attention_packed_backward),
-                         LF_FAST(rotate_heads), LF_FAST(rotate_backward), LF_FAST(rotate_train), LF_FAST(append_kv), LF_FAST(read_kv), LF_FAST(attention_cached),
+                         LF_FAST(rotate_heads), LF_FAST(rotate_backward), LF_FAST(rotate), LF_FAST(append_kv), LF_FAST(read_kv), LF_FAST(attention_cached),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lf_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
