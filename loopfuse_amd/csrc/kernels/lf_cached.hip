@@ -17,8 +17,8 @@
 //                   product number i has the elements D / 16 * row + i, so that a lane ends up with D / 4 neighbouring elements of O.
 //
 // Few rows: 16 of a kv head, a workgroup's four waves have a fourth of the pairs of tiles each and merge through LDS in the end; operands straight from memory, two pairs under way, no LDS
-// and no barrier in the loop.  Bound by memory where keys are many: 64 requests of one token up to 8192 keys, 32/8 heads of 128, 59 us and 5 for the joining (291 MB, 4.6 TB/s both); 4 up to
-// 100 000 53 and 5 (272 MB, 4.7); by one wave's chain where they are few: 2 up to 1000 10 us, of which lengths and shares 1.2, the first loads 0.9, eight pairs 4.2, the merge 0.8.
+// and no barrier in the loop.  Bound by memory where keys are many: 64 requests of one token up to 8192 keys, 32/8 heads of 128, 53 us and 5 for the joining (291 MB, 5.0 TB/s both); 4 up to
+// 100 000 47 and 5 (272 MB, 5.2); by one wave's chain where they are few: 2 up to 1000 10 us, of which lengths and shares 1.2, the first loads 0.9, eight pairs 4.2, the merge 0.8.
 // Many rows (LF_CACHED_ROWWAVES): 128, each wave has 32 of them over all pairs.  Of a pair two waves convert a tile of keys each, two one of values, into LDS, where all four find the operands as the
 // products take them: a fourth of the conversions, and fewer registers, so that three waves run on a SIMD.  Bound by the softmax and the products: 4 requests up to 6001 keys with up to 1000
 // new tokens 235 us (213 GFLOP, 905 TFLOP/s; each wave with keys and values of its own 257), 2 of 8192 with 4096 805 us (1025; 897).
@@ -305,18 +305,37 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES && LF_HEAD_
 #else
   constexpr int kStep = 4;
   const int first = wave;
+  // 128 MB of codes and more, which are not in a cache the next time anyhow, pass the caches by.  us, kept / by: 4 requests up to 100 000 keys 58.4 / 52.1, 64 up to 8192 64.2 / 57.7, 16 of 8000 (139 MB) 36.1 / 33.9;
+  // 8 of 8000 (70 MB) 21.6 / 22.2, 4 of 8192 with 4 new tokens (36 MB) 18.3 / 19.5.
+  constexpr int kStream = (128 << 20) / (34 * D);       // pairs of tiles
   struct Ids {
     int a, b;                  // (a pool has less than 2^31 pages)
   };
   auto fetch = [&](int pair) -> Ids { return {(int)ids[tile_of(pair, 0) >> p.shift], (int)ids[tile_of(pair, 1) >> p.shift]}; };
+  const bool streams = p.fixed >= 0 && line >= kStream;
   auto issue = [&](LfCachedStage& s, int pair, const Ids& id) {
+    long long codes[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) codes[w] = (w ? id.b : id.a) * p.page_bytes + (head_tiles + ((tile_of(pair, w) & in_page) >> 4)) * (8 * D);
+    if (streams) {
+      asm volatile("; streams");       // (or the compiler makes one load of both)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        s.k[w] = __builtin_nontemporal_load(reinterpret_cast<const lf_cached_codes*>(p.k + codes[w] + k_at));
+        s.v[w] = __builtin_nontemporal_load(reinterpret_cast<const lf_cached_codes*>(p.v + codes[w] + v_at));
+      }
+      asm volatile("; streams");
+    } else {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        s.k[w] = *reinterpret_cast<const lf_cached_codes*>(p.k + codes[w] + k_at);
+        s.v[w] = *reinterpret_cast<const lf_cached_codes*>(p.v + codes[w] + v_at);
+      }
+    }
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      const long long codes = (w ? id.b : id.a) * p.page_bytes + (head_tiles + ((tile_of(pair, w) & in_page) >> 4)) * (8 * D), scales = codes >> 4;
-      s.k[w] = *reinterpret_cast<const lf_cached_codes*>(p.k + codes + k_at);
-      s.ks[w] = p.k_scales[scales + ks_at];
-      s.v[w] = *reinterpret_cast<const lf_cached_codes*>(p.v + codes + v_at);
-      s.vs[w] = *reinterpret_cast<const unsigned*>(p.v_scales + scales + vs_at);
+      s.ks[w] = p.k_scales[(codes[w] >> 4) + ks_at];
+      s.vs[w] = *reinterpret_cast<const unsigned*>(p.v_scales + (codes[w] >> 4) + vs_at);
     }
   };
 #endif
