@@ -7,13 +7,14 @@
 // products are rounded before they are summed (no fused multiply-add), as the same formula in a tensor language rounds them: what a cache in
 // 4 bits takes for a row does not depend on who rotated it.
 //
-// LF_ROT_SLOTS threads have a row, 16 elements each: in rotated rows 8 of either half, the partners of each other, so that no value changes threads
-// but in the norm's sum (row permutations of 16 lanes).  A group of threads takes two heads of a token, whose row of the table it reads once: one, two and four
-// at a time take 134 / 129 / 133 us forwards and backwards together, 75 / 75 / 79 into pages and 50 / 48 / 50 into 4 bits and back, at the sizes below.
+// LF_ROT_SLOTS threads have a row, 16 elements each: 8 of either half of what is rotated, or of the rest, so that no value changes threads
+// but in the norm's sum (row permutations of 16 lanes) and a load or store of several threads has whole lines.  A group of threads takes two heads of a token, whose row of the table it
+// reads once: one, two and four at a time took 134 / 129 / 133 us forwards and backwards together, 75 / 75 / 79 into pages and 50 / 48 / 50 into 4 bits and back, at the sizes below and
+// before rows were read past the caches: 129 -> 118, 75 -> 66 and 49 -> 48 among passes over other rows.
 //
-// Bound by memory: 8192 rows of 32 and 32 heads of 128 in bf16 with norms 44 us forwards (268 MB, 6.1 TB/s) and 78 backwards with the weights' gradients (403 MB,
-// 5.2); 16384 rows of 32 and 8 heads into pages 74 (407 MB, 5.5); 8192 such rows into 4 bits 35 (177 MB, 5.1).
-// One new token each for up to 64 requests: 3.5 to 4 us, a launch and two round trips to memory.
+// Bound by memory: 8192 rows of 32 and 32 heads of 128 in bf16 with norms 43 us forwards (268 MB, 6.2 TB/s) and 69 backwards with the weights' gradients (403 MB, 5.8); 16384 rows of 32 and 8 heads into
+// pages 65 (407 MB, 6.2); 8192 such rows into 4 bits 37 (177 MB, 4.8).
+// One new token each for up to 64 requests: 3.5 to 4.5 us, a launch and two round trips to memory.
 //
 // In 4 bits: 32 neighbours of a row share a power of two, 2^e with the least e of which their largest size is below 7 * 2^e (what lies between
 // 6 and 7 of them rounds to 6, an error no larger than that of the step from 4 to 6), and each has a sign, two bits of exponent and one of mantissa
@@ -83,18 +84,20 @@ __device__ __forceinline__ float lf_rot_sum(float x) {
   return x;
 }
 
-// What a thread has of a row: 8 elements from `a` and 8 from `b`; `turns`: they are rotated, by pairs 8 slot ... of the table.
+// What a thread has of a row: 8 elements from `a` and 8 from `b`, of either half of the part that is rotated (`turns`) or of the rest, so that a load of several threads has whole lines.
 struct LfRotPlace {
   int a, b;
   bool turns;
 };
-__device__ __forceinline__ LfRotPlace lf_rot_place(int slot, int R, int pairs) {
+__device__ __forceinline__ LfRotPlace lf_rot_place(int slot, int R, int D) {
   const bool turns = 16 * slot < R;
-  return {turns && !pairs ? 8 * slot : 16 * slot, turns && !pairs ? R / 2 + 8 * slot : 16 * slot + 8, turns};
+  const int a = turns ? 8 * slot : R + 8 * (slot - R / 16);
+  return {a, a + (turns ? R : D - R) / 2, turns};
 }
 __device__ __forceinline__ void lf_rot_load(const lf_elem* row, const LfRotPlace& at, lf_elem8 (&raw)[2]) {
-  raw[0] = *reinterpret_cast<const lf_elem8*>(row + at.a);
-  raw[1] = *reinterpret_cast<const lf_elem8*>(row + at.b);
+  // (read once here)
+  raw[0] = __builtin_nontemporal_load(reinterpret_cast<const lf_elem8*>(row + at.a));
+  raw[1] = __builtin_nontemporal_load(reinterpret_cast<const lf_elem8*>(row + at.b));
 }
 __device__ __forceinline__ void lf_rot_floats(const lf_elem8 (&raw)[2], float (&x)[16]) {
 #pragma unroll
@@ -120,16 +123,17 @@ __device__ __forceinline__ void lf_rot_weights(const void* w, int wide, const Lf
       for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e];
     }
   } else {
-    lf_elem8 raw[2];
-    lf_rot_load(reinterpret_cast<const lf_elem*>(w), at, raw);
+    const lf_elem* f = reinterpret_cast<const lf_elem*>(w);
+    const lf_elem8 raw[2] = {*reinterpret_cast<const lf_elem8*>(f + at.a), *reinterpret_cast<const lf_elem8*>(f + at.b)};
     lf_rot_floats(raw, x);
   }
 }
-// cosines and sines of a thread's 8 pairs
-__device__ __forceinline__ void lf_rot_angles(const float* row, int R, int slot, float (&c)[8], float (&s)[8]) {
+// cosines and sines of a thread's 8 pairs, which are one behind the other, or with neighbours as partners four of either half
+__device__ __forceinline__ void lf_rot_angles(const float* row, int R, int pairs, int slot, float (&c)[8], float (&s)[8]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const lf_f32x4 x = *reinterpret_cast<const lf_f32x4*>(row + 8 * slot + 4 * i), y = *reinterpret_cast<const lf_f32x4*>(row + R / 2 + 8 * slot + 4 * i);
+    const float* at = row + (pairs ? 4 * slot + i * (R / 4) : 8 * slot + 4 * i);
+    const lf_f32x4 x = *reinterpret_cast<const lf_f32x4*>(at), y = *reinterpret_cast<const lf_f32x4*>(at + R / 2);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       c[4 * i + e] = x[e];
@@ -167,7 +171,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate(const LfRotate
     slot = p.slots[t];
     slot = slot < p.last ? slot : -1;
   }
-  const LfRotPlace at = lf_rot_place(slot_of_row, R, p.pairs);
+  const LfRotPlace at = lf_rot_place(slot_of_row, R, p.D);
   const lf_elem* x0 = which == 0 ? p.q + (long long)t * p.q_ss : which == 1 ? p.k + (long long)t * p.k_ss : p.v + (long long)t * p.v_ss;
   const long long x_sh = which == 0 ? p.q_sh : which == 1 ? p.k_sh : p.v_sh;
   const bool wanted = live && (!LF_ROT_STORE || which == 0 || slot >= 0);
@@ -178,7 +182,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate(const LfRotate
     if (wanted && h0 + u < H) lf_rot_load(x0 + (h0 + u) * x_sh, at, raw[u]);
   }
   float c[8], s[8], w[16];
-  if (wanted && at.turns) lf_rot_angles(p.table + (long long)position * p.table_stride, R, slot_of_row, c, s);
+  if (wanted && at.turns) lf_rot_angles(p.table + (long long)position * p.table_stride, R, p.pairs, slot_of_row, c, s);
   const bool norm = p.norm && which != 2;
   if (norm && in) lf_rot_weights(which ? p.k_weight : p.q_weight, p.wide, at, w);
 #if LF_ROT_STORE == 2
@@ -246,7 +250,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate_bwd(const LfRo
   const int which = (int)blockIdx.x < p.q_blocks ? 0 : 1;
   const int block = blockIdx.x - (which ? p.q_blocks : 0), blocks = which ? p.k_blocks : p.q_blocks;
   const int H = which ? p.Hkv : p.Hq, chunks = which ? p.k_chunks : p.q_chunks;
-  const LfRotPlace at = lf_rot_place(slot_of_row, p.R, p.pairs);
+  const LfRotPlace at = lf_rot_place(slot_of_row, p.R, p.D);
   const lf_elem* x0 = which ? p.k : p.q;
   const lf_elem* g0 = which ? p.dk_out : p.dq_out;
   lf_elem* out = which ? p.dk : p.dq;
@@ -275,7 +279,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate_bwd(const LfRo
       }
     }
     float c[8], s[8];
-    if (live && at.turns) lf_rot_angles(p.table + (long long)position * p.table_stride, p.R, slot_of_row, c, s);
+    if (live && at.turns) lf_rot_angles(p.table + (long long)position * p.table_stride, p.R, p.pairs, slot_of_row, c, s);
 #pragma unroll
     for (int u = 0; u < LF_ROT_HEADS; ++u) {
       float g[16];
