@@ -21,7 +21,7 @@
 // 100 000 47 and 5 (272 MB, 5.2); by one wave's chain where they are few: 2 up to 1000 10 us, of which lengths and shares 1.2, the first loads 0.9, eight pairs 4.2, the merge 0.8.
 // Many rows (LF_CACHED_ROWWAVES): 128, each wave has 32 of them over all pairs.  Of a pair two waves convert a tile of keys each, two one of values, into LDS, where all four find the operands as the
 // products take them: a fourth of the conversions, and fewer registers, so that three waves run on a SIMD.  Bound by the softmax and the products: 4 requests up to 6001 keys with up to 1000
-// new tokens 235 us (213 GFLOP, 905 TFLOP/s; each wave with keys and values of its own 257), 2 of 8192 with 4096 805 us (1025; 897).
+// new tokens 230 us (213 GFLOP, 926 TFLOP/s; each wave with keys and values of its own 257), 2 of 8192 with 4096 805 us (1025; 897).
 #ifndef LF_CACHED_CB
 #define LF_CACHED_CB 1
 #endif

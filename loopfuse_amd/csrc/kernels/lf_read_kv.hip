@@ -1,7 +1,7 @@
 // lf_read_kv.hip — rows of keys and values out of their slots of page pools of 16-bit rows, or of pools held in 4 bits (-DLF_READ4=1) as the
 // values that they stand for: rows[t] = pool[slot[t]], zeros where there is no such slot.  A thread has 8 neighbours of a K row and the same ones of
-// the V row, neighbouring threads the pieces of one row: each is a load of 16 bytes, or of 4 and a scale, and a store of 16.  Bound by memory: 10 240 rows of 8 heads of 128 out of 4 bits 12.7 us
-// (53 MB, 4.2 TB/s, 3 us of it a launch's own), 64 such rows 2.9.
+// the V row, neighbouring threads the pieces of one row: each is a load of 16 bytes, or of 4 and a scale, and a store of 16.  Bound by memory: 10 240 rows of 8 heads of 128 out of 4 bits 11.1 us
+// (53 MB, 4.8 TB/s, 3 us of it a launch's own), 64 such rows 3.1.
 #ifndef LF_READ4
 #define LF_READ4 0
 #endif
