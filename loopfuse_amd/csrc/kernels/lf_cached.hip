@@ -16,9 +16,10 @@
 //   O^T += V^T P^T: a lane holds 4 keys' D / 16 neighbouring elements; two conversions and two byte permutations make the two lanes' worth of operand of two elements out of them, and the
 //                   product number i has the elements D / 16 * row + i, so that a lane ends up with D / 4 neighbouring elements of O.
 //
-// Few rows: 16 of a kv head, a workgroup's four waves have a fourth of the pairs of tiles each and merge through LDS in the end; operands straight from memory, two pairs under way, no LDS
+// Few rows: 16 of a kv head, or 32, a workgroup's four waves have a fourth of the pairs of tiles each and merge through LDS in the end; operands straight from memory, two pairs under way, no LDS
 // and no barrier in the loop.  Bound by memory where keys are many: 64 requests of one token up to 8192 keys, 32/8 heads of 128, 53 us and 5 for the joining (291 MB, 5.0 TB/s both); 4 up to
-// 100 000 47 and 5 (272 MB, 5.2); by one wave's chain where they are few: 2 up to 1000 10 us, of which lengths and shares 1.2, the first loads 0.9, eight pairs 4.2, the merge 0.8.
+// 100 000 47 and 5 (272 MB, 5.2); by one wave's chain where they are few: 2 up to 1000 10 us, of which lengths and shares 1.2, the first loads 0.9, eight pairs 4.2, the merge 0.8;
+// by conversions, softmax and products in between: 64 up to 8192 with five new tokens each 74 us, 32 rows at a time (16: 99).
 // Many rows (LF_CACHED_ROWWAVES): 128, each wave has 32 of them over all pairs.  Of a pair two waves convert a tile of keys each, two one of values, into LDS, where all four find the operands as the
 // products take them: a fourth of the conversions, and fewer registers, so that three waves run on a SIMD.  Bound by the softmax and the products: 4 requests up to 6001 keys with up to 1000
 // new tokens 230 us (213 GFLOP, 926 TFLOP/s; each wave with keys and values of its own 257), 2 of 8192 with 4096 805 us (1025; 897).
@@ -182,7 +183,7 @@ struct LfCachedStage {
 };
 #endif
 
-extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES && LF_HEAD_DIM == 64 ? 4 : 3) lf_cached(const LfCachedParams p) {
+extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES && LF_HEAD_DIM == 64 ? 4 : LF_CACHED_ROWWAVES || LF_CACHED_CB == 1 ? 3 : 2) lf_cached(const LfCachedParams p) {
   constexpr int D = LF_HEAD_DIM, CB = LF_CACHED_CB, NJ = D / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const LfCachedRequest mine = lf_cached_request(p, lane);

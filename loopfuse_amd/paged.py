@@ -724,13 +724,18 @@ def _again(q, k_pool, v_pool, table, lengths, prefix_table, v_table, prefix_v_ta
     return out
 
 
-def cached_build(rows: float, all_rows: int, keys: int) -> tuple:
+def cached_build(rows: float, all_rows: int, keys: int, D: int) -> tuple:
     """(blocks of 16 rows of a wave, do a workgroup's waves have rows of their own) for so many rows of a kv head per request, ``all_rows`` of all heads and up to ``keys`` keys.
-    Few rows are taken 16 at a time by four waves that share their keys, many 128 at a time, whose keys and values are converted once, where there are workgroups or keys enough
-    for that.  us, 16 / 128: 32/8 heads of 128, 16 requests of 2048 keys, 64 new tokens each 66 / 70, 96 94 / 90, 512 476 / 276; 4 of 8192, 64 67 / 73, 96 89 / 90, 128 115 / 97; 1 of 32 768,
-    256 233 / 182; 8 of 4096, 64 63 / 71, 128 115 / 108; 16 of 4001, 33 53 / 67; 1 of 1000, all 45 / 42; 32 of 700, 64 67 / 44; 16/16 of 64, 32 of 1024, 64 31 / 40, 128 59 / 41."""
-    many = all_rows >= (32768 if keys <= 1536 else 49152) or all_rows * keys >= 10 ** 8
-    return (2, True) if rows > 64 and many else (1, False)
+    Up to 16 rows are taken by four waves that share their keys; more of them 32 at a time in the same way, whose keys and values are converted once for both blocks, where the work is enough for
+    half the workgroups (at head dimension 64, of which two run on a CU where four of the others do, also for pairs of blocks or long keys only); many 128 at a time, whose keys and
+    values are converted once for four waves.  us, 16 / 32: 32/8 heads of 128, 16 requests of 2048 keys, 8 new tokens each 17.5 / 21.3, 16 22.4 / 21.9, 64 65 / 53; 4 of 8192, 8 21.5 / 22.2, 32 46 / 38; 64 of
+    1500, 8 35 / 28; 64 up to 8192, 5 99 / 74; 2 of 100 000, 5 80 / 57; 64/2 heads, 64 up to 8192, 1 38 / 29; 4/4 of 64, 100 of 1200, 40 26 / 33.  32 / 128: 32/8 heads of 128, 16 of 2048, 96 82 / 91, 128 99 / 94,
+    512 390 / 273; 4 of 8192, 128 87 / 98, 256 166 / 159; 1 of 32 768, 256 182 / 159; 1 of 1000, all 36 / 42; 2 of 1500, all 122 / 70; 32 of 700, 64 57 / 43; 16/16 of 64, 32 of 1024, 64 28 / 38, 128 51 / 40."""
+    if rows > 64 and (all_rows >= 65536 or all_rows * keys >= 2 * 10 ** 8):
+        return 2, True
+    if rows > 16 and all_rows * keys >= 16 * 10 ** 6 and (D == 128 or keys > 4096 or math.ceil(rows / 16) % 2 == 0):
+        return 2, False
+    return 1, False
 
 
 def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64: bool, blocks: int, rowwaves: bool) -> lowering.KernelSpec:
@@ -738,20 +743,23 @@ def cached_spec(dtype: torch.dtype, D: int, mask: int, softcap: bool, table_i64:
                           extra=(f"-DLF_CACHED_CB={blocks}",) + (("-DLF_CACHED_ROWWAVES=1",) if rowwaves else ()))
 
 
-def cached_shares(units: int, keys: int, rows: float, rowwaves: bool, D: int) -> tuple:
+def cached_shares(units: int, keys: int, rows: float, build: tuple, D: int) -> tuple:
     """(workgroups, what a unit costs besides its pairs of tiles or -1, least share of a workgroup) for at most so many units of up to ``keys`` keys that a row can see, ``rows`` as
     above; -1: each workgroup has a unit.  Shares cost a second launch, 4 us, and the begin of every part of a unit; a unit of its own the chain of its pairs, 0.6 us a
     pair of each wave (1.2 us in 128 rows), and what the longest lasts longer than the others, which differ less where a request has many; under a causal mask the first of a request's new tokens
-    have fewer keys than shares are cut for.  As many workgroups as run at once: two on a CU (16 rows, head dimension 128), three (its 128 rows; 16 rows of 64), four.
-    us, shares / units: 16 rows, 2 requests up to 1000, 32/8 heads of 128, 12.5 / 10.8, 64 up to 8192 65 / 76, 4 up to 100 000 58 / 620, 75 up to 2063, 8/8, 32 / 30, 48 up to 1029 in a window,
+    have fewer keys than shares are cut for.  As many workgroups as run at once: two on a CU (16 rows of 128, 32 rows), three (128 rows of 128; 16 rows of 64), four.
+    us, shares / units: 16 rows, 2 requests up to 1000, 32/8 heads of 128, 12.5 / 10.8, 64 up to 8192 65 / 76, 4 up to 100 000 58 / 620, 75 up to 2063, 8/8, 32 / 30, 16 of 2048 with 8 new tokens each 21 / 18, 48 up to 1029 in a window,
     16/4 of 64, 21 / 17, 53 of 1681 with 75 new tokens each, 4/4, 54 / 40; workgroups, 512 / 768 / 1024: 64 up to 8192 64 / 66 / 73, 48 up to 12 341, 32/8 of 64, 57 / 52 / 50.  128 rows, 32/8 of
     128: 16 of 2048 with 128 new each 108 / 92, 8 of 4096 with 128 108 / 147, 4 up to 6001 with up to 1000 286 / 235, 1 of 12 000 with 1000 231 / 407, 1 of 32 768 with 3500 1820 / 2341, with 6144
-    2965 / 2854; workgroups, 512 / 768 / 1024: 4 of 8192 with 256 new each 195 / 161 / 199."""
-    if rowwaves:
+    2965 / 2854; workgroups, 512 / 768 / 1024: 4 of 8192 with 256 new each 195 / 161 / 199.  32 rows, 32/8 of 128: 64 up to 8192 with 5 new each 74 / 91, 24 of 1900 with 5 25 / 21, 32 of 4096 with 8
+    42 / 43, with 10 57 / 54, 4 of 8192 with 128 96 / 87, 1 of 32 768 with 256 182 / 221."""
+    if build == (2, True):
         if units >= (256 if keys <= 1536 else 512 if keys <= 4096 else 768 if keys <= 12288 else 1536):
             return units, -1, 1
         return 768 if D == 128 else 1024, 8, 20
-    if keys <= 1536 or (units >= 512 and (rows >= 64 or keys <= 2100)):
+    if build == (2, False):
+        return (units, -1, 1) if keys <= 2100 or (units >= 512 and (rows >= 32 or keys <= 4096)) else (512, 16, 20)
+    if keys <= 1536 or (units >= 512 and rows >= 64) or (units >= 256 and keys <= 2100):
         return units, -1, 1
     return 512 if D == 128 else 768, 16, 20
 
@@ -851,10 +859,10 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     P.window = min(int(plan.window), 1 << 30) if mask == lowering.MASK_SLIDING else 0
     P.scale, P.softcap = plan.scale, softcap or 0.0
     keys, per = min(room, P.window + T) if P.window else room, T * P.group / B
-    blocks, rowwaves = cached_build(per, T * Hq, keys)
+    blocks, rowwaves = build = cached_build(per, T * Hq, keys, D)
     rows = 16 * blocks * (4 if rowwaves else 1)
     units = (T * P.group // rows + min(T, B)) * Hkv       # (at most: a chunk that is not full for each request)
-    P.workgroups, P.fixed, P.least = cached_shares(units, keys, per, rowwaves, D)
+    P.workgroups, P.fixed, P.least = cached_shares(units, keys, per, build, D)
     P.per_group = (-(-(1 << 32) // P.group)) & 0xffffffff
     # (the line of all units, and rows times their division's error, are numbers in 32 bits)
     if units * (-(-room // 32) + 64) >= 1 << 31 or T * P.group ** 2 >= 1 << 32 or T * P.group >= 1 << 30:

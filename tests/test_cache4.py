@@ -212,11 +212,11 @@ def test_every_pair_has_one_workgroup_and_every_part_a_place(lengths, new, windo
     """The kernel's own arithmetic: the pairs of each unit are dealt once, parts lie in places of their own within the room for them, and the ones that lf_cached_combine looks
     for are those that were left."""
     B, T = len(lengths), sum(new)
-    for blocks, rowwaves in ((1, False), (2, True)):
+    for blocks, rowwaves in ((1, False), (2, False), (2, True)):
         rows = 16 * blocks * (4 if rowwaves else 1)
         most = (T * group // rows + min(T, B)) * Hkv
         keys = max(lengths)
-        workgroups, fixed, least = choice or paged.cached_shares(most, keys, T * group / B, rowwaves, 128)
+        workgroups, fixed, least = choice or paged.cached_shares(most, keys, T * group / B, (blocks, rowwaves), 128)
         requests = line_of(lengths, new, window, group, Hkv, rows, fixed)
         units = [(b, u) for b, (chunks, _, _) in enumerate(requests) for u in range(chunks * Hkv)]
         assert len(units) <= most
@@ -278,7 +278,8 @@ def test_builds_that_the_rules_choose_are_built_ahead():
             for mask in (0, 1, 2):
                 for cap in (False, True):
                     for rows in (1, 4, 16, 40, 64, 65, 500, 10000):
-                        assert paged.cached_spec(dtype, D, mask, cap, False, *paged.cached_build(rows, 32 * rows, 5000)) in built
+                        for keys in (500, 5000, 10 ** 6):
+                            assert paged.cached_spec(dtype, D, mask, cap, False, *paged.cached_build(rows, 32 * rows, keys, D)) in built
         for D in (16, 48, 64, 96, 128, 256):
             assert rotary.kernel_spec(dtype, D) in built and rotary.kernel_spec(dtype, D, 1) in built
             assert D not in (64, 128) or rotary.kernel_spec(dtype, D, 2) in built

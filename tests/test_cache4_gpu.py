@@ -291,7 +291,7 @@ def test_attention_over_a_cache_is_the_formula(lengths, new, page, Hkv, group, D
     assert torch.equal(given[inside], out[inside]) and bool((wide[:, 1::2] == 7).all()) and bool((given[:before] == 7).all()) and bool((given[before + sum(new):] == 7).all())
     # other shares, and other builds
     for choice in ((97, 3, 5), (1, 0, 1), None):
-        for build in ((1, False), (2, True)):
+        for build in ((1, False), (2, False), (2, True)):
             monkeypatch.setattr(paged, "cached_build", lambda *a: build)
             monkeypatch.setattr(paged, "cached_shares", lambda units, *a: choice or (units, -1, 1))
             paged._host.clear()
@@ -329,7 +329,7 @@ def test_offsets_that_descend_stay_within_the_rows_and_the_room():
 
 
 @pytest.mark.parametrize("D,dtype", [(64, HF), (128, BF)])
-@pytest.mark.parametrize("build", [(1, False), (2, True)])
+@pytest.mark.parametrize("build", [(1, False), (2, False), (2, True)])
 def test_nan_in_places_that_a_row_does_not_see_stays_there(D, dtype, build, monkeypatch):
     """A key and a value that are NaN, each in one block of a token, over rows some of which see the token: causal, behind a window, and alone."""
     monkeypatch.setattr(paged, "cached_build", lambda *a: build)
