@@ -10,7 +10,7 @@
 // LF_ROT_SLOTS threads have a row, 16 elements each: 8 of either half of what is rotated, or of the rest, so that no value changes threads
 // but in the norm's sum (row permutations of 16 lanes) and a load or store of several threads has whole lines.  A group of threads takes two heads of a token, whose row of the table it
 // reads once: one, two and four at a time took 134 / 129 / 133 us forwards and backwards together, 75 / 75 / 79 into pages and 50 / 48 / 50 into 4 bits and back, at the sizes below and
-// before rows were read past the caches: 129 -> 118, 75 -> 66 and 49 -> 48 among passes over other rows.
+// before rows were read past the caches: 129 -> 118, 75 -> 66 and 49 -> 48 in loops of 20 passes over other rows, 128 -> 125, 74 -> 76 and 53 -> 49 over seconds of nothing else.
 //
 // Bound by memory: 8192 rows of 32 and 32 heads of 128 in bf16 with norms 43 us forwards (268 MB, 6.2 TB/s) and 69 backwards with the weights' gradients (403 MB, 5.8); 16384 rows of 32 and 8 heads into
 // pages 65 (407 MB, 6.2); 8192 such rows into 4 bits 37 (177 MB, 4.8).
