@@ -83,7 +83,7 @@ __device__ __forceinline__ LfCachedRequest lf_cached_request(const LfCachedParam
   r.end = min(max(end, 0), p.room);
   r.start = 0;
 #if LF_MASK == 2
-  const int from = p.positions && r.n > 0 ? p.positions[r.first] : r.end - 1;
+  const int from = p.positions && r.n > 0 ? max(p.positions[r.first], 0) : r.end - 1;
   r.start = min(max(from - p.window + 1, 0), max(r.end - 1, 0)) & ~31;
 #endif
   r.chunks = (int)(((long long)r.n * p.group + LF_CACHED_ROWS - 1) / LF_CACHED_ROWS);
@@ -364,7 +364,7 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES && LF_HEAD_
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     hi[cb] = pos[cb] < 0 ? 0 : LF_MASK == 0 ? u.r.end : min(pos[cb], u.r.end - 1) + 1;
-    lo[cb] = LF_MASK == 2 ? max(pos[cb] - p.window + 1, 0) : 0;
+    lo[cb] = LF_MASK == 2 ? max(max(pos[cb], 0) - p.window + 1, 0) : 0;
     least_hi = min(least_hi, hi[cb]);
     most_hi = max(most_hi, hi[cb]);
     least_lo = min(least_lo, lo[cb]);

@@ -317,6 +317,19 @@ def test_lengths_that_tables_have_no_room_for_and_rows_of_no_token():
     assert int(torch.count_nonzero(paged.attention_cached(q, *empty, plan, table, n, offsets, positions))) == 0
 
 
+@pytest.mark.parametrize("build", [(1, False), (2, False), (2, True)])
+def test_rows_of_no_token_in_front_of_others_in_a_window(build, monkeypatch):
+    monkeypatch.setattr(paged, "cached_build", lambda *a: build)
+    pools, table, n, offsets, positions = batch([700, 90], [6, 3], 16, 2, 64, BF, 5)
+    plan = AttnPlan("sliding", 100, 0.1, None, True, True)
+    q = rnd((9, 4, 64), 2)
+    for none in (-1, -2 ** 31, -2 ** 31 + 50):
+        positions[0] = positions[6] = positions[7] = none
+        out = paged.attention_cached(q, *pools, plan, table, n, offsets, positions)
+        check(out, oracle(q, pools, plan, table, n, offsets, positions, BF), f"{none} {build}")
+        assert int(torch.count_nonzero(out[0])) == 0 and int(torch.count_nonzero(out[6:8])) == 0
+
+
 def test_offsets_that_descend_stay_within_the_rows_and_the_room():
     """Offsets that are none (they say of more rows than there are): numbers come out, and nothing beside O and the parts is written."""
     pools, table, n, _, _ = batch([5000] * 6, [1] * 6, 16, 2, 64, BF, 1)
