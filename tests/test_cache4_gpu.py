@@ -317,6 +317,20 @@ def test_lengths_that_tables_have_no_room_for_and_rows_of_no_token():
     assert int(torch.count_nonzero(paged.attention_cached(q, *empty, plan, table, n, offsets, positions))) == 0
 
 
+@pytest.mark.parametrize("D,dtype,group", [(128, BF, 4), (64, HF, 20)])
+def test_many_keys_pass_the_caches_by(D, dtype, group):
+    """Requests that share their pages count as if each had its own: 64 of 4100 keys are beyond the 128 MB from which codes are loaded so."""
+    B, Hkv = 64 if D == 128 else 128, 8
+    pools, table, n, _, _ = batch([4100], [1], 16, Hkv, D, dtype, 3)
+    assert B * (4100 // 32 * Hkv) * 34 * D > 128 << 20
+    table, n = table.expand(B, -1).contiguous(), n.expand(B).contiguous()
+    q, plan = rnd((B, Hkv * group, D), 4, dtype), AttnPlan("causal", 0, 0.1, None, True, True)
+    positions, offsets = torch.full((B,), 4099, dtype=torch.int32, device=DEV), i32(range(B + 1))
+    out = paged.attention_cached(q, *pools, plan, table, n, offsets, positions)
+    assert "lf_cached_combine" in lowering._last_launch["kernels"]
+    check(out, oracle(q, pools, plan, table, n, offsets, positions, dtype))
+
+
 @pytest.mark.parametrize("build", [(1, False), (2, False), (2, True)])
 def test_rows_of_no_token_in_front_of_others_in_a_window(build, monkeypatch):
     monkeypatch.setattr(paged, "cached_build", lambda *a: build)
