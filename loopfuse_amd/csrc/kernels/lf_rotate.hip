@@ -298,7 +298,8 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate_bwd(const LfRo
         lf_rot_floats(xr[u], x);
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += x[i] * x[i];
-        const float r = __builtin_amdgcn_rsqf(lf_rot_sum(sum) / (float)p.D + p.eps);
+        // (where there is no row, or no such head, eps may be 0 and the root infinite: the zeros there stay zeros)
+        const float y = lf_rot_sum(sum) / (float)p.D + p.eps, r = live && h0 + u < H ? __builtin_amdgcn_rsqf(y) : 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           x[i] *= r;

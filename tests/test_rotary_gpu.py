@@ -389,3 +389,24 @@ def test_inside_a_compiled_function():
     want = rotary.rotate_heads(q * 2, k, positions, table, **norm)
     got = torch.compile(lambda q, k: rotary.rotate_heads(q * 2, k, positions, table, **norm), backend="eager")(q, k)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-50])       # (the second is 0 in 32 bits)
+@pytest.mark.parametrize("T,Hq,Hkv,D,R,dtype,wtype,pairs", [(7, 3, 1, 64, 64, BF, BF, False), (300, 5, 8, 128, 0, HF, F32, False), (65, 2, 3, 80, 48, BF, F32, True)])
+def test_weights_gradients_without_eps(T, Hq, Hkv, D, R, dtype, wtype, pairs, eps):
+    """Rows of no token, odd numbers of heads and the last workgroup's rest add nothing to the weights' gradients, whose norms would divide by zero there."""
+    q, k, positions, table, norm = operands(T, Hq, Hkv, D, R, dtype, wtype, T)
+    positions[::3] = -1
+    norm["eps"] = eps
+    leaves = [t.requires_grad_() for t in (q, k, norm["q_weight"], norm["k_weight"])]
+    grads = [rnd(t.shape, 40 + i, dtype) for i, t in enumerate((q, k))]
+    rotary._host.clear()
+    for _ in range(3):       # the general path, then the host module's node
+        y = rotary.rotate_heads(q, k, positions, table, pairs=pairs, **norm)
+        got = torch.autograd.grad(y, leaves, grads)
+        for i, name in enumerate(("q_weight", "k_weight")):
+            want = oracle(leaves[i].detach(), grads[i], positions, table, norm[name].detach(), 0.0, pairs)
+            check(y[i], want["y"], "y")
+            check(got[i], want["dx"], "dx")
+            check(got[2 + i], want["dw"], "dw")
+    assert y[0].grad_fn.name() == "RotateHeadsBackward"
