@@ -84,6 +84,12 @@ __device__ __forceinline__ float lf_rot_sum(float x) {
   return x;
 }
 
+// 1 / sqrt(x).  The instruction takes numbers below the least normal one for zeros: those are brought up by 2^24 first (without an eps elements of 2^-64 have such means).
+__device__ __forceinline__ float lf_rot_root(float x) {
+  const bool small = x < 0x1p-126f;
+  return __builtin_amdgcn_rsqf(small ? x * 0x1p24f : x) * (small ? 0x1p12f : 1.0f);
+}
+
 // What a thread has of a row: 8 elements from `a` and 8 from `b`, of either half of the part that is rotated (`turns`) or of the rest, so that a load of several threads has whole lines.
 struct LfRotPlace {
   int a, b;
@@ -196,7 +202,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate(const LfRotate
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum += x[i] * x[i];
-      const float r = __builtin_amdgcn_rsqf(lf_rot_sum(sum) / (float)p.D + p.eps);
+      const float r = lf_rot_root(lf_rot_sum(sum) / (float)p.D + p.eps);
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
     }
@@ -299,7 +305,7 @@ extern "C" __global__ void __launch_bounds__(LF_ROT_NT) lf_rotate_bwd(const LfRo
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += x[i] * x[i];
         // (where there is no row, or no such head, eps may be 0 and the root infinite: the zeros there stay zeros)
-        const float y = lf_rot_sum(sum) / (float)p.D + p.eps, r = live && h0 + u < H ? __builtin_amdgcn_rsqf(y) : 0.0f;
+        const float y = lf_rot_sum(sum) / (float)p.D + p.eps, r = live && h0 + u < H ? lf_rot_root(y) : 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           x[i] *= r;

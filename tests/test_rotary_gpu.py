@@ -10,7 +10,7 @@ import threading
 import pytest
 import torch
 
-from loopfuse_amd import packed, rotary
+from loopfuse_amd import packed, paged, rotary
 from loopfuse_amd.lowering import AttnPlan, UnsupportedPlan
 
 pytestmark = pytest.mark.gpu
@@ -410,3 +410,29 @@ def test_weights_gradients_without_eps(T, Hq, Hkv, D, R, dtype, wtype, pairs, ep
             check(got[i], want["dx"], "dx")
             check(got[2 + i], want["dw"], "dw")
     assert y[0].grad_fn.name() == "RotateHeadsBackward"
+
+
+@pytest.mark.parametrize("power", [-62, -64, -70])
+def test_norms_of_rows_whose_squares_are_below_the_least_normal_number(power):
+    """Elements of 2^p and -2^p: squares of 2^(2 p), exact in 32 bits, have a mean of the same, and rows are signs after the norm, off by the root's 2^-22, which a
+    rounding to 16 bits takes away.  With one element's gradient 1 and the others' 0, dx is 2^-p times (1 - 1 / D) there and the signs' product by -1 / D elsewhere, all exact but for 2^-21,
+    which 2^-8 of each covers."""
+    D = 64
+    sign = torch.where(rnd((5, 2, D), 1, F32) < 0, -1.0, 1.0)
+    x = (sign * 2.0 ** power).to(BF).requires_grad_()
+    w = torch.ones(D, device=DEV).requires_grad_()
+    positions = torch.zeros(5, dtype=torch.int32, device=DEV)
+    g = torch.zeros_like(x.detach())
+    g[..., 7] = 1
+    n = sign.double()
+    want = (g.double() - n * n[..., 7:8] / D) * 2.0 ** -power
+    for _ in range(2):
+        y = rotary.rotate_heads(x, x, positions, None, q_weight=w, eps=0.0)
+        assert torch.equal(y[0], sign.to(BF)) and torch.equal(y[1], sign.to(BF))
+        dx, dw = torch.autograd.grad(y[0], (x, w), g)
+        assert ((dx.double() - want).abs() <= 2.0 ** -8 * want.abs()).all()
+        assert ((dw.double() - (g.double() * n).sum((0, 1))).abs() <= 10 * 2.0 ** -20).all()
+    pools = [torch.zeros((1, 8, 2, D), dtype=BF, device=DEV) for _ in range(2)]
+    slots = torch.arange(5, dtype=torch.int32, device=DEV)
+    q = paged.append_kv(x.detach(), x.detach(), x.detach(), *pools, slots, positions, None, eps=0.0)
+    assert torch.equal(q, sign.to(BF)) and torch.equal(pools[0][0, :5], sign.to(BF)) and torch.equal(pools[1][0, :5], x.detach())
