@@ -675,10 +675,11 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!takes(n, 9)) return nullptr;
   bool train = false;
-  if (c10::GradMode::is_enabled())
+  if (c10::GradMode::is_enabled()) {
+    if (THPVariable_Check(a[2]) && THPVariable_Unpack(a[2]).requires_grad()) return none();      // (refused)
     for (int i : {0, 1, 3, 4}) train = train || (THPVariable_Check(a[i]) && THPVariable_Unpack(a[i]).requires_grad());
+  }
   if (!train) return rotate_heads(nullptr, a, 8);
-  if (THPVariable_Check(a[2]) && THPVariable_Unpack(a[2]).requires_grad()) return none();      // (refused)
   if (!plain(a[0]) || (a[6] != Py_None && !PyFloat_CheckExact(a[6])) || !PyBool_Check(a[7]) || c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return none();
   PyObject* out = rotate_heads(nullptr, a, 8);
   if (!out || out == Py_None) return out;

@@ -162,14 +162,15 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     (``[D]``, of Q's dtype or float32; none: ones), before the rotation.  Sums and products in 32 bits, rounded once.
 
     Differentiable in q, k and the weights, as ``packed.attention_packed`` is: once, not forward-mode, and under graph capture not for leaves that another
-    autograd graph holds, nor for what a graph made outside the capture computed.  Kept for the backward: q and k as given where there is a norm."""
+    autograd graph holds, nor for what a graph made outside the capture computed.  A table
+    that asks for a gradient is refused.  Kept for the backward: q and k as given where there is a norm."""
     done = _host.rotate(q, k, table, q_weight, k_weight, positions, eps, bool(pairs), _differentiate)      # (gradients neither under capture nor with tangents)
     if done is not None:
         return done
     operands = [t for t in (q, k, q_weight, k_weight) if isinstance(t, torch.Tensor)]
+    if torch.is_grad_enabled() and isinstance(table, torch.Tensor) and table.requires_grad:
+        raise UnsupportedPlan("no gradient of the table is formed")
     if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
-        if isinstance(table, torch.Tensor) and table.requires_grad:
-            raise UnsupportedPlan("no gradient of the table is formed")
         from . import packed
         packed.refuse_outside_capture(operands, "Q, K and the weights")
         lowering._no_tangents(*operands)      # (not to be seen inside)

@@ -240,3 +240,13 @@ def test_parameter_blocks_of_c_hosts_are_the_mirrors(tmp_path, mirror, device, s
     subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-I" + include, str(tmp_path / "p.c"), "-o", str(tmp_path / "p")], check=True)
     out = dict(line.split() for line in subprocess.run([str(tmp_path / "p")], check=True, capture_output=True, text=True).stdout.splitlines())
     assert {n: int(out[n]) for n in own} == {n: getattr(mirror, n).offset for n in own} and int(out["sizeof"]) == ctypes.sizeof(mirror)
+
+
+def test_a_table_alone_gets_no_gradient_either(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    a = operands()
+    a["table"].requires_grad_()
+    with pytest.raises(UnsupportedPlan, match="table"):
+        rotary.rotate_heads(**a)
+    with torch.no_grad(), pytest.raises(AssertionError, match="a launch"):       # (nothing is asked for)
+        rotary.rotate_heads(**a)

@@ -436,3 +436,17 @@ def test_norms_of_rows_whose_squares_are_below_the_least_normal_number(power):
     slots = torch.arange(5, dtype=torch.int32, device=DEV)
     q = paged.append_kv(x.detach(), x.detach(), x.detach(), *pools, slots, positions, None, eps=0.0)
     assert torch.equal(q, sign.to(BF)) and torch.equal(pools[0][0, :5], sign.to(BF)) and torch.equal(pools[1][0, :5], x.detach())
+
+
+def test_a_repeated_call_refuses_a_table_that_asks_for_a_gradient():
+    q, k, positions, table, norm = operands(30, 4, 2, 64, 64, BF, BF, 5)
+    for _ in range(3):       # (the signature of a call does not say whether gradients are asked for)
+        want = rotary.rotate_heads(q, k, positions, table, **norm)
+    table.requires_grad_()
+    for leaf in (None, q):
+        if leaf is not None:
+            leaf.requires_grad_()
+        with pytest.raises(UnsupportedPlan, match="table"):
+            rotary.rotate_heads(q, k, positions, table, **norm)
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(rotary.rotate_heads(q, k, positions, table, **norm), want))
