@@ -301,7 +301,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pool: Union[t
 @lowering._on_device_of_first_argument
 def _append(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight, eps, pairs):
     """``positions`` None: only keys and values, into pools in 4 bits; ``q`` then stands for nothing."""
-    lowering._no_tangents(q, k, v, q_weight, k_weight)
+    lowering._no_tangents(q, k, v, table, q_weight, k_weight)
     keys_only = positions is None
     T, Hq, Hkv, D, R, wide = rotary.check_operands(q, k, positions, table, q_weight, k_weight, eps, (("V", v),), plain=True)
     _on_gpu("slots", slots, (torch.int32,), 1, q.device)

@@ -173,7 +173,7 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
         from . import packed
         packed.refuse_outside_capture(operands, "Q, K and the weights")
-        lowering._no_tangents(*operands)      # (not to be seen inside)
+        lowering._no_tangents(*operands, table)      # (not to be seen inside)
         return _Rotate.apply(q, k, _given(positions), table, q_weight, k_weight, eps, bool(pairs))
     return _general(q, k, positions, table, q_weight, k_weight, eps, bool(pairs))
 
@@ -191,7 +191,7 @@ def _given(positions):
 
 @lowering._on_device_of_first_argument
 def _general(q, k, positions, table, q_weight, k_weight, eps, pairs):
-    lowering._no_tangents(q, k, q_weight, k_weight)
+    lowering._no_tangents(q, k, table, q_weight, k_weight)
     T, Hq, Hkv, D, R, wide = check_operands(q, k, _given(positions), table, q_weight, k_weight, eps)
     if T:
         _checked_positions(positions, table.shape[0] if table is not None else _ALL)

@@ -250,3 +250,18 @@ def test_a_table_alone_gets_no_gradient_either(monkeypatch):
         rotary.rotate_heads(**a)
     with torch.no_grad(), pytest.raises(AssertionError, match="a launch"):       # (nothing is asked for)
         rotary.rotate_heads(**a)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_of_the_table_are_refused(grad, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    with forward_ad.dual_level():
+        a = operands()
+        if grad:
+            a["q"].requires_grad_()
+        a["table"] = forward_ad.make_dual(a["table"], torch.ones_like(a["table"]))
+        with pytest.raises(UnsupportedPlan, match="tangents"):
+            rotary.rotate_heads(**a)
+        rows = fake((10, 2, 64))
+        with pytest.raises(UnsupportedPlan, match="tangents"):
+            paged.append_kv(a["q"].detach(), rows, rows, fake((3, 4, 2, 64)), fake((3, 4, 2, 64)), a["positions"], a["positions"], a["table"])
