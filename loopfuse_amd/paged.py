@@ -272,9 +272,9 @@ def _two_pools(k_pool, v_pool, dtype, device, heads: int, D: int, written=True) 
     return pages, page, ks, vs
 
 
-def _checked_slots(slots, last) -> None:
+def _checked_slots(slots, last, positions=None, places=0) -> None:
     if lowering._checks_tables():
-        kept = slots[slots >= 0]
+        kept = slots[slots >= 0 if positions is None else (slots >= 0) & (positions >= 0) & (positions < places)]
         if len(kept) and (int(kept.max()) >= last or len(torch.unique(kept)) < len(kept)):
             raise ValueError(f"loopfuse_amd: slots must be distinct and below {last}")
 
@@ -324,7 +324,7 @@ def _append(q, k, v, k_pool, v_pool, slots, positions, table, q_weight, k_weight
         raise UnsupportedPlan(f"a launch for {T} rows of {Hq} and {Hkv} heads of {D} is too large")
     if T == 0:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _checked_slots(slots, P.last)
+    _checked_slots(slots, P.last, positions, P.places)
     if not keys_only:
         rotary._checked_positions(positions, P.places)
     if keys_only:

@@ -283,3 +283,23 @@ def test_builds_that_the_rules_choose_are_built_ahead():
         for D in (16, 48, 64, 96, 128, 256):
             assert rotary.kernel_spec(dtype, D) in built and rotary.kernel_spec(dtype, D, 1) in built
             assert D not in (64, 128) or rotary.kernel_spec(dtype, D, 2) in built
+
+
+def test_checked_slots_are_those_of_tokens(monkeypatch):
+    """A row of no token is left out of the pools whatever its slot, and so out of the check."""
+    monkeypatch.setattr(lowering, "_checks_tables", lambda: True)
+    apart, none = torch.arange(10, dtype=I32).as_subclass(OnGpu), fake((10,), I32)
+    none[[2, 5, 9]] = -1
+    twice, behind = apart.clone(), apart.clone()
+    twice[[2, 5]] = 7
+    behind[9] = 12
+    # (the pools hold 12 tokens)
+    for a, served in ((dict(slots=twice, positions=none), True), (dict(slots=behind, positions=none), True), (dict(slots=twice), False), (dict(slots=behind), False),
+                      (dict(slots=fake((10,), I32), positions=none), False), (dict(slots=fake((10,), I32), positions=none.clamp(max=-1)), True)):
+        for pools in ({}, dict(k_pool=pool(pages=1), v_pool=pool(pages=1))):
+            if pools and a["slots"] is behind:
+                continue       # (which hold 16)
+            with pytest.raises(AssertionError if served else ValueError):
+                paged.append_kv(**append(**pools, **a))
+    with pytest.raises(ValueError):       # a store knows no positions
+        paged.store_kv(fake((10, 2, 64)), fake((10, 2, 64)), pool(), pool(), twice)
