@@ -144,6 +144,14 @@ def grid(T: int, heads: int, D: int) -> tuple:
     return chunks, blocks
 
 
+def grids(T: int, Hq: int, Hkv: int, D: int) -> tuple:
+    """``grid`` of the queries and of the keys, which one launch has together."""
+    (q_chunks, q_blocks), (k_chunks, k_blocks) = grid(T, Hq, D), grid(T, Hkv, D)
+    if (q_blocks + k_blocks) * 256 >= 1 << 32:
+        raise UnsupportedPlan(f"a launch for {T} rows of {Hq} and {Hkv} heads of {D} is too large")
+    return q_chunks, q_blocks, k_chunks, k_blocks
+
+
 def _checked_positions(positions, places) -> None:
     if lowering._checks_tables() and len(positions) and int(positions.max()) >= places:
         raise ValueError(f"loopfuse_amd: positions must be below {places}")
@@ -215,8 +223,7 @@ def params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs) -> RotateParams:
     P.T, P.Hq, P.Hkv, P.D, P.R, P.pairs, P.norm, P.wide = T, Hq, Hkv, D, R, int(pairs), int(eps is not None), int(wide)
     P.eps = 0.0 if eps is None else float(eps)
     P.places, P.table_stride = (table.shape[0], table.stride(0)) if table is not None else (_ALL, 0)
-    P.q_chunks, P.q_blocks = grid(T, Hq, D)
-    P.k_chunks, P.k_blocks = grid(T, Hkv, D)
+    P.q_chunks, P.q_blocks, P.k_chunks, P.k_blocks = grids(T, Hq, Hkv, D)
     return P
 
 
@@ -256,7 +263,7 @@ def _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight
     for t, g in zip(saved, (dq_out, dk_out)):
         if t.shape != g.shape or t.dtype != g.dtype or t.device != g.device:
             raise UnsupportedPlan("gradients must be of the results' shape and dtype, with Q and K")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
+    weights, sizes = [w for w in (q_weight, k_weight) if w is not None], grids(T, Hq, Hkv, D)
     dq, dk = (torch.empty(t.shape, dtype=dtype, device=dev) for t in (dq_out, dk_out))
     dw = [torch.empty(D, dtype=weights[0].dtype, device=dev) if x else None for x in sums]
     if T == 0:
@@ -268,8 +275,7 @@ def _backward_general(dq_out, dk_out, q, k, positions, table, q_weight, k_weight
     P.T, P.Hq, P.Hkv, P.D, P.R, P.pairs, P.norm = T, Hq, Hkv, D, 0 if table is None else table.shape[1], int(pairs), int(eps is not None)
     P.wide, P.eps = int(bool(weights) and weights[0].dtype == torch.float32), 0.0 if eps is None else float(eps)
     P.places, P.table_stride = (table.shape[0], table.stride(0)) if table is not None else (_ALL, 0)
-    P.q_chunks, P.q_blocks = grid(T, Hq, D)
-    P.k_chunks, P.k_blocks = grid(T, Hkv, D)
+    P.q_chunks, P.q_blocks, P.k_chunks, P.k_blocks = sizes
     if any(sums):
         P.q_blocks, P.k_blocks = min(P.q_blocks, BWD_BLOCKS), min(P.k_blocks, BWD_BLOCKS)
     spec = kernel_spec(dtype, D)

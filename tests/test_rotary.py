@@ -265,3 +265,18 @@ def test_forward_mode_derivatives_of_the_table_are_refused(grad, monkeypatch):
         rows = fake((10, 2, 64))
         with pytest.raises(UnsupportedPlan, match="tangents"):
             paged.append_kv(a["q"].detach(), rows, rows, fake((3, 4, 2, 64)), fake((3, 4, 2, 64)), a["positions"], a["positions"], a["table"])
+
+
+def test_launches_whose_queries_and_keys_together_are_beyond_32_bits(monkeypatch):
+    """2^23 workgroups for the queries and as many for the keys, of 256 threads each."""
+    monkeypatch.setattr(lowering, "_check_tensor", lambda *a: None)
+    rows = fake((1, 1, 128)).expand(1 << 28, 1, 128)
+    positions, table = fake((1,), I32).expand(1 << 28), fake((4, 128), F32)
+    assert rotary.grid(1 << 28, 1, 128) == (1, 1 << 23)
+    for call in (lambda: rotary.rotate_heads(rows, rows, positions, table),
+                 lambda: rotary._backward(rows, rows, None, None, positions, table, None, None, None, False, (False, False))):
+        with pytest.raises(UnsupportedPlan, match="too large"):
+            call()
+    less = slice((1 << 28) - 32)
+    with pytest.raises(AssertionError, match="a launch"):
+        rotary.rotate_heads(rows[less], rows[less], positions[less], table)
