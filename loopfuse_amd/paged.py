@@ -863,6 +863,8 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     rows = 16 * blocks * (4 if rowwaves else 1)
     units = (T * P.group // rows + min(T, B)) * Hkv       # (at most: a chunk that is not full for each request)
     P.workgroups, P.fixed, P.least = cached_shares(units, keys, per, build, D)
+    if P.workgroups * 256 >= 1 << 32:
+        raise UnsupportedPlan(f"a launch for {T} rows of {Hq} heads, of {B} requests, is too large")
     P.per_group = (-(-(1 << 32) // P.group)) & 0xffffffff
     # (the line of all units, and rows times their division's error, are numbers in 32 bits)
     if units * (-(-room // 32) + 64) >= 1 << 31 or T * P.group ** 2 >= 1 << 32 or T * P.group >= 1 << 30:

@@ -303,3 +303,15 @@ def test_checked_slots_are_those_of_tokens(monkeypatch):
                 paged.append_kv(**append(**pools, **a))
     with pytest.raises(ValueError):       # a store knows no positions
         paged.store_kv(fake((10, 2, 64)), fake((10, 2, 64)), pool(), pool(), twice)
+
+
+def test_launches_of_a_unit_each_beyond_32_bits():
+    """2^24 requests of one token and few keys: 17 / 16 * 2^24 workgroups of 256 threads at most."""
+    def call(B):
+        one = lambda *shape: fake((1,) * len(shape), I32).expand(*shape)
+        return cached(q=fake((1, 1, 64)).expand(B, 1, 64), k_pool=pool(9, heads=1), v_pool=pool(9, heads=1), table=one(B, 1), lengths=one(B), offsets=None, positions=None)
+
+    for B, served in ((1 << 24, False), (15_800_000, False), (15_700_000, True)):
+        assert (B // 16 + B >= 1 << 24) != served
+        with pytest.raises(AssertionError if served else UnsupportedPlan):
+            paged.attention_cached(**call(B))
