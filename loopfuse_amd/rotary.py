@@ -45,7 +45,8 @@ class RotateBwdParams(ctypes.Structure):
 
 def rotary_table(length: int, dim: int, base: float = 10000.0, *, device=None, frequencies: Optional[torch.Tensor] = None) -> torch.Tensor:
     """float32 ``[length, dim]``: of each position the cosines of its ``dim / 2`` angles, then their sines.  Angle i is ``position * base ** (-2 i / dim)``, or
-    ``position * frequencies[i]``; formed in 64 bits, as angles of far positions have no digits left in 32."""
+    ``position * frequencies[i]``; formed in 64 bits, as angles of far positions have no digits left in 32.  On ``device``, or where the
+    frequencies are."""
     length, dim = operator.index(length), operator.index(dim)
     if length < 0 or dim < 2 or dim % 2:
         raise UnsupportedPlan("a table has 0 positions or more and an even number of rotated elements")
@@ -53,6 +54,8 @@ def rotary_table(length: int, dim: int, base: float = 10000.0, *, device=None, f
         frequencies = base ** (torch.arange(dim // 2, dtype=torch.float64, device=device) * (-2.0 / dim))
     elif frequencies.shape != (dim // 2,):
         raise UnsupportedPlan(f"frequencies must be [{dim // 2}]")
+    elif device is None:
+        device = frequencies.device
     angles = torch.arange(length, dtype=torch.float64, device=device)[:, None] * frequencies.to(device=device, dtype=torch.float64)
     return torch.cat((torch.cos(angles), torch.sin(angles)), 1).float()
 

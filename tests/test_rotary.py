@@ -280,3 +280,12 @@ def test_launches_whose_queries_and_keys_together_are_beyond_32_bits(monkeypatch
     less = slice((1 << 28) - 32)
     with pytest.raises(AssertionError, match="a launch"):
         rotary.rotate_heads(rows[less], rows[less], positions[less], table)
+
+
+def test_the_table_is_where_its_frequencies_are():
+    frequencies = torch.ones(4, device="meta")
+    assert rotary.rotary_table(3, 8, frequencies=frequencies).device.type == "meta"
+    assert rotary.rotary_table(3, 8, frequencies=torch.ones(4), device="meta").device.type == "meta"
+    with torch.device("meta"):
+        assert rotary.rotary_table(3, 8, frequencies=torch.ones(4, device="cpu")).device.type == "cpu"
+        assert rotary.rotary_table(3, 8).device.type == "meta"
