@@ -810,13 +810,14 @@ def _cached(q, k_pool, v_pool, plan, table, lengths, offsets, positions, out):
     mask = lowering._MASK_NAMES[plan.mask]
     if mask == lowering.MASK_SLIDING and plan.window < 1:
         raise UnsupportedPlan("sliding mask needs window >= 1")
-    if not (plan.scale > 0.0) or not math.isfinite(plan.scale):
-        raise UnsupportedPlan("score scale must be positive and finite")
+    narrow = lambda x: ctypes.c_float(x).value       # (as the kernels take it: masked scores, -inf, must not meet a scale of 0)
+    if not (narrow(plan.scale) > 0.0) or not math.isfinite(narrow(plan.scale)):
+        raise UnsupportedPlan("score scale must be positive and finite in 32 bits")
     softcap = None
     if plan.softcap is not None:
         softcap = abs(float(plan.softcap))
-        if not (softcap > 0.0) or not math.isfinite(softcap):
-            raise UnsupportedPlan("softcap must be finite and non-zero")
+        if not (narrow(softcap) > 0.0) or not math.isfinite(narrow(softcap)) or not math.isfinite(narrow(plan.scale / softcap)):
+            raise UnsupportedPlan("softcap, and the scale over it, must be finite, the cap non-zero, in 32 bits")
     _on_gpu("table", table, _TABLE_DTYPES, 2, q.device)
     _on_gpu("lengths", lengths, (torch.int32,), 1, q.device)
     B = table.shape[0]

@@ -315,3 +315,13 @@ def test_launches_of_a_unit_each_beyond_32_bits():
         assert (B // 16 + B >= 1 << 24) != served
         with pytest.raises(AssertionError if served else UnsupportedPlan):
             paged.attention_cached(**call(B))
+
+
+@pytest.mark.parametrize("scale,softcap", [(1e-46, None), (1e39, None), (0.1, 1e-46), (0.1, 1e39), (1.0, 1e-39), (1e-46, 1.0)])
+def test_scales_that_are_no_numbers_in_32_bits_are_refused(scale, softcap):
+    """The kernels multiply masked scores, -inf, with a scale that must not be 0, and divide by the cap."""
+    with pytest.raises(UnsupportedPlan):
+        paged.attention_cached(**cached(plan=AttnPlan("causal", scale=scale, softcap=softcap)))
+    for plan in (AttnPlan("causal", scale=1e-44), AttnPlan("causal", scale=1e38), AttnPlan("causal", scale=1e-30, softcap=1e30), AttnPlan("causal", scale=1.0, softcap=-1e-38)):
+        with pytest.raises(AssertionError, match="a launch"):
+            paged.attention_cached(**cached(plan=plan))

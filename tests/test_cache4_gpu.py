@@ -646,3 +646,12 @@ def test_inside_a_compiled_function():
     want = paged.attention_cached(q * 2, *pools, plan, table, n, offsets, positions)
     got = torch.compile(lambda q: paged.attention_cached(q * 2, *pools, plan, table, n, offsets, positions), backend="eager")(q)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("scale,cap", [(1e-44, None), (1e-30, 1e30), (1.0, 1e-30)])
+def test_scales_close_to_the_least_number(scale, cap):
+    """Scores that differ by nothing: rows are means of the values that they see."""
+    pools, table, n, offsets, positions = batch([70, 33], [9, 1], 16, 2, 64, BF, 1)
+    plan, q = AttnPlan("causal", 0, scale, cap, True, True), rnd((10, 8, 64), 2)
+    out = paged.attention_cached(q, *pools, plan, table, n, offsets, positions)
+    check(out, oracle(q, pools, plan, table, n, offsets, positions, BF))
