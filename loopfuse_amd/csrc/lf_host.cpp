@@ -693,8 +693,10 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   node->norm = a[6] != Py_None;
   node->eps = node->norm ? PyFloat_AS_DOUBLE(a[6]) : 0.0;
   node->pairs = a[7] == Py_True;
-  torch::autograd::SavedVariable* to[] = {&node->q, &node->k, &node->table, &node->q_weight, &node->k_weight, &node->positions};
-  for (int i = node->norm ? 0 : 2; i < 6; ++i) *to[i] = torch::autograd::SavedVariable(in[i], false);
+  // (in the order in which rotary._Rotate saves them: a recomputation may take either path, and what it saves is matched by its place)
+  const std::pair<torch::autograd::SavedVariable*, const at::Tensor*> saved[] = {{&node->q, &in[0]}, {&node->k, &in[1]}, {&node->positions, &in[5]},
+                                                                                 {&node->table, &in[2]}, {&node->q_weight, &in[3]}, {&node->k_weight, &in[4]}};
+  for (int i = node->norm ? 0 : 2; i < 6; ++i) *saved[i].first = torch::autograd::SavedVariable(*saved[i].second, false);
   for (int i = 0; i < 2; ++i) torch::autograd::set_history(THPVariable_Unpack(PyTuple_GET_ITEM(out, i)), node);
   return owned.release().ptr();
   END_HANDLE_TH_ERRORS

@@ -9,6 +9,7 @@ import threading
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from loopfuse_amd import packed, paged, rotary
 from loopfuse_amd.lowering import AttnPlan, UnsupportedPlan
@@ -450,3 +451,25 @@ def test_a_repeated_call_refuses_a_table_that_asks_for_a_gradient():
             rotary.rotate_heads(q, k, positions, table, **norm)
     with torch.no_grad():
         assert all(torch.equal(a, b) for a, b in zip(rotary.rotate_heads(q, k, positions, table, **norm), want))
+
+
+@pytest.mark.parametrize("norms", [True, False])
+@pytest.mark.parametrize("again", [False, True])
+def test_a_checkpointed_step_gives_the_gradients_of_a_plain_one(again, norms):
+    """What is saved in the forward is matched, one by one, with what the recomputation saves, which a call that is kept since then takes through the host module's node."""
+    q, k, positions, table, norm = operands(50, 4, 2, 64, 64, BF, BF, 9)
+    norm = norm if norms else {}
+    leaves = [t.requires_grad_() for t in (q, k, *(norm[n] for n in ("q_weight", "k_weight") if n in norm))]
+    grads = [rnd(t.shape, 30 + i) for i, t in enumerate((q, k))]
+    want = torch.autograd.grad(rotary.rotate_heads(q, k, positions, table, **norm), leaves, grads)
+    if not again:
+        rotary._host.clear()
+    for early in (True, False):
+        with torch.utils.checkpoint.set_checkpoint_early_stop(early):
+            y = torch.utils.checkpoint.checkpoint(lambda q, k: rotary.rotate_heads(q, k, positions, table, **norm), q, k, use_reentrant=False)
+            got = torch.autograd.grad(y, leaves, grads)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        if again:       # a recomputation whose call is no longer kept
+            y = torch.utils.checkpoint.checkpoint(lambda q, k: rotary.rotate_heads(q, k, positions, table, **norm), q, k, use_reentrant=False)
+            rotary._host.clear()
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, grads), want))
