@@ -121,7 +121,7 @@ typedef struct LfRotateParamsHost {
   const int32_t* positions;        /* [T]; null: all rows live */
   const int32_t* slots;    /* [T] */
   int64_t q_ss, q_sh, k_ss, k_sh, v_ss, v_sh;
-  int64_t kp_sb, kp_ss, kp_sh, vp_sb, vp_ss, vp_sh;  /* pools; in 4 bits bytes of a page's codes, of its scales, unused; without a pool the first and the last unused */
+  int64_t kp_sb, kp_ss, kp_sh, vp_sb, vp_ss, vp_sh;  /* pools; in 4 bits bytes of a page's codes, of its scales, unused; all unused without a pool */
   int64_t table_stride, last;      /* last: slots of a pool */
   int32_t T, Hq, Hkv, D, R, places;
   int32_t q_chunks, k_chunks;      /* items of a token */

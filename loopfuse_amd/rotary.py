@@ -209,7 +209,6 @@ def _general(q, k, positions, table, q_weight, k_weight, eps, pairs):
     P = params(q, k, table, T, Hq, Hkv, D, R, wide, eps, pairs)
     if T == 0:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    P.kp_ss, P.kp_sh = Hkv * D, D
     spec = kernel_spec(q.dtype, D)
     repeat = lowering._Repeat(P, [(lowering.get_kernel(spec, spec.entry()), (P.q_blocks + P.k_blocks, 1, 1), 256)], {"kernels": [spec.entry()]})
     even = positions.contiguous(), even_weight(q_weight), even_weight(k_weight)
