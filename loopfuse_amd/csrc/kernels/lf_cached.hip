@@ -18,8 +18,9 @@
 //
 // Few rows: 16 of a kv head, or 32, a workgroup's four waves have a fourth of the pairs of tiles each and merge through LDS in the end; operands straight from memory, two pairs under way, no LDS
 // and no barrier in the loop.  Bound by memory where keys are many: 64 requests of one token up to 8192 keys, 32/8 heads of 128, 53 us and 5 for the joining (291 MB, 5.0 TB/s both); 4 up to
-// 100 000 47 and 5 (272 MB, 5.2); by one wave's chain where they are few: 2 up to 1000 10 us, of which lengths and shares 1.2, the first loads 0.9, eight pairs 4.2, the merge 0.8;
-// by conversions, softmax and products in between: 64 up to 8192 with five new tokens each 74 us, 32 rows at a time (16: 99).
+// 100 000 47 and 5 (272 MB, 5.2); by one wave's chain where they are few: 2 up to 1000 10 us, 16 700 cycles of a wave: lengths and shares 2600, the first loads 2300, eight pairs 9800, the merge 1700; 48 requests of five new tokens in a
+// window of 1024 with a cap, 16/4 heads of 64, 15 us, 25 400 cycles: 3800, 3800, 14 300, 3000.  Of either's cycles waves wait in 0.47 and issue in 0.43.
+// By conversions, softmax and products in between: 64 up to 8192 with five new tokens each 74 us, 32 rows at a time (16: 99).
 // Many rows (LF_CACHED_ROWWAVES): 128, each wave has 32 of them over all pairs.  Of a pair two waves convert a tile of keys each, two one of values, into LDS, where all four find the operands as the
 // products take them: a fourth of the conversions, and fewer registers, so that three waves run on a SIMD.  Bound by the softmax and the products: 4 requests up to 6001 keys with up to 1000
 // new tokens 230 us (213 GFLOP, 926 TFLOP/s; each wave with keys and values of its own 257), 2 of 8192 with 4096 805 us (1025; 897).
@@ -306,8 +307,10 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES && LF_HEAD_
 #else
   constexpr int kStep = 4;
   const int first = wave;
-  // 128 MB of codes and more, which are not in a cache the next time anyhow, pass the caches by.  us, kept / by: 4 requests up to 100 000 keys 58.4 / 52.1, 64 up to 8192 64.2 / 57.7, 16 of 8000 (139 MB) 36.1 / 33.9;
-  // 8 of 8000 (70 MB) 21.6 / 22.2, 4 of 8192 with 4 new tokens (36 MB) 18.3 / 19.5.
+  // Codes that are not in a cache the next time anyhow pass the caches by: from 128 MB on, as the line counts them.  That is each request's keys once for each chunk of its rows, and `fixed` pairs more for every
+  // unit: more than there are where requests are short or have several chunks.  us, kept / by: 4 requests up to 100 000 keys 58.4 / 52.1, 64 up to 8192 64.2 / 57.7, 16 of 8000 (139 MB) 35.7 / 33.3;
+  // 8 of 8000 (70 MB) 20.7 / 21.6, 4 of 8192 with 4 new tokens (36 MB) 18.3 / 19.5.  By the line, but not by their codes, beyond it: 256 of 128 in wide tables (35 MB) 28.8 / 32.1,
+  // 8 of 8000 with 10 new tokens (70 MB, two chunks) 36.2 / 39.9.
   constexpr int kStream = (128 << 20) / (34 * D);       // pairs of tiles
   struct Ids {
     int a, b;                  // (a pool has less than 2^31 pages)
@@ -510,6 +513,8 @@ extern "C" __global__ void __launch_bounds__(256, LF_CACHED_ROWWAVES && LF_HEAD_
       for (int i = 0; i < 8; ++i) {
         const float e = lf_exp2(__builtin_fmaf(r[cb][i / 4][i % 4], cexp, -m_sub));
         l_part[cb] += e;
+        // (the second product's operand, so of the rows' type; two such parts of it would be twice the products.  Relative 2-norm against 64 bits 2.1e-3 to 2.3e-3 in bf16 and 2.8e-4 in fp16, where the
+        // result's own rounding is 1.7e-3 and 2.1e-4)
         pb[cb][i] = lf_from_float(e);
       }
     }

@@ -10,10 +10,10 @@
 // LF_ROT_SLOTS threads have a row, 16 elements each: 8 of either half of what is rotated, or of the rest, so that no value changes threads
 // but in the norm's sum (row permutations of 16 lanes) and a load or store of several threads has whole lines.  A group of threads takes two heads of a token, whose row of the table it
 // reads once: one, two and four at a time took 134 / 129 / 133 us forwards and backwards together, 75 / 75 / 79 into pages and 50 / 48 / 50 into 4 bits and back, at the sizes below and
-// before rows were read past the caches: 129 -> 118, 75 -> 66 and 49 -> 48 in loops of 20 passes over other rows, 128 -> 125, 74 -> 76 and 53 -> 49 over seconds of nothing else.
+// before rows were read past the caches.  Reading them so took 128 to 125, 74 to 76, which is slower, and 53 to 49 over seconds of nothing else; 129 to 118, 75 to 66 and 49 to 48 in loops of 20 passes over other rows.
 //
-// Bound by memory: 8192 rows of 32 and 32 heads of 128 in bf16 with norms 43 us forwards (268 MB, 6.2 TB/s) and 69 backwards with the weights' gradients (403 MB, 5.8); 16384 rows of 32 and 8 heads into
-// pages 65 (407 MB, 6.2); 8192 such rows into 4 bits 37 (177 MB, 4.8).
+// Bound by memory.  Seconds of nothing else: 8192 rows of 32 and 32 heads of 128 in bf16 with norms, forwards and backwards with the weights' gradients, 126 us (671 MB, 5.3 TB/s); 16384 rows of 32 and 8 heads
+// into pages 76 (407 MB, 5.3).  A kernel among 300 passes: the former's 43 forwards (268 MB, 6.2 TB/s) and 69 backwards (403 MB, 5.8), the latter 65 (6.2), 8192 such rows into 4 bits 37 (177 MB, 4.8).
 // One new token each for up to 64 requests: 3.5 to 4.5 us, a launch and two round trips to memory.
 //
 // In 4 bits: 32 neighbours of a row share a power of two, 2^e with the least e of which their largest size is below 7 * 2^e (what lies between

@@ -366,7 +366,7 @@ def read_kv(k_pool: Union[torch.Tensor, Pool4], v_pool: Union[torch.Tensor, Pool
     """Rows of keys and values out of the page pools, what ``store_kv`` and ``append_kv`` have put there: ``(k, v)``, each ``[rows, Hkv, D]``, row t of slot ``slots[t]``
     (int32 ``[rows]`` on the GPU, any number of times), zeros where it is below 0 or behind the pool's last.  From pools in 4 bits the values that they stand for,
     rounded to the type (those of fp16 have less than a bit below its least normal number).  For keys that go on elsewhere: into another cache, or beside
-    those of a prompt's next part."""
+    those of a prompt's next part.  No gradients are recorded."""
     dtype = k_pool.dtype if isinstance(k_pool, (Pool4, torch.Tensor)) else None
     parts = _parts(k_pool, v_pool, dtype)
     done = None if parts is None else _host.read_kv(*parts, slots, dtype is torch.float16)
